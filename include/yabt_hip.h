@@ -493,6 +493,67 @@ int yabt_predict(const float *X, int64_t ldx, int64_t n, int F, int T, const int
                  const int32_t *net_feats, const float *linear, const float *lo, const float *hi,
                  float base, int accumulate, float *out, yabt_stream_t stream);
 
+/* ---------------------------------------------------------------------------
+ * The expert layer: rows are normalised, a gate's scores route each to k of E
+ * experts, the experts' answers are weighted and added.  The learned, soft
+ * form of a tree with models in its leaves (yabt/neural_leaves.py:93-184),
+ * which routes a row to one leaf.  `dtype`: 0 fp32, 1 bf16, 2 fp16; rows of
+ * any leading dimension and alignment; sums and statistics are fp32, one
+ * rounding at the end; no atomics on sums, so results are the same every time.
+ * ------------------------------------------------------------------------- */
+
+/* Layer norm of n rows of width D:
+ *   mean = sum x / D, rstd = 1 / sqrt(sum (x - mean)^2 / D + eps),
+ *   y = (x - mean) * rstd * weight + bias
+ * weight, bias (D, fp32), mean and rstd (n, fp32) may be NULL. */
+int yabt_layer_norm(int dtype, const void *x, int64_t ldx, int64_t n, int D, const float *weight,
+                    const float *bias, float eps, void *y, int64_t ldy, float *mean, float *rstd,
+                    yabt_stream_t stream);
+
+/* Its gradients from dy and the forward pass's mean and rstd; with t = dy *
+ * weight and xh = (x - mean) * rstd:
+ *   dx = rstd * (t - sum t / D - xh * sum (t xh) / D)   (NULL: not wanted)
+ *   dweight = sum over rows of dy * xh, dbias = sum over rows of dy  (D, fp32; NULL: not wanted)
+ * weight NULL counts as ones.  The row sums are added in an order that n and D fix. */
+size_t yabt_layer_norm_grad_workspace_bytes(int64_t n, int D);
+int yabt_layer_norm_grad(int dtype, const void *dy, int64_t lddy, const void *x, int64_t ldx, int64_t n,
+                         int D, const float *weight, const float *mean, const float *rstd,
+                         void *workspace, size_t workspace_bytes, void *dx, int64_t lddx,
+                         float *dweight, float *dbias, yabt_stream_t stream);
+
+/* Route n rows to k of E experts (1 <= E <= 1024, 1 <= k <= min(E, 32)).
+ *   scores 0, softmax: p = softmax(logits), an expert's key is logit + bias
+ *   scores 1, sigmoid: p = 1 / (1 + exp(-logit)), its key is p + bias
+ * keys are fp32; bias (E, fp32) may be NULL and changes the choice alone.  A
+ * logit of -inf or NaN closes the expert to the row.  groups > 1 (at most 64,
+ * a divisor of E): the keep_groups groups of E / groups consecutive experts
+ * with the best score stay, the largest key of a group (softmax) or the sum
+ * of its two largest (sigmoid), equal ones by the lower group.  The k largest
+ * keys are chosen, equal ones by the lower expert, largest first:
+ *   out_ids (n, k) int32, -1 where no expert was left
+ *   out_weights (n, k) fp32 = scale * p, or with renormalise scale * p / sum
+ *     of the row's chosen p; 0 where the id is -1. */
+int yabt_route(int dtype, const void *logits, int64_t ldl, int64_t n, int E, int k, int scores,
+               const float *bias, int groups, int keep_groups, int renormalise, float scale,
+               int32_t *out_ids, float *out_weights, yabt_stream_t stream);
+
+/* Gradient of the weights of yabt_route in the logits, the choice held fixed:
+ * dweights (n, k) fp32 and the ids it gave, distinct within a row (others than
+ * 0..E-1 take no part), to out_dlogits (n, E) in the logits' type. */
+int yabt_route_grad(int dtype, const float *dweights, int64_t lddw, const void *logits, int64_t ldl,
+                    const int32_t *ids, int64_t n, int E, int k, int scores, int renormalise,
+                    float scale, void *out_dlogits, int64_t lddl, yabt_stream_t stream);
+
+/* The slots s = row * k + j of ids (n, k), sorted by expert (stable, so an
+ * expert's slots are in row order); slots whose id is not in [0, E) are left
+ * out.  n k < 2^31.
+ *   out_offsets (E + 1): expert e's slots are places offsets[e] .. offsets[e+1]
+ *   out_slots, out_rows (n k): the slot at a place and its row, -1 past the last. */
+size_t yabt_expert_plan_workspace_bytes(int64_t n, int k, int E);
+int yabt_expert_plan(const int32_t *ids, int64_t n, int k, int E, void *workspace,
+                     size_t workspace_bytes, int32_t *out_offsets, int32_t *out_slots,
+                     int32_t *out_rows, yabt_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -96,6 +96,15 @@ SIGNATURES = {
     "yabt_margin_update": (_int, [_vp, _i64, _vp, _vp, _i64, _int, _vp, _vp, _vp, _vp, _int, _vp, _i64, _vp]),
     "yabt_predict": (_int, [_vp, _i64, _i64, _int, _int, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _int, _vp, _vp,
                             _vp, _vp, _vp, _flt, _int, _vp, _vp]),
+    "yabt_layer_norm": (_int, [_int, _vp, _i64, _i64, _int, _vp, _vp, _flt, _vp, _i64, _vp, _vp, _vp]),
+    "yabt_layer_norm_grad_workspace_bytes": (_sz, [_i64, _int]),
+    "yabt_layer_norm_grad": (_int, [_int, _vp, _i64, _vp, _i64, _i64, _int, _vp, _vp, _vp, _vp, _sz, _vp, _i64,
+                                    _vp, _vp, _vp]),
+    "yabt_route": (_int, [_int, _vp, _i64, _i64, _int, _int, _int, _vp, _int, _int, _int, _flt, _vp, _vp, _vp]),
+    "yabt_route_grad": (_int, [_int, _vp, _i64, _vp, _i64, _vp, _i64, _int, _int, _int, _int, _flt, _vp, _i64,
+                               _vp]),
+    "yabt_expert_plan_workspace_bytes": (_sz, [_i64, _int, _int]),
+    "yabt_expert_plan": (_int, [_vp, _i64, _int, _int, _vp, _sz, _vp, _vp, _vp, _vp]),
 }
 
 

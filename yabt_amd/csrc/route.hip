@@ -1,0 +1,565 @@
+// Routing rows to experts: the k best of E scores, their weights, the weights'
+// gradient, and the plan that sorts the slots by expert.
+//
+//   p = softmax(l) or 1 / (1 + exp(-l)); an expert is chosen by its key,
+//   key = l + bias (softmax, whose order is the logits') or p + bias (sigmoid),
+//   in fp32; a logit of -inf or NaN closes the expert to the row.  With groups
+//   the best `keep` groups stay, by their largest key (softmax) or the sum of
+//   their two largest (sigmoid).  The k largest keys win, equal ones by the
+//   lower index; w_j = scale p_j, or scale p_j / sum of the chosen p.
+//
+// A row is held by G lanes, NV consecutive experts each.  A key and its expert
+// travel as one double: the key's 24 bits in front, the expert's number in low
+// bits that the key leaves free, so that one v_max_f64 compares both.  A lane
+// sorts its own keys once (an odd-even merge network); a round then takes the
+// largest of the G heads over DPP and the winner drops its head.
+
+#include "expert.h"
+#include "yabt_hip.h"
+
+namespace yabt {
+
+constexpr int ROUTE_NT = 256;
+constexpr int ROUTE_MAX_E = 1024, ROUTE_MAX_K = 32, ROUTE_MAX_GROUPS = 64;
+constexpr int SOFTMAX = 0, SIGMOID = 1;
+
+#define YABT_NEG_INF (-__builtin_inff())
+
+__device__ __forceinline__ float sigmoid(float x) { return 1.0f / (1.0f + expf(-x)); }
+
+// (key, e) as one double that orders by key, then by lower e; -inf carries no e.
+__device__ __forceinline__ double key_pack(float key, int e) {
+    if (!(key > YABT_NEG_INF)) return -__builtin_inf();
+    key += 0.0f;                                    // -0 is 0
+    const double d = key == __builtin_inff() ? 0x1p128 : (double)key;
+    const uint64_t low = (uint64_t)(key >= 0.0f ? ROUTE_MAX_E - 1 - e : e);
+    return __longlong_as_double((long long)((uint64_t)__double_as_longlong(d) | low));
+}
+__device__ __forceinline__ int key_expert(double m) {
+    const uint64_t u = (uint64_t)__double_as_longlong(m);
+    const int low = (int)(u & (ROUTE_MAX_E - 1));
+    return (u >> 63) ? low : ROUTE_MAX_E - 1 - low;
+}
+
+// h sorted descending by an odd-even merge network.
+template <int NV>
+__device__ __forceinline__ void sort_desc(double (&h)[NV]) {
+#pragma unroll
+    for (int p = 1; p < NV; p *= 2)
+#pragma unroll
+        for (int q = p; q >= 1; q /= 2)
+#pragma unroll
+            for (int j = q % p; j <= NV - 1 - q; j += 2 * q)
+#pragma unroll
+                for (int i = 0; i < q; ++i)
+                    if (i + j + q < NV && (i + j) / (p * 2) == (i + j + q) / (p * 2)) {
+                        const double a = h[i + j], b = h[i + j + q];
+                        h[i + j] = fmax(a, b);
+                        h[i + j + q] = fmin(a, b);
+                    }
+}
+
+// A lane's NV consecutive logits; -inf for those past E and for NaN.
+template <typename T, int NV>
+__device__ __forceinline__ void load_logits(const T* row, int e0, int E, float (&x)[NV]) {
+    typedef T VT __attribute__((ext_vector_type(NV), aligned(sizeof(T))));
+    if constexpr (NV > 1) {
+        if (e0 + NV <= E) {
+            const VT v = *reinterpret_cast<const VT*>(row + e0);
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const float f = (float)v[i];
+                x[i] = f > YABT_NEG_INF ? f : YABT_NEG_INF;
+            }
+            return;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const float f = e0 + i < E ? (float)row[e0 + i] : YABT_NEG_INF;
+        x[i] = f > YABT_NEG_INF ? f : YABT_NEG_INF;
+    }
+}
+
+// Max and sum of exp(x - max) of a row; those of a row without open experts
+// count as 0 and 1, so that its scores are 0.
+template <int G, int NV>
+__device__ __forceinline__ void softmax_stats(const float (&x)[NV], float* top, float* sum) {
+    float m = x[0];
+#pragma unroll
+    for (int i = 1; i < NV; ++i) m = fmaxf(m, x[i]);
+    m = lanes_max<G>(m);
+    if (m == YABT_NEG_INF) m = 0.0f;
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) s += expf(x[i] - m);
+    s = lanes_sum<G>(s);
+    *top = m;
+    *sum = s > 0.0f ? s : 1.0f;
+}
+
+struct RouteArgs {
+    int64_t ldl, n;
+    int E, k, scores, renormalise;
+    int groups, keep, per_group, magic;     // magic: ceil(2^20 / per_group)
+    float scale;
+};
+
+// The p of the chosen experts (lane j holds slots j and j + G) turned into v:
+// p / sum with `renorm`, p itself without; *total: the sum (softmax with
+// renorm: of the exponentials).
+template <int G, int S>
+__device__ __forceinline__ void chosen_scores(const RouteArgs& A, const float (&l)[S], const bool (&on)[S], float top,
+                                              float sum, float (&p)[S], float (&v)[S], float* total) {
+    float t = 0.0f;
+    if (A.scores == SOFTMAX && A.renormalise) {
+        // over the chosen alone: the others' exponentials cancel
+        float m = YABT_NEG_INF;
+#pragma unroll
+        for (int s = 0; s < S; ++s) m = on[s] ? fmaxf(m, l[s]) : m;
+        m = lanes_max<G>(m);
+#pragma unroll
+        for (int s = 0; s < S; ++s) p[s] = on[s] ? expf(l[s] - m) : 0.0f;
+    } else {
+#pragma unroll
+        for (int s = 0; s < S; ++s)
+            p[s] = !on[s] ? 0.0f : A.scores == SOFTMAX ? expf(l[s] - top) / sum : sigmoid(l[s]);
+    }
+#pragma unroll
+    for (int s = 0; s < S; ++s) t += p[s];
+    t = lanes_sum<G>(t);
+    *total = t;
+#pragma unroll
+    for (int s = 0; s < S; ++s) v[s] = !A.renormalise ? p[s] : t > 0.0f ? p[s] / t : 0.0f;
+}
+
+template <typename T, int G, int NV, bool GROUPS>
+__global__ void __launch_bounds__(ROUTE_NT) k_route(RouteArgs A, const T* __restrict__ logits,
+                                                    const float* __restrict__ bias, int32_t* __restrict__ ids,
+                                                    float* __restrict__ weights) {
+    constexpr int R = ROUTE_NT / G, S = (ROUTE_MAX_K + G - 1) / G;
+    __shared__ float s_key[GROUPS ? R : 1][GROUPS ? G * NV : 1];
+    __shared__ float s_score[GROUPS ? R : 1][GROUPS ? ROUTE_MAX_GROUPS : 1];
+    __shared__ int s_stay[GROUPS ? R : 1][GROUPS ? ROUTE_MAX_GROUPS : 1];
+    const int lane = threadIdx.x % G, sub = threadIdx.x / G, e0 = lane * NV;
+    float bv[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) bv[i] = bias && e0 + i < A.E ? bias[e0 + i] : 0.0f;
+    for (int64_t r0 = (int64_t)blockIdx.x * R; r0 < A.n; r0 += (int64_t)gridDim.x * R) {
+        // rows past the end are walked as the last one, and not written
+        const int64_t r = min(r0 + sub, A.n - 1);
+        const T* row = logits + (size_t)r * (size_t)A.ldl;
+        float x[NV], top = 0.0f, sum = 1.0f;
+        load_logits<T, NV>(row, e0, A.E, x);
+        if (A.scores == SOFTMAX && !A.renormalise) softmax_stats<G, NV>(x, &top, &sum);
+        float key[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const float p = A.scores == SOFTMAX ? x[i] : sigmoid(x[i]);
+            const float q = p + bv[i];
+            key[i] = x[i] > YABT_NEG_INF && q > YABT_NEG_INF ? q : YABT_NEG_INF;
+        }
+        if constexpr (GROUPS) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) s_key[sub][e0 + i] = key[i];
+            wave_sync_lds();
+            for (int g = lane; g < A.groups; g += G) {
+                float a = YABT_NEG_INF, b = YABT_NEG_INF;     // the group's two largest keys
+                int at = g % A.per_group;                     // lanes start apart: other banks
+                for (int i = 0; i < A.per_group; ++i) {
+                    const float q = s_key[sub][g * A.per_group + at];
+                    b = fmaxf(b, fminf(a, q));
+                    a = fmaxf(a, q);
+                    at = at + 1 == A.per_group ? 0 : at + 1;
+                }
+                s_score[sub][g] = A.scores == SIGMOID && b > YABT_NEG_INF ? a + b : a;
+            }
+            wave_sync_lds();
+            // a group stays if fewer than `keep` are before it
+            for (int g = lane; g < A.groups; g += G) {
+                const float own = s_score[sub][g];
+                int before = 0;
+                for (int o = 0; o < A.groups; ++o) {
+                    const float q = s_score[sub][o];
+                    before += q > own || (q == own && o < g);
+                }
+                s_stay[sub][g] = before < A.keep;
+            }
+            wave_sync_lds();
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int g = min((int)(((uint32_t)(e0 + i) * (uint32_t)A.magic) >> 20), A.groups - 1);
+                if (!s_stay[sub][g]) key[i] = YABT_NEG_INF;
+            }
+            wave_sync_lds();
+        }
+        double h[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) h[i] = key_pack(key[i], e0 + i);
+        sort_desc<NV>(h);
+        int mine[S];
+#pragma unroll
+        for (int s = 0; s < S; ++s) mine[s] = -1;
+        for (int j = 0; j < A.k; ++j) {
+            const double m = lanes_reduce<G>(h[0], [](double a, double b) { return fmax(a, b); });
+            const int e = m > -__builtin_inf() ? key_expert(m) : -1;
+#pragma unroll
+            for (int s = 0; s < S; ++s)
+                if (j == s * G + lane) mine[s] = e;
+            if (h[0] == m) {
+#pragma unroll
+                for (int i = 0; i + 1 < NV; ++i) h[i] = h[i + 1];
+                h[NV - 1] = -__builtin_inf();
+            }
+        }
+        float l[S], p[S], v[S], total;
+        bool on[S];
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            on[s] = mine[s] >= 0;
+            l[s] = on[s] ? (float)row[mine[s]] : 0.0f;
+        }
+        chosen_scores<G, S>(A, l, on, top, sum, p, v, &total);
+        if (r0 + sub < A.n) {
+#pragma unroll
+            for (int s = 0; s < S; ++s) {
+                const int j = s * G + lane;
+                if (j < A.k) {
+                    ids[(size_t)r * A.k + j] = mine[s];
+                    weights[(size_t)r * A.k + j] = A.scale * v[s];
+                }
+            }
+        }
+    }
+}
+
+// d(weights) to d(logits), the choice held fixed (ids as k_route left them;
+// one outside [0, E) takes no part):
+//   softmax, renormalised: v = softmax over the chosen, dl_j = v_j (dw_j - sum v dw)
+//   softmax:  dl_i = p_i ([i chosen] dw_i - sum_chosen p dw)
+//   sigmoid, renormalised: v = p / t, dl_j = (dw_j - sum v dw) / t p_j (1 - p_j)
+//   sigmoid:  dl_j = dw_j p_j (1 - p_j)                    with dw scaled by `scale`
+template <typename T, int G, int NV>
+__global__ void __launch_bounds__(ROUTE_NT) k_route_grad(RouteArgs A, const float* __restrict__ dweights, int64_t lddw,
+                                                         const T* __restrict__ logits,
+                                                         const int32_t* __restrict__ ids, T* __restrict__ dlogits,
+                                                         int64_t lddl) {
+    constexpr int R = ROUTE_NT / G, S = (ROUTE_MAX_K + G - 1) / G;
+    __shared__ float s_d[R][G * NV];
+    const int lane = threadIdx.x % G, sub = threadIdx.x / G, e0 = lane * NV;
+    for (int64_t r0 = (int64_t)blockIdx.x * R; r0 < A.n; r0 += (int64_t)gridDim.x * R) {
+        const int64_t r = min(r0 + sub, A.n - 1);
+        const T* row = logits + (size_t)r * (size_t)A.ldl;
+        const bool whole = A.scores == SOFTMAX && !A.renormalise;
+        float x[NV], top = 0.0f, sum = 1.0f;
+        if (whole) {
+            load_logits<T, NV>(row, e0, A.E, x);
+            softmax_stats<G, NV>(x, &top, &sum);
+        }
+        int id[S];
+        float l[S], dw[S], p[S], v[S], total, mean = 0.0f;
+        bool on[S];
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            const int j = s * G + lane;
+            id[s] = j < A.k ? ids[(size_t)r * A.k + j] : -1;
+            on[s] = id[s] >= 0 && id[s] < A.E;
+            l[s] = on[s] ? (float)row[id[s]] : 0.0f;
+            dw[s] = on[s] ? dweights[(size_t)r * (size_t)lddw + j] * A.scale : 0.0f;
+        }
+        chosen_scores<G, S>(A, l, on, top, sum, p, v, &total);
+#pragma unroll
+        for (int s = 0; s < S; ++s) mean += v[s] * dw[s];
+        mean = lanes_sum<G>(mean);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) s_d[sub][e0 + i] = whole ? -(expf(x[i] - top) / sum) * mean : 0.0f;
+        wave_sync_lds();
+#pragma unroll
+        for (int s = 0; s < S; ++s)
+            if (on[s]) {
+                float d;
+                if (A.scores == SOFTMAX) d = v[s] * (whole ? dw[s] : dw[s] - mean);
+                else if (A.renormalise) d = total > 0.0f ? (dw[s] - mean) / total * p[s] * (1.0f - p[s]) : 0.0f;
+                else d = dw[s] * p[s] * (1.0f - p[s]);
+                atomicAdd(&s_d[sub][id[s]], d);
+            }
+        wave_sync_lds();
+        if (r0 + sub < A.n) {
+            T* o = dlogits + (size_t)r * (size_t)lddl;
+            for (int e = lane; e < A.E; e += G) o[e] = (T)s_d[sub][e];
+        }
+        wave_sync_lds();
+    }
+}
+
+// ---------------------------------------------------------------------------
+// The plan: a stable counting sort of the slots (row, j) by expert.
+// ---------------------------------------------------------------------------
+
+constexpr int PLAN_NT = 512, PLAN_W = PLAN_NT / 64;
+constexpr int PLAN_CHUNK = 2048;        // slots a block sorts, at least
+constexpr int PLAN_BLOCKS = 1024;       // blocks at most
+
+struct PlanArgs {
+    const int32_t* ids;
+    int64_t S;
+    int k, E, bits;                     // bits: of an expert's number
+    int64_t chunk;                      // slots per block, a multiple of PLAN_NT
+    int blocks;
+};
+
+// Counts of each wave's part of the block's slots by expert, s_cnt[w][e].
+__device__ __forceinline__ void plan_count(const PlanArgs& A, int64_t lo, int64_t hi, uint32_t* s_cnt) {
+    const int w = threadIdx.x / 64, lane = threadIdx.x & 63;
+    for (int i = threadIdx.x; i < PLAN_W * A.E; i += PLAN_NT) s_cnt[i] = 0;
+    __syncthreads();
+    const int64_t per = A.chunk / PLAN_W;
+    const int64_t a = lo + w * per, b = min(hi, a + per);
+    for (int64_t s = a + lane; s < b; s += 64) {
+        const int e = A.ids[s];
+        if (e >= 0 && e < A.E) atomicAdd(&s_cnt[w * A.E + e], 1u);
+    }
+    __syncthreads();
+}
+
+// Slots of [lo, hi) to their places, base s_cnt[w][e] moving on as they go.
+__device__ __forceinline__ void plan_place(const PlanArgs& A, int64_t lo, int64_t hi, uint32_t* s_cnt,
+                                           int32_t* slots, int32_t* rows) {
+    const int w = threadIdx.x / 64, lane = threadIdx.x & 63;
+    const int64_t per = A.chunk / PLAN_W;
+    const int64_t a = lo + w * per, b = min(hi, a + per);
+    for (int64_t s0 = a; s0 < b; s0 += 64) {
+        const int64_t s = s0 + lane;
+        const int e = s < b ? A.ids[s] : -1;
+        const bool ok = e >= 0 && e < A.E;
+        uint64_t same = __ballot(ok);
+        for (int i = 0; i < A.bits; ++i) {
+            const uint64_t one = __ballot(e >> i & 1);
+            same &= (e >> i & 1) ? one : ~one;
+        }
+        if (ok) {
+            const int before = __popcll(same & ((1ull << lane) - 1ull));
+            const uint32_t pos = s_cnt[w * A.E + e] + (uint32_t)before;
+            slots[pos] = (int32_t)s;
+            rows[pos] = (int32_t)(s / A.k);
+        }
+        wave_sync_lds();
+        if (ok && (same >> lane) == 1ull) s_cnt[w * A.E + e] += (uint32_t)__popcll(same);
+        wave_sync_lds();
+    }
+}
+
+// Exclusive prefix of v over the block's threads; s: PLAN_W words.
+__device__ __forceinline__ uint32_t plan_scan(uint32_t v, uint32_t* s, uint32_t* total) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x / 64;
+    uint32_t t = v;
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+        const uint32_t o = (uint32_t)__shfl_up((int)t, m);
+        if (lane >= m) t += o;
+    }
+    __syncthreads();
+    if (lane == 63) s[w] = t;
+    __syncthreads();
+    uint32_t before = 0, all = 0;
+#pragma unroll
+    for (int i = 0; i < PLAN_W; ++i) {
+        before += i < w ? s[i] : 0u;
+        all += s[i];
+    }
+    *total = all;
+    return before + t - v;
+}
+
+__global__ void __launch_bounds__(PLAN_NT) k_plan_count(PlanArgs A, uint32_t* __restrict__ cnt) {
+    extern __shared__ uint32_t s_cnt[];
+    const int64_t lo = blockIdx.x * A.chunk, hi = min(A.S, lo + A.chunk);
+    plan_count(A, lo, hi, s_cnt);
+    for (int e = threadIdx.x; e < A.E; e += PLAN_NT) {
+        uint32_t t = 0;
+        for (int w = 0; w < PLAN_W; ++w) t += s_cnt[w * A.E + e];
+        cnt[(size_t)e * A.blocks + blockIdx.x] = t;
+    }
+}
+
+// Expert e = blockIdx.x: its counts over the blocks become a prefix, tot[e] their sum.
+__global__ void __launch_bounds__(PLAN_NT) k_plan_scan(PlanArgs A, uint32_t* __restrict__ cnt,
+                                                       uint32_t* __restrict__ tot) {
+    __shared__ uint32_t s_w[PLAN_W];
+    uint32_t* c = cnt + (size_t)blockIdx.x * A.blocks;
+    uint32_t carry = 0;
+    for (int b0 = 0; b0 < A.blocks; b0 += PLAN_NT) {
+        const int b = b0 + threadIdx.x;
+        const uint32_t v = b < A.blocks ? c[b] : 0u;
+        uint32_t all;
+        const uint32_t p = plan_scan(v, s_w, &all);
+        if (b < A.blocks) c[b] = carry + p;
+        carry += all;
+    }
+    if (threadIdx.x == 0) tot[blockIdx.x] = carry;
+}
+
+// One block (cnt null: A.blocks == 1, the counts are its own) or all of them
+// after the scan.
+__global__ void __launch_bounds__(PLAN_NT) k_plan_place(PlanArgs A, const uint32_t* __restrict__ cnt,
+                                                        const uint32_t* __restrict__ tot,
+                                                        int32_t* __restrict__ offsets, int32_t* __restrict__ slots,
+                                                        int32_t* __restrict__ rows) {
+    extern __shared__ uint32_t s_cnt[];
+    __shared__ uint32_t s_w[PLAN_W];
+    const int64_t lo = blockIdx.x * A.chunk, hi = min(A.S, lo + A.chunk);
+    plan_count(A, lo, hi, s_cnt);
+    uint32_t carry = 0;
+    for (int e0 = 0; e0 < A.E; e0 += PLAN_NT) {
+        const int e = e0 + threadIdx.x;
+        uint32_t mine = 0, all;
+        if (e < A.E) {
+            if (cnt) mine = tot[e];
+            else
+                for (int w = 0; w < PLAN_W; ++w) mine += s_cnt[w * A.E + e];
+        }
+        uint32_t at = carry + plan_scan(mine, s_w, &all);
+        carry += all;
+        if (e < A.E) {
+            if (blockIdx.x == 0) offsets[e] = (int32_t)at;
+            if (cnt) at += cnt[(size_t)e * A.blocks + blockIdx.x];
+            for (int w = 0; w < PLAN_W; ++w) {
+                const uint32_t c = s_cnt[w * A.E + e];
+                s_cnt[w * A.E + e] = at;
+                at += c;
+            }
+        }
+    }
+    if (blockIdx.x == 0 && threadIdx.x == 0) offsets[A.E] = (int32_t)carry;
+    // the places that no slot takes
+    for (int64_t i = max(lo, (int64_t)carry) + threadIdx.x; i < hi; i += PLAN_NT) slots[i] = rows[i] = -1;
+    __syncthreads();
+    plan_place(A, lo, hi, s_cnt, slots, rows);
+}
+
+inline PlanArgs plan_args(int64_t S, int k, int E) {
+    PlanArgs A = {};
+    A.S = S;
+    A.k = k;
+    A.E = E;
+    while ((1 << A.bits) < E) ++A.bits;
+    int64_t chunk = (S + PLAN_BLOCKS - 1) / PLAN_BLOCKS;
+    if (chunk < PLAN_CHUNK) chunk = PLAN_CHUNK;
+    A.chunk = (chunk + PLAN_NT - 1) / PLAN_NT * PLAN_NT;
+    A.blocks = (int)((S + A.chunk - 1) / A.chunk);
+    if (A.blocks < 1) A.blocks = 1;
+    return A;
+}
+
+// f with (G, NV) as constants for E experts.
+template <typename F>
+void route_shape(int E, const F& f) {
+#define YABT_SHAPE(g, nv) \
+    if (E <= g * nv) return f(std::integral_constant<int, g>(), std::integral_constant<int, nv>());
+    YABT_SHAPE(16, 1)
+    YABT_SHAPE(16, 2)
+    YABT_SHAPE(16, 4)
+    YABT_SHAPE(16, 8)
+    YABT_SHAPE(16, 16)
+    YABT_SHAPE(64, 8)
+    YABT_SHAPE(64, 16)
+#undef YABT_SHAPE
+}
+
+template <typename T>
+void run_route(const RouteArgs& A, const T* logits, const float* bias, int32_t* ids, float* weights,
+               hipStream_t stream) {
+    route_shape(A.E, [&](auto g, auto nv) {
+        constexpr int G = decltype(g)::value, NV = decltype(nv)::value;
+        const int grid = launch_grid(A.n, ROUTE_NT / G, 4096);
+        if (A.groups > 1) k_route<T, G, NV, true><<<grid, ROUTE_NT, 0, stream>>>(A, logits, bias, ids, weights);
+        else k_route<T, G, NV, false><<<grid, ROUTE_NT, 0, stream>>>(A, logits, bias, ids, weights);
+    });
+}
+
+template <typename T>
+void run_route_grad(const RouteArgs& A, const float* dweights, int64_t lddw, const T* logits, const int32_t* ids,
+                    T* dlogits, int64_t lddl, hipStream_t stream) {
+    route_shape(A.E, [&](auto g, auto nv) {
+        constexpr int G = decltype(g)::value, NV = decltype(nv)::value;
+        k_route_grad<T, G, NV><<<launch_grid(A.n, ROUTE_NT / G, 4096), ROUTE_NT, 0, stream>>>(
+            A, dweights, lddw, logits, ids, dlogits, lddl);
+    });
+}
+
+}  // namespace yabt
+
+using namespace yabt;
+
+extern "C" {
+
+int yabt_route(int dtype, const void* logits, int64_t ldl, int64_t n, int E, int k, int scores, const float* bias,
+               int groups, int keep_groups, int renormalise, float scale, int32_t* out_ids, float* out_weights,
+               yabt_stream_t stream) {
+    if (!dtype_ok(dtype)) return fail(-1, "yabt_route: dtype is 0 (fp32), 1 (bf16) or 2 (fp16)");
+    if (n < 0 || E < 1 || E > ROUTE_MAX_E || ldl < E) return fail(-1, "yabt_route: bad sizes (1 <= E <= 1024)");
+    if (k < 1 || k > ROUTE_MAX_K || k > E) return fail(-1, "yabt_route: 1 <= k <= min(E, 32)");
+    if (scores != SOFTMAX && scores != SIGMOID) return fail(-1, "yabt_route: scores is 0 (softmax) or 1 (sigmoid)");
+    if (groups < 1 || groups > ROUTE_MAX_GROUPS || E % groups != 0 || keep_groups < 1 || keep_groups > groups)
+        return fail(-1, "yabt_route: groups (at most 64) divide E, 1 <= keep_groups <= groups");
+    if (n == 0) return 0;
+    if (!logits || !out_ids || !out_weights) return fail(-1, "yabt_route: null pointer");
+    RouteArgs A = {ldl, n, E, k, scores, renormalise, keep_groups < groups ? groups : 1, keep_groups, E / groups, 0, scale};
+    A.magic = ((1 << 20) + A.per_group - 1) / A.per_group;
+    hipStream_t st = (hipStream_t)stream;
+    if (dtype == DT_F32) run_route<float>(A, (const float*)logits, bias, out_ids, out_weights, st);
+    else if (dtype == DT_BF16) run_route<bf16>(A, (const bf16*)logits, bias, out_ids, out_weights, st);
+    else run_route<f16>(A, (const f16*)logits, bias, out_ids, out_weights, st);
+    return launch_status("yabt_route");
+}
+
+int yabt_route_grad(int dtype, const float* dweights, int64_t lddw, const void* logits, int64_t ldl,
+                    const int32_t* ids, int64_t n, int E, int k, int scores, int renormalise, float scale,
+                    void* out_dlogits, int64_t lddl, yabt_stream_t stream) {
+    if (!dtype_ok(dtype)) return fail(-1, "yabt_route_grad: dtype is 0 (fp32), 1 (bf16) or 2 (fp16)");
+    if (n < 0 || E < 1 || E > ROUTE_MAX_E || ldl < E || lddl < E)
+        return fail(-1, "yabt_route_grad: bad sizes (1 <= E <= 1024)");
+    if (k < 1 || k > ROUTE_MAX_K || k > E || lddw < k) return fail(-1, "yabt_route_grad: 1 <= k <= min(E, 32)");
+    if (scores != SOFTMAX && scores != SIGMOID)
+        return fail(-1, "yabt_route_grad: scores is 0 (softmax) or 1 (sigmoid)");
+    if (n == 0) return 0;
+    if (!dweights || !logits || !ids || !out_dlogits) return fail(-1, "yabt_route_grad: null pointer");
+    RouteArgs A = {ldl, n, E, k, scores, renormalise, 1, 1, E, 0, scale};
+    hipStream_t st = (hipStream_t)stream;
+    if (dtype == DT_F32)
+        run_route_grad<float>(A, dweights, lddw, (const float*)logits, ids, (float*)out_dlogits, lddl, st);
+    else if (dtype == DT_BF16)
+        run_route_grad<bf16>(A, dweights, lddw, (const bf16*)logits, ids, (bf16*)out_dlogits, lddl, st);
+    else
+        run_route_grad<f16>(A, dweights, lddw, (const f16*)logits, ids, (f16*)out_dlogits, lddl, st);
+    return launch_status("yabt_route_grad");
+}
+
+size_t yabt_expert_plan_workspace_bytes(int64_t n, int k, int E) {
+    if (n < 0 || k < 1 || E < 1 || E > ROUTE_MAX_E || n > INT32_MAX / k) return 0;
+    const PlanArgs A = plan_args(n * k, k, E);
+    return ((size_t)A.blocks + 1) * (size_t)E * sizeof(uint32_t);
+}
+
+int yabt_expert_plan(const int32_t* ids, int64_t n, int k, int E, void* workspace, size_t workspace_bytes,
+                     int32_t* out_offsets, int32_t* out_slots, int32_t* out_rows, yabt_stream_t stream) {
+    const size_t need = yabt_expert_plan_workspace_bytes(n, k, E);
+    if (need == 0) return fail(-1, "yabt_expert_plan: bad sizes (1 <= E <= 1024, n k < 2^31)");
+    if (!workspace || workspace_bytes < need) return fail(-2, "yabt_expert_plan: workspace too small");
+    if (!out_offsets || (n > 0 && (!ids || !out_slots || !out_rows)))
+        return fail(-1, "yabt_expert_plan: null pointer");
+    PlanArgs A = plan_args(n * k, k, E);
+    A.ids = ids;
+    hipStream_t st = (hipStream_t)stream;
+    const size_t lds = (size_t)PLAN_W * E * sizeof(uint32_t);
+    uint32_t* cnt = A.blocks > 1 ? (uint32_t*)workspace : nullptr;
+    uint32_t* tot = (uint32_t*)workspace + (size_t)A.blocks * E;
+    if (cnt) {
+        k_plan_count<<<A.blocks, PLAN_NT, lds, st>>>(A, cnt);
+        k_plan_scan<<<E, PLAN_NT, 0, st>>>(A, cnt, tot);
+    }
+    k_plan_place<<<A.blocks, PLAN_NT, lds, st>>>(A, cnt, tot, out_offsets, out_slots, out_rows);
+    return launch_status("yabt_expert_plan");
+}
+
+}  // extern "C"

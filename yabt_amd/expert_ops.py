@@ -1,0 +1,210 @@
+"""The expert layer's operations on torch tensors (csrc/norm.hip, route.hip).
+
+Rows are normalised, a gate's scores route each row to k of E experts, and the
+experts' weighted answers are added up: the learned, soft form of a tree with
+models in its leaves (yabt/neural_leaves.py:93-184), which sends a row to one
+leaf.
+
+* ``layer_norm`` / ``layer_norm_grad``: rows to zero mean and unit variance,
+  times a weight, plus a bias;
+* ``route`` / ``route_grad``: the k best experts of each row and their weights;
+* ``expert_plan``: the (row, expert) slots sorted by expert.
+
+Values are float32, bfloat16 or float16; statistics, weights, parameters of
+the norm and all sums are float32.  Every call runs on the current stream and
+neither waits nor reads anything back, so it can be captured into a HIP graph.
+"""
+
+from __future__ import annotations
+
+from dataclasses import dataclass
+
+import torch
+
+from . import _lib
+
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+SCORES = {"softmax": 0, "sigmoid": 1}
+MAX_EXPERTS, MAX_K, MAX_GROUPS = 1024, 32, 64
+
+
+def _stream(dev: torch.device) -> int:
+    return torch.cuda.current_stream(dev).cuda_stream
+
+
+def _matrix(t: torch.Tensor, what: str, dtype: torch.dtype | None = None) -> torch.Tensor:
+    """t as a device matrix with unit column stride."""
+    if t.dim() != 2:
+        raise ValueError(f"{what} must be a matrix, got shape {tuple(t.shape)}")
+    if t.device.type != "cuda":
+        raise RuntimeError(f"{what} must be on a HIP device: the expert layer has no CPU form")
+    if t.dtype not in DTYPES or (dtype is not None and t.dtype != dtype):
+        raise ValueError(f"{what} must be {dtype or 'float32, bfloat16 or float16'}, got {t.dtype}")
+    rows, cols = t.shape
+    if rows > 1 and t.stride(0) < cols or cols > 1 and t.stride(1) != 1:
+        t = t.contiguous()
+    return t
+
+
+def _ld(t: torch.Tensor) -> int:
+    return max(t.stride(0), t.shape[1]) if t.shape[0] > 1 else t.shape[1]
+
+
+def _vector(t: torch.Tensor | None, size: int, dev: torch.device, what: str) -> torch.Tensor | None:
+    """t as a contiguous float32 vector on dev."""
+    if t is None:
+        return None
+    if t.dim() != 1 or t.shape[0] != size:
+        raise ValueError(f"{what} must have shape ({size},), got {tuple(t.shape)}")
+    if t.device != dev:
+        raise ValueError(f"{what} must be on {dev}")
+    return t if t.dtype == torch.float32 and t.is_contiguous() else t.float().contiguous()
+
+
+def _at(t: torch.Tensor | None) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
+               eps: float = 1e-5) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(y, mean, rstd) of the rows of x (n, D): y = (x - mean) * rstd * weight
+    + bias in x's type, mean and rstd (n,) float32 for the backward pass."""
+    x = _matrix(x, "x")
+    (n, D), dev = x.shape, x.device
+    if D == 0:
+        raise ValueError("layer_norm needs at least one column")
+    w, b = _vector(weight, D, dev, "weight"), _vector(bias, D, dev, "bias")
+    y = torch.empty((n, D), dtype=x.dtype, device=dev)
+    stats = torch.empty((2, n), dtype=torch.float32, device=dev)
+    mean, rstd = stats[0], stats[1]
+    _lib.check(_lib.load().yabt_layer_norm(DTYPES[x.dtype], x.data_ptr(), _ld(x), n, D, _at(w), _at(b), float(eps),
+                                           y.data_ptr(), D, mean.data_ptr(), rstd.data_ptr(), _stream(dev)),
+               "yabt_layer_norm")
+    return y, mean, rstd
+
+
+def layer_norm_grad(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor,
+                    weight: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(dx, dweight, dbias) of ``layer_norm`` at x, from dy and the mean and
+    rstd it returned: dx in x's type, dweight and dbias (D,) float32."""
+    x = _matrix(x, "x")
+    dy = _matrix(dy, "dy", x.dtype)
+    (n, D), dev = x.shape, x.device
+    if dy.shape != x.shape or dy.device != dev:
+        raise ValueError(f"dy must be like x, {tuple(x.shape)} on {dev}")
+    w, mu, rs = _vector(weight, D, dev, "weight"), _vector(mean, n, dev, "mean"), _vector(rstd, n, dev, "rstd")
+    if mu is None or rs is None:
+        raise ValueError("layer_norm_grad needs the mean and rstd of the forward pass")
+    lib = _lib.load()
+    nbytes = int(lib.yabt_layer_norm_grad_workspace_bytes(n, D))
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    dx = torch.empty((n, D), dtype=x.dtype, device=dev)
+    grads = torch.empty((2, D), dtype=torch.float32, device=dev)
+    dw, db = grads[0], grads[1]
+    _lib.check(lib.yabt_layer_norm_grad(DTYPES[x.dtype], dy.data_ptr(), _ld(dy), x.data_ptr(), _ld(x), n, D, _at(w),
+                                        mu.data_ptr(), rs.data_ptr(), ws.data_ptr(), nbytes, dx.data_ptr(), D,
+                                        dw.data_ptr(), db.data_ptr(), _stream(dev)), "yabt_layer_norm_grad")
+    return dx, dw, db
+
+
+def _scores(scores: str) -> int:
+    if scores not in SCORES:
+        raise ValueError(f"scores must be one of {sorted(SCORES)}, got {scores!r}")
+    return SCORES[scores]
+
+
+def route(logits: torch.Tensor, k: int, *, scores: str = "softmax", bias: torch.Tensor | None = None,
+          groups: int = 1, keep_groups: int = 1, renormalise: bool = True,
+          scale: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
+    """(ids, weights), (n, k) int32 and float32: the k best of each row's E
+    experts, best first, equal keys by the lower index.
+
+    An expert's key is logit + bias ("softmax") or sigmoid(logit) + bias
+    ("sigmoid"), in float32; the bias (for balance) changes the choice alone.
+    A logit of -inf or NaN closes the expert to the row; a slot that no expert
+    is left for has id -1 and weight 0.  With groups > 1 only the best
+    ``keep_groups`` groups of E / groups consecutive experts stay, by their
+    largest key ("softmax") or the sum of their two largest ("sigmoid").
+    Weights are scale * score, with ``renormalise`` divided by the sum of the
+    row's chosen scores."""
+    logits = _matrix(logits, "logits")
+    (n, E), dev = logits.shape, logits.device
+    how = _scores(scores)
+    if not 1 <= E <= MAX_EXPERTS:
+        raise ValueError(f"route takes 1 to {MAX_EXPERTS} experts, got {E}")
+    if not 1 <= k <= min(E, MAX_K):
+        raise ValueError(f"k must be 1 to {min(E, MAX_K)}, got {k}")
+    if not 1 <= groups <= MAX_GROUPS or E % groups or not 1 <= keep_groups <= groups:
+        raise ValueError(f"groups must divide {E} and be at most {MAX_GROUPS}, keep_groups 1 to groups; "
+                         f"got {groups}, {keep_groups}")
+    b = _vector(bias, E, dev, "bias")
+    ids = torch.empty((n, k), dtype=torch.int32, device=dev)
+    weights = torch.empty((n, k), dtype=torch.float32, device=dev)
+    _lib.check(_lib.load().yabt_route(DTYPES[logits.dtype], logits.data_ptr(), _ld(logits), n, E, int(k), how, _at(b),
+                                      int(groups), int(keep_groups), int(bool(renormalise)), float(scale),
+                                      ids.data_ptr(), weights.data_ptr(), _stream(dev)), "yabt_route")
+    return ids, weights
+
+
+def route_grad(dweights: torch.Tensor, logits: torch.Tensor, ids: torch.Tensor, *, scores: str = "softmax",
+               renormalise: bool = True, scale: float = 1.0) -> torch.Tensor:
+    """Gradient of ``route``'s weights in the logits, (n, E) in their type, the
+    choice (ids) held fixed; a balancing bias has none."""
+    logits = _matrix(logits, "logits")
+    (n, E), dev = logits.shape, logits.device
+    how = _scores(scores)
+    ids = _ids(ids, dev)
+    k = ids.shape[1]
+    if ids.shape[0] != n or not 1 <= E <= MAX_EXPERTS or not 1 <= k <= min(E, MAX_K):
+        raise ValueError(f"ids must be route's, (n, k) for logits {tuple(logits.shape)}; got {tuple(ids.shape)}")
+    if tuple(dweights.shape) != (n, k) or dweights.device != dev:
+        raise ValueError(f"dweights must have shape {(n, k)} on {dev}")
+    dweights = _matrix(dweights if dweights.dtype == torch.float32 else dweights.float(), "dweights")
+    out = torch.empty((n, E), dtype=logits.dtype, device=dev)
+    _lib.check(_lib.load().yabt_route_grad(DTYPES[logits.dtype], dweights.data_ptr(), _ld(dweights),
+                                           logits.data_ptr(), _ld(logits), ids.data_ptr(), n, E, k, how,
+                                           int(bool(renormalise)), float(scale), out.data_ptr(), E, _stream(dev)),
+               "yabt_route_grad")
+    return out
+
+
+def _ids(ids: torch.Tensor, dev: torch.device | None = None) -> torch.Tensor:
+    if ids.dim() != 2 or ids.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"ids must be an (n, k) integer matrix, got {tuple(ids.shape)} {ids.dtype}")
+    if ids.device.type != "cuda" or dev is not None and ids.device != dev:
+        raise RuntimeError("ids must be on the other tensors' HIP device")
+    # a wider id names no expert: it must not come out as one
+    return (ids if ids.dtype == torch.int32 else ids.clamp(-1, 2 ** 31 - 1).to(torch.int32)).contiguous()
+
+
+@dataclass
+class ExpertPlan:
+    """Slots (row * k + j) sorted by expert.  Expert e's are ``slots[offsets[e]
+    : offsets[e + 1]]``, in row order, and ``rows`` their rows; the places
+    after the last hold -1, as many as there are ids that name no expert."""
+    ids: torch.Tensor       # (n, k) int32
+    offsets: torch.Tensor   # (E + 1,) int32
+    slots: torch.Tensor     # (n k,) int32
+    rows: torch.Tensor      # (n k,) int32
+
+    @property
+    def experts(self) -> int:
+        return self.offsets.shape[0] - 1
+
+
+def expert_plan(ids: torch.Tensor, experts: int) -> ExpertPlan:
+    """The plan of ids (n, k); ids outside [0, experts) belong to no expert."""
+    ids = _ids(ids)
+    (n, k), dev = ids.shape, ids.device
+    lib = _lib.load()
+    nbytes = int(lib.yabt_expert_plan_workspace_bytes(n, k, int(experts)))
+    if nbytes == 0:
+        raise ValueError(f"expert_plan takes 1 to {MAX_EXPERTS} experts, k >= 1 and n k < 2^31; got {experts} "
+                         f"experts, ids {(n, k)}")
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    offsets = torch.empty(experts + 1, dtype=torch.int32, device=dev)
+    places = torch.empty((2, n * k), dtype=torch.int32, device=dev)
+    slots, rows = places[0], places[1]
+    _lib.check(lib.yabt_expert_plan(ids.data_ptr(), n, k, int(experts), ws.data_ptr(), nbytes, offsets.data_ptr(),
+                                    slots.data_ptr(), rows.data_ptr(), _stream(dev)), "yabt_expert_plan")
+    return ExpertPlan(ids, offsets, slots, rows)
