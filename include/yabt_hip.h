@@ -554,6 +554,31 @@ int yabt_expert_plan(const int32_t *ids, int64_t n, int k, int E, void *workspac
                      size_t workspace_bytes, int32_t *out_offsets, int32_t *out_slots,
                      int32_t *out_rows, yabt_stream_t stream);
 
+/* The experts' products.  Slot s = (row t, j) with expert e = ids[s]:
+ *   [g u] = w_in[e] x_t, h = silu(g) * u, y_t = sum over the row's slots of weights[s] * w_out[e] h
+ * x (n, D), y (n, D), w_in (E, 2 F, D): F gate rows, then F rows of u, w_out
+ * (E, D, F), all of `dtype`; weights (n, k) fp32; ids (n, k) and the plan
+ * yabt_expert_plan made of them.  A row none of whose slots has an expert gets
+ * zeros.  out_inner ((n k) x 2 F, fp32, or NULL) keeps g and u of every place
+ * of the plan for the backward pass; places past the plan's last are not written.
+ * h is rounded to `dtype` before the second product; sums are fp32. */
+size_t yabt_experts_workspace_bytes(int dtype, int64_t n, int k, int D, int F, int E);
+int yabt_experts(int dtype, const void *x, int64_t ldx, int64_t n, int k, int D, int F, int E,
+                 const int32_t *ids, const int32_t *offsets, const int32_t *slots, const int32_t *rows,
+                 const float *weights, const void *w_in, const void *w_out, void *workspace,
+                 size_t workspace_bytes, float *out_inner, void *y, int64_t ldy, yabt_stream_t stream);
+
+/* Their gradients from dy (n, D) and the forward pass's inner: dx (n, D),
+ * dw_in, dw_out like w_in and w_out, all of `dtype`, and dweights (n, k) fp32
+ * (0 for slots without an expert).  An expert without slots gets zeros. */
+size_t yabt_experts_grad_workspace_bytes(int dtype, int64_t n, int k, int D, int F, int E);
+int yabt_experts_grad(int dtype, const void *dy, int64_t lddy, const void *x, int64_t ldx, int64_t n,
+                      int k, int D, int F, int E, const int32_t *ids, const int32_t *offsets,
+                      const int32_t *slots, const int32_t *rows, const float *weights, const void *w_in,
+                      const void *w_out, const float *inner, void *workspace, size_t workspace_bytes,
+                      void *dx, int64_t lddx, float *dweights, void *dw_in, void *dw_out,
+                      yabt_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

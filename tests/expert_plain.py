@@ -92,3 +92,66 @@ def plan(ids, experts):
     offsets = np.concatenate([[0], np.cumsum([(flat == e).sum() for e in range(experts)])])
     rest = [-1] * (flat.size - len(slots))
     return offsets, np.array(slots + rest, np.int64), np.array([s // ids.shape[1] for s in slots] + rest, np.int64)
+
+
+
+def products(x, ids, w, w_in, w_out, dtype, dy=None, mask=None):
+    """{name: (value, bound)} of the experts' products and, with dy, of their
+    gradients, float64; the bounds carry every rounding of the way: sums of K
+    terms in float32 in any order (K + 8 units of the magnitudes' sum), h, w h,
+    dg and du to the inputs' type, the exponential and reciprocal (8 + 2 |g|
+    units), one rounding of the result."""
+    (n, D), k, E, F = x.shape, ids.shape[1], w_in.shape[0], w_out.shape[2]
+    u, tiny = UNIT[dtype], TINY[dtype]
+    gam = lambda terms: (terms + 8) * U32  # noqa: E731
+    out = {name: np.zeros(shape) for name, shape in (("y", (n, D)), ("dx", (n, D)), ("dweights", (n, k)),
+                                                     ("dw_in", w_in.shape), ("dw_out", w_out.shape))}
+    err, size = {m: np.zeros(v.shape) for m, v in out.items()}, {m: np.zeros(v.shape) for m, v in out.items()}
+    for e in range(E):
+        t, j = np.nonzero(ids == e)
+        if not len(t):
+            continue
+        xe, we, A, B = x[t], w[t, j][:, None], w_in[e], w_out[e]
+        pre, epre = xe @ A.T, gam(D) * (np.abs(xe) @ np.abs(A).T)
+        g, v, eg, ev = pre[:, :F], pre[:, F:], epre[:, :F], epre[:, F:]
+        sig = 1.0 / (1.0 + np.exp(-g))
+        silu, unit = g * sig, (8 + 2 * np.abs(g)) * U32
+        esilu = 1.1 * eg + unit * np.abs(silu)
+        h = silu * v
+        eh = esilu * np.abs(v) + np.abs(silu) * ev + 2 * U32 * np.abs(h)
+        eh16 = eh + u * (np.abs(h) + eh) + tiny
+        z = h @ B.T
+        ez = eh16 @ np.abs(B).T + gam(F) * (np.abs(h) @ np.abs(B).T)
+        np.add.at(out["y"], t, we * z)
+        np.add.at(err["y"], t, we * ez)
+        np.add.at(size["y"], t, np.abs(we * z))
+        if dy is None:
+            continue
+        de = dy[t]
+        a, ea = de @ B, gam(D) * (np.abs(de) @ np.abs(B))
+        out["dweights"][t, j] = (a * h).sum(axis=1)
+        err["dweights"][t, j] = (np.abs(a) * eh + np.abs(h) * ea).sum(axis=1) + gam(F) * np.abs(a * h).sum(axis=1)
+        slope = sig * (1.0 + g * (1.0 - sig))
+        du, dg = we * a * silu, we * a * v * slope
+        edu = np.abs(we) * (np.abs(silu) * ea + np.abs(a) * esilu)
+        edg = np.abs(we) * (np.abs(v * slope) * ea + np.abs(a * slope) * ev
+                            + np.abs(a * v) * (0.5 * eg + 1.5 * unit))
+        dpre, edpre = np.concatenate([dg, du], 1), np.concatenate([edg, edu], 1)
+        edpre = edpre + 4 * U32 * np.abs(dpre)
+        edpre = edpre + u * (np.abs(dpre) + edpre) + tiny
+        np.add.at(out["dx"], t, dpre @ A)
+        np.add.at(err["dx"], t, edpre @ np.abs(A) + gam(2 * F) * (np.abs(dpre) @ np.abs(A)))
+        np.add.at(size["dx"], t, np.abs(dpre @ A))
+        out["dw_in"][e] = dpre.T @ xe
+        err["dw_in"][e] = edpre.T @ np.abs(xe) + gam(len(t)) * (np.abs(dpre).T @ np.abs(xe))
+        hw = we * h
+        ehw = np.abs(we) * eh + U32 * np.abs(hw)
+        ehw = ehw + u * (np.abs(hw) + ehw) + tiny
+        out["dw_out"][e] = de.T @ hw
+        err["dw_out"][e] = np.abs(de).T @ ehw + gam(len(t)) * (np.abs(de).T @ np.abs(hw))
+    for m in ("y", "dx"):
+        err[m] = err[m] + (k + 2) * U32 * size[m]
+    names = ("y",) if dy is None else tuple(out)
+    last = {m: U32 if m == "dweights" else u for m in names}
+    return {m: (out[m], err[m] + last[m] * (np.abs(out[m]) + err[m]) + (0.0 if m == "dweights" else tiny) + 1e-38)
+            for m in names}

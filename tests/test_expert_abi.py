@@ -66,3 +66,53 @@ def test_plain_norm_gradient_against_differences():
             down = (norm(x, w, b, 1e-5)[0] * c).sum()
             flat[i] = keep
             assert abs((up - down) / (2 * h) - grad.reshape(-1)[i]) < 1e-7 * max(1.0, np.abs(grad).max()) + 1e-7
+
+
+def test_experts_refusals():
+    lib = _lib.load()
+    big = 1 << 40
+
+    def call(dt=0, ldx=8, n=4, k=2, D=8, F=4, E=3, p=4096, ws=big, ldy=8):
+        return lib.yabt_experts(dt, p, ldx, n, k, D, F, E, p, p, p, p, p, p, p, p, ws, 0, p, ldy, None)
+
+    def grad(dt=0, ldx=8, n=4, k=2, D=8, F=4, E=3, p=4096, ws=big, lddy=8, lddx=8):
+        return lib.yabt_experts_grad(dt, p, lddy, p, ldx, n, k, D, F, E, p, p, p, p, p, p, p, p, p, ws, p, lddx, p, p, p,
+                                     None)
+
+    for f in (call, grad):
+        for args, text in [(dict(dt=3), "dtype"), (dict(ldx=7), "bad sizes"), (dict(k=0), "bad sizes"),
+                           (dict(D=0), "bad sizes"), (dict(F=0), "bad sizes"), (dict(E=0), "bad sizes"),
+                           (dict(E=1025), "bad sizes"), (dict(n=-1), "bad sizes"), (dict(n=1 << 30), "bad sizes"),
+                           (dict(p=0), "null pointer"), (dict(ws=16), "workspace")]:
+            refused(f(**args), text)
+    assert call(n=0, p=0) == 0
+    for sizes in (lib.yabt_experts_workspace_bytes, lib.yabt_experts_grad_workspace_bytes):
+        assert sizes(0, 4, 2, 8, 0, 3) == 0 and sizes(9, 4, 2, 8, 4, 3) == 0
+        # h (or dg, du, w h) of every slot and the slots' fp32 answers
+        assert sizes(1, 1000, 4, 64, 32, 8) >= 4000 * (32 * 2 + 64 * 4)
+        assert sizes(1, 1000, 1, 64, 32, 8) >= 1000 * 32 * 2
+
+
+def test_plain_products_gradient_against_differences():
+    from expert_plain import products
+    rng = np.random.default_rng(3)
+    n, D, F, E, k = 6, 4, 3, 2, 2
+    ids = np.array([[0, 1], [1, -1], [0, 1], [-1, -1], [1, 0], [0, -1]])
+    a = dict(x=rng.normal(size=(n, D)), w=rng.random((n, k)), w_in=rng.normal(size=(E, 2 * F, D)),
+             w_out=rng.normal(size=(E, D, F)))
+    dy = rng.normal(size=(n, D))
+
+    def loss():
+        return (products(a["x"], ids, a["w"], a["w_in"], a["w_out"], "float32")["y"][0] * dy).sum()
+
+    got = products(a["x"], ids, a["w"], a["w_in"], a["w_out"], "float32", dy)
+    for m, grad in (("x", "dx"), ("w", "dweights"), ("w_in", "dw_in"), ("w_out", "dw_out")):
+        flat, ref = a[m].reshape(-1), got[grad][0].reshape(-1)
+        for i in range(flat.size):
+            keep, h = flat[i], 1e-6
+            flat[i] = keep + h
+            up = loss()
+            flat[i] = keep - h
+            down = loss()
+            flat[i] = keep
+            assert abs((up - down) / (2 * h) - ref[i]) < 1e-6

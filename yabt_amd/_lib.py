@@ -105,6 +105,12 @@ SIGNATURES = {
                                _vp]),
     "yabt_expert_plan_workspace_bytes": (_sz, [_i64, _int, _int]),
     "yabt_expert_plan": (_int, [_vp, _i64, _int, _int, _vp, _sz, _vp, _vp, _vp, _vp]),
+    "yabt_experts_workspace_bytes": (_sz, [_int, _i64, _int, _int, _int, _int]),
+    "yabt_experts": (_int, [_int, _vp, _i64, _i64, _int, _int, _int, _int, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+                            _sz, _vp, _vp, _i64, _vp]),
+    "yabt_experts_grad_workspace_bytes": (_sz, [_int, _i64, _int, _int, _int, _int]),
+    "yabt_experts_grad": (_int, [_int, _vp, _i64, _vp, _i64, _i64, _int, _int, _int, _int, _vp, _vp, _vp, _vp, _vp,
+                                 _vp, _vp, _vp, _vp, _sz, _vp, _i64, _vp, _vp, _vp, _vp]),
 }
 
 

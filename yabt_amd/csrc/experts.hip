@@ -1,0 +1,866 @@
+// The experts' products, forward and backward, on the matrix cores.
+//
+//   slot s = (row t, j), expert e:  [g u] = W_in[e] x_t,  h = silu(g) u,  z_s = W_out[e] h,  y_t = sum_j w_s z_s
+//   a = W_out[e]^T dy_t,  dw_s = a . h,  dh = w_s a,  du = dh silu(g),  dg = dh u silu'(g)
+//   dx_t = sum_j W_in[e]^T [dg du],  dW_in[e] = sum_s [dg du] x_t^T,  dW_out[e] = sum_s dy_t (w_s h)^T
+//
+// The slots come sorted by expert (yabt_expert_plan), so that every product is
+// one matrix product per expert over its slots; a launch does all experts'.
+// One kernel makes the tiles of all six products.  They differ in where a
+// tile's rows come from (gathered rows of x or dy, or the slots' own rows), in
+// whether an operand lies along the summed dimension in memory or across it,
+// and in what is done with the sums:
+//
+//   IN     [g u] of the slots, the tile's columns gate and up alternately by 32, then h = silu(g) u
+//   OUT    z = w (W_out h), by slot in fp32 (added up by k_combine), or y itself when k = 1
+//   DH     a, then dg, du, w h and dw in part
+//   DX     W_in^T [dg du] by slot in fp32, or dx itself when k = 1
+//   DWIN, DWOUT   the weights' gradients, summed over an expert's slots
+//
+// Both operands pass through LDS in 128-byte steps of the summed dimension,
+// two stages: the next one is on its way from memory straight into LDS while
+// the present one is multiplied.  16-byte pieces are stored at places that an
+// xor with the row spreads over the banks; the xor is applied to the global
+// address, as LDS is filled in lane order.  Operands across the summed
+// dimension are read with the transposing LDS loads.  Inputs whose rows are
+// not 16-byte aligned pass through registers instead.
+//
+// h, w h, dg and du are rounded to the inputs' type, as the matrix cores take
+// them; g and u are kept in fp32 for the backward pass, and z and the parts of
+// dx are added in fp32: so each output has two roundings behind it, its own
+// and that of one factor.
+
+#include "expert.h"
+#include "yabt_hip.h"
+
+namespace yabt {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef f16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) char lds_char;
+typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+typedef __attribute__((address_space(3))) float lds_float;
+
+enum Mode { IN, OUT, DH, DX, DWIN, DWOUT };
+
+constexpr int STEP = 128;             // bytes of the summed dimension a stage holds
+constexpr int XCDS = 8;               // blocks go to the 8 dies in turn
+constexpr int TILE_GROUP = 4;         // row tiles that walk the column tiles together
+
+struct ExpertArgs {
+    const void* x;
+    const void* dy;
+    const void* w_in;                 // (E, 2 F, D)
+    const void* w_out;                // (E, D, F)
+    const float* weights;             // (n, k)
+    const int32_t* ids;               // (n, k)
+    const int32_t* offsets;           // (E + 1), the plan
+    const int32_t* slots;
+    const int32_t* rows;
+    int64_t ldx, lddy, n;
+    int k, D, F, E;
+    int Fp;                           // F up to whole 16 bytes: the pitch of h and w h, half that of [dg du]
+    int Dp;                           // D up to whole 16 bytes: the pitch of z
+    void* h;                          // (S, Fp)
+    void* hw;                         // (S, Fp): w h
+    void* dpre;                       // (S, 2 Fp): dg from 0, du from Fp
+    float* pre;                       // (S, 2 F): g from 0, u from F, or NULL
+    float* z;                         // (S, Dp)
+    float* dwp;                       // (parts, S): dw by column tile
+    void* out;                        // y or dx (k = 1), dW_in or dW_out
+    int64_t ldo;
+    float* part;                      // (splits, E, M, N): the weights' gradients in part
+    int splits;
+};
+
+// 16 zero bytes for pieces past the end of the summed dimension.
+__device__ const u32x4 g_zeros = {0, 0, 0, 0};
+
+template <int BM_, int BN_, int WM_, int WN_>
+struct TileOf {
+    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_;
+    static constexpr int NT = 64 * WM * WN;
+    static constexpr int MI = BM / WM / 32, NI = BN / WN / 32;    // 32 x 32 blocks a wave makes
+    static constexpr int ABYTES = BM * STEP, BBYTES = BN * STEP, STAGE = ABYTES + BBYTES;
+    static constexpr int NA = ABYTES / 16 / NT, NB = BBYTES / 16 / NT;
+    static_assert(NA >= 1 && NB >= 1 && NI % 2 == 0, "whole pieces a thread, gate and up in one wave");
+};
+
+// silu by the hardware's exp2 and reciprocal (about one unit each).
+__device__ __forceinline__ float sigmoid_fast(float g) {
+    return __builtin_amdgcn_rcpf(1.0f + __expf(-g));
+}
+
+// 64 lanes' 16 bytes each from memory to LDS at base (the same for the wave), in lane order.
+__device__ __forceinline__ void lds_fill(const void* g, uint32_t base) {
+    typedef const __attribute__((address_space(1))) void global_void;
+    typedef __attribute__((address_space(3))) void lds_void;
+    __builtin_amdgcn_global_load_lds((global_void*)g, (lds_void*)(uintptr_t)base, 16, 0, 0);
+}
+
+__device__ __forceinline__ void stage_ready() {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+}
+
+// Row tile `id` of the slots in tiles of BM per expert; total: their number.
+struct TileAt {
+    int e, mi;
+};
+__device__ __forceinline__ int tiles_total(const int32_t* off, int E, int BM) {
+    const int lane = threadIdx.x & 63;
+    int t = 0;
+    for (int e = lane; e < E; e += 64) t += (off[e + 1] - off[e] + BM - 1) / BM;
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) t += __shfl_xor(t, m);
+    return t;
+}
+__device__ __forceinline__ TileAt tile_find(const int32_t* off, int E, int BM, int id) {
+    const int lane = threadIdx.x & 63;
+    int carry = 0;
+    for (int e0 = 0; e0 < E; e0 += 64) {
+        const int e = e0 + lane;
+        const int c = e < E ? (off[e + 1] - off[e] + BM - 1) / BM : 0;
+        int t = c;
+#pragma unroll
+        for (int m = 1; m < 64; m <<= 1) {
+            const int o = __shfl_up(t, m);
+            if (lane >= m) t += o;
+        }
+        const uint64_t hit = __ballot(id < carry + t);
+        if (hit) {
+            const int l = __ffsll((unsigned long long)hit) - 1;
+            return {e0 + l, id - carry - __shfl(t - c, l)};
+        }
+        carry += __shfl(t, 63);
+    }
+    return {-1, 0};
+}
+
+// The block's place in a grid that is walked die by die: consecutive tiles on
+// one die, whose L2 then holds the rows and weights they share.
+__device__ __forceinline__ int64_t die_order(int64_t b, int64_t total) {
+    const int64_t per = (total + XCDS - 1) / XCDS;
+    const int64_t in = b / XCDS;
+    return in < per ? (b % XCDS) * per + in : total;
+}
+
+template <typename T>
+__device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
+    if constexpr (sizeof(T) == 4) {
+        const f32x4 fa = __builtin_bit_cast(f32x4, a), fb = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) c = __builtin_amdgcn_mfma_f32_32x32x2f32(fa[q], fb[q], c, 0, 0, 0);
+        return c;
+    } else if constexpr (std::is_same_v<T, bf16>) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c,
+                                                      0, 0, 0);
+    } else {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0,
+                                                     0, 0);
+    }
+}
+
+// A lane's 16 bytes of block i of an operand at k-step ks (32 bytes of the
+// summed dimension): row (or column) lane % 32, half lane / 32.
+//   along: tile[row][128 bytes], piece c of a row stored at c ^ (row & 7)
+//   across: tile[k][W values], piece c of a row stored at c ^ 2 (k & 3)
+template <typename T, bool ACROSS, int W>
+struct Frag {
+    uint32_t at[ACROSS ? (sizeof(T) == 4 ? 4 : 2) : 4];
+    __device__ __forceinline__ Frag(int first) {
+        const int l = threadIdx.x & 63;
+        if constexpr (!ACROSS) {
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks)
+                at[ks] = (uint32_t)((first + (l & 31)) * STEP + (((ks * 2 + (l >> 5)) ^ (l & 7)) << 4));
+        } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                at[q] = (uint32_t)(((l >> 5) * 4 + q) * W * 4 + first * 4 + (((l & 31) * 4) ^ (q << 5)));
+        } else {
+            const int r = (l & 15) >> 2;                     // of four rows of k, this lane fetches row r
+            const int col = ((l >> 4) & 1) * 16 + (l & 3) * 4;
+            const uint32_t row = (uint32_t)(((l >> 5) * 8 + r) * W * 2 + first * 2);
+#pragma unroll
+            for (int odd = 0; odd < 2; ++odd) at[odd] = row + (uint32_t)((odd * 64 + col * 2) ^ (r << 5));
+        }
+    }
+    __device__ __forceinline__ u32x4 get(lds_char* tile, int i, int ks) const {
+        if constexpr (!ACROSS) {
+            return *(const lds_u32x4*)(tile + at[ks] + i * 32 * STEP);
+        } else if constexpr (sizeof(T) == 4) {
+            f32x4 v;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) v[q] = *(const lds_float*)(tile + at[q] + ks * 8 * W * 4 + i * 128);
+            return __builtin_bit_cast(u32x4, v);
+        } else {
+            lds_char* p = tile + at[i & 1] + (i >> 1) * 128 + ks * 16 * W * 2;
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
+            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 4 * W * 2));
+            return __builtin_bit_cast(u32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        }
+    }
+};
+
+// The pieces of an operand that a thread brings to LDS.  The mode says where a
+// row lies; pieces past the end of the summed dimension are zero, rows and
+// columns past the tile's end repeat the last (their sums are not stored).
+template <typename T, int MODE, bool SIDE_B, int W, int COUNT, int NT>
+struct Loader {
+    static constexpr bool ACROSS = SIDE_B ? MODE >= DH : MODE >= DWIN;
+    static constexpr bool GATHER = SIDE_B ? MODE == DWIN : MODE == IN || MODE == DH || MODE == DWOUT;
+    static constexpr int CH = VEC<T>;
+    static constexpr int PER_ROW = ACROSS ? W * (int)sizeof(T) / 16 : 8;
+    const T* ptr[COUNT];       // along: the row, at this piece; across: column of the piece, from row 0
+    int32_t src[COUNT];        // across and gathered: the next step's rows
+
+    __device__ __forceinline__ static int row_of(int i) { return (i * NT + (int)threadIdx.x) / PER_ROW; }
+    __device__ __forceinline__ static int piece_of(int i) {
+        const int c = (i * NT + (int)threadIdx.x) % PER_ROW, r = row_of(i);
+        return ACROSS ? c ^ ((r & 3) << 1) : c ^ (r & 7);
+    }
+
+    // p0: the tile's first slot place (along), or the split's (across); count:
+    // how many there are; first: the tile's first row or column of the operand
+    __device__ __forceinline__ void init(const ExpertArgs& P, int e, int p0, int count, int first) {
+#pragma unroll
+        for (int i = 0; i < COUNT; ++i) {
+            const int r = row_of(i), piece = piece_of(i) * CH;
+            if constexpr (!ACROSS && !SIDE_B) {
+                const int p = p0 + min(r, count - 1);
+                if constexpr (MODE == IN) ptr[i] = (const T*)P.x + (size_t)P.rows[p] * (size_t)P.ldx;
+                else if constexpr (MODE == DH) ptr[i] = (const T*)P.dy + (size_t)P.rows[p] * (size_t)P.lddy;
+                else if constexpr (MODE == OUT) ptr[i] = (const T*)P.h + (size_t)p * (size_t)P.Fp;
+                else ptr[i] = (const T*)P.dpre + (size_t)p * 2 * (size_t)P.Fp;
+                ptr[i] += piece;
+            } else if constexpr (!ACROSS) {
+                if constexpr (MODE == IN) {
+                    // gate and up rows alternately by 32
+                    const int f = min(first + (r >> 6) * 32 + (r & 31), P.F - 1);
+                    ptr[i] = (const T*)P.w_in + ((size_t)e * 2 * P.F + (r >> 5 & 1 ? P.F : 0) + f) * (size_t)P.D;
+                } else {
+                    ptr[i] = (const T*)P.w_out + ((size_t)e * P.D + min(first + r, P.D - 1)) * (size_t)P.F;
+                }
+                ptr[i] += piece;
+            } else {
+                const T* base;
+                int width;
+                if constexpr (SIDE_B) {
+                    if constexpr (MODE == DH) base = (const T*)P.w_out + (size_t)e * P.D * (size_t)P.F, width = P.F;
+                    else if constexpr (MODE == DX) base = (const T*)P.w_in + (size_t)e * 2 * P.F * (size_t)P.D, width = P.D;
+                    else if constexpr (MODE == DWIN) base = (const T*)P.x, width = P.D;
+                    else base = (const T*)P.hw + (size_t)p0 * (size_t)P.Fp, width = P.Fp;
+                } else {
+                    if constexpr (MODE == DWIN) base = (const T*)P.dpre + (size_t)p0 * 2 * (size_t)P.Fp, width = 2 * P.Fp;
+                    else base = (const T*)P.dy, width = P.D;
+                }
+                ptr[i] = base + min(first + piece, max(width - CH, 0));
+            }
+        }
+    }
+
+    // the summed dimension's length as this operand has it
+    __device__ __forceinline__ static int length(const ExpertArgs& P, int count) {
+        if constexpr (MODE == IN || MODE == DH) return P.D;
+        if constexpr (MODE == OUT) return SIDE_B ? P.F : P.Fp;
+        if constexpr (MODE == DX) return P.Fp + P.F;
+        return count;
+    }
+    __device__ __forceinline__ static int width(const ExpertArgs& P) {
+        if constexpr (SIDE_B) return MODE == DH ? P.F : MODE == DWOUT ? P.Fp : P.D;
+        return MODE == DWIN ? 2 * P.Fp : P.D;
+    }
+
+    // rows of x or dy of the step from k0 on
+    __device__ __forceinline__ void look_up(const ExpertArgs& P, int p0, int count, int k0) {
+        if constexpr (ACROSS && GATHER) {
+#pragma unroll
+            for (int i = 0; i < COUNT; ++i) {
+                const int kk = k0 + row_of(i);
+                src[i] = kk < count ? P.rows[p0 + kk] : -1;
+            }
+        }
+    }
+
+    // where piece i of the step from k0 on lies, or null past the end
+    __device__ __forceinline__ const T* at(const ExpertArgs& P, int i, int k0, int len) const {
+        if constexpr (!ACROSS) {
+            return k0 + piece_of(i) * CH < len ? ptr[i] + k0 : nullptr;
+        } else if constexpr (GATHER) {
+            const size_t ld = (size_t)(SIDE_B ? P.ldx : P.lddy);
+            return src[i] >= 0 ? ptr[i] + (size_t)src[i] * ld : nullptr;
+        } else {
+            int kk = k0 + row_of(i);
+            if (kk >= len) return nullptr;
+            size_t ld;
+            if constexpr (MODE == DH) ld = (size_t)P.F;
+            else if constexpr (MODE == DX) {
+                ld = (size_t)P.D;
+                if (kk >= P.F) {
+                    if (kk < P.Fp) return nullptr;
+                    kk += P.F - P.Fp;
+                }
+            } else {
+                ld = (size_t)(SIDE_B ? P.Fp : 2 * P.Fp);
+            }
+            return ptr[i] + (size_t)kk * ld;
+        }
+    }
+
+    __device__ __forceinline__ void fill(const ExpertArgs& P, int k0, int len, uint32_t lds) const {
+#pragma unroll
+        for (int i = 0; i < COUNT; ++i) {
+            const T* p = at(P, i, k0, len);
+            const uint32_t base = lds + (uint32_t)(i * NT * 16) + ((threadIdx.x & ~63u) << 4);
+            lds_fill(p ? (const void*)p : (const void*)&g_zeros, __builtin_amdgcn_readfirstlane(base));
+        }
+    }
+
+    // the same through registers, for rows at any address: the values that
+    // exist, zeros for the others
+    __device__ __forceinline__ void fetch(const ExpertArgs& P, int k0, int len, int first, u32x4* v) const {
+        typedef T VT __attribute__((ext_vector_type(CH)));
+#pragma unroll
+        for (int i = 0; i < COUNT; ++i) {
+            const T* p = at(P, i, k0, len);
+            u32x4 o = {0, 0, 0, 0};
+            if (p) {
+                const int piece = piece_of(i) * CH;
+                int have;
+                if constexpr (ACROSS) {
+                    // the column clamp of init() does not hold pieces that end past the row
+                    const int w = width(P);
+                    p += first + piece - min(first + piece, max(w - CH, 0));
+                    have = w - (first + piece);
+                } else {
+                    have = len - (k0 + piece);
+                }
+                if (have >= CH) o = *reinterpret_cast<const u32x4_any*>(p);
+                else {
+                    VT t = {};
+#pragma unroll
+                    for (int j = 0; j < CH; ++j)
+                        if (j < have) t[j] = p[j];
+                    o = __builtin_bit_cast(u32x4, t);
+                }
+            }
+            v[i] = o;
+        }
+    }
+    __device__ __forceinline__ static void put(lds_char* tile, const u32x4* v) {
+#pragma unroll
+        for (int i = 0; i < COUNT; ++i) *(lds_u32x4*)(tile + (i * NT + (int)threadIdx.x) * 16) = v[i];
+    }
+};
+
+template <typename T, int MODE, typename TL, bool DMA>
+__global__ void __launch_bounds__(TL::NT) k_experts(ExpertArgs P, int ntiles, int mtiles) {
+    constexpr bool ROWS = MODE < DWIN;
+    extern __shared__ __attribute__((aligned(128))) char s_tiles[];
+    __shared__ int s_slot[ROWS ? TL::BM : 1];
+    __shared__ float s_w[ROWS ? TL::BM : 1];
+    lds_char* const lds = (lds_char*)s_tiles;
+    const uint32_t lds_at = (uint32_t)(uintptr_t)lds;
+    const int wave = threadIdx.x / 64, lane = threadIdx.x & 63;
+    const int wm = wave / TL::WN, wn = wave % TL::WN;
+
+    // which tile: expert e, slots [p0, p0 + count), first row mf and column nf
+    int e, p0, count, mf = 0, nf, split = 0;
+    if constexpr (ROWS) {
+        const int total = tiles_total(P.offsets, P.E, TL::BM);
+        const int64_t all = (int64_t)total * ntiles, id = die_order(blockIdx.x, all);
+        if (id >= all) return;
+        const int group = (int)(id / ((int64_t)TILE_GROUP * ntiles));
+        const int in = (int)(id - (int64_t)group * TILE_GROUP * ntiles);
+        const int gm = min(TILE_GROUP, total - group * TILE_GROUP);
+        const TileAt t = tile_find(P.offsets, P.E, TL::BM, group * TILE_GROUP + in % gm);
+        e = t.e;
+        p0 = P.offsets[e] + t.mi * TL::BM;
+        count = min(TL::BM, P.offsets[e + 1] - p0);
+        nf = in / gm * (MODE == IN ? TL::BN / 2 : TL::BN);
+        for (int i = threadIdx.x; i < TL::BM; i += TL::NT) {
+            const int slot = i < count ? P.slots[p0 + i] : 0;
+            s_slot[i] = slot;
+            s_w[i] = MODE == OUT || MODE == DH ? P.weights[slot] : 1.0f;
+        }
+    } else {
+        const int64_t all = (int64_t)P.E * mtiles * ntiles * P.splits, id = die_order(blockIdx.x, all);
+        if (id >= all) return;
+        const int per = mtiles * ntiles;
+        const int es = (int)(id / per), in = (int)(id - (int64_t)es * per);
+        e = es / P.splits;
+        split = es % P.splits;
+        // column tiles together with a group of row tiles
+        const int group = in / (TILE_GROUP * ntiles), gin = in - group * TILE_GROUP * ntiles;
+        const int gm = min(TILE_GROUP, mtiles - group * TILE_GROUP);
+        mf = (group * TILE_GROUP + gin % gm) * TL::BM;
+        nf = gin / gm * TL::BN;
+        const int off = P.offsets[e], cnt = P.offsets[e + 1] - off;
+        const int step = STEP / (int)sizeof(T);
+        const int part = ((cnt + P.splits - 1) / P.splits + step - 1) / step * step;
+        const int lo = min(cnt, split * part);
+        p0 = off + lo;
+        count = min(part, cnt - lo);
+    }
+
+    Loader<T, MODE, false, TL::BM, TL::NA, TL::NT> la;
+    Loader<T, MODE, true, TL::BN, TL::NB, TL::NT> lb;
+    using LA = decltype(la);
+    using LB = decltype(lb);
+    const int ka = LA::length(P, count), kb = LB::length(P, count), K = max(ka, kb);
+    constexpr int BK = STEP / (int)sizeof(T);
+    const int steps = (K + BK - 1) / BK;
+    f32x16 acc[TL::MI][TL::NI];
+#pragma unroll
+    for (int i = 0; i < TL::MI; ++i)
+#pragma unroll
+        for (int j = 0; j < TL::NI; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
+
+    if (steps > 0) {
+        la.init(P, e, p0, count, mf);
+        lb.init(P, e, p0, count, nf);
+        la.look_up(P, p0, count, 0);
+        lb.look_up(P, p0, count, 0);
+        u32x4 ra[DMA ? 1 : TL::NA], rb[DMA ? 1 : TL::NB];
+        if constexpr (DMA) {
+            la.fill(P, 0, ka, lds_at);
+            lb.fill(P, 0, kb, lds_at + TL::ABYTES);
+        } else {
+            la.fetch(P, 0, ka, mf, ra);
+            lb.fetch(P, 0, kb, nf, rb);
+            LA::put(lds, ra);
+            LB::put(lds + TL::ABYTES, rb);
+        }
+        la.look_up(P, p0, count, BK);
+        lb.look_up(P, p0, count, BK);
+        const Frag<T, LA::ACROSS, TL::BM> fa(wm * TL::MI * 32);
+        const Frag<T, LB::ACROSS, TL::BN> fb(wn * TL::NI * 32);
+        for (int t = 0; t < steps; ++t) {
+            stage_ready();
+            const uint32_t next = (uint32_t)((t + 1) & 1) * TL::STAGE;
+            lds_char* const cur = lds + (t & 1) * TL::STAGE;
+            if (t + 1 < steps) {
+                const int k0 = (t + 1) * BK;
+                if constexpr (DMA) {
+                    la.fill(P, k0, ka, lds_at + next);
+                    lb.fill(P, k0, kb, lds_at + next + TL::ABYTES);
+                } else {
+                    la.fetch(P, k0, ka, mf, ra);
+                    lb.fetch(P, k0, kb, nf, rb);
+                }
+                la.look_up(P, p0, count, k0 + BK);
+                lb.look_up(P, p0, count, k0 + BK);
+            }
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) {
+                u32x4 a[TL::MI], b[TL::NI];
+#pragma unroll
+                for (int i = 0; i < TL::MI; ++i) a[i] = fa.get(cur, i, ks);
+#pragma unroll
+                for (int j = 0; j < TL::NI; ++j) b[j] = fb.get(cur + TL::ABYTES, j, ks);
+#pragma unroll
+                for (int i = 0; i < TL::MI; ++i)
+#pragma unroll
+                    for (int j = 0; j < TL::NI; ++j) acc[i][j] = mma<T>(a[i], b[j], acc[i][j]);
+            }
+            if constexpr (!DMA) {
+                if (t + 1 < steps) {
+                    LA::put(lds + next, ra);
+                    LB::put(lds + next + TL::ABYTES, rb);
+                }
+            }
+        }
+    }
+
+    // sum r of block (i, j): row m0 + i * 32 + 8 (r / 4) + r % 4, column n0 + j * 32
+    const int m0 = wm * TL::MI * 32 + 4 * (lane >> 5), n0 = wn * TL::NI * 32 + (lane & 31);
+    if constexpr (ROWS) __syncthreads();            // s_slot, s_w where there was no step
+#pragma unroll
+    for (int i = 0; i < TL::MI; ++i) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int m = m0 + i * 32 + 8 * (r / 4) + r % 4;
+            if constexpr (MODE == IN) {
+                if (m < count) {
+                    T* h = (T*)P.h + (size_t)(p0 + m) * (size_t)P.Fp;
+                    float* pre = P.pre ? P.pre + (size_t)(p0 + m) * 2 * (size_t)P.F : nullptr;
+#pragma unroll
+                    for (int j = 0; j < TL::NI; j += 2) {
+                        const int f = nf + (n0 >> 6) * 32 + (lane & 31) + j * 16;
+                        const float g = acc[i][j][r], u = acc[i][j + 1][r];
+                        if (f < P.F) {
+                            h[f] = (T)(g * sigmoid_fast(g) * u);
+                            if (pre) {
+                                pre[f] = g;
+                                pre[P.F + f] = u;
+                            }
+                        } else if (f < P.Fp) {
+                            h[f] = (T)0.0f;
+                        }
+                    }
+                }
+            } else if constexpr (MODE == OUT || MODE == DX) {
+                if (m < count) {
+                    const int slot = s_slot[m];
+                    const float w = s_w[m];
+#pragma unroll
+                    for (int j = 0; j < TL::NI; ++j) {
+                        const int d = nf + n0 + j * 32;
+                        if (d < P.D) {
+                            const float v = MODE == OUT ? acc[i][j][r] * w : acc[i][j][r];
+                            if (P.k == 1) ((T*)P.out)[(size_t)slot * (size_t)P.ldo + d] = (T)v;
+                            else P.z[(size_t)slot * (size_t)P.Dp + d] = v;
+                        }
+                    }
+                }
+            } else if constexpr (MODE == DH) {
+                float dot = 0.0f;
+                if (m < count) {
+                    const float w = s_w[m];
+                    const float* pre = P.pre + (size_t)(p0 + m) * 2 * (size_t)P.F;
+                    T* dpre = (T*)P.dpre + (size_t)(p0 + m) * 2 * (size_t)P.Fp;
+                    T* hw = (T*)P.hw + (size_t)(p0 + m) * (size_t)P.Fp;
+#pragma unroll
+                    for (int j = 0; j < TL::NI; ++j) {
+                        const int f = nf + n0 + j * 32;
+                        if (f < P.F) {
+                            const float g = pre[f], u = pre[P.F + f], a = acc[i][j][r];
+                            const float s = sigmoid_fast(g), h = g * s * u, dh = w * a;
+                            dot += a * h;
+                            dpre[f] = (T)(dh * u * s * (1.0f + g * (1.0f - s)));
+                            dpre[P.Fp + f] = (T)(dh * g * s);
+                            hw[f] = (T)(w * h);
+                        } else if (f < P.Fp) {
+                            dpre[f] = dpre[P.Fp + f] = hw[f] = (T)0.0f;
+                        }
+                    }
+                }
+                // over the 32 columns that the row's lanes hold
+                dot = lanes_reduce<32>(dot, [](float a, float b) { return a + b; });
+                if (m < count && (lane & 31) == 0)
+                    P.dwp[(size_t)(nf / TL::BN * TL::WN + wn) * (size_t)(P.n * P.k) + s_slot[m]] = dot;
+            } else {
+                int row = mf + m;
+                const int M = MODE == DWIN ? 2 * P.F : P.D, N = MODE == DWIN ? P.D : P.F;
+                if constexpr (MODE == DWIN) row = row < P.F ? row : row < P.Fp ? M : row + P.F - P.Fp;
+                if (row < M) {
+#pragma unroll
+                    for (int j = 0; j < TL::NI; ++j) {
+                        const int c = nf + n0 + j * 32;
+                        if (c < N) {
+                            const size_t at = ((size_t)e * M + row) * (size_t)N + c;
+                            if (P.splits == 1) ((T*)P.out)[at] = (T)acc[i][j][r];
+                            else P.part[(size_t)split * P.E * M * N + at] = acc[i][j][r];
+                        }
+                    }
+                }
+            }
+        }
+    }
+}
+
+// Rows' slots added up: out[t] = sum_j z[t k + j] over the slots that have an
+// expert, 4 columns a thread; and (dwp) the routing weights' gradient.
+template <typename T>
+__global__ void __launch_bounds__(256) k_combine(ExpertArgs P, T* __restrict__ out, int64_t ldo, int parts,
+                                                 float* __restrict__ dweights) {
+    const int per = P.Dp / 4;
+    const int64_t work = P.n * per;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < work; i += (int64_t)gridDim.x * 256) {
+        const int64_t t = i / per;
+        const int d = (int)(i - t * per) * 4;
+        f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int j = 0; j < P.k; ++j) {
+            const int e = P.ids[t * P.k + j];
+            if (e >= 0 && e < P.E) s += *(const f32x4*)(P.z + (size_t)(t * P.k + j) * (size_t)P.Dp + d);
+        }
+        T* o = out + (size_t)t * (size_t)ldo + d;
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+            if (d + c < P.D) o[c] = (T)s[c];
+    }
+    if (dweights) {
+        const int64_t S = P.n * P.k;
+        for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < S; i += (int64_t)gridDim.x * 256) {
+            const int e = P.ids[i];
+            float s = 0.0f;
+            if (e >= 0 && e < P.E)
+                for (int p = 0; p < parts; ++p) s += P.dwp[(size_t)p * (size_t)S + i];
+            dweights[i] = s;
+        }
+    }
+}
+
+// k = 1: rows whose slot has no expert get zeros, and dweights as in k_combine.
+template <typename T>
+__global__ void __launch_bounds__(256) k_unrouted(ExpertArgs P, T* __restrict__ out, int64_t ldo, int parts,
+                                                  float* __restrict__ dweights) {
+    for (int64_t t0 = (int64_t)blockIdx.x * 256; t0 < P.n; t0 += (int64_t)gridDim.x * 256) {
+        const int64_t t = t0 + threadIdx.x;
+        const int e = t < P.n ? P.ids[t] : 0;
+        const bool none = e < 0 || e >= P.E;
+        if (dweights && t < P.n) {
+            float s = 0.0f;
+            if (!none)
+                for (int p = 0; p < parts; ++p) s += P.dwp[(size_t)p * (size_t)P.n + t];
+            dweights[t] = s;
+        }
+        // a wave writes its rows without an expert one after the other
+        uint64_t left = __ballot(none);
+        while (left) {
+            const int l = __ffsll((unsigned long long)left) - 1;
+            left &= left - 1;
+            const int64_t row = t0 + (threadIdx.x & ~63) + l;
+            for (int d = threadIdx.x & 63; d < P.D; d += 64) out[(size_t)row * (size_t)ldo + d] = (T)0.0f;
+        }
+    }
+}
+
+// The parts of a weight gradient added in order.
+template <typename T>
+__global__ void __launch_bounds__(256) k_weight_parts(const float* __restrict__ part, int64_t count, int splits,
+                                                      T* __restrict__ out) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256) {
+        float s = 0.0f;
+        for (int p = 0; p < splits; ++p) s += part[(size_t)p * (size_t)count + i];
+        out[i] = (T)s;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------
+
+using TileSmall = TileOf<128, 128, 2, 2>;
+using TileLarge = TileOf<256, 256, 2, 4>;
+
+// Row tiles of 256 x 256 when the experts' slots fill them, else 128 x 128.
+inline bool large_tiles(int64_t S, int E, int M, int N) { return S >= (int64_t)E * 256 && M >= 192 && N >= 192; }
+
+constexpr int PART_BLOCKS = 512;      // blocks of weight gradients that keep the device busy
+
+inline int up16(int v, int bytes) { return (v * bytes + 15) / 16 * 16 / bytes; }
+
+struct ExpertPlanSizes {
+    int64_t S;
+    int Fp, Dp, splits_in, splits_out, parts;
+    bool large;
+};
+
+inline int weight_splits(int64_t S, int E, int M, int N, int bm, int bn, int bk) {
+    const int64_t tiles = (int64_t)E * ((M + bm - 1) / bm) * ((N + bn - 1) / bn);
+    int64_t s = PART_BLOCKS / tiles;
+    const int64_t longest = S / E / (4 * bk);          // at least four steps each for an average expert
+    if (s > longest) s = longest;
+    if (s > 64) s = 64;
+    return s < 1 ? 1 : (int)s;
+}
+
+inline ExpertPlanSizes expert_sizes(int dtype, int64_t n, int k, int D, int F, int E) {
+    ExpertPlanSizes z;
+    const int b = dtype_bytes(dtype);
+    z.S = n * k;
+    z.Fp = up16(F, b);
+    z.Dp = up16(D, 4);
+    z.large = large_tiles(z.S, E, D, F);
+    const int t = z.large ? 256 : 128, bk = STEP / b;
+    z.splits_in = weight_splits(z.S, E, z.Fp + F, D, t, t, bk);
+    z.splits_out = weight_splits(z.S, E, D, F, t, t, bk);
+    z.parts = (F + t - 1) / t * (z.large ? TileLarge::WN : TileSmall::WN);
+    return z;
+}
+
+inline size_t carve_forward(Carve& c, ExpertArgs* P, const ExpertPlanSizes& z, int dtype, int k) {
+    P->h = c.take<char>((size_t)z.S * z.Fp * dtype_bytes(dtype));
+    P->z = k > 1 ? c.take<float>((size_t)z.S * z.Dp) : nullptr;
+    return c.off;
+}
+
+inline size_t carve_backward(Carve& c, ExpertArgs* P, float** part, const ExpertPlanSizes& z, int dtype, int k, int D,
+                             int F, int E) {
+    const size_t b = (size_t)dtype_bytes(dtype);
+    P->dpre = c.take<char>((size_t)z.S * 2 * z.Fp * b);
+    P->hw = c.take<char>((size_t)z.S * z.Fp * b);
+    P->dwp = c.take<float>((size_t)z.parts * z.S);
+    P->z = k > 1 ? c.take<float>((size_t)z.S * z.Dp) : nullptr;
+    size_t p = z.splits_in > 1 ? (size_t)z.splits_in * E * 2 * F * (size_t)D : 0;
+    const size_t q = z.splits_out > 1 ? (size_t)z.splits_out * E * F * (size_t)D : 0;
+    if (q > p) p = q;
+    *part = p ? c.take<float>(p) : nullptr;
+    return c.off;
+}
+
+template <typename T, int MODE, typename TL, bool DMA>
+void launch_tiles(const ExpertArgs& P, int M, int N, hipStream_t stream) {
+    constexpr int cols = MODE == IN ? TL::BN / 2 : TL::BN;
+    const int nt = (N + cols - 1) / cols, mt = (M + TL::BM - 1) / TL::BM;
+    int64_t blocks;
+    if (MODE < DWIN) {
+        const int64_t S = P.n * P.k;
+        blocks = (S / TL::BM + (S < P.E ? S : P.E)) * nt;      // no plan has more tiles
+    } else {
+        blocks = (int64_t)P.E * mt * nt * P.splits;
+    }
+    if (blocks == 0) return;
+    blocks = (blocks + XCDS - 1) / XCDS * XCDS;
+    k_experts<T, MODE, TL, DMA><<<(unsigned)blocks, TL::NT, 2 * TL::STAGE, stream>>>(P, nt, mt);
+}
+
+template <typename T, int MODE>
+void run_tiles(const ExpertArgs& P, bool large, bool dma, int M, int N, hipStream_t stream) {
+    if (large) {
+        if (dma) launch_tiles<T, MODE, TileLarge, true>(P, M, N, stream);
+        else launch_tiles<T, MODE, TileLarge, false>(P, M, N, stream);
+    } else {
+        if (dma) launch_tiles<T, MODE, TileSmall, true>(P, M, N, stream);
+        else launch_tiles<T, MODE, TileSmall, false>(P, M, N, stream);
+    }
+}
+
+template <typename T>
+int run_experts(ExpertArgs P, const ExpertPlanSizes& z, T* y, int64_t ldy, bool dma, hipStream_t stream) {
+    P.out = y;
+    P.ldo = ldy;
+    run_tiles<T, IN>(P, z.large, dma, 0, P.F, stream);
+    run_tiles<T, OUT>(P, z.large, dma, 0, P.D, stream);
+    if (P.k > 1)
+        k_combine<T><<<launch_grid(P.n * (z.Dp / 4), 256, 8192), 256, 0, stream>>>(P, y, ldy, 0, nullptr);
+    else
+        k_unrouted<T><<<launch_grid(P.n, 256, 8192), 256, 0, stream>>>(P, y, ldy, 0, nullptr);
+    return launch_status("yabt_experts");
+}
+
+template <typename T>
+int run_experts_grad(ExpertArgs P, const ExpertPlanSizes& z, float* part, T* dx, int64_t lddx, float* dweights,
+                     T* dw_in, T* dw_out, bool dma, hipStream_t stream) {
+    run_tiles<T, DH>(P, z.large, dma, 0, P.F, stream);
+    P.out = dx;
+    P.ldo = lddx;
+    run_tiles<T, DX>(P, z.large, dma, 0, P.D, stream);
+    if (P.k > 1)
+        k_combine<T><<<launch_grid(P.n * (z.Dp / 4), 256, 8192), 256, 0, stream>>>(P, dx, lddx, z.parts, dweights);
+    else
+        k_unrouted<T><<<launch_grid(P.n, 256, 8192), 256, 0, stream>>>(P, dx, lddx, z.parts, dweights);
+    P.part = part;
+    P.out = dw_in;
+    P.splits = z.splits_in;
+    run_tiles<T, DWIN>(P, z.large, dma, z.Fp + P.F, P.D, stream);
+    const int64_t cin = (int64_t)P.E * 2 * P.F * P.D;
+    if (P.splits > 1)
+        k_weight_parts<T><<<launch_grid(cin, 256, 8192), 256, 0, stream>>>(part, cin, P.splits, dw_in);
+    P.out = dw_out;
+    P.splits = z.splits_out;
+    run_tiles<T, DWOUT>(P, z.large, dma, P.D, P.F, stream);
+    if (P.splits > 1)
+        k_weight_parts<T><<<launch_grid(cin / 2, 256, 8192), 256, 0, stream>>>(part, cin / 2, P.splits, dw_out);
+    return launch_status("yabt_experts_grad");
+}
+
+inline bool expert_sizes_ok(int64_t n, int k, int D, int F, int E) {
+    return n >= 0 && k >= 1 && D >= 1 && F >= 1 && E >= 1 && E <= 1024 && n <= INT32_MAX / k && D <= (1 << 24) &&
+           F <= (1 << 24);
+}
+
+// The grids' sizes; the tiles of the smallest shape.
+inline bool expert_grids_ok(int64_t n, int k, int D, int F, int E) {
+    const int64_t S = n * k, wide = D > F ? D : F;
+    return (S / 128 + E) * ((wide + 63) / 64) < INT32_MAX && (int64_t)E * ((2 * (int64_t)F + 255) / 128) * ((D + 127) / 128) < INT32_MAX / 64;
+}
+
+template <typename F>
+int by_dtype(int dtype, const F& f) {
+    if (dtype == DT_F32) return f((float*)nullptr);
+    if (dtype == DT_BF16) return f((bf16*)nullptr);
+    return f((f16*)nullptr);
+}
+
+// Whether rows of `width` values, ld apart, may be fetched in aligned 16-byte pieces.
+inline bool pieces_ok(const void* p, int64_t ld, int width, int bytes) {
+    return aligned16(p) && ld * bytes % 16 == 0 && (int64_t)width * bytes % 16 == 0;
+}
+
+}  // namespace yabt
+
+using namespace yabt;
+
+extern "C" {
+
+size_t yabt_experts_workspace_bytes(int dtype, int64_t n, int k, int D, int F, int E) {
+    if (!dtype_ok(dtype) || !expert_sizes_ok(n, k, D, F, E)) return 0;
+    ExpertArgs P;
+    Carve c{nullptr, 0};
+    return carve_forward(c, &P, expert_sizes(dtype, n, k, D, F, E), dtype, k) + 256;
+}
+
+int yabt_experts(int dtype, const void* x, int64_t ldx, int64_t n, int k, int D, int F, int E, const int32_t* ids,
+                 const int32_t* offsets, const int32_t* slots, const int32_t* rows, const float* weights,
+                 const void* w_in, const void* w_out, void* workspace, size_t workspace_bytes, float* out_inner,
+                 void* y, int64_t ldy, yabt_stream_t stream) {
+    if (!dtype_ok(dtype)) return fail(-1, "yabt_experts: dtype is 0 (fp32), 1 (bf16) or 2 (fp16)");
+    if (!expert_sizes_ok(n, k, D, F, E) || ldx < D || ldy < D || !expert_grids_ok(n, k, D, F, E))
+        return fail(-1, "yabt_experts: bad sizes");
+    if (n == 0) return 0;
+    if (!x || !ids || !offsets || !slots || !rows || !weights || !w_in || !w_out || !y)
+        return fail(-1, "yabt_experts: null pointer");
+    if (!workspace || workspace_bytes < yabt_experts_workspace_bytes(dtype, n, k, D, F, E))
+        return fail(-2, "yabt_experts: workspace too small");
+    const ExpertPlanSizes z = expert_sizes(dtype, n, k, D, F, E);
+    ExpertArgs P = {x, nullptr, w_in, w_out, weights, ids, offsets, slots, rows, ldx, 0, n, k, D, F, E, z.Fp, z.Dp};
+    P.pre = out_inner;
+    P.splits = 1;
+    Carve c{(char*)align_up((size_t)workspace, 256), 0};
+    carve_forward(c, &P, z, dtype, k);
+    const int b = dtype_bytes(dtype);
+    const bool dma = pieces_ok(x, ldx, D, b) && pieces_ok(w_in, D, D, b) && pieces_ok(w_out, F, F, b);
+    return by_dtype(dtype, [&](auto* t) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        return run_experts<T>(P, z, (T*)y, ldy, dma, (hipStream_t)stream);
+    });
+}
+
+size_t yabt_experts_grad_workspace_bytes(int dtype, int64_t n, int k, int D, int F, int E) {
+    if (!dtype_ok(dtype) || !expert_sizes_ok(n, k, D, F, E)) return 0;
+    ExpertArgs P;
+    float* part;
+    Carve c{nullptr, 0};
+    return carve_backward(c, &P, &part, expert_sizes(dtype, n, k, D, F, E), dtype, k, D, F, E) + 256;
+}
+
+int yabt_experts_grad(int dtype, const void* dy, int64_t lddy, const void* x, int64_t ldx, int64_t n, int k, int D,
+                      int F, int E, const int32_t* ids, const int32_t* offsets, const int32_t* slots,
+                      const int32_t* rows, const float* weights, const void* w_in, const void* w_out,
+                      const float* inner, void* workspace, size_t workspace_bytes, void* dx, int64_t lddx,
+                      float* dweights, void* dw_in, void* dw_out, yabt_stream_t stream) {
+    if (!dtype_ok(dtype)) return fail(-1, "yabt_experts_grad: dtype is 0 (fp32), 1 (bf16) or 2 (fp16)");
+    if (!expert_sizes_ok(n, k, D, F, E) || ldx < D || lddy < D || lddx < D || !expert_grids_ok(n, k, D, F, E))
+        return fail(-1, "yabt_experts_grad: bad sizes");
+    if (!offsets || !w_in || !w_out || !dw_in || !dw_out ||
+        (n > 0 && (!x || !dy || !ids || !slots || !rows || !weights || !inner || !dx || !dweights)))
+        return fail(-1, "yabt_experts_grad: null pointer");
+    if (!workspace || workspace_bytes < yabt_experts_grad_workspace_bytes(dtype, n, k, D, F, E))
+        return fail(-2, "yabt_experts_grad: workspace too small");
+    const ExpertPlanSizes z = expert_sizes(dtype, n, k, D, F, E);
+    ExpertArgs P = {x, dy, w_in, w_out, weights, ids, offsets, slots, rows, ldx, lddy, n, k, D, F, E, z.Fp, z.Dp};
+    P.pre = const_cast<float*>(inner);
+    Carve c{(char*)align_up((size_t)workspace, 256), 0};
+    float* part = nullptr;
+    carve_backward(c, &P, &part, z, dtype, k, D, F, E);
+    const int b = dtype_bytes(dtype);
+    const bool dma = pieces_ok(x, ldx, D, b) && pieces_ok(dy, lddy, D, b) && pieces_ok(w_in, D, D, b) &&
+                     pieces_ok(w_out, F, F, b);
+    return by_dtype(dtype, [&](auto* t) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        return run_experts_grad<T>(P, z, part, (T*)dx, lddx, dweights, (T*)dw_in, (T*)dw_out, dma,
+                                   (hipStream_t)stream);
+    });
+}
+
+}  // extern "C"

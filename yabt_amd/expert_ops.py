@@ -1,4 +1,5 @@
-"""The expert layer's operations on torch tensors (csrc/norm.hip, route.hip).
+"""The expert layer's operations on torch tensors (csrc/norm.hip, route.hip,
+experts.hip).
 
 Rows are normalised, a gate's scores route each row to k of E experts, and the
 experts' weighted answers are added up: the learned, soft form of a tree with
@@ -8,7 +9,8 @@ leaf.
 * ``layer_norm`` / ``layer_norm_grad``: rows to zero mean and unit variance,
   times a weight, plus a bias;
 * ``route`` / ``route_grad``: the k best experts of each row and their weights;
-* ``expert_plan``: the (row, expert) slots sorted by expert.
+* ``expert_plan``: the (row, expert) slots sorted by expert;
+* ``expert_products`` / ``expert_products_grad``: what the experts answer.
 
 Values are float32, bfloat16 or float16; statistics, weights, parameters of
 the norm and all sums are float32.  Every call runs on the current stream and
@@ -208,3 +210,80 @@ def expert_plan(ids: torch.Tensor, experts: int) -> ExpertPlan:
     _lib.check(lib.yabt_expert_plan(ids.data_ptr(), n, k, int(experts), ws.data_ptr(), nbytes, offsets.data_ptr(),
                                     slots.data_ptr(), rows.data_ptr(), _stream(dev)), "yabt_expert_plan")
     return ExpertPlan(ids, offsets, slots, rows)
+
+
+def _expert_args(x, plan, weights, w_in, w_out):
+    """Checked sizes and tensors of the products: (x, weights, w_in, w_out, n, k, D, F, E)."""
+    x = _matrix(x, "x")
+    (n, D), dev = x.shape, x.device
+    if w_in.dim() != 3 or w_out.dim() != 3:
+        raise ValueError(f"w_in and w_out must be (E, 2 F, D) and (E, D, F), got {tuple(w_in.shape)}, "
+                         f"{tuple(w_out.shape)}")
+    E, F = w_out.shape[0], w_out.shape[2]
+    if D < 1 or F < 1 or tuple(w_in.shape) != (E, 2 * F, D) or w_out.shape[1] != D:
+        raise ValueError(f"w_in and w_out must be (E, 2 F, {D}) and (E, {D}, F), got {tuple(w_in.shape)}, "
+                         f"{tuple(w_out.shape)}")
+    if w_in.dtype != x.dtype or w_out.dtype != x.dtype:
+        raise ValueError(f"x, w_in and w_out must have one type, got {x.dtype}, {w_in.dtype}, {w_out.dtype}")
+    if plan.experts != E or plan.ids.shape[0] != n:
+        raise ValueError(f"the plan is for {plan.experts} experts and {plan.ids.shape[0]} rows, not {E} and {n}")
+    k = plan.ids.shape[1]
+    if tuple(weights.shape) != (n, k):
+        raise ValueError(f"weights must have shape {(n, k)}, got {tuple(weights.shape)}")
+    if any(t.device != dev for t in (w_in, w_out, weights, plan.ids)):
+        raise ValueError(f"all tensors must be on {dev}")
+    weights = weights if weights.dtype == torch.float32 and weights.is_contiguous() else weights.float().contiguous()
+    return x, weights, w_in.contiguous(), w_out.contiguous(), n, k, D, F, E
+
+
+def expert_products(x: torch.Tensor, plan: ExpertPlan, weights: torch.Tensor, w_in: torch.Tensor,
+                    w_out: torch.Tensor, keep_inner: bool = False):
+    """y (n, D) in x's type: y_t = sum over row t's slots of weights * w_out[e]
+    (silu(g) * u) with [g u] = w_in[e] x_t, e the slot's expert.
+
+    w_in (E, 2 F, D) holds each expert's F gate rows, then its F rows of u;
+    w_out (E, D, F); both of x's type.  weights (n, k) as ``route`` gives them.
+    A row none of whose slots has an expert gets zeros.  With ``keep_inner``
+    returns (y, inner), inner (n k, 2 F) float32 being g and u by the plan's
+    places, which the backward pass takes."""
+    x, weights, w_in, w_out, n, k, D, F, E = _expert_args(x, plan, weights, w_in, w_out)
+    dev, dt, lib = x.device, DTYPES[x.dtype], _lib.load()
+    nbytes = int(lib.yabt_experts_workspace_bytes(dt, n, k, D, F, E))
+    if nbytes == 0:
+        raise ValueError("expert_products: sizes out of range (D, F <= 2^24, n k < 2^31)")
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    y = torch.empty((n, D), dtype=x.dtype, device=dev)
+    inner = torch.empty((n * k, 2 * F), dtype=torch.float32, device=dev) if keep_inner else None
+    _lib.check(lib.yabt_experts(dt, x.data_ptr(), _ld(x), n, k, D, F, E, plan.ids.data_ptr(), plan.offsets.data_ptr(),
+                                plan.slots.data_ptr(), plan.rows.data_ptr(), weights.data_ptr(), w_in.data_ptr(),
+                                w_out.data_ptr(), ws.data_ptr(), nbytes, _at(inner), y.data_ptr(), D, _stream(dev)),
+               "yabt_experts")
+    return (y, inner) if keep_inner else y
+
+
+def expert_products_grad(dy: torch.Tensor, x: torch.Tensor, plan: ExpertPlan, weights: torch.Tensor,
+                         w_in: torch.Tensor, w_out: torch.Tensor, inner: torch.Tensor):
+    """(dx, dweights, dw_in, dw_out) of ``expert_products`` from dy (n, D) and
+    the inner it kept: dx, dw_in and dw_out in x's type, dweights (n, k)
+    float32, 0 for slots without an expert."""
+    x, weights, w_in, w_out, n, k, D, F, E = _expert_args(x, plan, weights, w_in, w_out)
+    dy = _matrix(dy, "dy", x.dtype)
+    dev, dt, lib = x.device, DTYPES[x.dtype], _lib.load()
+    if dy.shape != x.shape or dy.device != dev:
+        raise ValueError(f"dy must be like x, {tuple(x.shape)} on {dev}")
+    if tuple(inner.shape) != (n * k, 2 * F) or inner.dtype != torch.float32 or not inner.is_contiguous() \
+            or inner.device != dev:
+        raise ValueError(f"inner must be what expert_products kept, {(n * k, 2 * F)} float32 on {dev}")
+    nbytes = int(lib.yabt_experts_grad_workspace_bytes(dt, n, k, D, F, E))
+    if nbytes == 0:
+        raise ValueError("expert_products_grad: sizes out of range (D, F <= 2^24, n k < 2^31)")
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    dx = torch.empty((n, D), dtype=x.dtype, device=dev)
+    dweights = torch.empty((n, k), dtype=torch.float32, device=dev)
+    dw_in, dw_out = torch.empty_like(w_in), torch.empty_like(w_out)
+    _lib.check(lib.yabt_experts_grad(dt, dy.data_ptr(), _ld(dy), x.data_ptr(), _ld(x), n, k, D, F, E,
+                                     plan.ids.data_ptr(), plan.offsets.data_ptr(), plan.slots.data_ptr(),
+                                     plan.rows.data_ptr(), weights.data_ptr(), w_in.data_ptr(), w_out.data_ptr(),
+                                     inner.data_ptr(), ws.data_ptr(), nbytes, dx.data_ptr(), D, dweights.data_ptr(),
+                                     dw_in.data_ptr(), dw_out.data_ptr(), _stream(dev)), "yabt_experts_grad")
+    return dx, dweights, dw_in, dw_out
