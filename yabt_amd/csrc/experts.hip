@@ -17,9 +17,9 @@
 //   DX     W_in^T [dg du] by slot in fp32, or dx itself when k = 1
 //   DWIN, DWOUT   the weights' gradients, summed over an expert's slots
 //
-// Both operands pass through LDS in 128-byte steps of the summed dimension,
-// two stages: the next one is on its way from memory straight into LDS while
-// the present one is multiplied.  16-byte pieces are stored at places that an
+// Both operands pass through LDS in steps of 64 or 128 bytes of the summed
+// dimension, two stages or more: the next ones are on their way from memory
+// straight into LDS while the present one is multiplied.  16-byte pieces are stored at places that an
 // xor with the row spreads over the banks; the xor is applied to the global
 // address, as LDS is filled in lane order.  Operands across the summed
 // dimension are read with the transposing LDS loads.  Inputs whose rows are
@@ -48,7 +48,6 @@ typedef __attribute__((address_space(3))) float lds_float;
 
 enum Mode { IN, OUT, DH, DX, DWIN, DWOUT };
 
-constexpr int STEP = 128;             // bytes of the summed dimension a stage holds
 constexpr int XCDS = 8;               // blocks go to the 8 dies in turn
 constexpr int TILE_GROUP = 4;         // row tiles that walk the column tiles together
 
@@ -81,31 +80,47 @@ struct ExpertArgs {
 // 16 zero bytes for pieces past the end of the summed dimension.
 __device__ const u32x4 g_zeros = {0, 0, 0, 0};
 
-template <int BM_, int BN_, int WM_, int WN_>
+// BM x BN sums by WM x WN waves; STAGES stages of STEP bytes of the summed dimension.
+template <int BM_, int BN_, int WM_, int WN_, int STEP_, int STAGES_>
 struct TileOf {
-    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_;
+    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, STEP = STEP_, STAGES = STAGES_;
     static constexpr int NT = 64 * WM * WN;
     static constexpr int MI = BM / WM / 32, NI = BN / WN / 32;    // 32 x 32 blocks a wave makes
     static constexpr int ABYTES = BM * STEP, BBYTES = BN * STEP, STAGE = ABYTES + BBYTES;
     static constexpr int NA = ABYTES / 16 / NT, NB = BBYTES / 16 / NT;
     static_assert(NA >= 1 && NB >= 1 && NI % 2 == 0, "whole pieces a thread, gate and up in one wave");
+    static_assert(STAGES * STAGE + 2048 <= 160 * 1024, "a block's LDS");
 };
+
+// Where piece c (16 bytes) of row r of a tile in LDS is kept: c ^ spread(r), so
+// that the lanes a read serves at once (16 of 16 bytes, 32 of 8, 64 of 4: 256
+// bytes, all banks) meet different banks.  ALONG: a row is STEP bytes of one
+// row of the operand; across: a row is one place of the summed dimension.
+template <typename T, bool ACROSS, int STEP>
+__device__ __forceinline__ constexpr int spread(int r) {
+    if (!ACROSS) return STEP == 128 ? r >> 1 & 7 : r >> 2 & 3;
+    return sizeof(T) == 4 ? (r >> 2 & 1) << 3 : (r & 3) << 2;
+}
 
 // silu by the hardware's exp2 and reciprocal (about one unit each).
 __device__ __forceinline__ float sigmoid_fast(float g) {
     return __builtin_amdgcn_rcpf(1.0f + __expf(-g));
 }
 
-// 64 lanes' 16 bytes each from memory to LDS at base (the same for the wave), in lane order.
+// 64 lanes' 16 bytes each from memory to LDS at base (the same for the wave),
+// in lane order.  By hand, because the compiler waits for all LDS reads at
+// every use of one where the builtin is about; it counts as a vector memory
+// access, which stage_ready waits for.
 __device__ __forceinline__ void lds_fill(const void* g, uint32_t base) {
-    typedef const __attribute__((address_space(1))) void global_void;
-    typedef __attribute__((address_space(3))) void lds_void;
-    __builtin_amdgcn_global_load_lds((global_void*)g, (lds_void*)(uintptr_t)base, 16, 0, 0);
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "s"(base));
 }
 
+// Until at most LATER of this wave's vector memory accesses are under way and
+// its LDS reads are done, then for the block's other waves: what was sent to
+// LDS before the last LATER accesses is there, and the stage read last is free.
+template <int LATER>
 __device__ __forceinline__ void stage_ready() {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LATER) : "memory");
 }
 
 // Row tile `id` of the slots in tiles of BM per expert; total: their number.
@@ -150,6 +165,18 @@ __device__ __forceinline__ int64_t die_order(int64_t b, int64_t total) {
     return in < per ? (b % XCDS) * per + in : total;
 }
 
+// Asks for the order in which MF products and RD LDS reads are issued: the reads
+// spread evenly between the products.
+template <int MF, int RD, int I = 0>
+__device__ __forceinline__ void interleave() {
+    if constexpr (I < MF) {
+        constexpr int reads = RD * (I + 1) / MF - RD * I / MF;
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        if constexpr (reads > 0) __builtin_amdgcn_sched_group_barrier(0x100, reads, 0);
+        interleave<MF, RD, I + 1>();
+    }
+}
+
 template <typename T>
 __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
     if constexpr (sizeof(T) == 4) {
@@ -168,27 +195,30 @@ __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
 
 // A lane's 16 bytes of block i of an operand at k-step ks (32 bytes of the
 // summed dimension): row (or column) lane % 32, half lane / 32.
-//   along: tile[row][128 bytes], piece c of a row stored at c ^ (row & 7)
-//   across: tile[k][W values], piece c of a row stored at c ^ 2 (k & 3)
-template <typename T, bool ACROSS, int W>
+template <typename T, bool ACROSS, int W, int STEP>
 struct Frag {
-    uint32_t at[ACROSS ? (sizeof(T) == 4 ? 4 : 2) : 4];
+    static constexpr int READS = !ACROSS ? 1 : sizeof(T) == 4 ? 4 : 2;   // LDS reads of get()
+    static constexpr int KEEP = ACROSS ? 4 : STEP / 32;
+    uint32_t at[KEEP];
     __device__ __forceinline__ Frag(int first) {
         const int l = threadIdx.x & 63;
         if constexpr (!ACROSS) {
 #pragma unroll
-            for (int ks = 0; ks < 4; ++ks)
-                at[ks] = (uint32_t)((first + (l & 31)) * STEP + (((ks * 2 + (l >> 5)) ^ (l & 7)) << 4));
+            for (int ks = 0; ks < KEEP; ++ks)
+                at[ks] = (uint32_t)((first + (l & 31)) * STEP +
+                                    (((ks * 2 + (l >> 5)) ^ spread<T, ACROSS, STEP>(l & 31)) << 4));
         } else if constexpr (sizeof(T) == 4) {
+            // four rows of k, a value of each; blocks of 32 columns are 128 bytes apart
+            const int r = (l >> 5) * 4;
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-                at[q] = (uint32_t)(((l >> 5) * 4 + q) * W * 4 + first * 4 + (((l & 31) * 4) ^ (q << 5)));
+            for (int i = 0; i < 2; ++i)
+                at[i] = (uint32_t)(r * W * 4 + first * 4 + ((i * 128 + (l & 31) * 4) ^ spread<T, ACROSS, STEP>(r) << 4));
         } else {
-            const int r = (l & 15) >> 2;                     // of four rows of k, this lane fetches row r
-            const int col = ((l >> 4) & 1) * 16 + (l & 3) * 4;
-            const uint32_t row = (uint32_t)(((l >> 5) * 8 + r) * W * 2 + first * 2);
+            // of four rows of k this lane fetches four values of one; blocks are 64 bytes apart
+            const int r = (l & 15) >> 2, col = ((l >> 4) & 1) * 16 + (l & 3) * 4;
 #pragma unroll
-            for (int odd = 0; odd < 2; ++odd) at[odd] = row + (uint32_t)((odd * 64 + col * 2) ^ (r << 5));
+            for (int i = 0; i < 4; ++i)
+                at[i] = (uint32_t)(((l >> 5) * 8 + r) * W * 2 + ((first * 2 + i * 64 + col * 2) ^ spread<T, ACROSS, STEP>(r) << 4));
         }
     }
     __device__ __forceinline__ u32x4 get(lds_char* tile, int i, int ks) const {
@@ -197,10 +227,11 @@ struct Frag {
         } else if constexpr (sizeof(T) == 4) {
             f32x4 v;
 #pragma unroll
-            for (int q = 0; q < 4; ++q) v[q] = *(const lds_float*)(tile + at[q] + ks * 8 * W * 4 + i * 128);
+            for (int q = 0; q < 4; ++q)
+                v[q] = *(const lds_float*)(tile + at[i & 1] + (ks * 8 + q) * W * 4 + (i >> 1) * 256);
             return __builtin_bit_cast(u32x4, v);
         } else {
-            lds_char* p = tile + at[i & 1] + (i >> 1) * 128 + ks * 16 * W * 2;
+            lds_char* p = tile + at[i & 3] + (i >> 2) * 256 + ks * 16 * W * 2;
             const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
             const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 4 * W * 2));
             return __builtin_bit_cast(u32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
@@ -211,19 +242,19 @@ struct Frag {
 // The pieces of an operand that a thread brings to LDS.  The mode says where a
 // row lies; pieces past the end of the summed dimension are zero, rows and
 // columns past the tile's end repeat the last (their sums are not stored).
-template <typename T, int MODE, bool SIDE_B, int W, int COUNT, int NT>
+template <typename T, int MODE, bool SIDE_B, int W, int COUNT, int NT, int STEP>
 struct Loader {
     static constexpr bool ACROSS = SIDE_B ? MODE >= DH : MODE >= DWIN;
     static constexpr bool GATHER = SIDE_B ? MODE == DWIN : MODE == IN || MODE == DH || MODE == DWOUT;
     static constexpr int CH = VEC<T>;
-    static constexpr int PER_ROW = ACROSS ? W * (int)sizeof(T) / 16 : 8;
+    static constexpr int PER_ROW = ACROSS ? W * (int)sizeof(T) / 16 : STEP / 16;
     const T* ptr[COUNT];       // along: the row, at this piece; across: column of the piece, from row 0
-    int32_t src[COUNT];        // across and gathered: the next step's rows
+    int32_t src[COUNT], nxt[COUNT];   // across and gathered: the rows of the step to send, and of the one after
 
     __device__ __forceinline__ static int row_of(int i) { return (i * NT + (int)threadIdx.x) / PER_ROW; }
     __device__ __forceinline__ static int piece_of(int i) {
         const int c = (i * NT + (int)threadIdx.x) % PER_ROW, r = row_of(i);
-        return ACROSS ? c ^ ((r & 3) << 1) : c ^ (r & 7);
+        return c ^ spread<T, ACROSS, STEP>(r);
     }
 
     // p0: the tile's first slot place (along), or the split's (across); count:
@@ -283,8 +314,14 @@ struct Loader {
 #pragma unroll
             for (int i = 0; i < COUNT; ++i) {
                 const int kk = k0 + row_of(i);
-                src[i] = kk < count ? P.rows[p0 + kk] : -1;
+                nxt[i] = kk < count ? P.rows[p0 + kk] : -1;
             }
+        }
+    }
+    __device__ __forceinline__ void move_on() {
+        if constexpr (ACROSS && GATHER) {
+#pragma unroll
+            for (int i = 0; i < COUNT; ++i) src[i] = nxt[i];
         }
     }
 
@@ -402,19 +439,19 @@ __global__ void __launch_bounds__(TL::NT) k_experts(ExpertArgs P, int ntiles, in
         mf = (group * TILE_GROUP + gin % gm) * TL::BM;
         nf = gin / gm * TL::BN;
         const int off = P.offsets[e], cnt = P.offsets[e + 1] - off;
-        const int step = STEP / (int)sizeof(T);
+        const int step = TL::STEP / (int)sizeof(T);
         const int part = ((cnt + P.splits - 1) / P.splits + step - 1) / step * step;
         const int lo = min(cnt, split * part);
         p0 = off + lo;
         count = min(part, cnt - lo);
     }
 
-    Loader<T, MODE, false, TL::BM, TL::NA, TL::NT> la;
-    Loader<T, MODE, true, TL::BN, TL::NB, TL::NT> lb;
+    Loader<T, MODE, false, TL::BM, TL::NA, TL::NT, TL::STEP> la;
+    Loader<T, MODE, true, TL::BN, TL::NB, TL::NT, TL::STEP> lb;
     using LA = decltype(la);
     using LB = decltype(lb);
     const int ka = LA::length(P, count), kb = LB::length(P, count), K = max(ka, kb);
-    constexpr int BK = STEP / (int)sizeof(T);
+    constexpr int BK = TL::STEP / (int)sizeof(T), AHEAD = DMA ? TL::STAGES - 1 : 1, KS = TL::STEP / 32;
     const int steps = (K + BK - 1) / BK;
     f32x16 acc[TL::MI][TL::NI];
 #pragma unroll
@@ -427,57 +464,79 @@ __global__ void __launch_bounds__(TL::NT) k_experts(ExpertArgs P, int ntiles, in
     if (steps > 0) {
         la.init(P, e, p0, count, mf);
         lb.init(P, e, p0, count, nf);
-        la.look_up(P, p0, count, 0);
-        lb.look_up(P, p0, count, 0);
+        // stage t % STAGES holds step t; AHEAD steps are under way
         u32x4 ra[DMA ? 1 : TL::NA], rb[DMA ? 1 : TL::NB];
+        auto look_up = [&](int t) {
+            la.look_up(P, p0, count, t * BK);
+            lb.look_up(P, p0, count, t * BK);
+        };
+        // step t on its way; the rows of the step after it are asked for first,
+        // so that a wait for them is none for the pieces
+        auto send = [&](int t) {
+            la.move_on();
+            lb.move_on();
+            look_up(t + 1);
+            if constexpr (DMA) {
+                const uint32_t to = lds_at + (uint32_t)(t % TL::STAGES) * TL::STAGE;
+                la.fill(P, t * BK, ka, to);
+                lb.fill(P, t * BK, kb, to + TL::ABYTES);
+            } else {
+                la.fetch(P, t * BK, ka, mf, ra);
+                lb.fetch(P, t * BK, kb, nf, rb);
+            }
+        };
+        look_up(0);
         if constexpr (DMA) {
-            la.fill(P, 0, ka, lds_at);
-            lb.fill(P, 0, kb, lds_at + TL::ABYTES);
+#pragma unroll
+            for (int t = 0; t <= AHEAD; ++t) send(t);
         } else {
-            la.fetch(P, 0, ka, mf, ra);
-            lb.fetch(P, 0, kb, nf, rb);
+            send(0);
             LA::put(lds, ra);
             LB::put(lds + TL::ABYTES, rb);
+            send(1);
         }
-        la.look_up(P, p0, count, BK);
-        lb.look_up(P, p0, count, BK);
-        const Frag<T, LA::ACROSS, TL::BM> fa(wm * TL::MI * 32);
-        const Frag<T, LB::ACROSS, TL::BN> fb(wn * TL::NI * 32);
+        const Frag<T, LA::ACROSS, TL::BM, TL::STEP> fa(wm * TL::MI * 32);
+        const Frag<T, LB::ACROSS, TL::BN, TL::STEP> fb(wn * TL::NI * 32);
+        u32x4 a[2][TL::MI], b[2][TL::NI];
+        auto read = [&](int t, int ks) {
+            lds_char* const cur = lds + t % TL::STAGES * TL::STAGE;
+#pragma unroll
+            for (int i = 0; i < TL::MI; ++i) a[ks & 1][i] = fa.get(cur, i, ks);
+#pragma unroll
+            for (int j = 0; j < TL::NI; ++j) b[ks & 1][j] = fb.get(cur + TL::ABYTES, j, ks);
+        };
+        // a step that was sent is EACH accesses of every wave, and steps past
+        // the last are sent too (zeros), so that every wait is the same
+        constexpr int EACH = TL::NA + TL::NB, READS = TL::MI * decltype(fa)::READS + TL::NI * decltype(fb)::READS;
+        constexpr int PRODUCTS = TL::MI * TL::NI * (sizeof(T) == 4 ? 4 : 1);
+        stage_ready<DMA ? AHEAD * EACH : 0>();
+        read(0, 0);
+        // A k-step's operands are read while the one before is multiplied, the
+        // next step's first ones too: the wait for it stands before the last
+        // k-step's products, and the step that takes the freed stage is sent there.
         for (int t = 0; t < steps; ++t) {
-            stage_ready();
-            const uint32_t next = (uint32_t)((t + 1) & 1) * TL::STAGE;
-            lds_char* const cur = lds + (t & 1) * TL::STAGE;
-            if (t + 1 < steps) {
-                const int k0 = (t + 1) * BK;
-                if constexpr (DMA) {
-                    la.fill(P, k0, ka, lds_at + next);
-                    lb.fill(P, k0, kb, lds_at + next + TL::ABYTES);
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                if (ks + 1 < KS) {
+                    read(t, ks + 1);
                 } else {
-                    la.fetch(P, k0, ka, mf, ra);
-                    lb.fetch(P, k0, kb, nf, rb);
+                    if constexpr (!DMA) {
+                        lds_char* const to = lds + (t + 1) % TL::STAGES * TL::STAGE;
+                        LA::put(to, ra);
+                        LB::put(to + TL::ABYTES, rb);
+                    }
+                    stage_ready<DMA ? (AHEAD - 1) * EACH : 0>();
+                    send(t + 1 + AHEAD);
+                    read(t + 1, 0);
                 }
-                la.look_up(P, p0, count, k0 + BK);
-                lb.look_up(P, p0, count, k0 + BK);
-            }
-#pragma unroll
-            for (int ks = 0; ks < 4; ++ks) {
-                u32x4 a[TL::MI], b[TL::NI];
-#pragma unroll
-                for (int i = 0; i < TL::MI; ++i) a[i] = fa.get(cur, i, ks);
-#pragma unroll
-                for (int j = 0; j < TL::NI; ++j) b[j] = fb.get(cur + TL::ABYTES, j, ks);
 #pragma unroll
                 for (int i = 0; i < TL::MI; ++i)
 #pragma unroll
-                    for (int j = 0; j < TL::NI; ++j) acc[i][j] = mma<T>(a[i], b[j], acc[i][j]);
-            }
-            if constexpr (!DMA) {
-                if (t + 1 < steps) {
-                    LA::put(lds + next, ra);
-                    LB::put(lds + next + TL::ABYTES, rb);
-                }
+                    for (int j = 0; j < TL::NI; ++j) acc[i][j] = mma<T>(a[ks & 1][i], b[ks & 1][j], acc[i][j]);
+                if constexpr (DMA) interleave<PRODUCTS, READS>();
             }
         }
+        stage_ready<0>();                            // nothing may reach the LDS of a block that is gone
     }
 
     // sum r of block (i, j): row m0 + i * 32 + 8 (r / 4) + r % 4, column n0 + j * 32
@@ -639,8 +698,8 @@ __global__ void __launch_bounds__(256) k_weight_parts(const float* __restrict__ 
 // host
 // ---------------------------------------------------------------------------
 
-using TileSmall = TileOf<128, 128, 2, 2>;
-using TileLarge = TileOf<256, 256, 2, 4>;
+using TileSmall = TileOf<128, 128, 2, 2, 128, 2>;
+using TileLarge = TileOf<256, 256, 2, 4, 128, 2>;
 
 // Row tiles of 256 x 256 when the experts' slots fill them, else 128 x 128.
 inline bool large_tiles(int64_t S, int E, int M, int N) { return S >= (int64_t)E * 256 && M >= 192 && N >= 192; }
@@ -671,7 +730,7 @@ inline ExpertPlanSizes expert_sizes(int dtype, int64_t n, int k, int D, int F, i
     z.Fp = up16(F, b);
     z.Dp = up16(D, 4);
     z.large = large_tiles(z.S, E, D, F);
-    const int t = z.large ? 256 : 128, bk = STEP / b;
+    const int t = z.large ? 256 : 128, bk = 128 / b;
     z.splits_in = weight_splits(z.S, E, z.Fp + F, D, t, t, bk);
     z.splits_out = weight_splits(z.S, E, D, F, t, t, bk);
     z.parts = (F + t - 1) / t * (z.large ? TileLarge::WN : TileSmall::WN);
@@ -711,7 +770,7 @@ void launch_tiles(const ExpertArgs& P, int M, int N, hipStream_t stream) {
     }
     if (blocks == 0) return;
     blocks = (blocks + XCDS - 1) / XCDS * XCDS;
-    k_experts<T, MODE, TL, DMA><<<(unsigned)blocks, TL::NT, 2 * TL::STAGE, stream>>>(P, nt, mt);
+    k_experts<T, MODE, TL, DMA><<<(unsigned)blocks, TL::NT, TL::STAGES * TL::STAGE, stream>>>(P, nt, mt);
 }
 
 template <typename T, int MODE>
