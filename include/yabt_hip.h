@@ -559,8 +559,9 @@ int yabt_expert_plan(const int32_t *ids, int64_t n, int k, int E, void *workspac
  * x (n, D), y (n, D), w_in (E, 2 F, D): F gate rows, then F rows of u, w_out
  * (E, D, F), all of `dtype`; weights (n, k) fp32; ids (n, k) and the plan
  * yabt_expert_plan made of them.  A row none of whose slots has an expert gets
- * zeros.  out_inner ((n k) x 2 F, fp32, or NULL) keeps g and u of every place
- * of the plan for the backward pass; places past the plan's last are not written.
+ * zeros.  out_inner ((n k) x 2 G, fp32, 16-byte aligned, or NULL), G being F up
+ * to a multiple of 4, keeps g and u of every place of the plan for the
+ * backward pass; places past the plan's last are not written.
  * h is rounded to `dtype` before the second product; sums are fp32. */
 size_t yabt_experts_workspace_bytes(int dtype, int64_t n, int k, int D, int F, int E);
 int yabt_experts(int dtype, const void *x, int64_t ldx, int64_t n, int k, int D, int F, int E,

@@ -45,6 +45,7 @@ typedef __attribute__((address_space(3))) char lds_char;
 typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 typedef __attribute__((address_space(3))) float lds_float;
+typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
 
 enum Mode { IN, OUT, DH, DX, DWIN, DWOUT };
 
@@ -64,11 +65,12 @@ struct ExpertArgs {
     int64_t ldx, lddy, n;
     int k, D, F, E;
     int Fp;                           // F up to whole 16 bytes: the pitch of h and w h, half that of [dg du]
-    int Dp;                           // D up to whole 16 bytes: the pitch of z
+    int Dp;                           // D up to a multiple of 4: the pitch of z
+    int Fi;                           // F up to a multiple of 4: half the pitch of pre
     void* h;                          // (S, Fp)
     void* hw;                         // (S, Fp): w h
     void* dpre;                       // (S, 2 Fp): dg from 0, du from Fp
-    float* pre;                       // (S, 2 F): g from 0, u from F, or NULL
+    float* pre;                       // (S, 2 Fi): g from 0, u from Fi, or NULL
     float* z;                         // (S, Dp)
     float* dwp;                       // (parts, S): dw by column tile
     void* out;                        // y or dx (k = 1), dW_in or dW_out
@@ -163,6 +165,25 @@ __device__ __forceinline__ int64_t die_order(int64_t b, int64_t total) {
     const int64_t per = (total + XCDS - 1) / XCDS;
     const int64_t in = b / XCDS;
     return in < per ? (b % XCDS) * per + in : total;
+}
+
+// Four values, at an address that is a multiple of four, or (store_part) any:
+// the first `have` of them.
+template <typename T>
+__device__ __forceinline__ void store4(T* p, const float* v) {
+    typedef T VT __attribute__((ext_vector_type(4)));
+    *(VT*)p = VT{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
+}
+template <typename T>
+__device__ __forceinline__ void store_part(T* p, f32x4 v, int have) {
+    typedef T VT __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+    if (have >= 4) {
+        *(VT*)p = VT{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
+    } else {
+#pragma unroll
+        for (int q = 0; q < 3; ++q)
+            if (q < have) p[q] = (T)v[q];
+    }
 }
 
 // Asks for the order in which MF products and RD LDS reads are issued: the reads
@@ -427,12 +448,13 @@ __global__ void __launch_bounds__(TL::NT) k_experts(ExpertArgs P, int ntiles, in
             s_w[i] = MODE == OUT || MODE == DH ? P.weights[slot] : 1.0f;
         }
     } else {
-        const int64_t all = (int64_t)P.E * mtiles * ntiles * P.splits, id = die_order(blockIdx.x, all);
+        // an expert's tiles over all dies: experts differ in how long theirs take
+        const int per = mtiles * ntiles, all = per * P.splits, up = (all + XCDS - 1) / XCDS * XCDS;
+        e = (int)(blockIdx.x / up);
+        const int64_t id = die_order(blockIdx.x - (int64_t)e * up, all);
         if (id >= all) return;
-        const int per = mtiles * ntiles;
-        const int es = (int)(id / per), in = (int)(id - (int64_t)es * per);
-        e = es / P.splits;
-        split = es % P.splits;
+        split = (int)(id / per);
+        const int in = (int)(id - (int64_t)split * per);
         // column tiles together with a group of row tiles
         const int group = in / (TILE_GROUP * ntiles), gin = in - group * TILE_GROUP * ntiles;
         const int gm = min(TILE_GROUP, mtiles - group * TILE_GROUP);
@@ -539,87 +561,93 @@ __global__ void __launch_bounds__(TL::NT) k_experts(ExpertArgs P, int ntiles, in
         stage_ready<0>();                            // nothing may reach the LDS of a block that is gone
     }
 
-    // sum r of block (i, j): row m0 + i * 32 + 8 (r / 4) + r % 4, column n0 + j * 32
-    const int m0 = wm * TL::MI * 32 + 4 * (lane >> 5), n0 = wn * TL::NI * 32 + (lane & 31);
-    if constexpr (ROWS) __syncthreads();            // s_slot, s_w where there was no step
+    // The sums go through LDS, 32 rows of a wave at a time, from the matrix
+    // cores' layout (a lane has one column) to four neighbouring columns a lane,
+    // so that what is read and written beside them goes in whole lines.
+    if constexpr (ROWS) __syncthreads();            // s_slot and s_w where there was no step
+    constexpr int W = TL::NI * 32;
+    static_assert(32 * W * 4 * TL::NT / 64 <= TL::STAGES * TL::STAGE, "the waves' 32 rows fit the stages");
+    lds_float* const mine = (lds_float*)(lds + wave * 32 * W * 4);
+    constexpr int LANES = MODE == IN ? W / 8 : W / 4, PASS = 64 / LANES;    // lanes a row, rows at once
+    const int c4 = lane % LANES * 4;
 #pragma unroll
     for (int i = 0; i < TL::MI; ++i) {
+        wave_sync_lds();
+        // sum r of block (i, j): row 8 (r / 4) + 4 (lane / 32) + r % 4, column 32 j + lane % 32;
+        // the rows of the upper lanes are kept with their blocks in pairs swapped: other banks
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const int m = m0 + i * 32 + 8 * (r / 4) + r % 4;
+        for (int j = 0; j < TL::NI; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                mine[(8 * (r / 4) + 4 * (lane >> 5) + r % 4) * W + ((j * 32) ^ (lane & 32)) + (lane & 31)] = acc[i][j][r];
+        wave_sync_lds();
+#pragma unroll 4
+        for (int p = 0; p < 32; p += PASS) {
+            const int in = p + lane / LANES, m = (wm * TL::MI + i) * 32 + in;
+            auto four = [&](int c) { return *(const lds_f32x4*)(mine + in * W + (c ^ ((in & 4) << 3))); };
             if constexpr (MODE == IN) {
-                if (m < count) {
-                    T* h = (T*)P.h + (size_t)(p0 + m) * (size_t)P.Fp;
-                    float* pre = P.pre ? P.pre + (size_t)(p0 + m) * 2 * (size_t)P.F : nullptr;
+                // columns 64 q + 0..31: gate of f 32 q + 0..31, the next 32: u
+                const int f = nf + wn * (W / 2) + c4, c = (c4 & ~31) * 2 + (c4 & 31);
+                const f32x4 g = four(c), u = four(c + 32);
+                if (m < count && f < P.Fp) {
+                    float h[4];
 #pragma unroll
-                    for (int j = 0; j < TL::NI; j += 2) {
-                        const int f = nf + (n0 >> 6) * 32 + (lane & 31) + j * 16;
-                        const float g = acc[i][j][r], u = acc[i][j + 1][r];
-                        if (f < P.F) {
-                            h[f] = (T)(g * sigmoid_fast(g) * u);
-                            if (pre) {
-                                pre[f] = g;
-                                pre[P.F + f] = u;
-                            }
-                        } else if (f < P.Fp) {
-                            h[f] = (T)0.0f;
-                        }
+                    for (int q = 0; q < 4; ++q) h[q] = f + q < P.F ? g[q] * sigmoid_fast(g[q]) * u[q] : 0.0f;
+                    store4((T*)P.h + (size_t)(p0 + m) * (size_t)P.Fp + f, h);
+                    if (P.pre && f < P.Fi) {
+                        float* pre = P.pre + (size_t)(p0 + m) * 2 * (size_t)P.Fi + f;
+                        *(f32x4*)pre = g;
+                        *(f32x4*)(pre + P.Fi) = u;
                     }
                 }
             } else if constexpr (MODE == OUT || MODE == DX) {
-                if (m < count) {
+                const int d = nf + wn * W + c4;
+                f32x4 v = four(c4);
+                if (m < count && d < P.D) {
                     const int slot = s_slot[m];
-                    const float w = s_w[m];
-#pragma unroll
-                    for (int j = 0; j < TL::NI; ++j) {
-                        const int d = nf + n0 + j * 32;
-                        if (d < P.D) {
-                            const float v = MODE == OUT ? acc[i][j][r] * w : acc[i][j][r];
-                            if (P.k == 1) ((T*)P.out)[(size_t)slot * (size_t)P.ldo + d] = (T)v;
-                            else P.z[(size_t)slot * (size_t)P.Dp + d] = v;
-                        }
-                    }
+                    if constexpr (MODE == OUT) v *= s_w[m];
+                    if (P.k > 1) *(f32x4*)(P.z + (size_t)slot * (size_t)P.Dp + d) = v;
+                    else store_part((T*)P.out + (size_t)slot * (size_t)P.ldo + d, v, P.D - d);
                 }
             } else if constexpr (MODE == DH) {
+                const int f = nf + wn * W + c4;
+                const f32x4 a = four(c4);
                 float dot = 0.0f;
-                if (m < count) {
+                if (m < count && f < P.Fp) {
                     const float w = s_w[m];
-                    const float* pre = P.pre + (size_t)(p0 + m) * 2 * (size_t)P.F;
-                    T* dpre = (T*)P.dpre + (size_t)(p0 + m) * 2 * (size_t)P.Fp;
-                    T* hw = (T*)P.hw + (size_t)(p0 + m) * (size_t)P.Fp;
-#pragma unroll
-                    for (int j = 0; j < TL::NI; ++j) {
-                        const int f = nf + n0 + j * 32;
-                        if (f < P.F) {
-                            const float g = pre[f], u = pre[P.F + f], a = acc[i][j][r];
-                            const float s = sigmoid_fast(g), h = g * s * u, dh = w * a;
-                            dot += a * h;
-                            dpre[f] = (T)(dh * u * s * (1.0f + g * (1.0f - s)));
-                            dpre[P.Fp + f] = (T)(dh * g * s);
-                            hw[f] = (T)(w * h);
-                        } else if (f < P.Fp) {
-                            dpre[f] = dpre[P.Fp + f] = hw[f] = (T)0.0f;
-                        }
+                    f32x4 g = {0.0f, 0.0f, 0.0f, 0.0f}, u = g;
+                    if (f < P.Fi) {
+                        const float* pre = P.pre + (size_t)(p0 + m) * 2 * (size_t)P.Fi + f;
+                        g = *(const f32x4*)pre;
+                        u = *(const f32x4*)(pre + P.Fi);
                     }
+                    float dg[4], du[4], hw[4];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const bool is = f + q < P.F;
+                        const float s = sigmoid_fast(g[q]), h = g[q] * s * u[q], dh = w * a[q];
+                        dot += is ? a[q] * h : 0.0f;
+                        dg[q] = is ? dh * u[q] * s * (1.0f + g[q] * (1.0f - s)) : 0.0f;
+                        du[q] = is ? dh * g[q] * s : 0.0f;
+                        hw[q] = is ? w * h : 0.0f;
+                    }
+                    T* dpre = (T*)P.dpre + (size_t)(p0 + m) * 2 * (size_t)P.Fp + f;
+                    store4(dpre, dg);
+                    store4(dpre + P.Fp, du);
+                    store4((T*)P.hw + (size_t)(p0 + m) * (size_t)P.Fp + f, hw);
                 }
-                // over the 32 columns that the row's lanes hold
-                dot = lanes_reduce<32>(dot, [](float a, float b) { return a + b; });
-                if (m < count && (lane & 31) == 0)
+                dot = lanes_sum<LANES>(dot);
+                if (m < count && lane % LANES == 0)
                     P.dwp[(size_t)(nf / TL::BN * TL::WN + wn) * (size_t)(P.n * P.k) + s_slot[m]] = dot;
             } else {
                 int row = mf + m;
-                const int M = MODE == DWIN ? 2 * P.F : P.D, N = MODE == DWIN ? P.D : P.F;
+                const int M = MODE == DWIN ? 2 * P.F : P.D, N = MODE == DWIN ? P.D : P.F, c = nf + wn * W + c4;
                 if constexpr (MODE == DWIN) row = row < P.F ? row : row < P.Fp ? M : row + P.F - P.Fp;
-                if (row < M) {
-#pragma unroll
-                    for (int j = 0; j < TL::NI; ++j) {
-                        const int c = nf + n0 + j * 32;
-                        if (c < N) {
-                            const size_t at = ((size_t)e * M + row) * (size_t)N + c;
-                            if (P.splits == 1) ((T*)P.out)[at] = (T)acc[i][j][r];
-                            else P.part[(size_t)split * P.E * M * N + at] = acc[i][j][r];
-                        }
-                    }
+                const f32x4 v = four(c4);
+                if (row < M && c < N) {
+                    const size_t at = ((size_t)e * M + row) * (size_t)N + c;
+                    if (P.splits == 1) store_part((T*)P.out + at, v, N - c);
+                    else store_part(P.part + (size_t)split * P.E * M * N + at, v, N - c);
                 }
             }
         }
@@ -699,7 +727,7 @@ __global__ void __launch_bounds__(256) k_weight_parts(const float* __restrict__ 
 // ---------------------------------------------------------------------------
 
 using TileSmall = TileOf<128, 128, 2, 2, 128, 2>;
-using TileLarge = TileOf<256, 256, 2, 4, 128, 2>;
+using TileLarge = TileOf<256, 256, 4, 2, 128, 2>;
 
 // Row tiles of 256 x 256 when the experts' slots fill them, else 128 x 128.
 inline bool large_tiles(int64_t S, int E, int M, int N) { return S >= (int64_t)E * 256 && M >= 192 && N >= 192; }
@@ -766,7 +794,7 @@ void launch_tiles(const ExpertArgs& P, int M, int N, hipStream_t stream) {
         const int64_t S = P.n * P.k;
         blocks = (S / TL::BM + (S < P.E ? S : P.E)) * nt;      // no plan has more tiles
     } else {
-        blocks = (int64_t)P.E * mt * nt * P.splits;
+        blocks = (int64_t)P.E * (((int64_t)mt * nt * P.splits + XCDS - 1) / XCDS * XCDS);
     }
     if (blocks == 0) return;
     blocks = (blocks + XCDS - 1) / XCDS * XCDS;
@@ -869,10 +897,11 @@ int yabt_experts(int dtype, const void* x, int64_t ldx, int64_t n, int k, int D,
     if (n == 0) return 0;
     if (!x || !ids || !offsets || !slots || !rows || !weights || !w_in || !w_out || !y)
         return fail(-1, "yabt_experts: null pointer");
+    if (!aligned16(out_inner)) return fail(-1, "yabt_experts: out_inner must be 16-byte aligned");
     if (!workspace || workspace_bytes < yabt_experts_workspace_bytes(dtype, n, k, D, F, E))
         return fail(-2, "yabt_experts: workspace too small");
     const ExpertPlanSizes z = expert_sizes(dtype, n, k, D, F, E);
-    ExpertArgs P = {x, nullptr, w_in, w_out, weights, ids, offsets, slots, rows, ldx, 0, n, k, D, F, E, z.Fp, z.Dp};
+    ExpertArgs P = {x, nullptr, w_in, w_out, weights, ids, offsets, slots, rows, ldx, 0, n, k, D, F, E, z.Fp, z.Dp, up16(F, 4)};
     P.pre = out_inner;
     P.splits = 1;
     Carve c{(char*)align_up((size_t)workspace, 256), 0};
@@ -904,10 +933,11 @@ int yabt_experts_grad(int dtype, const void* dy, int64_t lddy, const void* x, in
     if (!offsets || !w_in || !w_out || !dw_in || !dw_out ||
         (n > 0 && (!x || !dy || !ids || !slots || !rows || !weights || !inner || !dx || !dweights)))
         return fail(-1, "yabt_experts_grad: null pointer");
+    if (!aligned16(inner)) return fail(-1, "yabt_experts_grad: inner must be 16-byte aligned");
     if (!workspace || workspace_bytes < yabt_experts_grad_workspace_bytes(dtype, n, k, D, F, E))
         return fail(-2, "yabt_experts_grad: workspace too small");
     const ExpertPlanSizes z = expert_sizes(dtype, n, k, D, F, E);
-    ExpertArgs P = {x, dy, w_in, w_out, weights, ids, offsets, slots, rows, ldx, lddy, n, k, D, F, E, z.Fp, z.Dp};
+    ExpertArgs P = {x, dy, w_in, w_out, weights, ids, offsets, slots, rows, ldx, lddy, n, k, D, F, E, z.Fp, z.Dp, up16(F, 4)};
     P.pre = const_cast<float*>(inner);
     Carve c{(char*)align_up((size_t)workspace, 256), 0};
     float* part = nullptr;

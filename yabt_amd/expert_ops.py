@@ -236,6 +236,10 @@ def _expert_args(x, plan, weights, w_in, w_out):
     return x, weights, w_in.contiguous(), w_out.contiguous(), n, k, D, F, E
 
 
+def _inner_width(F: int) -> int:
+    return 2 * ((F + 3) // 4 * 4)
+
+
 def expert_products(x: torch.Tensor, plan: ExpertPlan, weights: torch.Tensor, w_in: torch.Tensor,
                     w_out: torch.Tensor, keep_inner: bool = False):
     """y (n, D) in x's type: y_t = sum over row t's slots of weights * w_out[e]
@@ -244,8 +248,8 @@ def expert_products(x: torch.Tensor, plan: ExpertPlan, weights: torch.Tensor, w_
     w_in (E, 2 F, D) holds each expert's F gate rows, then its F rows of u;
     w_out (E, D, F); both of x's type.  weights (n, k) as ``route`` gives them.
     A row none of whose slots has an expert gets zeros.  With ``keep_inner``
-    returns (y, inner), inner (n k, 2 F) float32 being g and u by the plan's
-    places, which the backward pass takes."""
+    returns (y, inner), inner (n k, 2 G) float32, G being F up to a multiple of
+    4: g and u by the plan's places, which the backward pass takes."""
     x, weights, w_in, w_out, n, k, D, F, E = _expert_args(x, plan, weights, w_in, w_out)
     dev, dt, lib = x.device, DTYPES[x.dtype], _lib.load()
     nbytes = int(lib.yabt_experts_workspace_bytes(dt, n, k, D, F, E))
@@ -253,7 +257,7 @@ def expert_products(x: torch.Tensor, plan: ExpertPlan, weights: torch.Tensor, w_
         raise ValueError("expert_products: sizes out of range (D, F <= 2^24, n k < 2^31)")
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     y = torch.empty((n, D), dtype=x.dtype, device=dev)
-    inner = torch.empty((n * k, 2 * F), dtype=torch.float32, device=dev) if keep_inner else None
+    inner = torch.empty((n * k, _inner_width(F)), dtype=torch.float32, device=dev) if keep_inner else None
     _lib.check(lib.yabt_experts(dt, x.data_ptr(), _ld(x), n, k, D, F, E, plan.ids.data_ptr(), plan.offsets.data_ptr(),
                                 plan.slots.data_ptr(), plan.rows.data_ptr(), weights.data_ptr(), w_in.data_ptr(),
                                 w_out.data_ptr(), ws.data_ptr(), nbytes, _at(inner), y.data_ptr(), D, _stream(dev)),
@@ -271,9 +275,9 @@ def expert_products_grad(dy: torch.Tensor, x: torch.Tensor, plan: ExpertPlan, we
     dev, dt, lib = x.device, DTYPES[x.dtype], _lib.load()
     if dy.shape != x.shape or dy.device != dev:
         raise ValueError(f"dy must be like x, {tuple(x.shape)} on {dev}")
-    if tuple(inner.shape) != (n * k, 2 * F) or inner.dtype != torch.float32 or not inner.is_contiguous() \
-            or inner.device != dev:
-        raise ValueError(f"inner must be what expert_products kept, {(n * k, 2 * F)} float32 on {dev}")
+    if tuple(inner.shape) != (n * k, _inner_width(F)) or inner.dtype != torch.float32 or not inner.is_contiguous() \
+            or inner.device != dev or inner.data_ptr() % 16:
+        raise ValueError(f"inner must be what expert_products kept, {(n * k, _inner_width(F))} float32 on {dev}")
     nbytes = int(lib.yabt_experts_grad_workspace_bytes(dt, n, k, D, F, E))
     if nbytes == 0:
         raise ValueError("expert_products_grad: sizes out of range (D, F <= 2^24, n k < 2^31)")
