@@ -11,8 +11,13 @@
 // A row is held by G lanes, NV consecutive experts each.  A key and its expert
 // travel as one double: the key's 24 bits in front, the expert's number in low
 // bits that the key leaves free, so that one v_max_f64 compares both.  A lane
-// sorts its own keys once (an odd-even merge network); a round then takes the
-// largest of the G heads over DPP and the winner drops its head.
+// sorts its own keys once (an odd-even merge network).  Up to k = 8 of 8 and
+// more a lane, the lanes then merge their best 8 pairwise (the larger of one
+// list and the other reversed, sorted by three rounds of a bitonic network),
+// log2 G times; else a round takes the largest of the G heads over DPP and the
+// winner drops its head, k times.
+//
+// What bounds it is instructions, not memory: ROUTE_FIGURES
 
 #include "expert.h"
 #include "yabt_hip.h"
@@ -25,7 +30,25 @@ constexpr int SOFTMAX = 0, SIGMOID = 1;
 
 #define YABT_NEG_INF (-__builtin_inff())
 
-__device__ __forceinline__ float sigmoid(float x) { return 1.0f / (1.0f + expf(-x)); }
+// p = 1 / (1 + exp(-x)) of N values, the quotient rounded correctly: the
+// hardware's reciprocal (one unit off at most) and one Newton step give it for
+// every divisor from 1 to 2^126 (all were tried), the compiler's division for
+// what is larger, which is rare.
+template <int N>
+__device__ __forceinline__ void sigmoids(const float (&x)[N], float (&p)[N]) {
+    float d[N], most = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        d[i] = 1.0f + expf(-x[i]);
+        most = fmaxf(most, d[i]);
+        const float r = __builtin_amdgcn_rcpf(d[i]);
+        p[i] = fmaf(fmaf(-d[i], r, 1.0f), r, r);
+    }
+    if (most > 0x1p126f) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) p[i] = 1.0f / d[i];
+    }
+}
 
 // (key, e) as one double that orders by key, then by lower e; -inf carries no e.
 __device__ __forceinline__ double key_pack(float key, int e) {
@@ -59,6 +82,42 @@ __device__ __forceinline__ void sort_desc(double (&h)[NV]) {
                     }
 }
 
+// The best 8 of each aligned run of G lanes, descending, from the lanes' own
+// (descending) lists: every lane gets them.
+template <int G, int M = 1>
+__device__ __forceinline__ void merge_best(double (&h)[8]) {
+    if constexpr (M < G) {
+        double t[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) t[i] = fmax(h[i], lanes_other<M>(h[7 - i]));
+#pragma unroll
+        for (int d = 4; d >= 1; d /= 2)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if ((i & d) == 0) {
+                    const double a = t[i], b = t[i + d];
+                    t[i] = fmax(a, b);
+                    t[i + d] = fmin(a, b);
+                }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) h[i] = t[i];
+        merge_best<G, M * 2>(h);
+    }
+}
+
+// The two largest of each run of q lanes (a power of two), from their own.
+template <int G, int M = 1>
+__device__ __forceinline__ void two_largest(float& a, float& b, int q) {
+    if constexpr (M < G) {
+        if (M < q) {
+            const float a2 = lanes_other<M>(a), b2 = lanes_other<M>(b);
+            b = fmaxf(fminf(a, a2), fmaxf(b, b2));
+            a = fmaxf(a, a2);
+            two_largest<G, M * 2>(a, b, q);
+        }
+    }
+}
+
 // A lane's NV consecutive logits; -inf for those past E and for NaN.
 template <typename T, int NV>
 __device__ __forceinline__ void load_logits(const T* row, int e0, int E, float (&x)[NV]) {
@@ -79,6 +138,16 @@ __device__ __forceinline__ void load_logits(const T* row, int e0, int E, float (
         const float f = e0 + i < E ? (float)row[e0 + i] : YABT_NEG_INF;
         x[i] = f > YABT_NEG_INF ? f : YABT_NEG_INF;
     }
+}
+
+template <int NV>
+__device__ __forceinline__ void load_any(int dtype, const void* logits, size_t at, int e0, int E, float (&x)[NV]) {
+    if (dtype == DT_F32) load_logits<float, NV>((const float*)logits + at, e0, E, x);
+    else if (dtype == DT_BF16) load_logits<bf16, NV>((const bf16*)logits + at, e0, E, x);
+    else load_logits<f16, NV>((const f16*)logits + at, e0, E, x);
+}
+__device__ __forceinline__ float value_at(int dtype, const void* p, size_t i) {
+    return dtype == DT_F32 ? ((const float*)p)[i] : dtype == DT_BF16 ? (float)((const bf16*)p)[i] : (float)((const f16*)p)[i];
 }
 
 // Max and sum of exp(x - max) of a row; those of a row without open experts
@@ -103,6 +172,7 @@ struct RouteArgs {
     int E, k, scores, renormalise;
     int groups, keep, per_group, magic;     // magic: ceil(2^20 / per_group)
     float scale;
+    int dtype;
 };
 
 // The p of the chosen experts (lane j holds slots j and j + G) turned into v:
@@ -121,9 +191,9 @@ __device__ __forceinline__ void chosen_scores(const RouteArgs& A, const float (&
 #pragma unroll
         for (int s = 0; s < S; ++s) p[s] = on[s] ? expf(l[s] - m) : 0.0f;
     } else {
+        if (A.scores == SIGMOID) sigmoids<S>(l, p);
 #pragma unroll
-        for (int s = 0; s < S; ++s)
-            p[s] = !on[s] ? 0.0f : A.scores == SOFTMAX ? expf(l[s] - top) / sum : sigmoid(l[s]);
+        for (int s = 0; s < S; ++s) p[s] = !on[s] ? 0.0f : A.scores == SOFTMAX ? expf(l[s] - top) / sum : p[s];
     }
 #pragma unroll
     for (int s = 0; s < S; ++s) t += p[s];
@@ -133,12 +203,13 @@ __device__ __forceinline__ void chosen_scores(const RouteArgs& A, const float (&
     for (int s = 0; s < S; ++s) v[s] = !A.renormalise ? p[s] : t > 0.0f ? p[s] / t : 0.0f;
 }
 
-template <typename T, int G, int NV, bool GROUPS>
-__global__ void __launch_bounds__(ROUTE_NT) k_route(RouteArgs A, const T* __restrict__ logits,
+// GROUPS: 0 none, 1 each a power of two of lanes, 2 any.
+template <int G, int NV, int SCORES, int GROUPS, bool MERGE>
+__global__ void __launch_bounds__(ROUTE_NT) k_route(RouteArgs A, const void* __restrict__ logits,
                                                     const float* __restrict__ bias, int32_t* __restrict__ ids,
                                                     float* __restrict__ weights) {
-    constexpr int R = ROUTE_NT / G, S = (ROUTE_MAX_K + G - 1) / G;
-    __shared__ float s_key[GROUPS ? R : 1][GROUPS ? G * NV : 1];
+    constexpr int R = ROUTE_NT / G, S = MERGE ? 1 : (ROUTE_MAX_K + G - 1) / G;
+    __shared__ float s_key[GROUPS == 2 ? R : 1][GROUPS == 2 ? G * NV : 1];
     __shared__ float s_score[GROUPS ? R : 1][GROUPS ? ROUTE_MAX_GROUPS : 1];
     __shared__ int s_stay[GROUPS ? R : 1][GROUPS ? ROUTE_MAX_GROUPS : 1];
     const int lane = threadIdx.x % G, sub = threadIdx.x / G, e0 = lane * NV;
@@ -148,31 +219,44 @@ __global__ void __launch_bounds__(ROUTE_NT) k_route(RouteArgs A, const T* __rest
     for (int64_t r0 = (int64_t)blockIdx.x * R; r0 < A.n; r0 += (int64_t)gridDim.x * R) {
         // rows past the end are walked as the last one, and not written
         const int64_t r = min(r0 + sub, A.n - 1);
-        const T* row = logits + (size_t)r * (size_t)A.ldl;
+        const size_t row = (size_t)r * (size_t)A.ldl;
         float x[NV], top = 0.0f, sum = 1.0f;
-        load_logits<T, NV>(row, e0, A.E, x);
-        if (A.scores == SOFTMAX && !A.renormalise) softmax_stats<G, NV>(x, &top, &sum);
+        load_any<NV>(A.dtype, logits, row, e0, A.E, x);
+        if (SCORES == SOFTMAX && !A.renormalise) softmax_stats<G, NV>(x, &top, &sum);
         float key[NV];
+        if constexpr (SCORES == SIGMOID) sigmoids<NV>(x, key);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const float p = A.scores == SOFTMAX ? x[i] : sigmoid(x[i]);
-            const float q = p + bv[i];
+            const float q = (SCORES == SOFTMAX ? x[i] : key[i]) + bv[i];
             key[i] = x[i] > YABT_NEG_INF && q > YABT_NEG_INF ? q : YABT_NEG_INF;
         }
-        if constexpr (GROUPS) {
+        if constexpr (GROUPS != 0) {
+            if constexpr (GROUPS == 1) {
+                float a = YABT_NEG_INF, b = YABT_NEG_INF;     // the lane's, then its group's two largest keys
 #pragma unroll
-            for (int i = 0; i < NV; ++i) s_key[sub][e0 + i] = key[i];
-            wave_sync_lds();
-            for (int g = lane; g < A.groups; g += G) {
-                float a = YABT_NEG_INF, b = YABT_NEG_INF;     // the group's two largest keys
-                int at = g % A.per_group;                     // lanes start apart: other banks
-                for (int i = 0; i < A.per_group; ++i) {
-                    const float q = s_key[sub][g * A.per_group + at];
-                    b = fmaxf(b, fminf(a, q));
-                    a = fmaxf(a, q);
-                    at = at + 1 == A.per_group ? 0 : at + 1;
+                for (int i = 0; i < NV; ++i) {
+                    b = fmaxf(b, fminf(a, key[i]));
+                    a = fmaxf(a, key[i]);
                 }
-                s_score[sub][g] = A.scores == SIGMOID && b > YABT_NEG_INF ? a + b : a;
+                const int q = A.per_group / NV;
+                two_largest<G>(a, b, q);
+                // lanes past the experts are in no group
+                if (e0 < A.E) s_score[sub][lane / q] = SCORES == SIGMOID && b > YABT_NEG_INF ? a + b : a;
+            } else {
+#pragma unroll
+                for (int i = 0; i < NV; ++i) s_key[sub][e0 + i] = key[i];
+                wave_sync_lds();
+                for (int g = lane; g < A.groups; g += G) {
+                    float a = YABT_NEG_INF, b = YABT_NEG_INF;
+                    int at = g % A.per_group;                 // lanes start apart: other banks
+                    for (int i = 0; i < A.per_group; ++i) {
+                        const float q = s_key[sub][g * A.per_group + at];
+                        b = fmaxf(b, fminf(a, q));
+                        a = fmaxf(a, q);
+                        at = at + 1 == A.per_group ? 0 : at + 1;
+                    }
+                    s_score[sub][g] = SCORES == SIGMOID && b > YABT_NEG_INF ? a + b : a;
+                }
             }
             wave_sync_lds();
             // a group stays if fewer than `keep` are before it
@@ -186,10 +270,16 @@ __global__ void __launch_bounds__(ROUTE_NT) k_route(RouteArgs A, const T* __rest
                 s_stay[sub][g] = before < A.keep;
             }
             wave_sync_lds();
+            if constexpr (GROUPS == 1) {
+                const bool stay = s_stay[sub][min(lane / (A.per_group / NV), A.groups - 1)];
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const int g = min((int)(((uint32_t)(e0 + i) * (uint32_t)A.magic) >> 20), A.groups - 1);
-                if (!s_stay[sub][g]) key[i] = YABT_NEG_INF;
+                for (int i = 0; i < NV; ++i) key[i] = stay ? key[i] : YABT_NEG_INF;
+            } else {
+#pragma unroll
+                for (int i = 0; i < NV; ++i) {
+                    const int g = min((int)(((uint32_t)(e0 + i) * (uint32_t)A.magic) >> 20), A.groups - 1);
+                    if (!s_stay[sub][g]) key[i] = YABT_NEG_INF;
+                }
             }
             wave_sync_lds();
         }
@@ -198,18 +288,27 @@ __global__ void __launch_bounds__(ROUTE_NT) k_route(RouteArgs A, const T* __rest
         for (int i = 0; i < NV; ++i) h[i] = key_pack(key[i], e0 + i);
         sort_desc<NV>(h);
         int mine[S];
+        if constexpr (MERGE) {
+            double b8[8];
 #pragma unroll
-        for (int s = 0; s < S; ++s) mine[s] = -1;
-        for (int j = 0; j < A.k; ++j) {
-            const double m = lanes_reduce<G>(h[0], [](double a, double b) { return fmax(a, b); });
-            const int e = m > -__builtin_inf() ? key_expert(m) : -1;
+            for (int i = 0; i < 8; ++i) b8[i] = h[i];
+            merge_best<G>(b8);
+            double m = b8[0];
 #pragma unroll
-            for (int s = 0; s < S; ++s)
-                if (j == s * G + lane) mine[s] = e;
-            if (h[0] == m) {
+            for (int i = 1; i < 8; ++i) m = lane == i ? b8[i] : m;
+            mine[0] = lane < A.k && m > -__builtin_inf() ? key_expert(m) : -1;
+        } else {
 #pragma unroll
-                for (int i = 0; i + 1 < NV; ++i) h[i] = h[i + 1];
-                h[NV - 1] = -__builtin_inf();
+            for (int s = 0; s < S; ++s) mine[s] = -1;
+            for (int j = 0; j < A.k; ++j) {
+                const double m = lanes_reduce<G>(h[0], [](double a, double b) { return fmax(a, b); });
+                const int e = m > -__builtin_inf() ? key_expert(m) : -1;
+#pragma unroll
+                for (int s = 0; s < S; ++s)
+                    if (j == s * G + lane) mine[s] = e;
+                const bool won = h[0] == m;
+#pragma unroll
+                for (int i = 0; i < NV; ++i) h[i] = won ? i + 1 < NV ? h[i + 1] : -__builtin_inf() : h[i];
             }
         }
         float l[S], p[S], v[S], total;
@@ -217,7 +316,7 @@ __global__ void __launch_bounds__(ROUTE_NT) k_route(RouteArgs A, const T* __rest
 #pragma unroll
         for (int s = 0; s < S; ++s) {
             on[s] = mine[s] >= 0;
-            l[s] = on[s] ? (float)row[mine[s]] : 0.0f;
+            l[s] = on[s] ? value_at(A.dtype, logits, row + mine[s]) : 0.0f;
         }
         chosen_scores<G, S>(A, l, on, top, sum, p, v, &total);
         if (r0 + sub < A.n) {
@@ -466,14 +565,27 @@ void route_shape(int E, const F& f) {
 #undef YABT_SHAPE
 }
 
-template <typename T>
-void run_route(const RouteArgs& A, const T* logits, const float* bias, int32_t* ids, float* weights,
+template <int SCORES>
+void run_route(const RouteArgs& A, const void* logits, const float* bias, int32_t* ids, float* weights,
                hipStream_t stream) {
     route_shape(A.E, [&](auto g, auto nv) {
         constexpr int G = decltype(g)::value, NV = decltype(nv)::value;
         const int grid = launch_grid(A.n, ROUTE_NT / G, 4096);
-        if (A.groups > 1) k_route<T, G, NV, true><<<grid, ROUTE_NT, 0, stream>>>(A, logits, bias, ids, weights);
-        else k_route<T, G, NV, false><<<grid, ROUTE_NT, 0, stream>>>(A, logits, bias, ids, weights);
+        auto go = [&](auto groups, auto merge) {
+            k_route<G, NV, SCORES, decltype(groups)::value, decltype(merge)::value>
+                <<<grid, ROUTE_NT, 0, stream>>>(A, logits, bias, ids, weights);
+        };
+        const int q = A.per_group % NV == 0 ? A.per_group / NV : 0;
+        const int kind = A.groups == 1 ? 0 : q >= 1 && q <= G && (q & (q - 1)) == 0 ? 1 : 2;
+        auto by_groups = [&](auto merge) {
+            if (kind == 0) go(std::integral_constant<int, 0>(), merge);
+            else if (kind == 1) go(std::integral_constant<int, 1>(), merge);
+            else go(std::integral_constant<int, 2>(), merge);
+        };
+        if constexpr (NV >= 8) {
+            if (A.k <= 8) return by_groups(std::true_type());
+        }
+        by_groups(std::false_type());
     });
 }
 
@@ -504,12 +616,11 @@ int yabt_route(int dtype, const void* logits, int64_t ldl, int64_t n, int E, int
         return fail(-1, "yabt_route: groups (at most 64) divide E, 1 <= keep_groups <= groups");
     if (n == 0) return 0;
     if (!logits || !out_ids || !out_weights) return fail(-1, "yabt_route: null pointer");
-    RouteArgs A = {ldl, n, E, k, scores, renormalise, keep_groups < groups ? groups : 1, keep_groups, E / groups, 0, scale};
+    RouteArgs A = {ldl, n, E, k, scores, renormalise, keep_groups < groups ? groups : 1, keep_groups, E / groups, 0, scale, dtype};
     A.magic = ((1 << 20) + A.per_group - 1) / A.per_group;
     hipStream_t st = (hipStream_t)stream;
-    if (dtype == DT_F32) run_route<float>(A, (const float*)logits, bias, out_ids, out_weights, st);
-    else if (dtype == DT_BF16) run_route<bf16>(A, (const bf16*)logits, bias, out_ids, out_weights, st);
-    else run_route<f16>(A, (const f16*)logits, bias, out_ids, out_weights, st);
+    if (scores == SOFTMAX) run_route<SOFTMAX>(A, logits, bias, out_ids, out_weights, st);
+    else run_route<SIGMOID>(A, logits, bias, out_ids, out_weights, st);
     return launch_status("yabt_route");
 }
 
@@ -524,7 +635,7 @@ int yabt_route_grad(int dtype, const float* dweights, int64_t lddw, const void* 
         return fail(-1, "yabt_route_grad: scores is 0 (softmax) or 1 (sigmoid)");
     if (n == 0) return 0;
     if (!dweights || !logits || !ids || !out_dlogits) return fail(-1, "yabt_route_grad: null pointer");
-    RouteArgs A = {ldl, n, E, k, scores, renormalise, 1, 1, E, 0, scale};
+    RouteArgs A = {ldl, n, E, k, scores, renormalise, 1, 1, E, 0, scale, dtype};
     hipStream_t st = (hipStream_t)stream;
     if (dtype == DT_F32)
         run_route_grad<float>(A, dweights, lddw, (const float*)logits, ids, (float*)out_dlogits, lddl, st);

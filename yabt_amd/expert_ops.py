@@ -31,7 +31,9 @@ MAX_EXPERTS, MAX_K, MAX_GROUPS = 1024, 32, 64
 
 
 def _stream(dev: torch.device) -> int:
-    return torch.cuda.current_stream(dev).cuda_stream
+    """The current stream's handle; ``torch.cuda.current_stream`` takes 2 us to
+    make an object of it, which a call for one row would notice."""
+    return torch._C._cuda_getCurrentRawStream(dev.index)
 
 
 def _matrix(t: torch.Tensor, what: str, dtype: torch.dtype | None = None) -> torch.Tensor:
@@ -77,8 +79,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
         raise ValueError("layer_norm needs at least one column")
     w, b = _vector(weight, D, dev, "weight"), _vector(bias, D, dev, "bias")
     y = torch.empty((n, D), dtype=x.dtype, device=dev)
-    stats = torch.empty((2, n), dtype=torch.float32, device=dev)
-    mean, rstd = stats[0], stats[1]
+    mean, rstd = torch.empty((2, n), dtype=torch.float32, device=dev).unbind()
     _lib.check(_lib.load().yabt_layer_norm(DTYPES[x.dtype], x.data_ptr(), _ld(x), n, D, _at(w), _at(b), float(eps),
                                            y.data_ptr(), D, mean.data_ptr(), rstd.data_ptr(), _stream(dev)),
                "yabt_layer_norm")
@@ -101,8 +102,7 @@ def layer_norm_grad(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd:
     nbytes = int(lib.yabt_layer_norm_grad_workspace_bytes(n, D))
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     dx = torch.empty((n, D), dtype=x.dtype, device=dev)
-    grads = torch.empty((2, D), dtype=torch.float32, device=dev)
-    dw, db = grads[0], grads[1]
+    dw, db = torch.empty((2, D), dtype=torch.float32, device=dev).unbind()
     _lib.check(lib.yabt_layer_norm_grad(DTYPES[x.dtype], dy.data_ptr(), _ld(dy), x.data_ptr(), _ld(x), n, D, _at(w),
                                         mu.data_ptr(), rs.data_ptr(), ws.data_ptr(), nbytes, dx.data_ptr(), D,
                                         dw.data_ptr(), db.data_ptr(), _stream(dev)), "yabt_layer_norm_grad")
@@ -198,16 +198,15 @@ def expert_plan(ids: torch.Tensor, experts: int) -> ExpertPlan:
     """The plan of ids (n, k); ids outside [0, experts) belong to no expert."""
     ids = _ids(ids)
     (n, k), dev = ids.shape, ids.device
-    lib = _lib.load()
-    nbytes = int(lib.yabt_expert_plan_workspace_bytes(n, k, int(experts)))
+    lib, experts = _lib.load(), int(experts)
+    nbytes = lib.yabt_expert_plan_workspace_bytes(n, k, experts)
     if nbytes == 0:
         raise ValueError(f"expert_plan takes 1 to {MAX_EXPERTS} experts, k >= 1 and n k < 2^31; got {experts} "
                          f"experts, ids {(n, k)}")
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    offsets = torch.empty(experts + 1, dtype=torch.int32, device=dev)
-    places = torch.empty((2, n * k), dtype=torch.int32, device=dev)
-    slots, rows = places[0], places[1]
-    _lib.check(lib.yabt_expert_plan(ids.data_ptr(), n, k, int(experts), ws.data_ptr(), nbytes, offsets.data_ptr(),
+    # one allocation: the plan's three arrays and the call's workspace behind them
+    sizes = (experts + 1, n * k, n * k, nbytes // 4)
+    offsets, slots, rows, ws = torch.empty(sum(sizes), dtype=torch.int32, device=dev).split_with_sizes(sizes)
+    _lib.check(lib.yabt_expert_plan(ids.data_ptr(), n, k, experts, ws.data_ptr(), nbytes, offsets.data_ptr(),
                                     slots.data_ptr(), rows.data_ptr(), _stream(dev)), "yabt_expert_plan")
     return ExpertPlan(ids, offsets, slots, rows)
 
