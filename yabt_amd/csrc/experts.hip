@@ -654,6 +654,180 @@ __global__ void __launch_bounds__(TL::NT) k_experts(ExpertArgs P, int ntiles, in
     }
 }
 
+// ---------------------------------------------------------------------------
+// Few rows: the products are bound by the weights' bytes, each read once, and
+// by the launches.  Weights and slots go straight from memory into the matrix
+// instructions' operands: a lane fetches 32 bytes in a row of one weight row,
+// two instructions' worth, 16 weight rows and 16 slots a wave.  Widths and
+// addresses are free.
+//   k_inner_few   h: a block has 16 gate rows and their 16 rows of u of one
+//                 expert; its waves share the summed dimension, 128 bytes a row
+//                 in turn, and their sums meet in LDS
+//   k_answer_few  y: a block has 16 columns of all rows; its waves share the
+//                 experts in use, and the weighted answers of a row's slots
+//                 are added up in LDS
+// ---------------------------------------------------------------------------
+
+template <typename T>
+__device__ __forceinline__ f32x4 mma16(u32x4 a, u32x4 b, f32x4 c) {
+    if constexpr (sizeof(T) == 4) {
+        const f32x4 fa = __builtin_bit_cast(f32x4, a), fb = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) c = __builtin_amdgcn_mfma_f32_16x16x4f32(fa[q], fb[q], c, 0, 0, 0);
+        return c;
+    } else if constexpr (std::is_same_v<T, bf16>) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c,
+                                                      0, 0, 0);
+    } else {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0,
+                                                     0, 0);
+    }
+}
+
+// 16 bytes of a row from value k on, the row's K values alone, zeros after them.
+template <typename T>
+__device__ __forceinline__ u32x4 row_piece(const T* row, int k, int K) {
+    typedef T VT __attribute__((ext_vector_type(VEC<T>)));
+    if (k + VEC<T> <= K) return *reinterpret_cast<const u32x4_any*>(row + k);
+    VT t = {};
+#pragma unroll
+    for (int j = 0; j < VEC<T>; ++j)
+        if (k + j < K) t[j] = row[k + j];
+    return __builtin_bit_cast(u32x4, t);
+}
+
+// The j-th of the experts that have slots, or -1.
+__device__ __forceinline__ int expert_in_use(const int32_t* off, int E, int j) {
+    const int lane = threadIdx.x & 63;
+    for (int e0 = 0; e0 < E; e0 += 64) {
+        const int e = e0 + lane;
+        const bool has = e < E && off[e + 1] > off[e];
+        const uint64_t all = __ballot(has);
+        const int before = __popcll(all & ((1ull << lane) - 1ull));
+        const uint64_t hit = __ballot(has && before == j);
+        if (hit) return e0 + __ffsll((unsigned long long)hit) - 1;
+        j -= __popcll(all);
+    }
+    return -1;
+}
+
+constexpr int FEW_NT = 256, FEW_W = FEW_NT / 64;
+constexpr int FEW_AHEAD = 4;                     // 128-byte pieces of a row under way in a wave
+constexpr int FEW_SLOTS = 512;                   // slots whose answers a block keeps in LDS
+
+// acc[m] += M matrices' 16 rows w[m] times the 16 slots' x, from piece `from` on, every `by`-th.
+template <typename T, int M>
+__device__ __forceinline__ void few_products(const T* const (&w)[M], const T* x, int K, int from, int by, f32x4 (&acc)[M]) {
+    constexpr int CH = VEC<T>, STEP = 8 * CH;    // values in 128 bytes
+    const int q = (threadIdx.x & 63) >> 4;
+    for (int k0 = from * STEP; k0 < K; k0 += by * FEW_AHEAD * STEP) {
+        u32x4 a[FEW_AHEAD][M][2], v[FEW_AHEAD][2];
+#pragma unroll
+        for (int s = 0; s < FEW_AHEAD; ++s)
+#pragma unroll
+            for (int o = 0; o < 2; ++o) {
+                const int k = k0 + s * by * STEP + (2 * q + o) * CH;
+#pragma unroll
+                for (int m = 0; m < M; ++m) a[s][m][o] = row_piece<T>(w[m], k, K);
+                v[s][o] = row_piece<T>(x, k, K);
+            }
+#pragma unroll
+        for (int s = 0; s < FEW_AHEAD; ++s)
+#pragma unroll
+            for (int o = 0; o < 2; ++o)
+#pragma unroll
+                for (int m = 0; m < M; ++m) acc[m] = mma16<T>(a[s][m][o], v[s][o], acc[m]);
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(FEW_NT) k_inner_few(ExpertArgs P) {
+    __shared__ f32x4 s_sum[FEW_W][2][64];
+    const int wave = threadIdx.x / 64, lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+    const int e = expert_in_use(P.offsets, P.E, blockIdx.y);
+    if (e < 0) return;
+    const int off = P.offsets[e], cnt = P.offsets[e + 1] - off, first = blockIdx.x * 16;
+    const T* const gate = (const T*)P.w_in + ((size_t)e * 2 * P.F + min(first + r, P.F - 1)) * (size_t)P.D;
+    const T* const w[2] = {gate, gate + (size_t)P.F * (size_t)P.D};
+    for (int p0 = 0; p0 < cnt; p0 += 16) {
+        const T* x = (const T*)P.x + (size_t)P.rows[off + min(p0 + r, cnt - 1)] * (size_t)P.ldx;
+        f32x4 acc[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+        few_products<T, 2>(w, x, P.D, wave, FEW_W, acc);
+        __syncthreads();                         // the sums of the slots before have been read
+        s_sum[wave][0][lane] = acc[0];
+        s_sum[wave][1][lane] = acc[1];
+        __syncthreads();
+        // a lane has slot r and f = first + 4 q .. + 3
+        const int at = p0 + r, f = first + 4 * q;
+        if (wave == 0 && at < cnt) {
+            f32x4 g = s_sum[0][0][lane], u = s_sum[0][1][lane];
+#pragma unroll
+            for (int o = 1; o < FEW_W; ++o) {
+                g += s_sum[o][0][lane];
+                u += s_sum[o][1][lane];
+            }
+            const size_t p = (size_t)(off + at);
+            if (f < P.Fp) {
+                float h[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) h[i] = f + i < P.F ? g[i] * sigmoid_fast(g[i]) * u[i] : 0.0f;
+                store4((T*)P.h + p * (size_t)P.Fp + f, h);
+            }
+            if (P.pre && f < P.Fi) {
+                float* pre = P.pre + p * 2 * (size_t)P.Fi + f;
+                *(f32x4*)pre = g;
+                *(f32x4*)(pre + P.Fi) = u;
+            }
+        }
+    }
+}
+
+constexpr int ANSWER_NT = 512;
+
+template <typename T>
+__global__ void __launch_bounds__(ANSWER_NT) k_answer_few(ExpertArgs P, T* __restrict__ y, int64_t ldy) {
+    __shared__ f32x4 s_z[FEW_SLOTS][4];          // the slots' weighted answers in the block's 16 columns
+    __shared__ int s_use[FEW_SLOTS];             // the experts in use: no more than slots
+    __shared__ int s_count;
+    const int wave = threadIdx.x / 64, lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+    const int first = blockIdx.x * 16;
+    if (wave == 0) {
+        int count = 0;
+        for (int e0 = 0; e0 < P.E; e0 += 64) {
+            const int e = e0 + lane;
+            const bool has = e < P.E && P.offsets[e + 1] > P.offsets[e];
+            const uint64_t all = __ballot(has);
+            if (has) s_use[count + __popcll(all & ((1ull << lane) - 1ull))] = e;
+            count += __popcll(all);
+        }
+        if (lane == 0) s_count = count;
+    }
+    __syncthreads();
+    for (int i = wave; i < s_count; i += ANSWER_NT / 64) {
+        const int e = s_use[i], off = P.offsets[e], cnt = P.offsets[e + 1] - off;
+        const T* const w[1] = {(const T*)P.w_out + ((size_t)e * P.D + min(first + r, P.D - 1)) * (size_t)P.F};
+        for (int p0 = 0; p0 < cnt; p0 += 16) {
+            const int p = off + min(p0 + r, cnt - 1);
+            f32x4 acc[1] = {{0.0f, 0.0f, 0.0f, 0.0f}};
+            few_products<T, 1>(w, (const T*)P.h + (size_t)p * (size_t)P.Fp, P.F, 0, 1, acc);
+            if (p0 + r < cnt) {
+                const int slot = P.slots[p];
+                s_z[slot][q] = acc[0] * P.weights[slot];
+            }
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < (int)P.n * 16; i += ANSWER_NT) {
+        const int t = i >> 4, c = i & 15;
+        float s = 0.0f;
+        for (int j = 0; j < P.k; ++j) {
+            const int e = P.ids[t * P.k + j];
+            if (e >= 0 && e < P.E) s += ((const float*)s_z[t * P.k + j])[c];
+        }
+        if (first + c < P.D) y[(size_t)t * (size_t)ldy + first + c] = (T)s;
+    }
+}
+
 // Rows' slots added up: out[t] = sum_j z[t k + j] over the slots that have an
 // expert, 4 columns a thread; and (dwp) the routing weights' gradient.
 template <typename T>
@@ -812,11 +986,34 @@ void run_tiles(const ExpertArgs& P, bool large, bool dma, int M, int N, hipStrea
     }
 }
 
+// The kernels for few rows by the slots an expert in use has on average.  They
+// pass over the weights once per 16 slots, the tiles once per 128 with a tile's
+// whole arithmetic, which fp32 does at a sixteenth of the rate.  h, few and
+// tiles: 2048 -> 1024 of 32 experts, fp16, 6 slots each 62 and 66 us, 16 each
+// 102 and 72; 1024 -> 512 of 64, bf16, one row's 6 slots 6 and 12 us, 192 slots
+// 20 and 21; 500 -> 101 of 4, fp32, 25 each 13 and 45 us.
+inline bool few_inner(int64_t S, int E, int bytes) {
+    const int64_t used = S < E ? S : E;
+    return S <= used * (bytes == 4 ? 32 : 8);
+}
+// y, few and tiles with k_combine: one row's 6 slots 6.6 and 12.7 us, two rows' 12
+// slots 11 and 14, 8 rows' 48 slots 26 and 18 (a wave has several experts in turn).
+inline bool few_answer(int64_t S, int E, int bytes) {
+    return few_inner(S, E, bytes) && S <= FEW_SLOTS && (S < E ? S : E) <= 16;
+}
+
 template <typename T>
 int run_experts(ExpertArgs P, const ExpertPlanSizes& z, T* y, int64_t ldy, bool dma, hipStream_t stream) {
     P.out = y;
     P.ldo = ldy;
-    run_tiles<T, IN>(P, z.large, dma, 0, P.F, stream);
+    if (few_inner(z.S, P.E, sizeof(T)))
+        k_inner_few<T><<<dim3((unsigned)((P.F + 15) / 16), (unsigned)(z.S < P.E ? z.S : P.E)), FEW_NT, 0, stream>>>(P);
+    else
+        run_tiles<T, IN>(P, z.large, dma, 0, P.F, stream);
+    if (few_answer(z.S, P.E, sizeof(T))) {
+        k_answer_few<T><<<(unsigned)((P.D + 15) / 16), ANSWER_NT, 0, stream>>>(P, y, ldy);
+        return launch_status("yabt_experts");
+    }
     run_tiles<T, OUT>(P, z.large, dma, 0, P.D, stream);
     if (P.k > 1)
         k_combine<T><<<launch_grid(P.n * (z.Dp / 4), 256, 8192), 256, 0, stream>>>(P, y, ldy, 0, nullptr);

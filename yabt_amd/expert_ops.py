@@ -214,25 +214,25 @@ def expert_plan(ids: torch.Tensor, experts: int) -> ExpertPlan:
 def _expert_args(x, plan, weights, w_in, w_out):
     """Checked sizes and tensors of the products: (x, weights, w_in, w_out, n, k, D, F, E)."""
     x = _matrix(x, "x")
-    (n, D), dev = x.shape, x.device
-    if w_in.dim() != 3 or w_out.dim() != 3:
-        raise ValueError(f"w_in and w_out must be (E, 2 F, D) and (E, D, F), got {tuple(w_in.shape)}, "
-                         f"{tuple(w_out.shape)}")
-    E, F = w_out.shape[0], w_out.shape[2]
-    if D < 1 or F < 1 or tuple(w_in.shape) != (E, 2 * F, D) or w_out.shape[1] != D:
+    (n, D), dev, dt = x.shape, x.device, x.dtype
+    if w_in.dim() != 3 or w_out.dim() != 3 or w_in.shape[0] != w_out.shape[0] or w_out.shape[1] != D or D < 1 \
+            or w_in.shape[2] != D or w_out.shape[2] < 1 or w_in.shape[1] != 2 * w_out.shape[2]:
         raise ValueError(f"w_in and w_out must be (E, 2 F, {D}) and (E, {D}, F), got {tuple(w_in.shape)}, "
                          f"{tuple(w_out.shape)}")
-    if w_in.dtype != x.dtype or w_out.dtype != x.dtype:
-        raise ValueError(f"x, w_in and w_out must have one type, got {x.dtype}, {w_in.dtype}, {w_out.dtype}")
-    if plan.experts != E or plan.ids.shape[0] != n:
-        raise ValueError(f"the plan is for {plan.experts} experts and {plan.ids.shape[0]} rows, not {E} and {n}")
-    k = plan.ids.shape[1]
-    if tuple(weights.shape) != (n, k):
+    E, _, F = w_out.shape
+    if w_in.dtype != dt or w_out.dtype != dt:
+        raise ValueError(f"x, w_in and w_out must have one type, got {dt}, {w_in.dtype}, {w_out.dtype}")
+    ids = plan.ids
+    k = ids.shape[1]
+    if plan.offsets.shape[0] != E + 1 or ids.shape[0] != n:
+        raise ValueError(f"the plan is for {plan.experts} experts and {ids.shape[0]} rows, not {E} and {n}")
+    if weights.shape != ids.shape:
         raise ValueError(f"weights must have shape {(n, k)}, got {tuple(weights.shape)}")
-    if any(t.device != dev for t in (w_in, w_out, weights, plan.ids)):
+    if w_in.device != dev or w_out.device != dev or weights.device != dev or ids.device != dev:
         raise ValueError(f"all tensors must be on {dev}")
-    weights = weights if weights.dtype == torch.float32 and weights.is_contiguous() else weights.float().contiguous()
-    return x, weights, w_in.contiguous(), w_out.contiguous(), n, k, D, F, E
+    if weights.dtype != torch.float32:
+        weights = weights.float()
+    return x, weights.contiguous(), w_in.contiguous(), w_out.contiguous(), n, k, D, F, E
 
 
 def _inner_width(F: int) -> int:
@@ -251,7 +251,7 @@ def expert_products(x: torch.Tensor, plan: ExpertPlan, weights: torch.Tensor, w_
     4: g and u by the plan's places, which the backward pass takes."""
     x, weights, w_in, w_out, n, k, D, F, E = _expert_args(x, plan, weights, w_in, w_out)
     dev, dt, lib = x.device, DTYPES[x.dtype], _lib.load()
-    nbytes = int(lib.yabt_experts_workspace_bytes(dt, n, k, D, F, E))
+    nbytes = lib.yabt_experts_workspace_bytes(dt, n, k, D, F, E)
     if nbytes == 0:
         raise ValueError("expert_products: sizes out of range (D, F <= 2^24, n k < 2^31)")
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
