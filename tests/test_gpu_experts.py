@@ -85,6 +85,22 @@ def test_large_tiles(n, D, F, E, k, dt):
     check(inputs(n, D, F, E, k, dt, n))
 
 
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16], ids=name)
+@pytest.mark.parametrize("n,D,F,E,k", [(7000, 400, 520, 16, 1), (6001, 397, 515, 8, 2), (9000, 1032, 392, 16, 1)])
+def test_large_tiles_of_every_product(n, D, F, E, k, dt):
+    """Enough tiles and sums long enough that 256 x 256 tiles make all six products or some of them."""
+    check(inputs(n, D, F, E, k, dt, n))
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=name)
+@pytest.mark.parametrize("n,D,F,E,k", [(1, 300, 70, 64, 6), (2, 129, 33, 20, 8), (9, 64, 48, 3, 1), (60, 96, 130, 2, 1),
+                                       (250, 40, 33, 100, 2), (120, 33, 20, 4, 1), (500, 24, 17, 200, 1)])
+def test_few_rows(n, D, F, E, k, dt):
+    """The kernels for few rows: one, several and more than 16 slots an expert, more experts than waves."""
+    check(inputs(n, D, F, E, k, dt, n + E), grad=False)
+    check(inputs(n, D, F, E, k, dt, n + E, unused=0.5))
+
+
 @pytest.mark.parametrize("dt", TYPES, ids=name)
 def test_uneven_experts(dt):
     """One expert with most rows, others with a few or none; an expert that no id names."""

@@ -12,7 +12,7 @@
 // and in what is done with the sums:
 //
 //   IN     [g u] of the slots, the tile's columns gate and up alternately by 32, then h = silu(g) u
-//   OUT    z = w (W_out h), by slot in fp32 (added up by k_combine), or y itself when k = 1
+//   OUT    z = w (W_out h), by slot in fp32 (added up by k_finish), or y itself when k = 1
 //   DH     a, then dg, du, w h and dw in part
 //   DX     W_in^T [dg du] by slot in fp32, or dx itself when k = 1
 //   DWIN, DWOUT   the weights' gradients, summed over an expert's slots
@@ -73,10 +73,15 @@ struct ExpertArgs {
     float* pre;                       // (S, 2 Fi): g from 0, u from Fi, or NULL
     float* z;                         // (S, Dp)
     float* dwp;                       // (parts, S): dw by column tile
-    void* out;                        // y or dx (k = 1), dW_in or dW_out
+    void* out;                        // y or dx
     int64_t ldo;
-    float* part;                      // (splits, E, M, N): the weights' gradients in part
-    int splits;
+    void* dw_in;                      // (E, 2 F, D)
+    void* dw_out;                     // (E, D, F)
+    float* part_in;                   // (splits_in, E, 2 F, D): dw_in in part, where splits_in > 1
+    float* part_out;                  // (splits_out, E, D, F)
+    int splits_in, splits_out;
+    float* dweights;                  // (n, k), or NULL: not wanted
+    int parts;                        // of dwp
 };
 
 // 16 zero bytes for pieces past the end of the summed dimension.
@@ -97,11 +102,14 @@ struct TileOf {
 // Where piece c (16 bytes) of row r of a tile in LDS is kept: c ^ spread(r), so
 // that the lanes a read serves at once (16 of 16 bytes, 32 of 8, 64 of 4: 256
 // bytes, all banks) meet different banks.  ALONG: a row is STEP bytes of one
-// row of the operand; across: a row is one place of the summed dimension.
-template <typename T, bool ACROSS, int STEP>
+// row of the operand; across: a row is one place of the summed dimension, W
+// values of the operand's rows.
+template <typename T, bool ACROSS, int W, int STEP>
 __device__ __forceinline__ constexpr int spread(int r) {
     if (!ACROSS) return STEP == 128 ? r >> 1 & 7 : r >> 2 & 3;
-    return sizeof(T) == 4 ? (r >> 2 & 1) << 3 : (r & 3) << 2;
+    constexpr int bytes = W * (int)sizeof(T);
+    static_assert(!ACROSS || bytes >= 256 || (bytes == 128 && sizeof(T) == 2), "the places stay in their row");
+    return sizeof(T) == 4 ? (r >> 2 & 1) << 3 : bytes == 128 ? (r >> 1 & 1) << 2 : (r & 3) << 2;
 }
 
 // silu by the hardware's exp2 and reciprocal (about one unit each).
@@ -227,19 +235,19 @@ struct Frag {
 #pragma unroll
             for (int ks = 0; ks < KEEP; ++ks)
                 at[ks] = (uint32_t)((first + (l & 31)) * STEP +
-                                    (((ks * 2 + (l >> 5)) ^ spread<T, ACROSS, STEP>(l & 31)) << 4));
+                                    (((ks * 2 + (l >> 5)) ^ spread<T, ACROSS, W, STEP>(l & 31)) << 4));
         } else if constexpr (sizeof(T) == 4) {
             // four rows of k, a value of each; blocks of 32 columns are 128 bytes apart
             const int r = (l >> 5) * 4;
 #pragma unroll
             for (int i = 0; i < 2; ++i)
-                at[i] = (uint32_t)(r * W * 4 + first * 4 + ((i * 128 + (l & 31) * 4) ^ spread<T, ACROSS, STEP>(r) << 4));
+                at[i] = (uint32_t)(r * W * 4 + ((first * 4 + i * 128 + (l & 31) * 4) ^ spread<T, ACROSS, W, STEP>(r) << 4));
         } else {
             // of four rows of k this lane fetches four values of one; blocks are 64 bytes apart
             const int r = (l & 15) >> 2, col = ((l >> 4) & 1) * 16 + (l & 3) * 4;
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                at[i] = (uint32_t)(((l >> 5) * 8 + r) * W * 2 + ((first * 2 + i * 64 + col * 2) ^ spread<T, ACROSS, STEP>(r) << 4));
+                at[i] = (uint32_t)(((l >> 5) * 8 + r) * W * 2 + ((first * 2 + i * 64 + col * 2) ^ spread<T, ACROSS, W, STEP>(r) << 4));
         }
     }
     __device__ __forceinline__ u32x4 get(lds_char* tile, int i, int ks) const {
@@ -275,7 +283,7 @@ struct Loader {
     __device__ __forceinline__ static int row_of(int i) { return (i * NT + (int)threadIdx.x) / PER_ROW; }
     __device__ __forceinline__ static int piece_of(int i) {
         const int c = (i * NT + (int)threadIdx.x) % PER_ROW, r = row_of(i);
-        return c ^ spread<T, ACROSS, STEP>(r);
+        return c ^ spread<T, ACROSS, W, STEP>(r);
     }
 
     // p0: the tile's first slot place (along), or the split's (across); count:
@@ -417,10 +425,15 @@ struct Loader {
     }
 };
 
+extern __shared__ __attribute__((aligned(128))) char s_tiles[];
+
+// One tile of the product MODE: that of the block with number `block` of its
+// product's grid of `ntiles` column tiles (and, of a weight's gradient, `mtiles`
+// row tiles).
 template <typename T, int MODE, typename TL, bool DMA>
-__global__ void __launch_bounds__(TL::NT) k_experts(ExpertArgs P, int ntiles, int mtiles) {
+__device__ __forceinline__ void expert_tile(const ExpertArgs& P, uint32_t block, int ntiles, int mtiles) {
     constexpr bool ROWS = MODE < DWIN;
-    extern __shared__ __attribute__((aligned(128))) char s_tiles[];
+    const int splits = MODE == DWIN ? P.splits_in : P.splits_out;
     __shared__ int s_slot[ROWS ? TL::BM : 1];
     __shared__ float s_w[ROWS ? TL::BM : 1];
     lds_char* const lds = (lds_char*)s_tiles;
@@ -432,7 +445,7 @@ __global__ void __launch_bounds__(TL::NT) k_experts(ExpertArgs P, int ntiles, in
     int e, p0, count, mf = 0, nf, split = 0;
     if constexpr (ROWS) {
         const int total = tiles_total(P.offsets, P.E, TL::BM);
-        const int64_t all = (int64_t)total * ntiles, id = die_order(blockIdx.x, all);
+        const int64_t all = (int64_t)total * ntiles, id = die_order(block, all);
         if (id >= all) return;
         const int group = (int)(id / ((int64_t)TILE_GROUP * ntiles));
         const int in = (int)(id - (int64_t)group * TILE_GROUP * ntiles);
@@ -449,9 +462,10 @@ __global__ void __launch_bounds__(TL::NT) k_experts(ExpertArgs P, int ntiles, in
         }
     } else {
         // an expert's tiles over all dies: experts differ in how long theirs take
-        const int per = mtiles * ntiles, all = per * P.splits, up = (all + XCDS - 1) / XCDS * XCDS;
-        e = (int)(blockIdx.x / up);
-        const int64_t id = die_order(blockIdx.x - (int64_t)e * up, all);
+        const int per = mtiles * ntiles, all = per * splits, up = (all + XCDS - 1) / XCDS * XCDS;
+        e = (int)(block / up);
+        if (e >= P.E) return;
+        const int64_t id = die_order(block - (int64_t)e * up, all);
         if (id >= all) return;
         split = (int)(id / per);
         const int in = (int)(id - (int64_t)split * per);
@@ -462,7 +476,7 @@ __global__ void __launch_bounds__(TL::NT) k_experts(ExpertArgs P, int ntiles, in
         nf = gin / gm * TL::BN;
         const int off = P.offsets[e], cnt = P.offsets[e + 1] - off;
         const int step = TL::STEP / (int)sizeof(T);
-        const int part = ((cnt + P.splits - 1) / P.splits + step - 1) / step * step;
+        const int part = ((cnt + splits - 1) / splits + step - 1) / step * step;
         const int lo = min(cnt, split * part);
         p0 = off + lo;
         count = min(part, cnt - lo);
@@ -646,12 +660,30 @@ __global__ void __launch_bounds__(TL::NT) k_experts(ExpertArgs P, int ntiles, in
                 const f32x4 v = four(c4);
                 if (row < M && c < N) {
                     const size_t at = ((size_t)e * M + row) * (size_t)N + c;
-                    if (P.splits == 1) store_part((T*)P.out + at, v, N - c);
-                    else store_part(P.part + (size_t)split * P.E * M * N + at, v, N - c);
+                    if (splits == 1) store_part((T*)(MODE == DWIN ? P.dw_in : P.dw_out) + at, v, N - c);
+                    else store_part((MODE == DWIN ? P.part_in : P.part_out) + (size_t)split * P.E * M * N + at, v, N - c);
                 }
             }
         }
     }
+}
+
+template <typename T, int MODE, typename TL, bool DMA>
+__global__ void __launch_bounds__(TL::NT) k_experts(ExpertArgs P, int ntiles) {
+    expert_tile<T, MODE, TL, DMA>(P, blockIdx.x, ntiles, 0);
+}
+
+// DX, DWIN and DWOUT need nothing of each other: one grid, so that one's last
+// tiles run beside the next one's first.
+struct GradGrid {
+    int nt[3], mt[3];
+    uint32_t first[2];                // DWIN's and DWOUT's first blocks, multiples of XCDS
+};
+template <typename T, typename TL, bool DMA>
+__global__ void __launch_bounds__(TL::NT) k_expert_grads(ExpertArgs P, GradGrid G) {
+    if (blockIdx.x < G.first[0]) expert_tile<T, DX, TL, DMA>(P, blockIdx.x, G.nt[0], 0);
+    else if (blockIdx.x < G.first[1]) expert_tile<T, DWIN, TL, DMA>(P, blockIdx.x - G.first[0], G.nt[1], G.mt[1]);
+    else expert_tile<T, DWOUT, TL, DMA>(P, blockIdx.x - G.first[1], G.nt[2], G.mt[2]);
 }
 
 // ---------------------------------------------------------------------------
@@ -828,96 +860,107 @@ __global__ void __launch_bounds__(ANSWER_NT) k_answer_few(ExpertArgs P, T* __res
     }
 }
 
-// Rows' slots added up: out[t] = sum_j z[t k + j] over the slots that have an
-// expert, 4 columns a thread; and (dwp) the routing weights' gradient.
+// The parts of a weight's gradient added in order, four values a thread.
 template <typename T>
-__global__ void __launch_bounds__(256) k_combine(ExpertArgs P, T* __restrict__ out, int64_t ldo, int parts,
-                                                 float* __restrict__ dweights) {
-    const int per = P.Dp / 4;
-    const int64_t work = P.n * per;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < work; i += (int64_t)gridDim.x * 256) {
-        const int64_t t = i / per;
-        const int d = (int)(i - t * per) * 4;
+__device__ __forceinline__ void add_parts(const float* part, int64_t count, int splits, T* out) {
+    typedef f32x4 f32x4_any __attribute__((aligned(4)));
+    for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < count; i += (int64_t)gridDim.x * 1024) {
+        const int have = (int)min(count - i, (int64_t)4);
         f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int j = 0; j < P.k; ++j) {
-            const int e = P.ids[t * P.k + j];
-            if (e >= 0 && e < P.E) s += *(const f32x4*)(P.z + (size_t)(t * P.k + j) * (size_t)P.Dp + d);
-        }
-        T* o = out + (size_t)t * (size_t)ldo + d;
+        if (have == 4) {
+#pragma unroll 8
+            for (int p = 0; p < splits; ++p) s += *(const f32x4_any*)(part + (size_t)p * (size_t)count + i);
+        } else {
+            for (int p = 0; p < splits; ++p)
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
-            if (d + c < P.D) o[c] = (T)s[c];
-    }
-    if (dweights) {
-        const int64_t S = P.n * P.k;
-        for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < S; i += (int64_t)gridDim.x * 256) {
-            const int e = P.ids[i];
-            float s = 0.0f;
-            if (e >= 0 && e < P.E)
-                for (int p = 0; p < parts; ++p) s += P.dwp[(size_t)p * (size_t)S + i];
-            dweights[i] = s;
+                for (int q = 0; q < 3; ++q)
+                    if (q < have) s[q] += part[(size_t)p * (size_t)count + i + q];
         }
+        store_part(out + i, s, have);
     }
 }
 
-// k = 1: rows whose slot has no expert get zeros, and dweights as in k_combine.
+// What is left once the tiles are made: out[t] = sum_j z[t k + j] over row t's
+// slots that have an expert (k = 1: zeros for rows without one, the others are
+// there), and in the backward pass dw = the sum of its parts and the weights'
+// gradients of theirs.
 template <typename T>
-__global__ void __launch_bounds__(256) k_unrouted(ExpertArgs P, T* __restrict__ out, int64_t ldo, int parts,
-                                                  float* __restrict__ dweights) {
-    for (int64_t t0 = (int64_t)blockIdx.x * 256; t0 < P.n; t0 += (int64_t)gridDim.x * 256) {
-        const int64_t t = t0 + threadIdx.x;
-        const int e = t < P.n ? P.ids[t] : 0;
-        const bool none = e < 0 || e >= P.E;
-        if (dweights && t < P.n) {
-            float s = 0.0f;
-            if (!none)
-                for (int p = 0; p < parts; ++p) s += P.dwp[(size_t)p * (size_t)P.n + t];
-            dweights[t] = s;
+__global__ void __launch_bounds__(256) k_finish(ExpertArgs P) {
+    T* const out = (T*)P.out;
+    if (P.k > 1) {
+        const int per = P.Dp / 4;
+        const int64_t work = P.n * per;
+        for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < work; i += (int64_t)gridDim.x * 256) {
+            const int64_t t = i / per;
+            const int d = (int)(i - t * per) * 4;
+            f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (int j = 0; j < P.k; ++j) {
+                const int e = P.ids[t * P.k + j];
+                if (e >= 0 && e < P.E) s += *(const f32x4*)(P.z + (size_t)(t * P.k + j) * (size_t)P.Dp + d);
+            }
+            store_part(out + (size_t)t * (size_t)P.ldo + d, s, P.D - d);
         }
-        // a wave writes its rows without an expert one after the other
-        uint64_t left = __ballot(none);
-        while (left) {
-            const int l = __ffsll((unsigned long long)left) - 1;
-            left &= left - 1;
-            const int64_t row = t0 + (threadIdx.x & ~63) + l;
-            for (int d = threadIdx.x & 63; d < P.D; d += 64) out[(size_t)row * (size_t)ldo + d] = (T)0.0f;
+    } else {
+        for (int64_t t0 = (int64_t)blockIdx.x * 256; t0 < P.n; t0 += (int64_t)gridDim.x * 256) {
+            const int64_t t = t0 + threadIdx.x;
+            const int e = t < P.n ? P.ids[t] : 0;
+            // a wave writes its rows without an expert one after the other
+            uint64_t left = __ballot(e < 0 || e >= P.E);
+            while (left) {
+                const int l = __ffsll((unsigned long long)left) - 1;
+                left &= left - 1;
+                const int64_t row = t0 + (threadIdx.x & ~63) + l;
+                for (int d = threadIdx.x & 63; d < P.D; d += 64) out[(size_t)row * (size_t)P.ldo + d] = (T)0.0f;
+            }
         }
     }
-}
-
-// The parts of a weight gradient added in order.
-template <typename T>
-__global__ void __launch_bounds__(256) k_weight_parts(const float* __restrict__ part, int64_t count, int splits,
-                                                      T* __restrict__ out) {
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256) {
+    if (!P.dweights) return;
+    const int64_t S = P.n * P.k;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < S; i += (int64_t)gridDim.x * 256) {
+        const int e = P.ids[i];
         float s = 0.0f;
-        for (int p = 0; p < splits; ++p) s += part[(size_t)p * (size_t)count + i];
-        out[i] = (T)s;
+        if (e >= 0 && e < P.E)
+            for (int p = 0; p < P.parts; ++p) s += P.dwp[(size_t)p * (size_t)S + i];
+        P.dweights[i] = s;
     }
+    const int64_t count = (int64_t)P.E * P.F * P.D;
+    if (P.splits_in > 1) add_parts(P.part_in, 2 * count, P.splits_in, (T*)P.dw_in);
+    if (P.splits_out > 1) add_parts(P.part_out, count, P.splits_out, (T*)P.dw_out);
 }
 
 // ---------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------
 
-using TileSmall = TileOf<128, 128, 2, 2, 128, 2>;
+using TileSmall = TileOf<64, 128, 2, 2, 128, 2>;
 using TileLarge = TileOf<256, 256, 4, 2, 128, 2>;
-
-// Row tiles of 256 x 256 when the experts' slots fill them, else 128 x 128.
-inline bool large_tiles(int64_t S, int E, int M, int N) { return S >= (int64_t)E * 256 && M >= 192 && N >= 192; }
 
 constexpr int PART_BLOCKS = 512;      // blocks of weight gradients that keep the device busy
 
 inline int up16(int v, int bytes) { return (v * bytes + 15) / 16 * 16 / bytes; }
+inline int64_t over(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-struct ExpertPlanSizes {
-    int64_t S;
-    int Fp, Dp, splits_in, splits_out, parts;
-    bool large;
+struct ExpertSizes {
+    int64_t S, used;                  // slots, and the experts that can have some
+    int D, F, E, bytes, Fp, Dp;
+    bool large[4];                    // tiles of h, of y, of the inner gradient, of the three others
+    int splits_in, splits_out, parts;
 };
 
+// Whether 256 x 256 tiles make the product of M x K by K x N of `count` experts
+// faster than 64 x 128: they fetch a third of the bytes, but there have to be
+// enough of them, and a block of theirs has its CU to itself, so that nothing
+// covers its beginning and end unless K is long.  Large and small, bf16, us: h of
+// 8000 slots, 250 an expert, 2048 -> 1024: 151 and 165, of 32 768, 256 -> 256 of 8:
+// 38 and 33; dx of 8000, 1024, 16 experts: 64 and 76; dw_in of the same 84 and 107,
+// of 4000, 256 x 256, 8 experts 38 and 19.  fp32 is bound by its arithmetic, of which
+// small tiles waste less at the edges (6000 x 500 -> 512 of 8: 949 and 625 for all six).
+inline bool large_product(int bytes, int64_t count, int64_t M, int64_t N, int64_t K) {
+    return bytes == 2 && K >= 384 && M >= 192 && N >= 192 && count * over(M, 256) * over(N, 256) >= 128;
+}
+
 inline int weight_splits(int64_t S, int E, int M, int N, int bm, int bn, int bk) {
-    const int64_t tiles = (int64_t)E * ((M + bm - 1) / bm) * ((N + bn - 1) / bn);
+    const int64_t tiles = (int64_t)E * over(M, bm) * over(N, bn);
     int64_t s = PART_BLOCKS / tiles;
     const int64_t longest = S / E / (4 * bk);          // at least four steps each for an average expert
     if (s > longest) s = longest;
@@ -925,65 +968,96 @@ inline int weight_splits(int64_t S, int E, int M, int N, int bm, int bn, int bk)
     return s < 1 ? 1 : (int)s;
 }
 
-inline ExpertPlanSizes expert_sizes(int dtype, int64_t n, int k, int D, int F, int E) {
-    ExpertPlanSizes z;
+inline ExpertSizes expert_sizes(int dtype, int64_t n, int k, int D, int F, int E) {
+    ExpertSizes z;
     const int b = dtype_bytes(dtype);
     z.S = n * k;
+    z.used = z.S < E ? z.S : E;
+    z.D = D, z.F = F, z.E = E, z.bytes = b;
     z.Fp = up16(F, b);
     z.Dp = up16(D, 4);
-    z.large = large_tiles(z.S, E, D, F);
-    const int t = z.large ? 256 : 128, bk = 128 / b;
-    z.splits_in = weight_splits(z.S, E, z.Fp + F, D, t, t, bk);
-    z.splits_out = weight_splits(z.S, E, D, F, t, t, bk);
-    z.parts = (F + t - 1) / t * (z.large ? TileLarge::WN : TileSmall::WN);
+    const int64_t each = z.used ? over(z.S, z.used) : 0;
+    z.large[0] = large_product(b, z.used, each, 2 * (int64_t)F, D);
+    z.large[1] = large_product(b, z.used, each, D, F);
+    z.large[2] = large_product(b, z.used, each, F, D);
+    z.large[3] = large_product(b, z.used, each, D, 2 * (int64_t)F) && large_product(b, E, 2 * (int64_t)F, D, z.S / E);
+    const int bm = z.large[3] ? 256 : 64, bn = z.large[3] ? 256 : 128;
+    z.splits_in = weight_splits(z.S, E, z.Fp + F, D, bm, bn, 128 / b);
+    z.splits_out = weight_splits(z.S, E, D, F, bm, bn, 128 / b);
+    z.parts = (int)(z.large[2] ? over(F, TileLarge::BN) * TileLarge::WN : over(F, TileSmall::BN) * TileSmall::WN);
     return z;
 }
 
-inline size_t carve_forward(Carve& c, ExpertArgs* P, const ExpertPlanSizes& z, int dtype, int k) {
-    P->h = c.take<char>((size_t)z.S * z.Fp * dtype_bytes(dtype));
+inline size_t carve_forward(Carve& c, ExpertArgs* P, const ExpertSizes& z, int k) {
+    P->h = c.take<char>((size_t)z.S * z.Fp * z.bytes);
     P->z = k > 1 ? c.take<float>((size_t)z.S * z.Dp) : nullptr;
     return c.off;
 }
 
-inline size_t carve_backward(Carve& c, ExpertArgs* P, float** part, const ExpertPlanSizes& z, int dtype, int k, int D,
-                             int F, int E) {
-    const size_t b = (size_t)dtype_bytes(dtype);
-    P->dpre = c.take<char>((size_t)z.S * 2 * z.Fp * b);
-    P->hw = c.take<char>((size_t)z.S * z.Fp * b);
+inline size_t carve_backward(Carve& c, ExpertArgs* P, const ExpertSizes& z, int k) {
+    P->dpre = c.take<char>((size_t)z.S * 2 * z.Fp * z.bytes);
+    P->hw = c.take<char>((size_t)z.S * z.Fp * z.bytes);
     P->dwp = c.take<float>((size_t)z.parts * z.S);
     P->z = k > 1 ? c.take<float>((size_t)z.S * z.Dp) : nullptr;
-    size_t p = z.splits_in > 1 ? (size_t)z.splits_in * E * 2 * F * (size_t)D : 0;
-    const size_t q = z.splits_out > 1 ? (size_t)z.splits_out * E * F * (size_t)D : 0;
-    if (q > p) p = q;
-    *part = p ? c.take<float>(p) : nullptr;
+    const size_t count = (size_t)z.E * z.F * (size_t)z.D;
+    P->part_in = z.splits_in > 1 ? c.take<float>(z.splits_in * 2 * count) : nullptr;
+    P->part_out = z.splits_out > 1 ? c.take<float>(z.splits_out * count) : nullptr;
+    P->splits_in = z.splits_in;
+    P->splits_out = z.splits_out;
+    P->parts = z.parts;
     return c.off;
 }
 
-template <typename T, int MODE, typename TL, bool DMA>
-void launch_tiles(const ExpertArgs& P, int M, int N, hipStream_t stream) {
-    constexpr int cols = MODE == IN ? TL::BN / 2 : TL::BN;
-    const int nt = (N + cols - 1) / cols, mt = (M + TL::BM - 1) / TL::BM;
-    int64_t blocks;
-    if (MODE < DWIN) {
-        const int64_t S = P.n * P.k;
-        blocks = (S / TL::BM + (S < P.E ? S : P.E)) * nt;      // no plan has more tiles
-    } else {
-        blocks = (int64_t)P.E * (((int64_t)mt * nt * P.splits + XCDS - 1) / XCDS * XCDS);
+template <typename TL, int MODE>
+int64_t tile_blocks(const ExpertSizes& z, int* nt, int* mt) {
+    const int N = MODE == OUT || MODE == DX || MODE == DWIN ? z.D : z.F, cols = MODE == IN ? TL::BN / 2 : TL::BN;
+    const int M = MODE == DWIN ? z.Fp + z.F : z.D;
+    *nt = (int)over(N, cols);
+    *mt = (int)over(M, TL::BM);
+    if (MODE < DWIN) return over((z.S / TL::BM + z.used) * *nt, XCDS) * XCDS;      // no plan has more tiles
+    return z.E * (over((int64_t)*mt * *nt * (MODE == DWIN ? z.splits_in : z.splits_out), XCDS) * XCDS);
+}
+
+// fp32 has no large tiles (large_product).
+template <typename T, typename F>
+void by_tile(bool large, bool dma, const F& f) {
+    if constexpr (sizeof(T) == 2) {
+        if (large) return dma ? f(TileLarge(), std::true_type()) : f(TileLarge(), std::false_type());
     }
-    if (blocks == 0) return;
-    blocks = (blocks + XCDS - 1) / XCDS * XCDS;
-    k_experts<T, MODE, TL, DMA><<<(unsigned)blocks, TL::NT, TL::STAGES * TL::STAGE, stream>>>(P, nt, mt);
+    dma ? f(TileSmall(), std::true_type()) : f(TileSmall(), std::false_type());
 }
 
 template <typename T, int MODE>
-void run_tiles(const ExpertArgs& P, bool large, bool dma, int M, int N, hipStream_t stream) {
-    if (large) {
-        if (dma) launch_tiles<T, MODE, TileLarge, true>(P, M, N, stream);
-        else launch_tiles<T, MODE, TileLarge, false>(P, M, N, stream);
-    } else {
-        if (dma) launch_tiles<T, MODE, TileSmall, true>(P, M, N, stream);
-        else launch_tiles<T, MODE, TileSmall, false>(P, M, N, stream);
-    }
+void run_tiles(const ExpertArgs& P, const ExpertSizes& z, bool large, bool dma, hipStream_t stream) {
+    by_tile<T>(large, dma, [&](auto tl, auto d) {
+        using TL = decltype(tl);
+        int nt, mt;
+        const int64_t blocks = tile_blocks<TL, MODE>(z, &nt, &mt);
+        if (blocks)
+            k_experts<T, MODE, TL, decltype(d)::value><<<(unsigned)blocks, TL::NT, TL::STAGES * TL::STAGE, stream>>>(P, nt);
+    });
+}
+
+template <typename T>
+void run_grads(const ExpertArgs& P, const ExpertSizes& z, bool dma, hipStream_t stream) {
+    by_tile<T>(z.large[3], dma, [&](auto tl, auto d) {
+        using TL = decltype(tl);
+        GradGrid G;
+        const int64_t dx = tile_blocks<TL, DX>(z, &G.nt[0], &G.mt[0]);
+        const int64_t in = tile_blocks<TL, DWIN>(z, &G.nt[1], &G.mt[1]);
+        const int64_t out = tile_blocks<TL, DWOUT>(z, &G.nt[2], &G.mt[2]);
+        G.first[0] = (uint32_t)dx;
+        G.first[1] = (uint32_t)(dx + in);
+        k_expert_grads<T, TL, decltype(d)::value>
+            <<<(unsigned)(dx + in + out), TL::NT, TL::STAGES * TL::STAGE, stream>>>(P, G);
+    });
+}
+
+template <typename T>
+void run_finish(const ExpertArgs& P, const ExpertSizes& z, hipStream_t stream) {
+    int64_t work = P.k > 1 ? P.n * (z.Dp / 4) : P.n;
+    if (P.dweights && (z.splits_in > 1 || z.splits_out > 1)) work += (int64_t)z.E * z.F * z.D / 4;
+    k_finish<T><<<launch_grid(work, 256, 8192), 256, 0, stream>>>(P);
 }
 
 // The kernels for few rows by the slots an expert in use has on average.  They
@@ -996,55 +1070,32 @@ inline bool few_inner(int64_t S, int E, int bytes) {
     const int64_t used = S < E ? S : E;
     return S <= used * (bytes == 4 ? 32 : 8);
 }
-// y, few and tiles with k_combine: one row's 6 slots 6.6 and 12.7 us, two rows' 12
+// y, few and tiles with k_finish: one row's 6 slots 6.6 and 12.7 us, two rows' 12
 // slots 11 and 14, 8 rows' 48 slots 26 and 18 (a wave has several experts in turn).
 inline bool few_answer(int64_t S, int E, int bytes) {
     return few_inner(S, E, bytes) && S <= FEW_SLOTS && (S < E ? S : E) <= 16;
 }
 
 template <typename T>
-int run_experts(ExpertArgs P, const ExpertPlanSizes& z, T* y, int64_t ldy, bool dma, hipStream_t stream) {
-    P.out = y;
-    P.ldo = ldy;
+int run_experts(const ExpertArgs& P, const ExpertSizes& z, bool dma, hipStream_t stream) {
     if (few_inner(z.S, P.E, sizeof(T)))
-        k_inner_few<T><<<dim3((unsigned)((P.F + 15) / 16), (unsigned)(z.S < P.E ? z.S : P.E)), FEW_NT, 0, stream>>>(P);
+        k_inner_few<T><<<dim3((unsigned)over(P.F, 16), (unsigned)z.used), FEW_NT, 0, stream>>>(P);
     else
-        run_tiles<T, IN>(P, z.large, dma, 0, P.F, stream);
+        run_tiles<T, IN>(P, z, z.large[0], dma, stream);
     if (few_answer(z.S, P.E, sizeof(T))) {
-        k_answer_few<T><<<(unsigned)((P.D + 15) / 16), ANSWER_NT, 0, stream>>>(P, y, ldy);
-        return launch_status("yabt_experts");
+        k_answer_few<T><<<(unsigned)over(P.D, 16), ANSWER_NT, 0, stream>>>(P, (T*)P.out, P.ldo);
+    } else {
+        run_tiles<T, OUT>(P, z, z.large[1], dma, stream);
+        run_finish<T>(P, z, stream);
     }
-    run_tiles<T, OUT>(P, z.large, dma, 0, P.D, stream);
-    if (P.k > 1)
-        k_combine<T><<<launch_grid(P.n * (z.Dp / 4), 256, 8192), 256, 0, stream>>>(P, y, ldy, 0, nullptr);
-    else
-        k_unrouted<T><<<launch_grid(P.n, 256, 8192), 256, 0, stream>>>(P, y, ldy, 0, nullptr);
     return launch_status("yabt_experts");
 }
 
 template <typename T>
-int run_experts_grad(ExpertArgs P, const ExpertPlanSizes& z, float* part, T* dx, int64_t lddx, float* dweights,
-                     T* dw_in, T* dw_out, bool dma, hipStream_t stream) {
-    run_tiles<T, DH>(P, z.large, dma, 0, P.F, stream);
-    P.out = dx;
-    P.ldo = lddx;
-    run_tiles<T, DX>(P, z.large, dma, 0, P.D, stream);
-    if (P.k > 1)
-        k_combine<T><<<launch_grid(P.n * (z.Dp / 4), 256, 8192), 256, 0, stream>>>(P, dx, lddx, z.parts, dweights);
-    else
-        k_unrouted<T><<<launch_grid(P.n, 256, 8192), 256, 0, stream>>>(P, dx, lddx, z.parts, dweights);
-    P.part = part;
-    P.out = dw_in;
-    P.splits = z.splits_in;
-    run_tiles<T, DWIN>(P, z.large, dma, z.Fp + P.F, P.D, stream);
-    const int64_t cin = (int64_t)P.E * 2 * P.F * P.D;
-    if (P.splits > 1)
-        k_weight_parts<T><<<launch_grid(cin, 256, 8192), 256, 0, stream>>>(part, cin, P.splits, dw_in);
-    P.out = dw_out;
-    P.splits = z.splits_out;
-    run_tiles<T, DWOUT>(P, z.large, dma, P.D, P.F, stream);
-    if (P.splits > 1)
-        k_weight_parts<T><<<launch_grid(cin / 2, 256, 8192), 256, 0, stream>>>(part, cin / 2, P.splits, dw_out);
+int run_experts_grad(const ExpertArgs& P, const ExpertSizes& z, bool dma, hipStream_t stream) {
+    run_tiles<T, DH>(P, z, z.large[2], dma, stream);
+    run_grads<T>(P, z, dma, stream);
+    run_finish<T>(P, z, stream);
     return launch_status("yabt_experts_grad");
 }
 
@@ -1053,10 +1104,11 @@ inline bool expert_sizes_ok(int64_t n, int k, int D, int F, int E) {
            F <= (1 << 24);
 }
 
-// The grids' sizes; the tiles of the smallest shape.
+// The grids' sizes, in tiles of the small shape and with the most splits.
 inline bool expert_grids_ok(int64_t n, int k, int D, int F, int E) {
-    const int64_t S = n * k, wide = D > F ? D : F;
-    return (S / 128 + E) * ((wide + 63) / 64) < INT32_MAX && (int64_t)E * ((2 * (int64_t)F + 255) / 128) * ((D + 127) / 128) < INT32_MAX / 64;
+    const int64_t S = n * k, wide = D > F ? D : F, rows = (S / 64 + E) * over(wide, 64);
+    const int64_t weights = (int64_t)E * (over(2 * (int64_t)F + 8, 64) * over(D, 128) + over(D, 64) * over(F, 128) + 2 * XCDS);
+    return rows < (INT32_MAX >> 2) && weights < (INT32_MAX >> 2);
 }
 
 template <typename F>
@@ -1081,7 +1133,7 @@ size_t yabt_experts_workspace_bytes(int dtype, int64_t n, int k, int D, int F, i
     if (!dtype_ok(dtype) || !expert_sizes_ok(n, k, D, F, E)) return 0;
     ExpertArgs P;
     Carve c{nullptr, 0};
-    return carve_forward(c, &P, expert_sizes(dtype, n, k, D, F, E), dtype, k) + 256;
+    return carve_forward(c, &P, expert_sizes(dtype, n, k, D, F, E), k) + 256;
 }
 
 int yabt_experts(int dtype, const void* x, int64_t ldx, int64_t n, int k, int D, int F, int E, const int32_t* ids,
@@ -1097,26 +1149,26 @@ int yabt_experts(int dtype, const void* x, int64_t ldx, int64_t n, int k, int D,
     if (!aligned16(out_inner)) return fail(-1, "yabt_experts: out_inner must be 16-byte aligned");
     if (!workspace || workspace_bytes < yabt_experts_workspace_bytes(dtype, n, k, D, F, E))
         return fail(-2, "yabt_experts: workspace too small");
-    const ExpertPlanSizes z = expert_sizes(dtype, n, k, D, F, E);
+    const ExpertSizes z = expert_sizes(dtype, n, k, D, F, E);
     ExpertArgs P = {x, nullptr, w_in, w_out, weights, ids, offsets, slots, rows, ldx, 0, n, k, D, F, E, z.Fp, z.Dp, up16(F, 4)};
     P.pre = out_inner;
-    P.splits = 1;
+    P.out = y;
+    P.ldo = ldy;
     Carve c{(char*)align_up((size_t)workspace, 256), 0};
-    carve_forward(c, &P, z, dtype, k);
+    carve_forward(c, &P, z, k);
     const int b = dtype_bytes(dtype);
     const bool dma = pieces_ok(x, ldx, D, b) && pieces_ok(w_in, D, D, b) && pieces_ok(w_out, F, F, b);
     return by_dtype(dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        return run_experts<T>(P, z, (T*)y, ldy, dma, (hipStream_t)stream);
+        return run_experts<T>(P, z, dma, (hipStream_t)stream);
     });
 }
 
 size_t yabt_experts_grad_workspace_bytes(int dtype, int64_t n, int k, int D, int F, int E) {
     if (!dtype_ok(dtype) || !expert_sizes_ok(n, k, D, F, E)) return 0;
     ExpertArgs P;
-    float* part;
     Carve c{nullptr, 0};
-    return carve_backward(c, &P, &part, expert_sizes(dtype, n, k, D, F, E), dtype, k, D, F, E) + 256;
+    return carve_backward(c, &P, expert_sizes(dtype, n, k, D, F, E), k) + 256;
 }
 
 int yabt_experts_grad(int dtype, const void* dy, int64_t lddy, const void* x, int64_t ldx, int64_t n, int k, int D,
@@ -1133,19 +1185,22 @@ int yabt_experts_grad(int dtype, const void* dy, int64_t lddy, const void* x, in
     if (!aligned16(inner)) return fail(-1, "yabt_experts_grad: inner must be 16-byte aligned");
     if (!workspace || workspace_bytes < yabt_experts_grad_workspace_bytes(dtype, n, k, D, F, E))
         return fail(-2, "yabt_experts_grad: workspace too small");
-    const ExpertPlanSizes z = expert_sizes(dtype, n, k, D, F, E);
+    const ExpertSizes z = expert_sizes(dtype, n, k, D, F, E);
     ExpertArgs P = {x, dy, w_in, w_out, weights, ids, offsets, slots, rows, ldx, lddy, n, k, D, F, E, z.Fp, z.Dp, up16(F, 4)};
     P.pre = const_cast<float*>(inner);
+    P.out = dx;
+    P.ldo = lddx;
+    P.dw_in = dw_in;
+    P.dw_out = dw_out;
+    P.dweights = dweights;
     Carve c{(char*)align_up((size_t)workspace, 256), 0};
-    float* part = nullptr;
-    carve_backward(c, &P, &part, z, dtype, k, D, F, E);
+    carve_backward(c, &P, z, k);
     const int b = dtype_bytes(dtype);
     const bool dma = pieces_ok(x, ldx, D, b) && pieces_ok(dy, lddy, D, b) && pieces_ok(w_in, D, D, b) &&
                      pieces_ok(w_out, F, F, b);
     return by_dtype(dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        return run_experts_grad<T>(P, z, part, (T*)dx, lddx, dweights, (T*)dw_in, (T*)dw_out, dma,
-                                   (hipStream_t)stream);
+        return run_experts_grad<T>(P, z, dma, (hipStream_t)stream);
     });
 }
 
