@@ -17,7 +17,14 @@
 
 namespace yabt {
 
-constexpr int NORM_GRAD_BLOCKS = 512;   // row blocks whose weight gradients are added afterwards, at most
+// Blocks at most: they stay and walk rows, the next row's chunks on their way
+// while one is worked on, and keep the weights in registers.  16384 x 4096 bf16,
+// us: forward with 512, 768, 1024, 2048 and 16384 blocks 55, 57, 59, 68 and 244 (a
+// copy of as many bytes takes 52), backward with 512, 768 and 1024, the parts of
+// the weights' gradients and their sum included, 106, 100 and 103 (its 403 MB as a
+// copy: 78); 20000 x 500 fp32: forward with 768 and 2048 17 and 19, backward 33, 29 and 30.
+constexpr int NORM_BLOCKS = 768;
+constexpr int NORM_GRAD_BLOCKS = 768;
 
 // Sum over the G threads of a row; s: 2 * (G / 64) floats in LDS when G > 64,
 // `flip` alternates between its halves so that one barrier is enough.
@@ -371,7 +378,7 @@ void run_norm(const T* x, int64_t ldx, int64_t n, int D, const float* w, const f
     const bool fits = norm_shape<T>(D, [&](auto g, auto nv, auto nn) {
         constexpr int G = decltype(g)::value, NV = decltype(nv)::value, N = decltype(nn)::value;
         constexpr int NT = G < 256 ? 256 : G;
-        k_norm<T, G, NV, N><<<launch_grid(n, NT / G, 2048), NT, 0, stream>>>(x, ldx, n, D, w, c, eps, y, ldy, mean,
+        k_norm<T, G, NV, N><<<launch_grid(n, NT / G, NORM_BLOCKS), NT, 0, stream>>>(x, ldx, n, D, w, c, eps, y, ldy, mean,
                                                                            rstd);
     });
     if (!fits)
