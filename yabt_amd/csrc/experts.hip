@@ -17,9 +17,9 @@
 //   DX     W_in^T [dg du] by slot in fp32, or dx itself when k = 1
 //   DWIN, DWOUT   the weights' gradients, summed over an expert's slots
 //
-// Both operands pass through LDS in steps of 64 or 128 bytes of the summed
-// dimension, two stages or more: the next ones are on their way from memory
-// straight into LDS while the present one is multiplied.  16-byte pieces are stored at places that an
+// Both operands pass through LDS in steps of 128 bytes of the summed dimension:
+// the next steps are on their way from memory straight into LDS while the
+// present one is multiplied.  16-byte pieces are stored at places that an
 // xor with the row spreads over the banks; the xor is applied to the global
 // address, as LDS is filled in lane order.  Operands across the summed
 // dimension are read with the transposing LDS loads.  Inputs whose rows are
@@ -45,6 +45,7 @@ typedef __attribute__((address_space(3))) char lds_char;
 typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 typedef __attribute__((address_space(3))) float lds_float;
+typedef __attribute__((address_space(3))) int lds_int;
 typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
 
 enum Mode { IN, OUT, DH, DX, DWIN, DWOUT };
@@ -87,16 +88,19 @@ struct ExpertArgs {
 // 16 zero bytes for pieces past the end of the summed dimension.
 __device__ const u32x4 g_zeros = {0, 0, 0, 0};
 
-// BM x BN sums by WM x WN waves; STAGES stages of STEP bytes of the summed dimension.
-template <int BM_, int BN_, int WM_, int WN_, int STEP_, int STAGES_>
+// BM x BN sums by WM x WN waves, in steps of STEP bytes of the summed dimension;
+// LDS holds AS steps of the rows' operand and BS <= AS of the columns'.
+template <int BM_, int BN_, int WM_, int WN_, int STEP_, int AS_, int BS_>
 struct TileOf {
-    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, STEP = STEP_, STAGES = STAGES_;
+    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, STEP = STEP_, AS = AS_, BS = BS_;
     static constexpr int NT = 64 * WM * WN;
     static constexpr int MI = BM / WM / 32, NI = BN / WN / 32;    // 32 x 32 blocks a wave makes
-    static constexpr int ABYTES = BM * STEP, BBYTES = BN * STEP, STAGE = ABYTES + BBYTES;
+    static constexpr int ABYTES = BM * STEP, BBYTES = BN * STEP;
+    static constexpr int LDS = AS * ABYTES + BS * BBYTES;
     static constexpr int NA = ABYTES / 16 / NT, NB = BBYTES / 16 / NT;
+    static constexpr int SUMS = BM / MI * BN * 4;                 // 32 rows of every wave, as the sums leave
     static_assert(NA >= 1 && NB >= 1 && NI % 2 == 0, "whole pieces a thread, gate and up in one wave");
-    static_assert(STAGES * STAGE + 2048 <= 160 * 1024, "a block's LDS");
+    static_assert(LDS <= 160 * 1024 && SUMS + BM * 8 <= LDS && BS <= AS && BM <= NT, "a block's LDS");
 };
 
 // Where piece c (16 bytes) of row r of a tile in LDS is kept: c ^ spread(r), so
@@ -127,7 +131,7 @@ __device__ __forceinline__ void lds_fill(const void* g, uint32_t base) {
 
 // Until at most LATER of this wave's vector memory accesses are under way and
 // its LDS reads are done, then for the block's other waves: what was sent to
-// LDS before the last LATER accesses is there, and the stage read last is free.
+// LDS before the last LATER accesses is there, and the places read last are free.
 template <int LATER>
 __device__ __forceinline__ void stage_ready() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LATER) : "memory");
@@ -434,15 +438,14 @@ template <typename T, int MODE, typename TL, bool DMA>
 __device__ __forceinline__ void expert_tile(const ExpertArgs& P, uint32_t block, int ntiles, int mtiles) {
     constexpr bool ROWS = MODE < DWIN;
     const int splits = MODE == DWIN ? P.splits_in : P.splits_out;
-    __shared__ int s_slot[ROWS ? TL::BM : 1];
-    __shared__ float s_w[ROWS ? TL::BM : 1];
     lds_char* const lds = (lds_char*)s_tiles;
     const uint32_t lds_at = (uint32_t)(uintptr_t)lds;
     const int wave = threadIdx.x / 64, lane = threadIdx.x & 63;
     const int wm = wave / TL::WN, wn = wave % TL::WN;
 
     // which tile: expert e, slots [p0, p0 + count), first row mf and column nf
-    int e, p0, count, mf = 0, nf, split = 0;
+    int e, p0, count, mf = 0, nf, split = 0, my_slot = 0;
+    float my_w = 1.0f;
     if constexpr (ROWS) {
         const int total = tiles_total(P.offsets, P.E, TL::BM);
         const int64_t all = (int64_t)total * ntiles, id = die_order(block, all);
@@ -455,10 +458,12 @@ __device__ __forceinline__ void expert_tile(const ExpertArgs& P, uint32_t block,
         p0 = P.offsets[e] + t.mi * TL::BM;
         count = min(TL::BM, P.offsets[e + 1] - p0);
         nf = in / gm * (MODE == IN ? TL::BN / 2 : TL::BN);
-        for (int i = threadIdx.x; i < TL::BM; i += TL::NT) {
-            const int slot = i < count ? P.slots[p0 + i] : 0;
-            s_slot[i] = slot;
-            s_w[i] = MODE == OUT || MODE == DH ? P.weights[slot] : 1.0f;
+        // a row a thread, kept until the sums are there
+        if constexpr (MODE != IN) {
+            if ((int)threadIdx.x < count) {
+                my_slot = P.slots[p0 + threadIdx.x];
+                if constexpr (MODE != DX) my_w = P.weights[my_slot];
+            }
         }
     } else {
         // an expert's tiles over all dies: experts differ in how long theirs take
@@ -487,7 +492,7 @@ __device__ __forceinline__ void expert_tile(const ExpertArgs& P, uint32_t block,
     using LA = decltype(la);
     using LB = decltype(lb);
     const int ka = LA::length(P, count), kb = LB::length(P, count), K = max(ka, kb);
-    constexpr int BK = TL::STEP / (int)sizeof(T), AHEAD = DMA ? TL::STAGES - 1 : 1, KS = TL::STEP / 32;
+    constexpr int BK = TL::STEP / (int)sizeof(T), KS = TL::STEP / 32;
     const int steps = (K + BK - 1) / BK;
     f32x16 acc[TL::MI][TL::NI];
 #pragma unroll
@@ -500,70 +505,79 @@ __device__ __forceinline__ void expert_tile(const ExpertArgs& P, uint32_t block,
     if (steps > 0) {
         la.init(P, e, p0, count, mf);
         lb.init(P, e, p0, count, nf);
-        // stage t % STAGES holds step t; AHEAD steps are under way
+        // Step t of the rows' operand lies at place t % AS, of the columns' at t % BS.
+        // A step is sent as soon as its place is free: the columns' BS, then the
+        // rows' AS steps ahead.  For operands whose rows are looked up the rows of
+        // the step after are asked for first, so that a wait for them is none for
+        // the pieces.  Steps past the last are sent too (zeros), so that every wait
+        // is the same.  Without DMA a step waits in registers for its place.
+        constexpr int AS = DMA ? TL::AS : 2, BS = 2;
+        static_assert(TL::BS == 2, "two places for the columns' steps");
         u32x4 ra[DMA ? 1 : TL::NA], rb[DMA ? 1 : TL::NB];
-        auto look_up = [&](int t) {
-            la.look_up(P, p0, count, t * BK);
-            lb.look_up(P, p0, count, t * BK);
-        };
-        // step t on its way; the rows of the step after it are asked for first,
-        // so that a wait for them is none for the pieces
-        auto send = [&](int t) {
+        auto send_a = [&](int t, int place) {
             la.move_on();
-            lb.move_on();
-            look_up(t + 1);
-            if constexpr (DMA) {
-                const uint32_t to = lds_at + (uint32_t)(t % TL::STAGES) * TL::STAGE;
-                la.fill(P, t * BK, ka, to);
-                lb.fill(P, t * BK, kb, to + TL::ABYTES);
-            } else {
-                la.fetch(P, t * BK, ka, mf, ra);
-                lb.fetch(P, t * BK, kb, nf, rb);
-            }
+            la.look_up(P, p0, count, (t + 1) * BK);
+            if constexpr (DMA) la.fill(P, t * BK, ka, lds_at + (uint32_t)place * TL::ABYTES);
+            else la.fetch(P, t * BK, ka, mf, ra);
         };
-        look_up(0);
+        auto send_b = [&](int t) {
+            lb.move_on();
+            lb.look_up(P, p0, count, (t + 1) * BK);
+            if constexpr (DMA) lb.fill(P, t * BK, kb, lds_at + TL::AS * TL::ABYTES + (uint32_t)(t & 1) * TL::BBYTES);
+            else lb.fetch(P, t * BK, kb, nf, rb);
+        };
+        auto put = [&](int t) {
+            LA::put(lds + (t & 1) * TL::ABYTES, ra);
+            LB::put(lds + TL::AS * TL::ABYTES + (t & 1) * TL::BBYTES, rb);
+        };
+        la.look_up(P, p0, count, 0);
+        lb.look_up(P, p0, count, 0);
+        // accesses of every wave after step 0's and, in the loop, after the next step's
+        constexpr int AFTER_0 = DMA ? (AS - 1) * TL::NA + (BS - 1) * TL::NB : 0, AFTER = DMA ? (AS - BS) * TL::NA : 0;
         if constexpr (DMA) {
 #pragma unroll
-            for (int t = 0; t <= AHEAD; ++t) send(t);
+            for (int t = 0; t < AS; ++t) {
+                send_a(t, t);
+                if (t < BS) send_b(t);
+            }
         } else {
-            send(0);
-            LA::put(lds, ra);
-            LB::put(lds + TL::ABYTES, rb);
-            send(1);
+            send_a(0, 0);
+            send_b(0);
+            put(0);
+            send_a(1, 0);
+            send_b(1);
         }
         const Frag<T, LA::ACROSS, TL::BM, TL::STEP> fa(wm * TL::MI * 32);
         const Frag<T, LB::ACROSS, TL::BN, TL::STEP> fb(wn * TL::NI * 32);
         u32x4 a[2][TL::MI], b[2][TL::NI];
-        auto read = [&](int t, int ks) {
-            lds_char* const cur = lds + t % TL::STAGES * TL::STAGE;
+        auto read = [&](int place, int t, int ks) {
+            lds_char* const ta = lds + place * TL::ABYTES;
+            lds_char* const tb = lds + TL::AS * TL::ABYTES + (t & 1) * TL::BBYTES;
 #pragma unroll
-            for (int i = 0; i < TL::MI; ++i) a[ks & 1][i] = fa.get(cur, i, ks);
+            for (int i = 0; i < TL::MI; ++i) a[ks & 1][i] = fa.get(ta, i, ks);
 #pragma unroll
-            for (int j = 0; j < TL::NI; ++j) b[ks & 1][j] = fb.get(cur + TL::ABYTES, j, ks);
+            for (int j = 0; j < TL::NI; ++j) b[ks & 1][j] = fb.get(tb, j, ks);
         };
-        // a step that was sent is EACH accesses of every wave, and steps past
-        // the last are sent too (zeros), so that every wait is the same
-        constexpr int EACH = TL::NA + TL::NB, READS = TL::MI * decltype(fa)::READS + TL::NI * decltype(fb)::READS;
+        constexpr int READS = TL::MI * decltype(fa)::READS + TL::NI * decltype(fb)::READS;
         constexpr int PRODUCTS = TL::MI * TL::NI * (sizeof(T) == 4 ? 4 : 1);
-        stage_ready<DMA ? AHEAD * EACH : 0>();
-        read(0, 0);
+        stage_ready<AFTER_0>();
+        read(0, 0, 0);
         // A k-step's operands are read while the one before is multiplied, the
         // next step's first ones too: the wait for it stands before the last
-        // k-step's products, and the step that takes the freed stage is sent there.
+        // k-step's products, and what takes the freed places is sent there.
+        int place = 0;
         for (int t = 0; t < steps; ++t) {
+            const int next = place + 1 == AS ? 0 : place + 1;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 if (ks + 1 < KS) {
-                    read(t, ks + 1);
+                    read(place, t, ks + 1);
                 } else {
-                    if constexpr (!DMA) {
-                        lds_char* const to = lds + (t + 1) % TL::STAGES * TL::STAGE;
-                        LA::put(to, ra);
-                        LB::put(to + TL::ABYTES, rb);
-                    }
-                    stage_ready<DMA ? (AHEAD - 1) * EACH : 0>();
-                    send(t + 1 + AHEAD);
-                    read(t + 1, 0);
+                    if constexpr (!DMA) put(t + 1);
+                    stage_ready<AFTER>();
+                    send_b(t + 2);
+                    send_a(t + AS, place);
+                    read(next, t + 1, 0);
                 }
 #pragma unroll
                 for (int i = 0; i < TL::MI; ++i)
@@ -571,6 +585,7 @@ __device__ __forceinline__ void expert_tile(const ExpertArgs& P, uint32_t block,
                     for (int j = 0; j < TL::NI; ++j) acc[i][j] = mma<T>(a[ks & 1][i], b[ks & 1][j], acc[i][j]);
                 if constexpr (DMA) interleave<PRODUCTS, READS>();
             }
+            place = next;
         }
         stage_ready<0>();                            // nothing may reach the LDS of a block that is gone
     }
@@ -578,9 +593,16 @@ __device__ __forceinline__ void expert_tile(const ExpertArgs& P, uint32_t block,
     // The sums go through LDS, 32 rows of a wave at a time, from the matrix
     // cores' layout (a lane has one column) to four neighbouring columns a lane,
     // so that what is read and written beside them goes in whole lines.
-    if constexpr (ROWS) __syncthreads();            // s_slot and s_w where there was no step
+    lds_int* const s_slot = (lds_int*)(lds + TL::SUMS);
+    lds_float* const s_w = (lds_float*)(lds + TL::SUMS + TL::BM * 4);
+    if constexpr (ROWS && MODE != IN) {
+        if (threadIdx.x < TL::BM) {
+            s_slot[threadIdx.x] = my_slot;
+            s_w[threadIdx.x] = my_w;
+        }
+        __syncthreads();
+    }
     constexpr int W = TL::NI * 32;
-    static_assert(32 * W * 4 * TL::NT / 64 <= TL::STAGES * TL::STAGE, "the waves' 32 rows fit the stages");
     lds_float* const mine = (lds_float*)(lds + wave * 32 * W * 4);
     constexpr int LANES = MODE == IN ? W / 8 : W / 4, PASS = 64 / LANES;    // lanes a row, rows at once
     const int c4 = lane % LANES * 4;
@@ -932,8 +954,8 @@ __global__ void __launch_bounds__(256) k_finish(ExpertArgs P) {
 // host
 // ---------------------------------------------------------------------------
 
-using TileSmall = TileOf<64, 128, 2, 2, 128, 2>;
-using TileLarge = TileOf<256, 256, 4, 2, 128, 2>;
+using TileSmall = TileOf<64, 128, 2, 2, 128, 2, 2>;
+using TileLarge = TileOf<256, 256, 4, 2, 128, 3, 2>;
 
 constexpr int PART_BLOCKS = 512;      // blocks of weight gradients that keep the device busy
 
@@ -1034,7 +1056,7 @@ void run_tiles(const ExpertArgs& P, const ExpertSizes& z, bool large, bool dma, 
         int nt, mt;
         const int64_t blocks = tile_blocks<TL, MODE>(z, &nt, &mt);
         if (blocks)
-            k_experts<T, MODE, TL, decltype(d)::value><<<(unsigned)blocks, TL::NT, TL::STAGES * TL::STAGE, stream>>>(P, nt);
+            k_experts<T, MODE, TL, decltype(d)::value><<<(unsigned)blocks, TL::NT, TL::LDS, stream>>>(P, nt);
     });
 }
 
@@ -1049,7 +1071,7 @@ void run_grads(const ExpertArgs& P, const ExpertSizes& z, bool dma, hipStream_t 
         G.first[0] = (uint32_t)dx;
         G.first[1] = (uint32_t)(dx + in);
         k_expert_grads<T, TL, decltype(d)::value>
-            <<<(unsigned)(dx + in + out), TL::NT, TL::STAGES * TL::STAGE, stream>>>(P, G);
+            <<<(unsigned)(dx + in + out), TL::NT, TL::LDS, stream>>>(P, G);
     });
 }
 
