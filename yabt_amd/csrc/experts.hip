@@ -137,39 +137,49 @@ __device__ __forceinline__ void stage_ready() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LATER) : "memory");
 }
 
-// Row tile `id` of the slots in tiles of BM per expert; total: their number.
-struct TileAt {
-    int e, mi;
-};
-__device__ __forceinline__ int tiles_total(const int32_t* off, int E, int BM) {
-    const int lane = threadIdx.x & 63;
-    int t = 0;
-    for (int e = lane; e < E; e += 64) t += (off[e + 1] - off[e] + BM - 1) / BM;
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) t += __shfl_xor(t, m);
-    return t;
-}
-__device__ __forceinline__ TileAt tile_find(const int32_t* off, int E, int BM, int id) {
-    const int lane = threadIdx.x & 63;
-    int carry = 0;
-    for (int e0 = 0; e0 < E; e0 += 64) {
-        const int e = e0 + lane;
-        const int c = e < E ? (off[e + 1] - off[e] + BM - 1) / BM : 0;
-        int t = c;
+// The slots' row tiles, BM slots of one expert each: a lane counts those of
+// expert e0 + lane, and up to 64 experts are read once.
+struct RowTiles {
+    const int32_t* off;
+    int E, BM;
+    int first, count, upto;           // of the 64 experts in view: this lane's first slot, slots, and tiles up to it
+    __device__ __forceinline__ void view(int e0) {
+        const int lane = threadIdx.x & 63, e = e0 + lane;
+        first = e < E ? off[e] : 0;
+        count = e < E ? off[e + 1] - first : 0;
+        upto = (count + BM - 1) / BM;
 #pragma unroll
         for (int m = 1; m < 64; m <<= 1) {
-            const int o = __shfl_up(t, m);
-            if (lane >= m) t += o;
+            const int o = __shfl_up(upto, m);
+            if (lane >= m) upto += o;
         }
-        const uint64_t hit = __ballot(id < carry + t);
-        if (hit) {
-            const int l = __ffsll((unsigned long long)hit) - 1;
-            return {e0 + l, id - carry - __shfl(t - c, l)};
-        }
-        carry += __shfl(t, 63);
     }
-    return {-1, 0};
-}
+    __device__ __forceinline__ int total() {
+        int t = 0;
+        for (int e0 = 0; e0 < E; e0 += 64) {
+            view(e0);
+            t += __shfl(upto, 63);
+        }
+        return t;
+    }
+    // Tile id < total(): its expert, first place and slots.
+    __device__ __forceinline__ void find(int id, int* e, int* p0, int* slots) {
+        int carry = 0;
+        for (int e0 = 0;; e0 += 64) {
+            if (E > 64) view(e0);
+            const uint64_t hit = __ballot(id < carry + upto);
+            if (hit) {
+                const int l = __ffsll((unsigned long long)hit) - 1;
+                const int c = __shfl(count, l), mi = id - carry - (__shfl(upto, l) - (c + BM - 1) / BM);
+                *e = e0 + l;
+                *p0 = __shfl(first, l) + mi * BM;
+                *slots = min(BM, c - mi * BM);
+                return;
+            }
+            carry += __shfl(upto, 63);
+        }
+    }
+};
 
 // The block's place in a grid that is walked die by die: consecutive tiles on
 // one die, whose L2 then holds the rows and weights they share.
@@ -447,16 +457,14 @@ __device__ __forceinline__ void expert_tile(const ExpertArgs& P, uint32_t block,
     int e, p0, count, mf = 0, nf, split = 0, my_slot = 0;
     float my_w = 1.0f;
     if constexpr (ROWS) {
-        const int total = tiles_total(P.offsets, P.E, TL::BM);
+        RowTiles tiles{P.offsets, P.E, TL::BM};
+        const int total = tiles.total();
         const int64_t all = (int64_t)total * ntiles, id = die_order(block, all);
         if (id >= all) return;
         const int group = (int)(id / ((int64_t)TILE_GROUP * ntiles));
         const int in = (int)(id - (int64_t)group * TILE_GROUP * ntiles);
         const int gm = min(TILE_GROUP, total - group * TILE_GROUP);
-        const TileAt t = tile_find(P.offsets, P.E, TL::BM, group * TILE_GROUP + in % gm);
-        e = t.e;
-        p0 = P.offsets[e] + t.mi * TL::BM;
-        count = min(TL::BM, P.offsets[e + 1] - p0);
+        tiles.find(group * TILE_GROUP + in % gm, &e, &p0, &count);
         nf = in / gm * (MODE == IN ? TL::BN / 2 : TL::BN);
         // a row a thread, kept until the sums are there
         if constexpr (MODE != IN) {

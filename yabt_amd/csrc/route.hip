@@ -22,6 +22,8 @@
 #include "expert.h"
 #include "yabt_hip.h"
 
+#include <cfloat>
+
 namespace yabt {
 
 constexpr int ROUTE_NT = 256;
@@ -50,13 +52,14 @@ __device__ __forceinline__ void sigmoids(const float (&x)[N], float (&p)[N]) {
     }
 }
 
-// (key, e) as one double that orders by key, then by lower e; -inf carries no e.
+// (key, e) as one double that orders by key, then by lower e; a key of -inf
+// carries no e, +inf counts as the largest number.
 __device__ __forceinline__ double key_pack(float key, int e) {
-    if (!(key > YABT_NEG_INF)) return -__builtin_inf();
-    key += 0.0f;                                    // -0 is 0
-    const double d = key == __builtin_inff() ? 0x1p128 : (double)key;
-    const uint64_t low = (uint64_t)(key >= 0.0f ? ROUTE_MAX_E - 1 - e : e);
-    return __longlong_as_double((long long)((uint64_t)__double_as_longlong(d) | low));
+    key = fminf(key, FLT_MAX) + 0.0f;               // -0 is 0
+    const uint64_t u = (uint64_t)__double_as_longlong((double)key);
+    // the lower e is larger in front of a positive key and smaller in front of a negative one
+    const uint32_t low = (uint32_t)(ROUTE_MAX_E - 1 - e) ^ ((uint32_t)((int32_t)__float_as_uint(key) >> 31) & (ROUTE_MAX_E - 1));
+    return __longlong_as_double((long long)(u | (key == YABT_NEG_INF ? 0u : low)));
 }
 __device__ __forceinline__ int key_expert(double m) {
     const uint64_t u = (uint64_t)__double_as_longlong(m);
@@ -235,7 +238,7 @@ __global__ void __launch_bounds__(ROUTE_NT) k_route(RouteArgs A, const void* __r
                 float a = YABT_NEG_INF, b = YABT_NEG_INF;     // the lane's, then its group's two largest keys
 #pragma unroll
                 for (int i = 0; i < NV; ++i) {
-                    b = fmaxf(b, fminf(a, key[i]));
+                    b = __builtin_amdgcn_fmed3f(a, b, key[i]);        // a >= b
                     a = fmaxf(a, key[i]);
                 }
                 const int q = A.per_group / NV;
