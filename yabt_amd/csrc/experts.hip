@@ -393,9 +393,11 @@ struct Loader {
         }
     }
 
+    // pieces LO .. HI - 1 of the step from k0 on
+    template <int LO = 0, int HI = COUNT>
     __device__ __forceinline__ void fill(const ExpertArgs& P, int k0, int len, uint32_t lds) const {
 #pragma unroll
-        for (int i = 0; i < COUNT; ++i) {
+        for (int i = LO; i < HI; ++i) {
             const T* p = at(P, i, k0, len);
             const uint32_t base = lds + (uint32_t)(i * NT * 16) + ((threadIdx.x & ~63u) << 4);
             lds_fill(p ? (const void*)p : (const void*)&g_zeros, __builtin_amdgcn_readfirstlane(base));
@@ -513,14 +515,18 @@ __device__ __forceinline__ void expert_tile(const ExpertArgs& P, uint32_t block,
     if (steps > 0) {
         la.init(P, e, p0, count, mf);
         lb.init(P, e, p0, count, nf);
-        // Step t of the rows' operand lies at place t % AS, of the columns' at t % BS.
-        // A step is sent as soon as its place is free: the columns' BS, then the
-        // rows' AS steps ahead.  For operands whose rows are looked up the rows of
-        // the step after are asked for first, so that a wait for them is none for
-        // the pieces.  Steps past the last are sent too (zeros), so that every wait
-        // is the same.  Without DMA a step waits in registers for its place.
-        constexpr int AS = DMA ? TL::AS : 2, BS = 2;
-        static_assert(TL::BS == 2, "two places for the columns' steps");
+        // Step t of the rows' operand lies at place t % AS, of the columns' at t % 2.
+        // The columns' step t + 2 is sent as soon as its place is free, at the end of
+        // step t; the rows' step t + 2 there too, or, with a third place, in two
+        // halves between the products of step t: a wave that sends waits for the
+        // address units, which take a piece of 1 KB in 16 cycles for the whole CU,
+        // and multiplies nothing meanwhile.  For operands whose rows are looked up
+        // the rows of the step after are asked for first, so that a wait for them is
+        // none for the pieces.  Steps past the last are sent too (zeros), so that
+        // every wait is the same.  Without DMA a step waits in registers for its place.
+        constexpr int AS = DMA ? TL::AS : 2;
+        constexpr bool HALVES = AS == 3;
+        static_assert(TL::BS == 2 && (AS == 2 || AS == 3), "places that the order of the steps is made for");
         u32x4 ra[DMA ? 1 : TL::NA], rb[DMA ? 1 : TL::NB];
         auto send_a = [&](int t, int place) {
             la.move_on();
@@ -541,12 +547,12 @@ __device__ __forceinline__ void expert_tile(const ExpertArgs& P, uint32_t block,
         la.look_up(P, p0, count, 0);
         lb.look_up(P, p0, count, 0);
         // accesses of every wave after step 0's and, in the loop, after the next step's
-        constexpr int AFTER_0 = DMA ? (AS - 1) * TL::NA + (BS - 1) * TL::NB : 0, AFTER = DMA ? (AS - BS) * TL::NA : 0;
+        constexpr int AFTER_0 = DMA ? TL::NA + TL::NB : 0, AFTER = HALVES ? TL::NA : 0;
         if constexpr (DMA) {
 #pragma unroll
-            for (int t = 0; t < AS; ++t) {
+            for (int t = 0; t < 2; ++t) {
                 send_a(t, t);
-                if (t < BS) send_b(t);
+                send_b(t);
             }
         } else {
             send_a(0, 0);
@@ -575,16 +581,26 @@ __device__ __forceinline__ void expert_tile(const ExpertArgs& P, uint32_t block,
         // k-step's products, and what takes the freed places is sent there.
         int place = 0;
         for (int t = 0; t < steps; ++t) {
-            const int next = place + 1 == AS ? 0 : place + 1;
+            const int next = place + 1 == AS ? 0 : place + 1, free = next + 1 == AS ? 0 : next + 1;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 if (ks + 1 < KS) {
+                    if constexpr (HALVES) {
+                        const uint32_t to = lds_at + (uint32_t)free * TL::ABYTES;
+                        if (ks == 0) {
+                            la.move_on();
+                            la.look_up(P, p0, count, (t + 3) * BK);
+                            la.template fill<0, TL::NA / 2>(P, (t + 2) * BK, ka, to);
+                        } else if (ks == 1) {
+                            la.template fill<TL::NA / 2, TL::NA>(P, (t + 2) * BK, ka, to);
+                        }
+                    }
                     read(place, t, ks + 1);
                 } else {
                     if constexpr (!DMA) put(t + 1);
                     stage_ready<AFTER>();
                     send_b(t + 2);
-                    send_a(t + AS, place);
+                    if constexpr (!HALVES) send_a(t + 2, place);
                     read(next, t + 1, 0);
                 }
 #pragma unroll
