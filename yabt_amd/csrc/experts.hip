@@ -25,6 +25,17 @@
 // dimension are read with the transposing LDS loads.  Inputs whose rows are
 // not 16-byte aligned pass through registers instead.
 //
+// 16 384 x 2048 rows, 2 of 8 experts of 2048, bf16 (550 GFLOP for h, 275 for y and the
+// inner gradient, 1375 for the other three): 0.60, 0.32, 0.51 and 1.58 ms, the matrix
+// cores at work 59, 61, 34 and 50% of the CUs' busy time; the library's plain
+// product of 275 GFLOP alone takes 0.21 ms.  What is between them: a block has its
+// CU to itself (its sums are 256 KB of registers), so that what a tile reads and
+// writes besides (h with the kept g and u 0.67 GB, the inner gradient 0.95 GB) and its
+// first loads are not covered, a quarter of what the steps take comes from behind
+// L2 (h: 1.1 of 4.3 GB), and the experts' last tiles are partly empty.  Two blocks
+// of 128 x 256 a CU, which cover each other, fetch half more: 0.69, 0.36, 0.52 and
+// 1.80 ms.
+//
 // h, w h, dg and du are rounded to the inputs' type, as the matrix cores take
 // them; g and u are kept in fp32 for the backward pass, and z and the parts of
 // dx are added in fp32: so each output has two roundings behind it, its own
@@ -744,6 +755,9 @@ __global__ void __launch_bounds__(TL::NT) k_expert_grads(ExpertArgs P, GradGrid 
 //   k_answer_few  y: a block has 16 columns of all rows; its waves share the
 //                 experts in use, and the weighted answers of a row's slots
 //                 are added up in LDS
+// One row, 6 of 64 experts, 1024 -> 512 -> 1024, bf16: 6.8 and 7.6 us, mostly launch and
+// three dependent loads before the weights' first (19 MB); h of 48 rows, 2048 -> 1024,
+// all of 32 experts: 62 us for 268 MB, 4.3 TB/s.
 // ---------------------------------------------------------------------------
 
 template <typename T>
@@ -791,7 +805,7 @@ __device__ __forceinline__ int expert_in_use(const int32_t* off, int E, int j) {
 
 constexpr int FEW_NT = 256, FEW_W = FEW_NT / 64;
 constexpr int FEW_AHEAD = 4;                     // 128-byte pieces of a row under way in a wave
-constexpr int FEW_SLOTS = 512;                   // slots whose answers a block keeps in LDS
+constexpr int FEW_SLOTS = 128;                   // slots whose answers a block keeps in LDS
 
 // acc[m] += M matrices' 16 rows w[m] times the 16 slots' x, from piece `from` on, every `by`-th.
 template <typename T, int M>
@@ -929,7 +943,8 @@ __device__ __forceinline__ void add_parts(const float* part, int64_t count, int 
 // What is left once the tiles are made: out[t] = sum_j z[t k + j] over row t's
 // slots that have an expert (k = 1: zeros for rows without one, the others are
 // there), and in the backward pass dw = the sum of its parts and the weights'
-// gradients of theirs.
+// gradients of theirs.  z in fp32 because y is a sum; 16 384 x 2048, k = 2: 67 us,
+// 5.0 TB/s, a copy's rate.
 template <typename T>
 __global__ void __launch_bounds__(256) k_finish(ExpertArgs P) {
     T* const out = (T*)P.out;
@@ -1107,17 +1122,20 @@ void run_finish(const ExpertArgs& P, const ExpertSizes& z, hipStream_t stream) {
 }
 
 // The kernels for few rows by the slots an expert in use has on average.  They
-// pass over the weights once per 16 slots, the tiles once per 128 with a tile's
+// pass over the weights once per 16 slots, the tiles once per 64 with a tile's
 // whole arithmetic, which fp32 does at a sixteenth of the rate.  h, few and
-// tiles: 2048 -> 1024 of 32 experts, fp16, 6 slots each 62 and 66 us, 16 each
-// 102 and 72; 1024 -> 512 of 64, bf16, one row's 6 slots 6 and 12 us, 192 slots
-// 20 and 21; 500 -> 101 of 4, fp32, 25 each 13 and 45 us.
+// tiles, us: 2048 -> 1024 of 32 experts, fp16, 6 slots each 61 and 66, 12 each 79
+// and 70; 1024 -> 512 of 64, bf16, one row's 6 slots 6 and 10, 3 each 20 and 19,
+// 6 each 24 and 21; of 8, fp32, 4 each 14 and 40, 32 each 35 and 41; 500 -> 101 of
+// 4, fp32, 25 each 12 and 28, 50 each 19 and 28.
 inline bool few_inner(int64_t S, int E, int bytes) {
     const int64_t used = S < E ? S : E;
     return S <= used * (bytes == 4 ? 32 : 8);
 }
-// y, few and tiles with k_finish: one row's 6 slots 6.6 and 12.7 us, two rows' 12
-// slots 11 and 14, 8 rows' 48 slots 26 and 18 (a wave has several experts in turn).
+// y, few and tiles with k_finish, us: bf16, one row's 6 slots 6.8 and 11.4, two rows'
+// 12 slots 11.3 and 12.1, 8 rows' 48 slots of about 33 experts, so that a wave
+// has several in turn, 26 and 15; fp32 of 8 experts 32 slots 15 and 27, 128 slots
+// 26 and 27, 256 slots 44 and 27.
 inline bool few_answer(int64_t S, int E, int bytes) {
     return few_inner(S, E, bytes) && S <= FEW_SLOTS && (S < E ? S : E) <= 16;
 }

@@ -17,7 +17,11 @@
 // log2 G times; else a round takes the largest of the G heads over DPP and the
 // winner drops its head, k times.
 //
-// What bounds it is instructions, not memory: ROUTE_FIGURES
+// What bounds it is instructions, not memory: 65 536 rows of 256 bf16 logits,
+// sigmoid, 8 experts in 4 of 8 groups, take 44 us, of which the VALU issues for 40
+// (1258 instructions a wave of 4 rows, a third of them the exponentials; 38 MB
+// are 7 us of a copy).  72 us with k rounds in place of the merge, the
+// compiler's division and the groups' keys scanned in LDS.
 
 #include "expert.h"
 #include "yabt_hip.h"
@@ -341,6 +345,9 @@ __global__ void __launch_bounds__(ROUTE_NT) k_route(RouteArgs A, const void* __r
 //   softmax:  dl_i = p_i ([i chosen] dw_i - sum_chosen p dw)
 //   sigmoid, renormalised: v = p / t, dl_j = (dw_j - sum v dw) / t p_j (1 - p_j)
 //   sigmoid:  dl_j = dw_j p_j (1 - p_j)                    with dw scaled by `scale`
+// A row's gradient is put together in LDS, so that it leaves in whole lines
+// whatever experts were chosen.  8191 x 60 fp32, k = 4: 4.8 us, a launch's length
+// and its loads' latency (4 MB).
 template <typename T, int G, int NV>
 __global__ void __launch_bounds__(ROUTE_NT) k_route_grad(RouteArgs A, const float* __restrict__ dweights, int64_t lddw,
                                                          const T* __restrict__ logits,
