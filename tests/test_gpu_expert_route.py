@@ -163,6 +163,12 @@ def test_plan(n, k, E):
     assert got.experts == E
 
 
+@pytest.mark.parametrize("n,k,E", [(8193, 1, 2), (65_536, 2, 64), (131_073, 1, 64), (16_384, 4, 512), (16_385, 4, 513),
+                                   (16_400, 8, 1024)])
+def test_plan_of_few_and_many_blocks(n, k, E):
+    test_plan(n, k, E)
+
+
 def test_nothing_routed():
     plan_ = X.expert_plan(torch.full((10, 2), -1, dtype=torch.int32, device="cuda"), 4)
     assert plan_.offsets.tolist() == [0] * 5 and plan_.slots.tolist() == [-1] * 20

@@ -407,15 +407,20 @@ __global__ void __launch_bounds__(ROUTE_NT) k_route_grad(RouteArgs A, const floa
 // a slot's rank is its wave's count so far plus the lanes before it with the
 // same expert, which one ballot per bit of the expert's number finds.  Up to
 // PLAN_ONE slots are sorted in one block's LDS, in one launch; more are counted
-// by blocks, the counts' prefix taken per expert, then ranked and placed: 32 764
-// slots of 60 experts take 12.6 us in these three launches and 30 in one block,
-// whose CU alone is bound by the ballots.
+// by blocks, then ranked and placed: 32 764 slots of 60 experts take 12.6 us with a
+// launch between that takes the counts' prefix per expert, and 30 in one block,
+// whose CU alone is bound by the ballots.  Few blocks take the prefix each by
+// itself, without the launch between, us of kernels with and without it: 20 000
+// slots of 7 experts 13.1 and 9.3, 131 072 of 64 13.9 and 11.0, 65 536 of 1024 17.4 and
+// 16.1; many do not, 524 288 of 256 18.8 and 24.3.
 // ---------------------------------------------------------------------------
 
 constexpr int PLAN_NT = 512, PLAN_R = 4;
 constexpr int PLAN_TILE = PLAN_NT * PLAN_R;      // slots a block ranks at a time
 constexpr int PLAN_BLOCKS = 1024;                // blocks at most
 constexpr int PLAN_ONE = 8192;                   // slots one block sorts, at most
+constexpr int PLAN_FEW = 64;                     // blocks that add up each other's counts, at most,
+constexpr int PLAN_FEW_COUNTS = 32768;           // and their counts
 constexpr size_t PLAN_LDS = 156 * 1024;
 
 // LDS of one block of nt threads that sorts S slots.
@@ -518,7 +523,8 @@ __global__ void __launch_bounds__(PLAN_NT) k_plan_scan(PlanArgs A, uint32_t* __r
     if (threadIdx.x == 0) tot[blockIdx.x] = carry;
 }
 
-// ONE: the only block, whose own counts are all there is; else after k_plan_scan.
+// ONE: the only block, whose own counts are all there is; else after k_plan_scan,
+// or, tot NULL, from all blocks' counts as they are.
 template <int NT, int R, int BITS, bool ONE>
 __global__ void __launch_bounds__(NT) k_plan_place(PlanArgs A, const uint32_t* __restrict__ cnt,
                                                    const uint32_t* __restrict__ tot, int32_t* __restrict__ offsets,
@@ -533,17 +539,29 @@ __global__ void __launch_bounds__(NT) k_plan_place(PlanArgs A, const uint32_t* _
     auto experts_places = [&]() {
         for (int e0 = 0; e0 < A.E; e0 += NT) {
             const int e = e0 + threadIdx.x;
-            uint32_t mine = 0, all;
+            uint32_t mine = 0, before = 0, all;
             if (e < A.E) {
-                if (!ONE) mine = tot[e];
-                else
+                if (ONE) {
                     for (int w = 0; w < W; ++w) mine += s_cnt[w * A.E + e];
+                } else {
+                    const uint32_t* c = cnt + (size_t)e * A.blocks;
+                    if (tot) {
+                        mine = tot[e];
+                        before = c[blockIdx.x];
+                    } else {
+#pragma unroll 8
+                        for (int b = 0; b < A.blocks; ++b) {
+                            mine += c[b];
+                            before += b < (int)blockIdx.x ? c[b] : 0u;
+                        }
+                    }
+                }
             }
             const uint32_t at = carry + plan_scan<NT>(mine, s_w, &all);
             carry += all;
             if (e < A.E) {
                 if (blockIdx.x == 0) offsets[e] = (int32_t)at;
-                s_next[e] = ONE ? at : at + cnt[(size_t)e * A.blocks + blockIdx.x];
+                s_next[e] = at + before;
             }
         }
         if (blockIdx.x == 0 && threadIdx.x == 0) offsets[A.E] = (int32_t)carry;
@@ -620,8 +638,10 @@ void run_plan(const PlanArgs& A, uint32_t* cnt, int32_t* offsets, int32_t* slots
     if (A.blocks > 1) {
         uint32_t* tot = cnt + (size_t)A.blocks * A.E;
         k_plan_count<<<A.blocks, PLAN_NT, (size_t)A.E * sizeof(uint32_t), st>>>(A, cnt);
-        k_plan_scan<<<A.E, PLAN_NT, 0, st>>>(A, cnt, tot);
-        k_plan_place<PLAN_NT, PLAN_R, BITS, false><<<A.blocks, PLAN_NT, lds(PLAN_NT), st>>>(A, cnt, tot, offsets, slots, rows);
+        const bool scan = A.blocks > PLAN_FEW || A.blocks * A.E > PLAN_FEW_COUNTS;
+        if (scan) k_plan_scan<<<A.E, PLAN_NT, 0, st>>>(A, cnt, tot);
+        k_plan_place<PLAN_NT, PLAN_R, BITS, false>
+            <<<A.blocks, PLAN_NT, lds(PLAN_NT), st>>>(A, cnt, scan ? tot : nullptr, offsets, slots, rows);
     } else {
         auto one = [&](auto nt, auto r) {
             constexpr int NT = decltype(nt)::value, R = decltype(r)::value;
