@@ -125,6 +125,22 @@ def test_rows_without_an_expert(k, dt):
 
 
 @pytest.mark.parametrize("dt", TYPES, ids=name)
+def test_one_slot_a_row_writes_every_row(dt):
+    """k = 1 in tiles: rows without an expert, single, in runs and at the end, in
+    memory that held NaN before."""
+    n, D, F, E = 1500, 70, 40, 3
+    args = list(inputs(n, D, F, E, 1, dt, 9))
+    for rows in (slice(0, 1), slice(100, 400), slice(1499, 1500), slice(700, 900, 2)):
+        args[1][rows] = -1
+        args[2][rows] = 0.0
+    out = torch.full((n, D), float("nan"), dtype=dt, device="cuda")
+    del out                                           # y is likely to get this memory
+    got = check(args)
+    empty = (args[1] < 0).flatten()
+    assert torch.all(got["y"].cpu()[empty] == 0) and torch.all(got["dx"].cpu()[empty] == 0)
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=name)
 def test_nothing_leaks_between_rows_and_experts(dt):
     """NaN in an unused expert's weights and in a row of its own stay there, at
     sizes that end inside pieces, steps and tiles."""

@@ -725,8 +725,28 @@ __device__ __forceinline__ void expert_tile(const ExpertArgs& P, uint32_t block,
     }
 }
 
+// k = 1: the rows that have no expert, to which no tile writes, become zero; a
+// wave writes those among its 64 rows one after the other.
+template <typename T, int NT>
+__device__ __forceinline__ void zero_rows(const ExpertArgs& P) {
+    for (int64_t t0 = (int64_t)blockIdx.x * NT; t0 < P.n; t0 += (int64_t)gridDim.x * NT) {
+        const int64_t t = t0 + threadIdx.x;
+        const int e = t < P.n ? P.ids[t] : 0;
+        uint64_t left = __ballot(e < 0 || e >= P.E);
+        while (left) {
+            const int l = __ffsll((unsigned long long)left) - 1;
+            left &= left - 1;
+            T* const row = (T*)P.out + (size_t)(t0 + (threadIdx.x & ~63) + l) * (size_t)P.ldo;
+            for (int d = threadIdx.x & 63; d < P.D; d += 64) row[d] = (T)0.0f;
+        }
+    }
+}
+
 template <typename T, int MODE, typename TL, bool DMA>
 __global__ void __launch_bounds__(TL::NT) k_experts(ExpertArgs P, int ntiles) {
+    // y of one slot a row is made here whole, without a launch of k_finish
+    if constexpr (MODE == OUT)
+        if (P.k == 1) zero_rows<T, TL::NT>(P);
     expert_tile<T, MODE, TL, DMA>(P, blockIdx.x, ntiles, 0);
 }
 
@@ -941,8 +961,8 @@ __device__ __forceinline__ void add_parts(const float* part, int64_t count, int 
 }
 
 // What is left once the tiles are made: out[t] = sum_j z[t k + j] over row t's
-// slots that have an expert (k = 1: zeros for rows without one, the others are
-// there), and in the backward pass dw = the sum of its parts and the weights'
+// slots that have an expert (k = 1, dx alone: zeros for rows without one, the others
+// are there), and in the backward pass dw = the sum of its parts and the weights'
 // gradients of theirs.  z in fp32 because y is a sum; 16 384 x 2048, k = 2: 67 us,
 // 5.0 TB/s, a copy's rate.
 template <typename T>
@@ -962,18 +982,7 @@ __global__ void __launch_bounds__(256) k_finish(ExpertArgs P) {
             store_part(out + (size_t)t * (size_t)P.ldo + d, s, P.D - d);
         }
     } else {
-        for (int64_t t0 = (int64_t)blockIdx.x * 256; t0 < P.n; t0 += (int64_t)gridDim.x * 256) {
-            const int64_t t = t0 + threadIdx.x;
-            const int e = t < P.n ? P.ids[t] : 0;
-            // a wave writes its rows without an expert one after the other
-            uint64_t left = __ballot(e < 0 || e >= P.E);
-            while (left) {
-                const int l = __ffsll((unsigned long long)left) - 1;
-                left &= left - 1;
-                const int64_t row = t0 + (threadIdx.x & ~63) + l;
-                for (int d = threadIdx.x & 63; d < P.D; d += 64) out[(size_t)row * (size_t)P.ldo + d] = (T)0.0f;
-            }
-        }
+        zero_rows<T, 256>(P);
     }
     if (!P.dweights) return;
     const int64_t S = P.n * P.k;
@@ -1150,7 +1159,7 @@ int run_experts(const ExpertArgs& P, const ExpertSizes& z, bool dma, hipStream_t
         k_answer_few<T><<<(unsigned)over(P.D, 16), ANSWER_NT, 0, stream>>>(P, (T*)P.out, P.ldo);
     } else {
         run_tiles<T, OUT>(P, z, z.large[1], dma, stream);
-        run_finish<T>(P, z, stream);
+        if (P.k > 1) run_finish<T>(P, z, stream);
     }
     return launch_status("yabt_experts");
 }
