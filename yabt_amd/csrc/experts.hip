@@ -32,9 +32,9 @@
 // CU to itself (its sums are 256 KB of registers), so that what a tile reads and
 // writes besides (h with the kept g and u 0.67 GB, the inner gradient 0.95 GB) and its
 // first loads are not covered, a quarter of what the steps take comes from behind
-// L2 (h: 1.1 of 4.3 GB), and the experts' last tiles are partly empty.  Two blocks
-// of 128 x 256 a CU, which cover each other, fetch half more: 0.69, 0.36, 0.52 and
-// 1.80 ms.
+// L2 (h: 1.1 of 4.3 GB), the experts' last tiles are partly empty, and so is the last
+// round of 256 tiles (h has 8.5, y 4.25).  Two blocks of 128 x 256 a CU, which cover
+// each other, fetch half more: 0.69, 0.36, 0.52 and 1.80 ms.
 //
 // h, w h, dg and du are rounded to the inputs' type, as the matrix cores take
 // them; g and u are kept in fp32 for the backward pass, and z and the parts of
