@@ -11,7 +11,8 @@ the booster's predictions as they are:
     stage = ExpertStage(ExpertParams(experts=16, k=2), LogLoss()).fit(X, y, margin)
     stage.predict_margin(X_new, booster.predict_margin(X_new))
 
-Per row, with x the standardised inputs (missing ones at their mean, 0):
+Per row, with x the standardised inputs (missing ones at their mean, 0, and
+columns that the fit saw no spread in always 0):
 
     r = x A;  a = layer_norm(r);  ids, weights = route(a G, k);
     out = (r + sum_j weights_j expert_{ids_j}(a)) h
@@ -52,6 +53,27 @@ class ExpertParams:
 _DTYPES = {"float32": torch.float32, "bfloat16": torch.bfloat16, "float16": torch.float16}
 
 
+def _statistics(raw: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Mean and spread of the values of each column of raw (n, F).  A
+    column whose values differ by their last bits alone, or that has none, has an
+    infinite spread: whatever comes later, its input is 0, as in the fit, which
+    learned nothing about it.  Sums are taken in units of the power of two below
+    a column's largest value, so that no square leaves float32."""
+    if raw.shape[0] == 0:
+        return raw.new_zeros(raw.shape[1]), raw.new_full((raw.shape[1],), float("inf"))
+    seen = ~torch.isnan(raw)
+    count = seen.sum(dim=0).clamp_min(1)
+    high = torch.where(seen, raw, float("-inf")).amax(dim=0)
+    low = torch.where(seen, raw, float("inf")).amin(dim=0)
+    most = torch.where(seen, raw.abs(), 0.0).amax(dim=0)
+    unit = (most.view(torch.int32) & 0x7F800000).view(torch.float32).clamp_min(2.0 ** -126)
+    mean = torch.where(seen, raw / unit, 0.0).sum(dim=0) / count
+    spread = torch.where(seen, raw / unit - mean, 0.0).square().sum(dim=0) / count
+    std = spread.sqrt() * unit
+    flat = ~(high - low > 2.0 ** -22 * most) | (std == 0.0)
+    return mean * unit, torch.where(flat, float("inf"), std)
+
+
 class ExpertStage:
     """See the module's text; ``loss`` as a ``Booster`` takes it."""
 
@@ -73,7 +95,8 @@ class ExpertStage:
         Xt = torch.as_tensor(np.asarray(X, dtype=np.float32), device=self.device_)
         if Xt.dim() != 2 or Xt.shape[1] != self.mean_.shape[0]:
             raise ValueError(f"X must be (n, {self.mean_.shape[0]}), got {tuple(Xt.shape)}")
-        return torch.nan_to_num((Xt - self.mean_) / self.std_, nan=0.0)
+        x = torch.where(torch.isfinite(self.std_), (Xt - self.mean_) / self.std_, 0.0)
+        return torch.nan_to_num(x, nan=0.0)
 
     def _forward(self, x: torch.Tensor, keep: bool):
         """(out (n,), what the backward pass needs)."""
@@ -115,12 +138,7 @@ class ExpertStage:
         X = np.asarray(X, dtype=np.float32)
         n, F = X.shape
         self.device_ = dev
-        raw = torch.as_tensor(X, device=dev)
-        seen = ~torch.isnan(raw)
-        count = seen.sum(dim=0).clamp_min(1)
-        self.mean_ = torch.where(seen, raw, 0.0).sum(dim=0) / count
-        spread = torch.where(seen, raw - self.mean_, 0.0).square().sum(dim=0) / count
-        self.std_ = spread.sqrt().clamp_min(1e-6)
+        self.mean_, self.std_ = _statistics(torch.as_tensor(X, device=dev))
         x = self._inputs(X)
         yt = torch.as_tensor(np.asarray(y, dtype=np.float32), device=dev)
         base = torch.as_tensor(np.broadcast_to(np.asarray(margin, dtype=np.float32), (n,)).copy(), device=dev)
