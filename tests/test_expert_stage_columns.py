@@ -1,4 +1,4 @@
-"""The stage's column statistics on the CPU: the same
+"""The stage's column statistics on the CPU: those of the finite values, the same
 bits as plain sums for ordinary columns, and no spread where there is none."""
 
 import torch
@@ -17,11 +17,15 @@ def test_ordinary_columns_have_plain_statistics():
     spread = torch.where(seen, raw - mean, 0.0).square().sum(dim=0) / count
     got_mean, got_std = _statistics(raw)
     assert torch.equal(got_mean, mean) and torch.equal(got_std, spread.sqrt())
+    raw[7, 3], raw[8, 3] = INF, -INF
+    clean = raw.clone()
+    clean[7, 3], clean[8, 3] = float("nan"), float("nan")
+    assert all(torch.equal(a, b) for a, b in zip(_statistics(raw), _statistics(clean)))
 
 
 def test_columns_without_spread():
     raw = torch.randn((400, 7), generator=torch.Generator().manual_seed(1))
-    raw[:, 0], raw[:, 1], raw[:, 2], raw[:, 3] = 0.0, 0.1, float("nan"), -2.0
+    raw[:, 0], raw[:, 1], raw[:, 2], raw[:, 3] = 0.0, 0.1, float("nan"), INF
     raw[:, 4] = torch.tensor([1.0, 1.0 + 2.0 ** -23]).repeat(200)
     raw[:, 5] = torch.tensor([1e6, 1e6 + 1.0]).repeat(200)          # small beside its values, and real
     mean, std = _statistics(raw)

@@ -11,8 +11,8 @@ the booster's predictions as they are:
     stage = ExpertStage(ExpertParams(experts=16, k=2), LogLoss()).fit(X, y, margin)
     stage.predict_margin(X_new, booster.predict_margin(X_new))
 
-Per row, with x the standardised inputs (missing ones at their mean, 0, and
-columns that the fit saw no spread in always 0):
+Per row, with x the standardised inputs (missing ones, NaN or infinite, at their
+mean, 0, and columns that the fit saw no spread in always 0):
 
     r = x A;  a = layer_norm(r);  ids, weights = route(a G, k);
     out = (r + sum_j weights_j expert_{ids_j}(a)) h
@@ -53,15 +53,20 @@ class ExpertParams:
 _DTYPES = {"float32": torch.float32, "bfloat16": torch.bfloat16, "float16": torch.float16}
 
 
+# Standardised inputs are held to +-2^40: the squares of a row of them, which the
+# layer norm adds, stay in float32 (a row past that is no row of the fit's table).
+_FAR = 2.0 ** 40
+
+
 def _statistics(raw: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
-    """Mean and spread of the values of each column of raw (n, F).  A
+    """Mean and spread of the finite values of each column of raw (n, F).  A
     column whose values differ by their last bits alone, or that has none, has an
     infinite spread: whatever comes later, its input is 0, as in the fit, which
     learned nothing about it.  Sums are taken in units of the power of two below
     a column's largest value, so that no square leaves float32."""
     if raw.shape[0] == 0:
         return raw.new_zeros(raw.shape[1]), raw.new_full((raw.shape[1],), float("inf"))
-    seen = ~torch.isnan(raw)
+    seen = torch.isfinite(raw)
     count = seen.sum(dim=0).clamp_min(1)
     high = torch.where(seen, raw, float("-inf")).amax(dim=0)
     low = torch.where(seen, raw, float("inf")).amin(dim=0)
@@ -95,8 +100,8 @@ class ExpertStage:
         Xt = torch.as_tensor(np.asarray(X, dtype=np.float32), device=self.device_)
         if Xt.dim() != 2 or Xt.shape[1] != self.mean_.shape[0]:
             raise ValueError(f"X must be (n, {self.mean_.shape[0]}), got {tuple(Xt.shape)}")
-        x = torch.where(torch.isfinite(self.std_), (Xt - self.mean_) / self.std_, 0.0)
-        return torch.nan_to_num(x, nan=0.0)
+        known = torch.isfinite(Xt) & torch.isfinite(self.std_)
+        return torch.where(known, (Xt - self.mean_) / self.std_, 0.0).clamp_(-_FAR, _FAR)
 
     def _forward(self, x: torch.Tensor, keep: bool):
         """(out (n,), what the backward pass needs)."""
