@@ -182,11 +182,12 @@ class ExpertStage:
         return self
 
     def predict_margin(self, X: np.ndarray, margin: np.ndarray | float = 0.0) -> np.ndarray:
-        """margin + the stage's answer for each row."""
+        """margin + the stage's answer for each row; margin (n,) or one number."""
         x = self._inputs(X)
+        base = np.broadcast_to(np.asarray(margin, dtype=np.float32), (x.shape[0],))
         parts = [self._forward(x[lo:lo + (1 << 18)], keep=False)[0] for lo in range(0, x.shape[0], 1 << 18)]
         out = torch.cat(parts) if parts else x.new_zeros(0)
-        return np.asarray(margin, dtype=np.float32) + out.cpu().numpy()
+        return base + out.cpu().numpy()
 
     def loads(self, X: np.ndarray) -> np.ndarray:
         """How many of X's slots each expert gets."""
