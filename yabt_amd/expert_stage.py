@@ -46,6 +46,7 @@ class ExpertParams:
     batch_rows: int = 512
     learning_rate: float = 3e-3
     dtype: str = "float32"        # of the rows and the experts' weights in the passes; parameters are float32
+                                  # ("float16" ends at 65504: a fit or an answer that leaves it is an error)
     random_state: int = 0
     device: str = "cuda"
 
@@ -56,6 +57,29 @@ _DTYPES = {"float32": torch.float32, "bfloat16": torch.bfloat16, "float16": torc
 # Standardised inputs are held to +-2^40: the squares of a row of them, which the
 # layer norm adds, stay in float32 (a row past that is no row of the fit's table).
 _FAR = 2.0 ** 40
+
+# What the rows' gradients are made to add up to before they become float16.  No
+# column of a weight's gradient is larger than that times an inner value and an
+# input, which leaves those 2^10 below the type's 2^16; and of 65536 rows with
+# equal gradients each has 2^-10, which leaves 14 bits above its smallest step 2^-24.
+_HALF_SUM = 2.0 ** 6
+
+# An answer in float16 ends at 65504: the answers are counted in a unit in which
+# the median gradient before the first step is about this, if it is larger.
+_HALF_ANSWER = 2.0 ** 4
+
+
+def _power_of_two(t: torch.Tensor) -> torch.Tensor:
+    """The power of two below each of t's positive normal float32 values."""
+    return (t.view(torch.int32) & 0x7F800000).view(torch.float32)
+
+
+def _half_unit(g: torch.Tensor, head: torch.Tensor) -> torch.Tensor:
+    """The power of two, as a 0-d tensor, that the rows' gradients g head are
+    multiplied by for float16; 1 where they are all 0 or not finite."""
+    total = g.abs().sum() * head.abs().amax()
+    unit = _power_of_two((_HALF_SUM / total).clamp(2.0 ** -100, 2.0 ** 100))
+    return torch.where((total > 0.0) & torch.isfinite(total), unit, 1.0)
 
 
 def _statistics(raw: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -71,7 +95,7 @@ def _statistics(raw: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     high = torch.where(seen, raw, float("-inf")).amax(dim=0)
     low = torch.where(seen, raw, float("inf")).amin(dim=0)
     most = torch.where(seen, raw.abs(), 0.0).amax(dim=0)
-    unit = (most.view(torch.int32) & 0x7F800000).view(torch.float32).clamp_min(2.0 ** -126)
+    unit = _power_of_two(most).clamp_min(2.0 ** -126)
     mean = torch.where(seen, raw / unit, 0.0).sum(dim=0) / count
     spread = torch.where(seen, raw / unit - mean, 0.0).square().sum(dim=0) / count
     std = spread.sqrt() * unit
@@ -103,6 +127,9 @@ class ExpertStage:
         known = torch.isfinite(Xt) & torch.isfinite(self.std_)
         return torch.where(known, (Xt - self.mean_) / self.std_, 0.0).clamp_(-_FAR, _FAR)
 
+    def _head(self) -> torch.Tensor:
+        return self.weights_["head"] if self.unit_ is None else self.weights_["head"] * self.unit_
+
     def _forward(self, x: torch.Tensor, keep: bool):
         """(out (n,), what the backward pass needs)."""
         w, p, dt = self.weights_, self.p, _DTYPES[self.p.dtype]
@@ -114,19 +141,27 @@ class ExpertStage:
         ac, w_in, w_out = a.to(dt), w["w_in"].to(dt), w["w_out"].to(dt)
         if not keep:
             y = expert_ops.expert_products(ac, plan, weights, w_in, w_out)
-            return (r + y) @ w["head"], None
+            return (r + y) @ self._head(), None
         y, inner = expert_ops.expert_products(ac, plan, weights, w_in, w_out, keep_inner=True)
         s = r + y
-        return s @ w["head"], (x, r, mean, rstd, a, logits, ids, plan, weights, ac, w_in, w_out, inner, s)
+        return s @ self._head(), (x, r, mean, rstd, a, logits, ids, plan, weights, ac, w_in, w_out, inner, s)
 
     def _backward(self, g: torch.Tensor, kept) -> dict[str, torch.Tensor]:
         """Gradients of sum_t L_t / n, g = dL/dout, in every parameter."""
         x, r, mean, rstd, a, logits, ids, plan, weights, ac, w_in, w_out, inner, s = kept
         w = self.weights_
         g = g / g.shape[0]
+        if self.unit_ is not None:
+            g = g * self.unit_
         ds = g[:, None] * w["head"]
-        dac, dweights, dw_in, dw_out = expert_ops.expert_products_grad(ds.to(ac.dtype), ac, plan, weights, w_in,
-                                                                       w_out, inner)
+        if ac.dtype == torch.float16:
+            # float16 has too few powers of two for gradients as they come
+            unit = _half_unit(g, w["head"])
+            grads = expert_ops.expert_products_grad((ds * unit).half(), ac, plan, weights, w_in, w_out, inner)
+            dac, dweights, dw_in, dw_out = (t.float() / unit for t in grads)
+        else:
+            dac, dweights, dw_in, dw_out = expert_ops.expert_products_grad(ds.to(ac.dtype), ac, plan, weights, w_in,
+                                                                           w_out, inner)
         dlogits = expert_ops.route_grad(dweights, logits, ids, scores=self.p.scores)
         da = dac.float() + dlogits @ w["gate"]
         dr, dnorm, dshift = expert_ops.layer_norm_grad(da, r, mean, rstd, w["norm"])
@@ -161,6 +196,10 @@ class ExpertStage:
                              w_out=normal(p.experts, p.width, p.inner, scale=p.inner ** -0.5),
                              head=torch.zeros(p.width, device=dev))
         self.bias_ = torch.zeros(p.experts, device=dev)
+        self.unit_ = None             # of the answers, where it is not 1
+        if p.dtype == "float16" and n:
+            g, _ = boost_ops.grad_hess(self.loss, base, yt)
+            self.unit_ = _power_of_two((g.abs().median() / _HALF_ANSWER).clamp(1.0, 2.0 ** 100))
         first = {m: torch.zeros_like(t) for m, t in self.weights_.items()}
         second = {m: torch.zeros_like(t) for m, t in self.weights_.items()}
         step = 0
@@ -179,6 +218,9 @@ class ExpertStage:
                 # experts with more than their share become a little less likely
                 share = kept[7].offsets.diff().float()
                 self.bias_ -= p.balance_step * torch.sign(share - share.mean())
+        if not all(bool(torch.isfinite(t).all()) for t in self.weights_.values()):
+            raise RuntimeError(f"the fit's parameters are not finite: y or margin are not, or passes in {p.dtype} "
+                               "left the type's range")
         return self
 
     def predict_margin(self, X: np.ndarray, margin: np.ndarray | float = 0.0) -> np.ndarray:
@@ -187,6 +229,8 @@ class ExpertStage:
         base = np.broadcast_to(np.asarray(margin, dtype=np.float32), (x.shape[0],))
         parts = [self._forward(x[lo:lo + (1 << 18)], keep=False)[0] for lo in range(0, x.shape[0], 1 << 18)]
         out = torch.cat(parts) if parts else x.new_zeros(0)
+        if not bool(torch.isfinite(out).all()):
+            raise RuntimeError(f"answers are not finite: passes in {self.p.dtype} left the type's range")
         return base + out.cpu().numpy()
 
     def loads(self, X: np.ndarray) -> np.ndarray:
