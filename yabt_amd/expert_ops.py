@@ -30,10 +30,18 @@ SCORES = {"softmax": 0, "sigmoid": 1}
 MAX_EXPERTS, MAX_K, MAX_GROUPS = 1024, 32, 64
 
 
-def _stream(dev: torch.device) -> int:
-    """The current stream's handle; ``torch.cuda.current_stream`` takes 2 us to
-    make an object of it, which a call for one row would notice."""
-    return torch._C._cuda_getCurrentRawStream(dev.index)
+def _call(name: str, dev: torch.device, *args) -> None:
+    """The library's ``name`` with args and dev's current stream, dev being the
+    current device meanwhile: the default stream's handle is 0 on every device,
+    and a launch on it goes to the current one.  ``torch.cuda.current_stream``
+    takes 2 us to make an object of the handle and ``torch.cuda.device`` more,
+    which a call for one row would notice."""
+    lib = _lib.load()
+    if torch._C._cuda_getDevice() == dev.index:
+        _lib.check(getattr(lib, name)(*args, torch._C._cuda_getCurrentRawStream(dev.index)), name)
+    else:
+        with torch.cuda.device(dev):
+            _lib.check(getattr(lib, name)(*args, torch._C._cuda_getCurrentRawStream(dev.index)), name)
 
 
 def _matrix(t: torch.Tensor, what: str, dtype: torch.dtype | None = None) -> torch.Tensor:
@@ -80,9 +88,8 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     w, b = _vector(weight, D, dev, "weight"), _vector(bias, D, dev, "bias")
     y = torch.empty((n, D), dtype=x.dtype, device=dev)
     mean, rstd = torch.empty((2, n), dtype=torch.float32, device=dev).unbind()
-    _lib.check(_lib.load().yabt_layer_norm(DTYPES[x.dtype], x.data_ptr(), _ld(x), n, D, _at(w), _at(b), float(eps),
-                                           y.data_ptr(), D, mean.data_ptr(), rstd.data_ptr(), _stream(dev)),
-               "yabt_layer_norm")
+    _call("yabt_layer_norm", dev, DTYPES[x.dtype], x.data_ptr(), _ld(x), n, D, _at(w), _at(b), float(eps),
+          y.data_ptr(), D, mean.data_ptr(), rstd.data_ptr())
     return y, mean, rstd
 
 
@@ -103,9 +110,8 @@ def layer_norm_grad(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd:
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     dx = torch.empty((n, D), dtype=x.dtype, device=dev)
     dw, db = torch.empty((2, D), dtype=torch.float32, device=dev).unbind()
-    _lib.check(lib.yabt_layer_norm_grad(DTYPES[x.dtype], dy.data_ptr(), _ld(dy), x.data_ptr(), _ld(x), n, D, _at(w),
-                                        mu.data_ptr(), rs.data_ptr(), ws.data_ptr(), nbytes, dx.data_ptr(), D,
-                                        dw.data_ptr(), db.data_ptr(), _stream(dev)), "yabt_layer_norm_grad")
+    _call("yabt_layer_norm_grad", dev, DTYPES[x.dtype], dy.data_ptr(), _ld(dy), x.data_ptr(), _ld(x), n, D, _at(w),
+          mu.data_ptr(), rs.data_ptr(), ws.data_ptr(), nbytes, dx.data_ptr(), D, dw.data_ptr(), db.data_ptr())
     return dx, dw, db
 
 
@@ -142,9 +148,8 @@ def route(logits: torch.Tensor, k: int, *, scores: str = "softmax", bias: torch.
     b = _vector(bias, E, dev, "bias")
     ids = torch.empty((n, k), dtype=torch.int32, device=dev)
     weights = torch.empty((n, k), dtype=torch.float32, device=dev)
-    _lib.check(_lib.load().yabt_route(DTYPES[logits.dtype], logits.data_ptr(), _ld(logits), n, E, int(k), how, _at(b),
-                                      int(groups), int(keep_groups), int(bool(renormalise)), float(scale),
-                                      ids.data_ptr(), weights.data_ptr(), _stream(dev)), "yabt_route")
+    _call("yabt_route", dev, DTYPES[logits.dtype], logits.data_ptr(), _ld(logits), n, E, int(k), how, _at(b),
+          int(groups), int(keep_groups), int(bool(renormalise)), float(scale), ids.data_ptr(), weights.data_ptr())
     return ids, weights
 
 
@@ -163,10 +168,8 @@ def route_grad(dweights: torch.Tensor, logits: torch.Tensor, ids: torch.Tensor, 
         raise ValueError(f"dweights must have shape {(n, k)} on {dev}")
     dweights = _matrix(dweights if dweights.dtype == torch.float32 else dweights.float(), "dweights")
     out = torch.empty((n, E), dtype=logits.dtype, device=dev)
-    _lib.check(_lib.load().yabt_route_grad(DTYPES[logits.dtype], dweights.data_ptr(), _ld(dweights),
-                                           logits.data_ptr(), _ld(logits), ids.data_ptr(), n, E, k, how,
-                                           int(bool(renormalise)), float(scale), out.data_ptr(), E, _stream(dev)),
-               "yabt_route_grad")
+    _call("yabt_route_grad", dev, DTYPES[logits.dtype], dweights.data_ptr(), _ld(dweights), logits.data_ptr(),
+          _ld(logits), ids.data_ptr(), n, E, k, how, int(bool(renormalise)), float(scale), out.data_ptr(), E)
     return out
 
 
@@ -206,8 +209,8 @@ def expert_plan(ids: torch.Tensor, experts: int) -> ExpertPlan:
     # one allocation: the plan's three arrays and the call's workspace behind them
     sizes = (experts + 1, n * k, n * k, nbytes // 4)
     offsets, slots, rows, ws = torch.empty(sum(sizes), dtype=torch.int32, device=dev).split_with_sizes(sizes)
-    _lib.check(lib.yabt_expert_plan(ids.data_ptr(), n, k, experts, ws.data_ptr(), nbytes, offsets.data_ptr(),
-                                    slots.data_ptr(), rows.data_ptr(), _stream(dev)), "yabt_expert_plan")
+    _call("yabt_expert_plan", dev, ids.data_ptr(), n, k, experts, ws.data_ptr(), nbytes, offsets.data_ptr(),
+          slots.data_ptr(), rows.data_ptr())
     return ExpertPlan(ids, offsets, slots, rows)
 
 
@@ -257,10 +260,9 @@ def expert_products(x: torch.Tensor, plan: ExpertPlan, weights: torch.Tensor, w_
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     y = torch.empty((n, D), dtype=x.dtype, device=dev)
     inner = torch.empty((n * k, _inner_width(F)), dtype=torch.float32, device=dev) if keep_inner else None
-    _lib.check(lib.yabt_experts(dt, x.data_ptr(), _ld(x), n, k, D, F, E, plan.ids.data_ptr(), plan.offsets.data_ptr(),
-                                plan.slots.data_ptr(), plan.rows.data_ptr(), weights.data_ptr(), w_in.data_ptr(),
-                                w_out.data_ptr(), ws.data_ptr(), nbytes, _at(inner), y.data_ptr(), D, _stream(dev)),
-               "yabt_experts")
+    _call("yabt_experts", dev, dt, x.data_ptr(), _ld(x), n, k, D, F, E, plan.ids.data_ptr(), plan.offsets.data_ptr(),
+          plan.slots.data_ptr(), plan.rows.data_ptr(), weights.data_ptr(), w_in.data_ptr(), w_out.data_ptr(),
+          ws.data_ptr(), nbytes, _at(inner), y.data_ptr(), D)
     return (y, inner) if keep_inner else y
 
 
@@ -284,9 +286,8 @@ def expert_products_grad(dy: torch.Tensor, x: torch.Tensor, plan: ExpertPlan, we
     dx = torch.empty((n, D), dtype=x.dtype, device=dev)
     dweights = torch.empty((n, k), dtype=torch.float32, device=dev)
     dw_in, dw_out = torch.empty_like(w_in), torch.empty_like(w_out)
-    _lib.check(lib.yabt_experts_grad(dt, dy.data_ptr(), _ld(dy), x.data_ptr(), _ld(x), n, k, D, F, E,
-                                     plan.ids.data_ptr(), plan.offsets.data_ptr(), plan.slots.data_ptr(),
-                                     plan.rows.data_ptr(), weights.data_ptr(), w_in.data_ptr(), w_out.data_ptr(),
-                                     inner.data_ptr(), ws.data_ptr(), nbytes, dx.data_ptr(), D, dweights.data_ptr(),
-                                     dw_in.data_ptr(), dw_out.data_ptr(), _stream(dev)), "yabt_experts_grad")
+    _call("yabt_experts_grad", dev, dt, dy.data_ptr(), _ld(dy), x.data_ptr(), _ld(x), n, k, D, F, E,
+          plan.ids.data_ptr(), plan.offsets.data_ptr(), plan.slots.data_ptr(), plan.rows.data_ptr(),
+          weights.data_ptr(), w_in.data_ptr(), w_out.data_ptr(), inner.data_ptr(), ws.data_ptr(), nbytes,
+          dx.data_ptr(), D, dweights.data_ptr(), dw_in.data_ptr(), dw_out.data_ptr())
     return dx, dweights, dw_in, dw_out

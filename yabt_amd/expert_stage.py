@@ -172,12 +172,18 @@ class ExpertStage:
         """Fit to the loss at margin + out; margin (n,), the booster's on these rows, or one number."""
         self._check()
         p = self.p
+        # "cuda" is the current device, any other is made current while the stage works
         dev = torch.device(p.device if p.device != "cuda" else f"cuda:{torch.cuda.current_device()}")
         if dev.type != "cuda":
             raise RuntimeError("ExpertStage needs a HIP device: the expert layer has no CPU form")
-        X = np.asarray(X, dtype=np.float32)
-        n, F = X.shape
         self.device_ = dev
+        with torch.cuda.device(dev):
+            self._fit(np.asarray(X, dtype=np.float32), y, margin)
+        return self
+
+    def _fit(self, X: np.ndarray, y: np.ndarray, margin: np.ndarray | float) -> None:
+        p, dev = self.p, self.device_
+        n, F = X.shape
         self.mean_, self.std_ = _statistics(torch.as_tensor(X, device=dev))
         x = self._inputs(X)
         yt = torch.as_tensor(np.asarray(y, dtype=np.float32), device=dev)
@@ -221,21 +227,22 @@ class ExpertStage:
         if not all(bool(torch.isfinite(t).all()) for t in self.weights_.values()):
             raise RuntimeError(f"the fit's parameters are not finite: y or margin are not, or passes in {p.dtype} "
                                "left the type's range")
-        return self
 
     def predict_margin(self, X: np.ndarray, margin: np.ndarray | float = 0.0) -> np.ndarray:
         """margin + the stage's answer for each row; margin (n,) or one number."""
-        x = self._inputs(X)
-        base = np.broadcast_to(np.asarray(margin, dtype=np.float32), (x.shape[0],))
-        parts = [self._forward(x[lo:lo + (1 << 18)], keep=False)[0] for lo in range(0, x.shape[0], 1 << 18)]
-        out = torch.cat(parts) if parts else x.new_zeros(0)
+        with torch.cuda.device(self.device_):
+            x = self._inputs(X)
+            base = np.broadcast_to(np.asarray(margin, dtype=np.float32), (x.shape[0],))
+            parts = [self._forward(x[lo:lo + (1 << 18)], keep=False)[0] for lo in range(0, x.shape[0], 1 << 18)]
+            out = torch.cat(parts) if parts else x.new_zeros(0)
         if not bool(torch.isfinite(out).all()):
             raise RuntimeError(f"answers are not finite: passes in {self.p.dtype} left the type's range")
         return base + out.cpu().numpy()
 
     def loads(self, X: np.ndarray) -> np.ndarray:
         """How many of X's slots each expert gets."""
-        x, w = self._inputs(X), self.weights_
-        a = expert_ops.layer_norm(x @ w["embed"], w["norm"], w["shift"])[0]
-        ids, _ = expert_ops.route(a @ w["gate"].t(), self.p.k, scores=self.p.scores, bias=self.bias_)
-        return expert_ops.expert_plan(ids, self.p.experts).offsets.diff().cpu().numpy()
+        with torch.cuda.device(self.device_):
+            x, w = self._inputs(X), self.weights_
+            a = expert_ops.layer_norm(x @ w["embed"], w["norm"], w["shift"])[0]
+            ids, _ = expert_ops.route(a @ w["gate"].t(), self.p.k, scores=self.p.scores, bias=self.bias_)
+            return expert_ops.expert_plan(ids, self.p.experts).offsets.diff().cpu().numpy()
