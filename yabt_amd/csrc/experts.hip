@@ -127,9 +127,21 @@ __device__ __forceinline__ constexpr int spread(int r) {
     return sizeof(T) == 4 ? (r >> 2 & 1) << 3 : bytes == 128 ? (r >> 1 & 1) << 2 : (r & 3) << 2;
 }
 
-// silu by the hardware's exp2 and reciprocal (about one unit each).
-__device__ __forceinline__ float sigmoid_fast(float g) {
-    return __builtin_amdgcn_rcpf(1.0f + __expf(-g));
+// 1 / (1 + exp(-g)), the gates' factor in silu.  fp32: right to a unit for any g.
+// 16 bits: the hardware's exp2 and reciprocal, off by more the larger |g| is, as the
+// rounding of g log2 e counts whole in the exponent (y at most 3 units of 2^-24 for
+// g near 0, 10 to -10, 18 to -20, 59 to -60; with fp32's 3 everywhere): the rounding
+// of h that follows is 2^13 or 2^16 units.  fp32's form costs 20 000 x 100 -> 60 2 of 107 us.
+template <typename T>
+__device__ __forceinline__ float gate_sigmoid(float g) {
+    if constexpr (sizeof(T) == 4) {
+        const float x[1] = {g};
+        float p[1];
+        sigmoids<1>(x, p);
+        return p[0];
+    } else {
+        return __builtin_amdgcn_rcpf(1.0f + __expf(-g));
+    }
 }
 
 // 64 lanes' 16 bytes each from memory to LDS at base (the same for the wave),
@@ -663,7 +675,7 @@ __device__ __forceinline__ void expert_tile(const ExpertArgs& P, uint32_t block,
                 if (m < count && f < P.Fp) {
                     float h[4];
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) h[q] = f + q < P.F ? g[q] * sigmoid_fast(g[q]) * u[q] : 0.0f;
+                    for (int q = 0; q < 4; ++q) h[q] = f + q < P.F ? g[q] * gate_sigmoid<T>(g[q]) * u[q] : 0.0f;
                     store4((T*)P.h + (size_t)(p0 + m) * (size_t)P.Fp + f, h);
                     if (P.pre && f < P.Fi) {
                         float* pre = P.pre + (size_t)(p0 + m) * 2 * (size_t)P.Fi + f;
@@ -696,7 +708,7 @@ __device__ __forceinline__ void expert_tile(const ExpertArgs& P, uint32_t block,
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
                         const bool is = f + q < P.F;
-                        const float s = sigmoid_fast(g[q]), h = g[q] * s * u[q], dh = w * a[q];
+                        const float s = gate_sigmoid<T>(g[q]), h = g[q] * s * u[q], dh = w * a[q];
                         dot += is ? a[q] * h : 0.0f;
                         dg[q] = is ? dh * u[q] * s * (1.0f + g[q] * (1.0f - s)) : 0.0f;
                         du[q] = is ? dh * g[q] * s : 0.0f;
@@ -882,7 +894,7 @@ __global__ void __launch_bounds__(FEW_NT) k_inner_few(ExpertArgs P) {
             if (f < P.Fp) {
                 float h[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) h[i] = f + i < P.F ? g[i] * sigmoid_fast(g[i]) * u[i] : 0.0f;
+                for (int i = 0; i < 4; ++i) h[i] = f + i < P.F ? g[i] * gate_sigmoid<T>(g[i]) * u[i] : 0.0f;
                 store4((T*)P.h + p * (size_t)P.Fp + f, h);
             }
             if (P.pre && f < P.Fi) {

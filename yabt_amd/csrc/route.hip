@@ -36,26 +36,6 @@ constexpr int SOFTMAX = 0, SIGMOID = 1;
 
 #define YABT_NEG_INF (-__builtin_inff())
 
-// p = 1 / (1 + exp(-x)) of N values, the quotient rounded correctly: the
-// hardware's reciprocal (one unit off at most) and one Newton step give it for
-// every divisor from 1 to 2^126 (all were tried), the compiler's division for
-// what is larger, which is rare.
-template <int N>
-__device__ __forceinline__ void sigmoids(const float (&x)[N], float (&p)[N]) {
-    float d[N], most = 0.0f;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        d[i] = 1.0f + expf(-x[i]);
-        most = fmaxf(most, d[i]);
-        const float r = __builtin_amdgcn_rcpf(d[i]);
-        p[i] = fmaf(fmaf(-d[i], r, 1.0f), r, r);
-    }
-    if (most > 0x1p126f) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) p[i] = 1.0f / d[i];
-    }
-}
-
 // (key, e) as one double that orders by key, then by lower e; a key of -inf
 // carries no e, +inf counts as the largest number.
 __device__ __forceinline__ double key_pack(float key, int e) {
