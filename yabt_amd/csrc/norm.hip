@@ -453,21 +453,33 @@ void run_norm(const T* x, int64_t ldx, int64_t n, int D, const float* w, const f
         k_norm_long<T><<<launch_grid(n, 1, 2048), LONG_NT, 0, stream>>>(x, ldx, n, D, w, c, eps, y, ldy, mean, rstd);
 }
 
-// Blocks that walk the rows in the backward pass: each gets a few rows of its
-// own before the parts' traffic (8 D bytes a block, written and read) counts.
-inline int norm_grad_blocks(int64_t n, int rows_per_block) {
-    return launch_grid(n, rows_per_block * 4, NORM_GRAD_BLOCKS);
+// Blocks that walk the rows in the backward pass, a part of the weights' gradients
+// each: a block gets a few rows of its own before the parts' traffic (8 D bytes a
+// block, written and read) counts.  Rows too long for registers: the slices of
+// rows, which `across` blocks share.
+template <typename T>
+int norm_long_across(int D) {
+    return (int)((D + 256 * (int64_t)VEC<T> - 1) / (256 * VEC<T>));
+}
+template <typename T>
+int norm_grad_blocks(int64_t n, int D) {
+    int blocks = 1;
+    const bool fits = norm_shape<T>(D, [&](auto g, auto, auto) {
+        constexpr int G = decltype(g)::value, R = (G < 256 ? 256 : G) / G;
+        blocks = launch_grid(n, R * 4, NORM_GRAD_BLOCKS);
+    });
+    const int across = norm_long_across<T>(D);
+    return fits ? blocks : launch_grid(n, 32, (NORM_GRAD_BLOCKS + across - 1) / across);
 }
 
 template <typename T>
 void run_norm_grad(const T* dy, int64_t lddy, const T* x, int64_t ldx, int64_t n, int D, const float* w,
                    const float* mean, const float* rstd, float* part, T* dx, int64_t lddx, float* dw, float* dc,
                    hipStream_t stream) {
-    int blocks = 1;
+    const int blocks = norm_grad_blocks<T>(n, D);
     const bool fits = norm_shape<T>(D, [&](auto g, auto nv, auto nn) {
         constexpr int G = decltype(g)::value, NV = decltype(nv)::value, N = decltype(nn)::value;
         constexpr int NT = G < 256 ? 256 : G;
-        blocks = norm_grad_blocks(n, NT / G);
         k_norm_grad<T, G, NV, N><<<blocks, NT, 0, stream>>>(dy, lddy, x, ldx, n, D, w, mean, rstd, dx, lddx, dw, dc,
                                                             blocks > 1 ? part : nullptr);
     });
@@ -475,10 +487,8 @@ void run_norm_grad(const T* dy, int64_t lddy, const T* x, int64_t ldx, int64_t n
         if (dx)
             k_norm_long_dx<T><<<launch_grid(n, 1, 2048), LONG_NT, 0, stream>>>(dy, lddy, x, ldx, n, D, w, mean, rstd,
                                                                              dx, lddx);
-        const int across = (int)((D + 256 * (int64_t)VEC<T> - 1) / (256 * VEC<T>));
-        blocks = launch_grid(n, 32, (NORM_GRAD_BLOCKS + across - 1) / across);
         if (dw || dc)
-            k_norm_long_dw<T><<<dim3((unsigned)across, (unsigned)blocks), 256, 0, stream>>>(
+            k_norm_long_dw<T><<<dim3((unsigned)norm_long_across<T>(D), (unsigned)blocks), 256, 0, stream>>>(
                 dy, lddy, x, ldx, n, D, mean, rstd, blocks, dw, dc, blocks > 1 ? part : nullptr);
     }
     if (blocks > 1 && (dw || dc))
@@ -509,7 +519,9 @@ int yabt_layer_norm(int dtype, const void* x, int64_t ldx, int64_t n, int D, con
 
 size_t yabt_layer_norm_grad_workspace_bytes(int64_t n, int D) {
     if (n < 0 || D < 1) return 0;
-    return (size_t)norm_grad_blocks(n, 1) * 2 * (size_t)D * sizeof(float);
+    // bf16 and fp16 rows have the same chunks
+    const int blocks = norm_grad_blocks<float>(n, D), half = norm_grad_blocks<bf16>(n, D);
+    return (size_t)(blocks > half ? blocks : half) * 2 * (size_t)D * sizeof(float);
 }
 
 int yabt_layer_norm_grad(int dtype, const void* dy, int64_t lddy, const void* x, int64_t ldx, int64_t n, int D,
