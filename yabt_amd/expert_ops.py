@@ -15,6 +15,11 @@ leaf.
 Values are float32, bfloat16 or float16; statistics, weights, parameters of
 the norm and all sums are float32.  Every call runs on the current stream and
 neither waits nor reads anything back, so it can be captured into a HIP graph.
+
+Autograd does not see these calls: a program takes the gradients from the
+``_grad`` functions itself.  A tensor that requires a gradient is therefore
+refused while autograd records; under ``torch.no_grad()``, as in a backward pass
+of one's own, it is taken as it is.
 """
 
 from __future__ import annotations
@@ -42,6 +47,16 @@ def _call(name: str, dev: torch.device, *args) -> None:
     else:
         with torch.cuda.device(dev):
             _lib.check(getattr(lib, name)(*args, torch._C._cuda_getCurrentRawStream(dev.index)), name)
+
+
+def _unrecorded(*tensors: torch.Tensor | None) -> None:
+    """Refuses tensors whose gradients autograd would silently not get."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError("the expert layer's calls are not recorded by autograd, and a tensor requires a "
+                                   "gradient: call them under torch.no_grad() and take the gradients from the _grad "
+                                   "functions, or detach it")
 
 
 def _matrix(t: torch.Tensor, what: str, dtype: torch.dtype | None = None) -> torch.Tensor:
@@ -81,6 +96,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
                eps: float = 1e-5) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """(y, mean, rstd) of the rows of x (n, D): y = (x - mean) * rstd * weight
     + bias in x's type, mean and rstd (n,) float32 for the backward pass."""
+    _unrecorded(x, weight, bias)
     x = _matrix(x, "x")
     (n, D), dev = x.shape, x.device
     if D == 0:
@@ -97,6 +113,7 @@ def layer_norm_grad(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd:
                     weight: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """(dx, dweight, dbias) of ``layer_norm`` at x, from dy and the mean and
     rstd it returned: dx in x's type, dweight and dbias (D,) float32."""
+    _unrecorded(dy, x, mean, rstd, weight)
     x = _matrix(x, "x")
     dy = _matrix(dy, "dy", x.dtype)
     (n, D), dev = x.shape, x.device
@@ -135,6 +152,7 @@ def route(logits: torch.Tensor, k: int, *, scores: str = "softmax", bias: torch.
     largest key ("softmax") or the sum of their two largest ("sigmoid").
     Weights are scale * score, with ``renormalise`` divided by the sum of the
     row's chosen scores."""
+    _unrecorded(logits, bias)
     logits = _matrix(logits, "logits")
     (n, E), dev = logits.shape, logits.device
     how = _scores(scores)
@@ -157,6 +175,7 @@ def route_grad(dweights: torch.Tensor, logits: torch.Tensor, ids: torch.Tensor, 
                renormalise: bool = True, scale: float = 1.0) -> torch.Tensor:
     """Gradient of ``route``'s weights in the logits, (n, E) in their type, the
     choice (ids) held fixed; a balancing bias has none."""
+    _unrecorded(dweights, logits)
     logits = _matrix(logits, "logits")
     (n, E), dev = logits.shape, logits.device
     how = _scores(scores)
@@ -252,6 +271,7 @@ def expert_products(x: torch.Tensor, plan: ExpertPlan, weights: torch.Tensor, w_
     A row none of whose slots has an expert gets zeros.  With ``keep_inner``
     returns (y, inner), inner (n k, 2 G) float32, G being F up to a multiple of
     4: g and u by the plan's places, which the backward pass takes."""
+    _unrecorded(x, weights, w_in, w_out)
     x, weights, w_in, w_out, n, k, D, F, E = _expert_args(x, plan, weights, w_in, w_out)
     dev, dt, lib = x.device, DTYPES[x.dtype], _lib.load()
     nbytes = lib.yabt_experts_workspace_bytes(dt, n, k, D, F, E)
@@ -271,6 +291,7 @@ def expert_products_grad(dy: torch.Tensor, x: torch.Tensor, plan: ExpertPlan, we
     """(dx, dweights, dw_in, dw_out) of ``expert_products`` from dy (n, D) and
     the inner it kept: dx, dw_in and dw_out in x's type, dweights (n, k)
     float32, 0 for slots without an expert."""
+    _unrecorded(dy, x, weights, w_in, w_out, inner)
     x, weights, w_in, w_out, n, k, D, F, E = _expert_args(x, plan, weights, w_in, w_out)
     dy = _matrix(dy, "dy", x.dtype)
     dev, dt, lib = x.device, DTYPES[x.dtype], _lib.load()
