@@ -1188,23 +1188,57 @@ int run_experts_grad(const ExpertArgs& P, const ExpertSizes& z, bool dma, hipStr
     return launch_status("yabt_experts_grad");
 }
 
-inline bool expert_sizes_ok(int64_t n, int k, int D, int F, int E) {
+inline bool expert_ranges_ok(int64_t n, int k, int D, int F, int E) {
     return n >= 0 && k >= 1 && D >= 1 && F >= 1 && E >= 1 && E <= 1024 && n <= INT32_MAX / k && D <= (1 << 24) &&
            F <= (1 << 24);
 }
 
-// The grids' sizes, in tiles of the small shape and with the most splits.
-inline bool expert_grids_ok(int64_t n, int k, int D, int F, int E) {
-    const int64_t S = n * k, wide = D > F ? D : F, rows = (S / 64 + E) * over(wide, 64);
-    const int64_t weights = (int64_t)E * (over(2 * (int64_t)F + 8, 64) * over(D, 128) + over(D, 64) * over(F, 128) + 2 * XCDS);
-    return rows < (INT32_MAX >> 2) && weights < (INT32_MAX >> 2);
-}
-
 template <typename F>
-int by_dtype(int dtype, const F& f) {
+auto by_dtype(int dtype, const F& f) {
     if (dtype == DT_F32) return f((float*)nullptr);
     if (dtype == DT_BF16) return f((bf16*)nullptr);
     return f((f16*)nullptr);
+}
+
+// A launch has fewer than 2^32 threads.
+template <typename T>
+bool forward_grids_ok(const ExpertSizes& z) {
+    bool ok = true;
+    auto tiles = [&](auto mode, bool large) {
+        by_tile<T>(large, true, [&](auto tl, auto) {
+            using TL = decltype(tl);
+            int nt, mt;
+            ok = ok && tile_blocks<TL, decltype(mode)::value>(z, &nt, &mt) <= UINT32_MAX / TL::NT;
+        });
+    };
+    if (!few_inner(z.S, z.E, sizeof(T))) tiles(std::integral_constant<int, IN>(), z.large[0]);
+    if (!few_answer(z.S, z.E, sizeof(T))) tiles(std::integral_constant<int, OUT>(), z.large[1]);
+    return ok;
+}
+template <typename T>
+bool backward_grids_ok(const ExpertSizes& z) {
+    bool ok = true;
+    int nt, mt;
+    by_tile<T>(z.large[2], true, [&](auto tl, auto) {
+        using TL = decltype(tl);
+        ok = tile_blocks<TL, DH>(z, &nt, &mt) <= UINT32_MAX / TL::NT;
+    });
+    by_tile<T>(z.large[3], true, [&](auto tl, auto) {
+        using TL = decltype(tl);
+        ok = ok && tile_blocks<TL, DX>(z, &nt, &mt) + tile_blocks<TL, DWIN>(z, &nt, &mt) +
+                           tile_blocks<TL, DWOUT>(z, &nt, &mt) <= UINT32_MAX / TL::NT;
+    });
+    return ok;
+}
+
+// Whether the sizes can be run, and what they lead to.
+inline bool expert_sizes_ok(bool backward, int dtype, int64_t n, int k, int D, int F, int E, ExpertSizes* z) {
+    if (!dtype_ok(dtype) || !expert_ranges_ok(n, k, D, F, E)) return false;
+    *z = expert_sizes(dtype, n, k, D, F, E);
+    return by_dtype(dtype, [&](auto* t) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        return backward ? backward_grids_ok<T>(*z) : forward_grids_ok<T>(*z);
+    });
 }
 
 // Whether rows of `width` values, ld apart, may be fetched in aligned 16-byte pieces.
@@ -1219,10 +1253,11 @@ using namespace yabt;
 extern "C" {
 
 size_t yabt_experts_workspace_bytes(int dtype, int64_t n, int k, int D, int F, int E) {
-    if (!dtype_ok(dtype) || !expert_sizes_ok(n, k, D, F, E)) return 0;
+    ExpertSizes z;
+    if (!expert_sizes_ok(false, dtype, n, k, D, F, E, &z)) return 0;
     ExpertArgs P;
     Carve c{nullptr, 0};
-    return carve_forward(c, &P, expert_sizes(dtype, n, k, D, F, E), k) + 256;
+    return carve_forward(c, &P, z, k) + 256;
 }
 
 int yabt_experts(int dtype, const void* x, int64_t ldx, int64_t n, int k, int D, int F, int E, const int32_t* ids,
@@ -1230,7 +1265,8 @@ int yabt_experts(int dtype, const void* x, int64_t ldx, int64_t n, int k, int D,
                  const void* w_in, const void* w_out, void* workspace, size_t workspace_bytes, float* out_inner,
                  void* y, int64_t ldy, yabt_stream_t stream) {
     if (!dtype_ok(dtype)) return fail(-1, "yabt_experts: dtype is 0 (fp32), 1 (bf16) or 2 (fp16)");
-    if (!expert_sizes_ok(n, k, D, F, E) || ldx < D || ldy < D || !expert_grids_ok(n, k, D, F, E))
+    ExpertSizes z;
+    if (!expert_sizes_ok(false, dtype, n, k, D, F, E, &z) || ldx < D || ldy < D)
         return fail(-1, "yabt_experts: bad sizes");
     if (n == 0) return 0;
     if (!x || !ids || !offsets || !slots || !rows || !weights || !w_in || !w_out || !y)
@@ -1238,7 +1274,6 @@ int yabt_experts(int dtype, const void* x, int64_t ldx, int64_t n, int k, int D,
     if (!aligned16(out_inner)) return fail(-1, "yabt_experts: out_inner must be 16-byte aligned");
     if (!workspace || workspace_bytes < yabt_experts_workspace_bytes(dtype, n, k, D, F, E))
         return fail(-2, "yabt_experts: workspace too small");
-    const ExpertSizes z = expert_sizes(dtype, n, k, D, F, E);
     ExpertArgs P = {x, nullptr, w_in, w_out, weights, ids, offsets, slots, rows, ldx, 0, n, k, D, F, E, z.Fp, z.Dp, up16(F, 4)};
     P.pre = out_inner;
     P.out = y;
@@ -1254,10 +1289,11 @@ int yabt_experts(int dtype, const void* x, int64_t ldx, int64_t n, int k, int D,
 }
 
 size_t yabt_experts_grad_workspace_bytes(int dtype, int64_t n, int k, int D, int F, int E) {
-    if (!dtype_ok(dtype) || !expert_sizes_ok(n, k, D, F, E)) return 0;
+    ExpertSizes z;
+    if (!expert_sizes_ok(true, dtype, n, k, D, F, E, &z)) return 0;
     ExpertArgs P;
     Carve c{nullptr, 0};
-    return carve_backward(c, &P, expert_sizes(dtype, n, k, D, F, E), k) + 256;
+    return carve_backward(c, &P, z, k) + 256;
 }
 
 int yabt_experts_grad(int dtype, const void* dy, int64_t lddy, const void* x, int64_t ldx, int64_t n, int k, int D,
@@ -1266,7 +1302,8 @@ int yabt_experts_grad(int dtype, const void* dy, int64_t lddy, const void* x, in
                       const float* inner, void* workspace, size_t workspace_bytes, void* dx, int64_t lddx,
                       float* dweights, void* dw_in, void* dw_out, yabt_stream_t stream) {
     if (!dtype_ok(dtype)) return fail(-1, "yabt_experts_grad: dtype is 0 (fp32), 1 (bf16) or 2 (fp16)");
-    if (!expert_sizes_ok(n, k, D, F, E) || ldx < D || lddy < D || lddx < D || !expert_grids_ok(n, k, D, F, E))
+    ExpertSizes z;
+    if (!expert_sizes_ok(true, dtype, n, k, D, F, E, &z) || ldx < D || lddy < D || lddx < D)
         return fail(-1, "yabt_experts_grad: bad sizes");
     if (!offsets || !w_in || !w_out || !dw_in || !dw_out ||
         (n > 0 && (!x || !dy || !ids || !slots || !rows || !weights || !inner || !dx || !dweights)))
@@ -1274,7 +1311,6 @@ int yabt_experts_grad(int dtype, const void* dy, int64_t lddy, const void* x, in
     if (!aligned16(inner)) return fail(-1, "yabt_experts_grad: inner must be 16-byte aligned");
     if (!workspace || workspace_bytes < yabt_experts_grad_workspace_bytes(dtype, n, k, D, F, E))
         return fail(-2, "yabt_experts_grad: workspace too small");
-    const ExpertSizes z = expert_sizes(dtype, n, k, D, F, E);
     ExpertArgs P = {x, dy, w_in, w_out, weights, ids, offsets, slots, rows, ldx, lddy, n, k, D, F, E, z.Fp, z.Dp, up16(F, 4)};
     P.pre = const_cast<float*>(inner);
     P.out = dx;
