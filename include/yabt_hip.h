@@ -569,6 +569,12 @@ int yabt_experts(int dtype, const void *x, int64_t ldx, int64_t n, int k, int D,
                  const float *weights, const void *w_in, const void *w_out, void *workspace,
                  size_t workspace_bytes, float *out_inner, void *y, int64_t ldy, yabt_stream_t stream);
 
+/* Which kernels make the products of these sizes, for tests and profiles; -1
+ * where they are out of range.  Bit 0: h by the kernel for few rows, bit 1: y by
+ * its kernel for few rows; bits 2 to 5: 256 x 256 tiles (else 64 x 128) for h, y,
+ * the inner gradient, and the three other gradients. */
+int yabt_experts_forms(int dtype, int64_t n, int k, int D, int F, int E);
+
 /* Their gradients from dy (n, D) and the forward pass's inner: dx (n, D),
  * dw_in, dw_out like w_in and w_out, all of `dtype`, and dweights (n, k) fp32
  * (0 for slots without an expert).  An expert without slots gets zeros. */

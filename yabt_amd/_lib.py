@@ -108,6 +108,7 @@ SIGNATURES = {
     "yabt_experts_workspace_bytes": (_sz, [_int, _i64, _int, _int, _int, _int]),
     "yabt_experts": (_int, [_int, _vp, _i64, _i64, _int, _int, _int, _int, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
                             _sz, _vp, _vp, _i64, _vp]),
+    "yabt_experts_forms": (_int, [_int, _i64, _int, _int, _int, _int]),
     "yabt_experts_grad_workspace_bytes": (_sz, [_int, _i64, _int, _int, _int, _int]),
     "yabt_experts_grad": (_int, [_int, _vp, _i64, _vp, _i64, _i64, _int, _int, _int, _int, _vp, _vp, _vp, _vp, _vp,
                                  _vp, _vp, _vp, _vp, _sz, _vp, _i64, _vp, _vp, _vp, _vp]),

@@ -1288,6 +1288,14 @@ int yabt_experts(int dtype, const void* x, int64_t ldx, int64_t n, int k, int D,
     });
 }
 
+int yabt_experts_forms(int dtype, int64_t n, int k, int D, int F, int E) {
+    if (!dtype_ok(dtype) || !expert_ranges_ok(n, k, D, F, E)) return -1;
+    const ExpertSizes z = expert_sizes(dtype, n, k, D, F, E);
+    const bool inner = few_inner(z.S, E, z.bytes), answer = few_answer(z.S, E, z.bytes);
+    int forms = (int)inner | (int)answer << 1 | (int)(z.large[0] && !inner) << 2 | (int)(z.large[1] && !answer) << 3;
+    return forms | (int)z.large[2] << 4 | (int)z.large[3] << 5;
+}
+
 size_t yabt_experts_grad_workspace_bytes(int dtype, int64_t n, int k, int D, int F, int E) {
     ExpertSizes z;
     if (!expert_sizes_ok(true, dtype, n, k, D, F, E, &z)) return 0;
