@@ -41,22 +41,23 @@ def _call(name: str, dev: torch.device, *args) -> None:
     and a launch on it goes to the current one.  ``torch.cuda.current_stream``
     takes 2 us to make an object of the handle and ``torch.cuda.device`` more,
     which a call for one row would notice."""
-    lib = _lib.load()
-    if torch._C._cuda_getDevice() == dev.index:
-        _lib.check(getattr(lib, name)(*args, torch._C._cuda_getCurrentRawStream(dev.index)), name)
+    call, index = getattr(_lib.load(), name), dev.index
+    if torch._C._cuda_getDevice() == index:
+        rc = call(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(dev):
-            _lib.check(getattr(lib, name)(*args, torch._C._cuda_getCurrentRawStream(dev.index)), name)
+            rc = call(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        _lib.check(rc, name)
 
 
 def _unrecorded(*tensors: torch.Tensor | None) -> None:
     """Refuses tensors whose gradients autograd would silently not get."""
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                raise RuntimeError("the expert layer's calls are not recorded by autograd, and a tensor requires a "
-                                   "gradient: call them under torch.no_grad() and take the gradients from the _grad "
-                                   "functions, or detach it")
+    for t in tensors:
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("the expert layer's calls are not recorded by autograd, and a tensor requires a "
+                               "gradient: call them under torch.no_grad() and take the gradients from the _grad "
+                               "functions, or detach it")
 
 
 def _matrix(t: torch.Tensor, what: str, dtype: torch.dtype | None = None) -> torch.Tensor:
