@@ -76,10 +76,9 @@ def _power_of_two(t: torch.Tensor) -> torch.Tensor:
 
 def _half_unit(g: torch.Tensor, head: torch.Tensor) -> torch.Tensor:
     """The power of two, as a 0-d tensor, that the rows' gradients g head are
-    multiplied by for float16; 1 where they are all 0 or not finite."""
-    total = g.abs().sum() * head.abs().amax()
-    unit = _power_of_two((_HALF_SUM / total).clamp(2.0 ** -100, 2.0 ** 100))
-    return torch.where((total > 0.0) & torch.isfinite(total), unit, 1.0)
+    multiplied by for float16 (any, where they are all 0)."""
+    total = torch.linalg.vector_norm(g, 1) * torch.linalg.vector_norm(head, float("inf"))
+    return _power_of_two((_HALF_SUM / total).clamp_(2.0 ** -100, 2.0 ** 100))
 
 
 def _statistics(raw: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
