@@ -499,7 +499,8 @@ int yabt_predict(const float *X, int64_t ldx, int64_t n, int F, int T, const int
  * form of a tree with models in its leaves (yabt/neural_leaves.py:93-184),
  * which routes a row to one leaf.  `dtype`: 0 fp32, 1 bf16, 2 fp16; rows of
  * any leading dimension and alignment; sums and statistics are fp32, one
- * rounding at the end; no atomics on sums, so results are the same every time.
+ * rounding at the end; no sum depends on the order of atomics, so results are the
+ * same every time.
  * ------------------------------------------------------------------------- */
 
 /* Layer norm of n rows of width D:
@@ -514,7 +515,8 @@ int yabt_layer_norm(int dtype, const void *x, int64_t ldx, int64_t n, int D, con
  * weight and xh = (x - mean) * rstd:
  *   dx = rstd * (t - sum t / D - xh * sum (t xh) / D)   (NULL: not wanted)
  *   dweight = sum over rows of dy * xh, dbias = sum over rows of dy  (D, fp32; NULL: not wanted)
- * weight NULL counts as ones.  The row sums are added in an order that n and D fix. */
+ * weight NULL counts as ones.  The row sums are added in an order that n, D and the
+ * size of a value fix. */
 size_t yabt_layer_norm_grad_workspace_bytes(int64_t n, int D);
 int yabt_layer_norm_grad(int dtype, const void *dy, int64_t lddy, const void *x, int64_t ldx, int64_t n,
                          int D, const float *weight, const float *mean, const float *rstd,
@@ -562,7 +564,9 @@ int yabt_expert_plan(const int32_t *ids, int64_t n, int k, int E, void *workspac
  * zeros.  out_inner ((n k) x 2 G, fp32, 16-byte aligned, or NULL), G being F up
  * to a multiple of 4, keeps g and u of every place of the plan for the
  * backward pass; places past the plan's last are not written.
- * h is rounded to `dtype` before the second product; sums are fp32. */
+ * h is rounded to `dtype` before the second product, so that in fp16 one beyond
+ * 65504 makes its row's y infinite or NaN; sums are fp32.  Sizes whose launches
+ * would have 2^32 threads are refused; the size query then answers 0. */
 size_t yabt_experts_workspace_bytes(int dtype, int64_t n, int k, int D, int F, int E);
 int yabt_experts(int dtype, const void *x, int64_t ldx, int64_t n, int k, int D, int F, int E,
                  const int32_t *ids, const int32_t *offsets, const int32_t *slots, const int32_t *rows,
@@ -577,7 +581,8 @@ int yabt_experts_forms(int dtype, int64_t n, int k, int D, int F, int E);
 
 /* Their gradients from dy (n, D) and the forward pass's inner: dx (n, D),
  * dw_in, dw_out like w_in and w_out, all of `dtype`, and dweights (n, k) fp32
- * (0 for slots without an expert).  An expert without slots gets zeros. */
+ * (0 for slots without an expert).  An expert without slots gets zeros.  The inner
+ * gradients and w h are rounded to `dtype`, in fp16 with its range. */
 size_t yabt_experts_grad_workspace_bytes(int dtype, int64_t n, int k, int D, int F, int E);
 int yabt_experts_grad(int dtype, const void *dy, int64_t lddy, const void *x, int64_t ldx, int64_t n,
                       int k, int D, int F, int E, const int32_t *ids, const int32_t *offsets,

@@ -26,7 +26,8 @@
 // not 16-byte aligned pass through registers instead.
 //
 // 16 384 x 2048 rows, 2 of 8 experts of 2048, bf16 (550 GFLOP for h, 275 for y and the
-// inner gradient, 1375 for the other three): 0.60, 0.32, 0.51 and 1.58 ms, the matrix
+// inner gradient, 1375 for the other three): 0.60, 0.32, 0.51 and 1.58 ms over the
+// first dozen passes, 0.57, 0.30, 0.48 and 1.46 over a hundred, the matrix
 // cores at work 59, 61, 34 and 50% of the CUs' busy time; the library's plain
 // product of 275 GFLOP alone takes 0.21 ms.  What is between them: a block has its
 // CU to itself (its sums are 256 KB of registers), so that what a tile reads and
@@ -39,7 +40,10 @@
 // h, w h, dg and du are rounded to the inputs' type, as the matrix cores take
 // them; g and u are kept in fp32 for the backward pass, and z and the parts of
 // dx are added in fp32: so each output has two roundings behind it, its own
-// and that of one factor.
+// and that of one factor (0.0023 from the formulas in 64 bits where its own alone
+// leaves 0.0017, bf16).  In fp16 they have the type's range: an h beyond 65504 is
+// infinite.  Two parts of 16 bits each would take that rounding away for
+// twice the arithmetic of all products but h and dh; float32 tensors have none.
 
 #include "expert.h"
 #include "yabt_hip.h"
@@ -131,7 +135,8 @@ __device__ __forceinline__ constexpr int spread(int r) {
 // 16 bits: the hardware's exp2 and reciprocal, off by more the larger |g| is, as the
 // rounding of g log2 e counts whole in the exponent (y at most 3 units of 2^-24 for
 // g near 0, 10 to -10, 18 to -20, 59 to -60; with fp32's 3 everywhere): the rounding
-// of h that follows is 2^13 or 2^16 units.  fp32's form costs 20 000 x 100 -> 60 2 of 107 us.
+// of h that follows is 2^13 or 2^16 units.  fp32's form costs 2 of 107 us of 20 000 x
+// 100 -> 60 of 7, forward and backward.
 template <typename T>
 __device__ __forceinline__ float gate_sigmoid(float g) {
     if constexpr (sizeof(T) == 4) {
@@ -147,7 +152,8 @@ __device__ __forceinline__ float gate_sigmoid(float g) {
 // 64 lanes' 16 bytes each from memory to LDS at base (the same for the wave),
 // in lane order.  By hand, because the compiler waits for all LDS reads at
 // every use of one where the builtin is about; it counts as a vector memory
-// access, which stage_ready waits for.
+// access, which stage_ready waits for.  m0 is the compiler's reserved register: it
+// keeps nothing there from one instruction to another and refuses it as a clobber.
 __device__ __forceinline__ void lds_fill(const void* g, uint32_t base) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "s"(base));
 }
@@ -1151,8 +1157,8 @@ void run_finish(const ExpertArgs& P, const ExpertSizes& z, hipStream_t stream) {
 // whole arithmetic, which fp32 does at a sixteenth of the rate.  h, few and
 // tiles, us: 2048 -> 1024 of 32 experts, fp16, 6 slots each 61 and 66, 12 each 79
 // and 70; 1024 -> 512 of 64, bf16, one row's 6 slots 6 and 10, 3 each 20 and 19,
-// 6 each 24 and 21; of 8, fp32, 4 each 14 and 40, 32 each 35 and 41; 500 -> 101 of
-// 4, fp32, 25 each 12 and 28, 50 each 19 and 28.
+// 6 each 24 and 21; of 8, fp32, 4 each 15 and 40, 32 each 22 and 42; 500 -> 101 of
+// 4, fp32, 25 each 10 and 29, 50 each 17 and 29 (fp32 with as many for every expert).
 inline bool few_inner(int64_t S, int E, int bytes) {
     const int64_t used = S < E ? S : E;
     return S <= used * (bytes == 4 ? 32 : 8);

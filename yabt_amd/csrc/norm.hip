@@ -239,7 +239,8 @@ __global__ void __launch_bounds__(G < 256 ? 256 : G) k_norm_grad(
 
 // Rows too long for registers: a block per row, read once per sum (the later
 // reads come from the caches), by chunks as above.  4096 x 20000 bf16: 108 us forward
-// (3.0 TB/s over one read and write), 193 backward; value by value 195 and 329.
+// (3.0 TB/s over one read and write), 193 backward, 93 and 175 back to
+// back; value by value 195 and 329.
 constexpr int LONG_NT = 1024;
 
 // chunk c's values of a parameter vector, or `none` where there is no vector

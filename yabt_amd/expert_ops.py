@@ -271,7 +271,10 @@ def expert_products(x: torch.Tensor, plan: ExpertPlan, weights: torch.Tensor, w_
     w_out (E, D, F); both of x's type.  weights (n, k) as ``route`` gives them.
     A row none of whose slots has an expert gets zeros.  With ``keep_inner``
     returns (y, inner), inner (n k, 2 G) float32, G being F up to a multiple of
-    4: g and u by the plan's places, which the backward pass takes."""
+    4: g and u by the plan's places, which the backward pass takes.
+
+    16-bit types round silu(g) * u to theirs before w_out, which float32 does
+    not; in float16 one beyond 65504 makes its row infinite or NaN."""
     _unrecorded(x, weights, w_in, w_out)
     x, weights, w_in, w_out, n, k, D, F, E = _expert_args(x, plan, weights, w_in, w_out)
     dev, dt, lib = x.device, DTYPES[x.dtype], _lib.load()
@@ -291,7 +294,8 @@ def expert_products_grad(dy: torch.Tensor, x: torch.Tensor, plan: ExpertPlan, we
                          w_in: torch.Tensor, w_out: torch.Tensor, inner: torch.Tensor):
     """(dx, dweights, dw_in, dw_out) of ``expert_products`` from dy (n, D) and
     the inner it kept: dx, dw_in and dw_out in x's type, dweights (n, k)
-    float32, 0 for slots without an expert."""
+    float32, 0 for slots without an expert.  In float16 the inner gradients have
+    its range too: scale dy for them and the results back."""
     _unrecorded(dy, x, weights, w_in, w_out, inner)
     x, weights, w_in, w_out, n, k, D, F, E = _expert_args(x, plan, weights, w_in, w_out)
     dy = _matrix(dy, "dy", x.dtype)
