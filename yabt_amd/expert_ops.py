@@ -206,7 +206,8 @@ def _ids(ids: torch.Tensor, dev: torch.device | None = None) -> torch.Tensor:
 class ExpertPlan:
     """Slots (row * k + j) sorted by expert.  Expert e's are ``slots[offsets[e]
     : offsets[e + 1]]``, in row order, and ``rows`` their rows; the places
-    after the last hold -1, as many as there are ids that name no expert."""
+    after the last hold -1, as many as there are ids that name no expert.  ids
+    are kept, not copied: they stay as they are while the plan is in use."""
     ids: torch.Tensor       # (n, k) int32
     offsets: torch.Tensor   # (E + 1,) int32
     slots: torch.Tensor     # (n k,) int32

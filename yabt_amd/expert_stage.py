@@ -105,6 +105,8 @@ def _statistics(raw: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 class ExpertStage:
     """See the module's text; ``loss`` as a ``Booster`` takes it."""
 
+    unit_: torch.Tensor | None = None     # of the answers, where it may not be 1
+
     def __init__(self, params: ExpertParams, loss):
         self.p, self.loss = params, loss
 
@@ -201,7 +203,7 @@ class ExpertStage:
                              w_out=normal(p.experts, p.width, p.inner, scale=p.inner ** -0.5),
                              head=torch.zeros(p.width, device=dev))
         self.bias_ = torch.zeros(p.experts, device=dev)
-        self.unit_ = None             # of the answers, where it is not 1
+        self.unit_ = None
         if p.dtype == "float16" and n:
             g, _ = boost_ops.grad_hess(self.loss, base, yt)
             self.unit_ = _power_of_two((g.abs().median() / _HALF_ANSWER).clamp(1.0, 2.0 ** 100))
