@@ -51,20 +51,19 @@ def _call(name: str, dev: torch.device, *args) -> None:
         _lib.check(rc, name)
 
 
-def _unrecorded(*tensors: torch.Tensor | None) -> None:
-    """Refuses tensors whose gradients autograd would silently not get."""
-    for t in tensors:
-        if t is not None and t.requires_grad and torch.is_grad_enabled():
-            raise RuntimeError("the expert layer's calls are not recorded by autograd, and a tensor requires a "
-                               "gradient: call them under torch.no_grad() and take the gradients from the _grad "
-                               "functions, or detach it")
+def _unrecorded() -> None:
+    """A call's tensor requires a gradient, which autograd would silently not get."""
+    if torch.is_grad_enabled():
+        raise RuntimeError("the expert layer's calls are not recorded by autograd, and a tensor requires a gradient: "
+                           "call them under torch.no_grad() and take the gradients from the _grad functions, or "
+                           "detach it")
 
 
 def _matrix(t: torch.Tensor, what: str, dtype: torch.dtype | None = None) -> torch.Tensor:
     """t as a device matrix with unit column stride."""
     if t.dim() != 2:
         raise ValueError(f"{what} must be a matrix, got shape {tuple(t.shape)}")
-    if t.device.type != "cuda":
+    if not t.is_cuda:
         raise RuntimeError(f"{what} must be on a HIP device: the expert layer has no CPU form")
     if t.dtype not in DTYPES or (dtype is not None and t.dtype != dtype):
         raise ValueError(f"{what} must be {dtype or 'float32, bfloat16 or float16'}, got {t.dtype}")
@@ -97,7 +96,8 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
                eps: float = 1e-5) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """(y, mean, rstd) of the rows of x (n, D): y = (x - mean) * rstd * weight
     + bias in x's type, mean and rstd (n,) float32 for the backward pass."""
-    _unrecorded(x, weight, bias)
+    if x.requires_grad or weight is not None and weight.requires_grad or bias is not None and bias.requires_grad:
+        _unrecorded()
     x = _matrix(x, "x")
     (n, D), dev = x.shape, x.device
     if D == 0:
@@ -114,7 +114,8 @@ def layer_norm_grad(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd:
                     weight: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """(dx, dweight, dbias) of ``layer_norm`` at x, from dy and the mean and
     rstd it returned: dx in x's type, dweight and dbias (D,) float32."""
-    _unrecorded(dy, x, mean, rstd, weight)
+    if any(t is not None and t.requires_grad for t in (dy, x, mean, rstd, weight)):
+        _unrecorded()
     x = _matrix(x, "x")
     dy = _matrix(dy, "dy", x.dtype)
     (n, D), dev = x.shape, x.device
@@ -153,7 +154,8 @@ def route(logits: torch.Tensor, k: int, *, scores: str = "softmax", bias: torch.
     largest key ("softmax") or the sum of their two largest ("sigmoid").
     Weights are scale * score, with ``renormalise`` divided by the sum of the
     row's chosen scores."""
-    _unrecorded(logits, bias)
+    if logits.requires_grad or bias is not None and bias.requires_grad:
+        _unrecorded()
     logits = _matrix(logits, "logits")
     (n, E), dev = logits.shape, logits.device
     how = _scores(scores)
@@ -176,7 +178,8 @@ def route_grad(dweights: torch.Tensor, logits: torch.Tensor, ids: torch.Tensor, 
                renormalise: bool = True, scale: float = 1.0) -> torch.Tensor:
     """Gradient of ``route``'s weights in the logits, (n, E) in their type, the
     choice (ids) held fixed; a balancing bias has none."""
-    _unrecorded(dweights, logits)
+    if dweights.requires_grad or logits.requires_grad:
+        _unrecorded()
     logits = _matrix(logits, "logits")
     (n, E), dev = logits.shape, logits.device
     how = _scores(scores)
@@ -196,7 +199,7 @@ def route_grad(dweights: torch.Tensor, logits: torch.Tensor, ids: torch.Tensor, 
 def _ids(ids: torch.Tensor, dev: torch.device | None = None) -> torch.Tensor:
     if ids.dim() != 2 or ids.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"ids must be an (n, k) integer matrix, got {tuple(ids.shape)} {ids.dtype}")
-    if ids.device.type != "cuda" or dev is not None and ids.device != dev:
+    if not ids.is_cuda or dev is not None and ids.device != dev:
         raise RuntimeError("ids must be on the other tensors' HIP device")
     # a wider id names no expert: it must not come out as one
     return (ids if ids.dtype == torch.int32 else ids.clamp(-1, 2 ** 31 - 1).to(torch.int32)).contiguous()
@@ -276,7 +279,8 @@ def expert_products(x: torch.Tensor, plan: ExpertPlan, weights: torch.Tensor, w_
 
     16-bit types round silu(g) * u to theirs before w_out, which float32 does
     not; in float16 one beyond 65504 makes its row infinite or NaN."""
-    _unrecorded(x, weights, w_in, w_out)
+    if x.requires_grad or weights.requires_grad or w_in.requires_grad or w_out.requires_grad:
+        _unrecorded()
     x, weights, w_in, w_out, n, k, D, F, E = _expert_args(x, plan, weights, w_in, w_out)
     dev, dt, lib = x.device, DTYPES[x.dtype], _lib.load()
     nbytes = lib.yabt_experts_workspace_bytes(dt, n, k, D, F, E)
@@ -297,7 +301,9 @@ def expert_products_grad(dy: torch.Tensor, x: torch.Tensor, plan: ExpertPlan, we
     the inner it kept: dx, dw_in and dw_out in x's type, dweights (n, k)
     float32, 0 for slots without an expert.  In float16 the inner gradients have
     its range too: scale dy for them and the results back."""
-    _unrecorded(dy, x, weights, w_in, w_out, inner)
+    if dy.requires_grad or x.requires_grad or weights.requires_grad or w_in.requires_grad or w_out.requires_grad or \
+            inner.requires_grad:
+        _unrecorded()
     x, weights, w_in, w_out, n, k, D, F, E = _expert_args(x, plan, weights, w_in, w_out)
     dy = _matrix(dy, "dy", x.dtype)
     dev, dt, lib = x.device, DTYPES[x.dtype], _lib.load()
