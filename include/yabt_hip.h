@@ -591,6 +591,45 @@ int yabt_experts_grad(int dtype, const void *dy, int64_t lddy, const void *x, in
                       void *dx, int64_t lddx, float *dweights, void *dw_in, void *dw_out,
                       yabt_stream_t stream);
 
+/* ---------------------------------------------------------------------------
+ * The dense stage: the block that every row passes beside the routed experts,
+ * its fit and its answers in 8 bits.  Types and rows as for the expert layer.
+ * ------------------------------------------------------------------------- */
+
+/* One tensor of an AdamW step: n values one behind the other, of any alignment
+ * their types have.  `first` and `second`: its moments, n floats each, or with 8 bits
+ * n int8 and n uint8, whose blocks of 256 values share a float of first_scale and
+ * second_scale (ceil(n / 256) each).  The moments' largest magnitude in a block is
+ * its scale; a code c of `first` stands for sign(c) (c / 127)^2 scale, one of
+ * `second` for ((c / 255)^2 scale)^2, the scale being of the square roots.  Zeroed
+ * moments are those before the first step. */
+typedef struct {
+    void *param;
+    const void *grad;
+    void *first, *second;
+    float *first_scale, *second_scale; /* NULL with 32 bits */
+    int64_t n;
+    int32_t param_dtype, grad_dtype; /* 0 fp32, 1 bf16, 2 fp16 */
+} yabt_adamw_tensor;
+
+/* Step number `step`, from 1, over `count` tensors (`tensors` is host memory and
+ * free again on return), in fp32:
+ *   m = m + (1 - beta1) (g - m), v = v + (1 - beta2) (g^2 - v)
+ *   p = p (1 - lr weight_decay) - lr sqrt(1 - beta2^t) / (1 - beta1^t) m / (sqrt(v) + eps sqrt(1 - beta2^t))
+ * the last product of each rounded with its sum, every other operation by itself.
+ * p is written in its type, rounded once, the moments in `bits` (32 or 8).  With 8
+ * bits p moves by the moments before they are rounded; a v above 0 keeps a code above
+ * 0; a block whose largest magnitude is below 2^-100 is held as zeros, one that is not
+ * finite as NaN.  step_device, if not NULL, is read on the device in place of `step`, so
+ * that a captured call counts on; numbers below 1 count as 1. */
+int yabt_adamw_step(int count, const yabt_adamw_tensor *tensors, int bits, int64_t step,
+                    const int32_t *step_device, double lr, double beta1, double beta2, double eps,
+                    double weight_decay, yabt_stream_t stream);
+
+/* The values that 8-bit moments stand for: those of `first` as n floats to
+ * `param`, those of `second` to `grad`, which is written here; the types are not read. */
+int yabt_adamw_values(int count, const yabt_adamw_tensor *tensors, yabt_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -112,6 +112,8 @@ SIGNATURES = {
     "yabt_experts_grad_workspace_bytes": (_sz, [_int, _i64, _int, _int, _int, _int]),
     "yabt_experts_grad": (_int, [_int, _vp, _i64, _vp, _i64, _i64, _int, _int, _int, _int, _vp, _vp, _vp, _vp, _vp,
                                  _vp, _vp, _vp, _vp, _sz, _vp, _i64, _vp, _vp, _vp, _vp]),
+    "yabt_adamw_step": (_int, [_int, _vp, _int, _i64, _vp, _dbl, _dbl, _dbl, _dbl, _dbl, _vp]),
+    "yabt_adamw_values": (_int, [_int, _vp, _vp]),
 }
 
 
