@@ -630,6 +630,56 @@ int yabt_adamw_step(int count, const yabt_adamw_tensor *tensors, int bits, int64
  * `param`, those of `second` to `grad`, which is written here; the types are not read. */
 int yabt_adamw_values(int count, const yabt_adamw_tensor *tensors, yabt_stream_t stream);
 
+/* A gated feed-forward block over n rows:
+ *   [g u] = x w_in^T, h = act(g) * u, y = h w_out^T
+ * x (n, D), y (n, O), w_in (2 F, D): F gate rows, then F rows of u, w_out (O, F),
+ * all of `dtype`; act 0 silu (g / (1 + exp(-g))), 1 gelu (g times the normal
+ * distribution function), 2 gelu_tanh (its usual form by tanh), 3 relu.
+ * out_inner (yabt_feed_forward_inner_bytes, or NULL) keeps g and u in fp32 and h for
+ * the backward pass.  h is rounded to `dtype` before the second product (16-bit
+ * types, 64 rows or fewer: to two parts of it), so that in fp16 one beyond 65504
+ * makes its row infinite or NaN; sums are fp32.  n below 2^31 - 256, D, F, O to 2^24.
+ * Sums are added in an order that the sizes fix. */
+size_t yabt_feed_forward_inner_bytes(int dtype, int64_t n, int D, int F, int O);
+size_t yabt_feed_forward_workspace_bytes(int dtype, int64_t n, int D, int F, int O);
+int yabt_feed_forward(int dtype, int act, const void *x, int64_t ldx, int64_t n, int D, int F, int O,
+                      const void *w_in, const void *w_out, void *workspace, size_t workspace_bytes,
+                      void *out_inner, void *y, int64_t ldy, yabt_stream_t stream);
+
+/* Its gradients from dy (n, O) and the forward pass's inner: dx (n, D), dw_in
+ * (2 F, D), dw_out (O, F), all of `dtype`.  The inner gradients are rounded to
+ * `dtype`, in fp16 with its range.  n = 0 gives zeros for the weights. */
+size_t yabt_feed_forward_grad_workspace_bytes(int dtype, int64_t n, int D, int F, int O);
+int yabt_feed_forward_grad(int dtype, int act, const void *dy, int64_t lddy, const void *x, int64_t ldx,
+                           int64_t n, int D, int F, int O, const void *w_in, const void *w_out,
+                           const void *inner, void *workspace, size_t workspace_bytes, void *dx,
+                           int64_t lddx, void *dw_in, void *dw_out, yabt_stream_t stream);
+
+/* Rows of x (n, D) in 8 bits: with m the row's largest magnitude
+ *   code = round(x * (127 / m)) to the nearest, ties to even, scale = m * (1 / 127)
+ * in fp32.  A row with m below 2^-100 gets zeros and scale 0, one that is not finite
+ * zeros and scale NaN.  n below 2^24, D to 2^24. */
+int yabt_quantize_rows(int dtype, const void *x, int64_t ldx, int64_t n, int D, int8_t *out_codes,
+                       int64_t ldq, float *out_scale, yabt_stream_t stream);
+
+/* y = a_scale[i] * (b_scale[o] * sum_k a[i, k] b[o, k]): codes a (n, K) with a scale for each
+ * row, b (N, K) with one for each output column, to y (n, N) of out_dtype.  The sum
+ * is exact (32 bits, K at most 131071) and rounded to fp32 once. */
+size_t yabt_product_int8_workspace_bytes(int64_t n, int K, int N);
+int yabt_product_int8(const int8_t *a, int64_t lda, const float *a_scale, int64_t n, int K,
+                      const int8_t *b, int64_t ldb, const float *b_scale, int N, int out_dtype,
+                      void *workspace, size_t workspace_bytes, void *y, int64_t ldy,
+                      yabt_stream_t stream);
+
+/* yabt_feed_forward with both weights in 8 bits (w_in (2 F, D) and w_out (O, F), a
+ * scale for each row): x's rows are put in 8 bits as yabt_quantize_rows does, g, u
+ * and h are fp32, and h's rows are put in 8 bits in the same way.  D and F to 131071. */
+size_t yabt_feed_forward_int8_workspace_bytes(int64_t n, int D, int F, int O);
+int yabt_feed_forward_int8(int dtype, int act, const void *x, int64_t ldx, int64_t n, int D, int F, int O,
+                           const int8_t *w_in, const float *in_scale, const int8_t *w_out,
+                           const float *out_scale, void *workspace, size_t workspace_bytes, void *y,
+                           int64_t ldy, yabt_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

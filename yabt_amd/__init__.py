@@ -15,7 +15,7 @@ Kernels live in ``yabt_amd/csrc`` and are reached through the C ABI of
 ``include/yabt_hip.h`` (``libyabt_hip.so``, loaded with ctypes).
 """
 
-from . import expert_ops, optim
+from . import expert_ops, feed_ops, optim
 from .binning import MAX_BINS, Binner, IdentityBinner
 from .boosting import Booster, BoostParams, MulticlassBooster
 from .expert_stage import ExpertParams, ExpertStage
@@ -26,4 +26,5 @@ from .tree import LEAF, Tree, TreeParams
 
 __all__ = ["MAX_BINS", "Binner", "IdentityBinner", "apply_hip", "grow_tree_hip", "is_available",
            "LEAF", "Tree", "TreeParams", "Booster", "BoostParams", "MulticlassBooster", "LogLoss", "MSELoss",
-           "YABTClassifier", "YABTRegressor", "ExpertParams", "ExpertStage", "expert_ops", "optim"]
+           "YABTClassifier", "YABTRegressor", "ExpertParams", "ExpertStage", "expert_ops",
+           "feed_ops", "optim"]

@@ -114,6 +114,19 @@ SIGNATURES = {
                                  _vp, _vp, _vp, _vp, _sz, _vp, _i64, _vp, _vp, _vp, _vp]),
     "yabt_adamw_step": (_int, [_int, _vp, _int, _i64, _vp, _dbl, _dbl, _dbl, _dbl, _dbl, _vp]),
     "yabt_adamw_values": (_int, [_int, _vp, _vp]),
+    "yabt_feed_forward_inner_bytes": (_sz, [_int, _i64, _int, _int, _int]),
+    "yabt_feed_forward_workspace_bytes": (_sz, [_int, _i64, _int, _int, _int]),
+    "yabt_feed_forward": (_int, [_int, _int, _vp, _i64, _i64, _int, _int, _int, _vp, _vp, _vp, _sz, _vp, _vp, _i64,
+                                 _vp]),
+    "yabt_feed_forward_grad_workspace_bytes": (_sz, [_int, _i64, _int, _int, _int]),
+    "yabt_feed_forward_grad": (_int, [_int, _int, _vp, _i64, _vp, _i64, _i64, _int, _int, _int, _vp, _vp, _vp, _vp,
+                                      _sz, _vp, _i64, _vp, _vp, _vp]),
+    "yabt_quantize_rows": (_int, [_int, _vp, _i64, _i64, _int, _vp, _i64, _vp, _vp]),
+    "yabt_product_int8_workspace_bytes": (_sz, [_i64, _int, _int]),
+    "yabt_product_int8": (_int, [_vp, _i64, _vp, _i64, _int, _vp, _i64, _vp, _int, _int, _vp, _sz, _vp, _i64, _vp]),
+    "yabt_feed_forward_int8_workspace_bytes": (_sz, [_i64, _int, _int, _int]),
+    "yabt_feed_forward_int8": (_int, [_int, _int, _vp, _i64, _i64, _int, _int, _int, _vp, _vp, _vp, _vp, _vp, _sz,
+                                      _vp, _i64, _vp]),
 }
 
 

@@ -1,0 +1,1299 @@
+// The dense stage's products on the matrix cores: a gated feed-forward block,
+// forward and backward, and products of 8-bit integers.
+//
+//   [g u] = x W_in^T,  h = act(g) u,  y = h W_out^T
+//   dh = dy W_out,  du = dh act(g),  dg = dh u act'(g)
+//   dx = [dg du] W_in,  dW_in = [dg du]^T x,  dW_out = dy^T h
+//   8 bits:  x_ij = q_ij s_i,  w_oj = p_oj t_o  (q, p whole numbers):  (x w^T)_io = s_i t_o sum_j q_ij p_oj
+//
+// One kernel makes the tiles of all these products; they differ in whether an
+// operand lies along the summed dimension in memory or across it, and in what
+// is done with the sums:
+//
+//   IN, IN8     a tile's columns are gate and up alternately by 32; h = act(g) u leaves it
+//   OUT, OUT8   x w^T as it is; the sums of whole numbers times their rows' and columns' scales
+//   DH          dh, which becomes dg and du on the spot
+//   DX, DWIN, DWOUT   the gradients, side by side in one grid
+//
+// Both operands pass through LDS in steps of 128 bytes of the summed dimension:
+// an instruction takes 32 of them a row whatever they hold, so that 8-bit products
+// are the 16-bit ones with twice the values.  Operands across the summed dimension
+// are read with the transposing LDS loads.  Few rows have kernels of their own,
+// which are bound by the weights' bytes.
+//
+// 16-bit types: h, dg and du are rounded to the inputs' type, as the matrix cores
+// take them (for few rows, whose time is the weights', h is taken in two parts and
+// keeps 16 bits); g and u are kept in fp32 for the backward pass.  So an output has
+// two roundings behind it, its own and that of one factor.  8 bits: h is kept in fp32
+// until its row's largest magnitude is known, sums of codes are whole numbers.
+
+#include "tiles.h"
+#include "yabt_hip.h"
+
+namespace yabt {
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x16 __attribute__((ext_vector_type(16)));
+
+enum Mode { IN, IN8, OUT, OUT8, DH, DX, DWIN, DWOUT };
+enum Act { SILU, GELU, GELU_TANH, RELU };
+
+// One product of M rows by N columns (IN: N of h) over K.
+struct Product {
+    const void* a;                    // the rows' operand and the columns', lda and ldb values from row to row
+    const void* b;
+    int64_t lda, ldb;
+    int M, N, K;
+    int aw, bw;                       // an operand across K: its width in memory
+    int F, Fp, Fi;                    // inner width; up to whole 16 bytes: the pitch of h, half of [dg du]'s; up to a multiple of 4
+    int act;
+    float* pre;                       // (M, 2 Fi): g from 0, u from Fi, or NULL
+    void* h;                          // (M, Fp), or NULL
+    float* h32;                       // (M, Fi): h of 8-bit products and of few rows
+    void* dpre;                       // (M, 2 Fp): dg from 0, du from Fp
+    void* out;
+    int64_t ldo;
+    int out_dtype;
+    const float* sa;                  // scales of rows and columns (IN8: of gates, then of u)
+    const float* sb;
+    float* part;                      // (splits, M, N) where splits > 1: the sums in part (OUT8: as int32)
+    int splits;
+    int x_dtype;                      // few rows of 8 bits: the type of a's values
+};
+
+template <typename T> struct Sums { using Four = f32x4; using Block = f32x16; };
+template <> struct Sums<int8_t> { using Four = i32x4; using Block = i32x16; };
+
+__device__ __forceinline__ i32x16 mma8(u32x4 a, u32x4 b, i32x16 c) {
+    return __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ i32x4 mma8(u32x4 a, u32x4 b, i32x4 c) {
+    return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), c, 0, 0, 0);
+}
+
+// The activation of four gates and its derivative.  16 bits: the hardware's exp2 and
+// reciprocal (gate_sigmoid), and for the normal distribution function the approximation
+// 7.1.26 of Abramowitz and Stegun's handbook, off by 7.5e-8 at most; fp32 and 8 bits, whose
+// codes a small error would move: the accurate functions.
+template <typename T>
+__device__ __forceinline__ float gate_normal(float g) {
+    const float x = fabsf(g) * 0.70710678f;
+    float tail;                        // of the distribution, beyond |g|
+    if constexpr (sizeof(T) == 2) {
+        const float t = __builtin_amdgcn_rcpf(1.0f + 0.3275911f * x);
+        const float p = t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+        tail = 0.5f * p * __expf(-x * x);
+    } else {
+        tail = 0.5f * erfcf(x);
+    }
+    return g > 0.0f ? 1.0f - tail : tail;
+}
+template <typename T>
+__device__ __forceinline__ void activate(int act, f32x4 g, float (&v)[4], float (&slope)[4]) {
+    using S = std::conditional_t<sizeof(T) == 2, T, float>;
+    switch (act) {
+        case SILU:
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const float s = gate_sigmoid<S>(g[q]);
+                v[q] = g[q] * s;
+                slope[q] = s * (1.0f + g[q] * (1.0f - s));
+            }
+            break;
+        case GELU:
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const float p = gate_normal<S>(g[q]), e = -0.5f * g[q] * g[q];
+                v[q] = g[q] * p;
+                // far out the density is 0, and g times it too
+                slope[q] = p + (e > -87.0f ? g[q] * 0.39894228f * (sizeof(T) == 2 ? __expf(e) : expf(e)) : 0.0f);
+            }
+            break;
+        case GELU_TANH:
+            // 0.5 (1 + tanh(z)) = sigmoid(2 z); where g^2 is held at 10^8 it is 0 or 1 already
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const float g2 = fminf(g[q] * g[q], 1e8f);
+                const float s = gate_sigmoid<S>(1.5957691216f * g[q] * (1.0f + 0.044715f * g2));
+                v[q] = g[q] * s;
+                slope[q] = s + g[q] * s * (1.0f - s) * 1.5957691216f * (1.0f + 0.134145f * g2);
+            }
+            break;
+        default:
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                v[q] = g[q] <= 0.0f ? 0.0f : g[q];
+                slope[q] = g[q] > 0.0f ? 1.0f : 0.0f;
+            }
+    }
+}
+
+// The pieces of an operand that a thread brings to LDS.  Pieces past the end of the
+// summed dimension are zero, rows and columns past the product's end repeat the last
+// (their sums are not stored).
+template <typename T, int MODE, bool SIDE_B, int W, int COUNT, int NT, int STEP>
+struct Loader {
+    static constexpr bool ACROSS = SIDE_B ? MODE >= DH : MODE >= DWIN;
+    static constexpr bool GATED = SIDE_B && (MODE == IN || MODE == IN8);
+    static constexpr int CH = VEC<T>;
+    static constexpr int PER_ROW = ACROSS ? W * (int)sizeof(T) / 16 : STEP / 16;
+    const T* ptr[COUNT];       // along: the row, at this piece; across: column of the piece, from row 0
+
+    __device__ __forceinline__ static int row_of(int i) { return (i * NT + (int)threadIdx.x) / PER_ROW; }
+    __device__ __forceinline__ static int piece_of(int i) {
+        const int c = (i * NT + (int)threadIdx.x) % PER_ROW, r = row_of(i);
+        return c ^ spread<T, ACROSS, W, STEP>(r);
+    }
+    __device__ __forceinline__ static int width(const Product& P) { return SIDE_B ? P.bw : P.aw; }
+
+    // first: the tile's first row or column of the operand
+    __device__ __forceinline__ void init(const Product& P, int first) {
+        const T* const base = (const T*)(SIDE_B ? P.b : P.a);
+        const size_t ld = (size_t)(SIDE_B ? P.ldb : P.lda);
+#pragma unroll
+        for (int i = 0; i < COUNT; ++i) {
+            const int r = row_of(i), piece = piece_of(i) * CH;
+            if constexpr (GATED) {
+                // gate and up rows alternately by 32
+                const int f = min(first + (r >> 6) * 32 + (r & 31), P.F - 1);
+                ptr[i] = base + (size_t)((r >> 5 & 1 ? P.F : 0) + f) * ld + piece;
+            } else if constexpr (!ACROSS) {
+                ptr[i] = base + (size_t)min(first + r, (SIDE_B ? P.N : P.M) - 1) * ld + piece;
+            } else {
+                ptr[i] = base + min(first + piece, max(width(P) - CH, 0));
+            }
+        }
+    }
+
+    // where piece i of the step from k0 on lies, or null past the end
+    __device__ __forceinline__ const T* at(const Product& P, int i, int k0, int end) const {
+        if constexpr (!ACROSS) {
+            return k0 + piece_of(i) * CH < end ? ptr[i] + k0 : nullptr;
+        } else {
+            int kk = k0 + row_of(i);
+            if (kk >= end) return nullptr;
+            if constexpr (MODE == DX) {
+                // [dg du] has du from Fp on, W_in its rows from F on
+                if (kk >= P.F) {
+                    if (kk < P.Fp) return nullptr;
+                    kk += P.F - P.Fp;
+                }
+            }
+            return ptr[i] + (size_t)kk * (size_t)(SIDE_B ? P.ldb : P.lda);
+        }
+    }
+
+    // pieces LO .. HI - 1 of the step from k0 on
+    template <int LO = 0, int HI = COUNT>
+    __device__ __forceinline__ void fill(const Product& P, int k0, int end, uint32_t lds) const {
+#pragma unroll
+        for (int i = LO; i < HI; ++i) {
+            const T* p = at(P, i, k0, end);
+            const uint32_t base = lds + (uint32_t)(i * NT * 16) + ((threadIdx.x & ~63u) << 4);
+            lds_fill(p ? (const void*)p : (const void*)&g_zeros, __builtin_amdgcn_readfirstlane(base));
+        }
+    }
+
+    // the same through registers, for rows at any address: the values that
+    // exist, zeros for the others
+    __device__ __forceinline__ void fetch(const Product& P, int k0, int end, int first, u32x4* v) const {
+        typedef T VT __attribute__((ext_vector_type(CH)));
+#pragma unroll
+        for (int i = 0; i < COUNT; ++i) {
+            const T* p = at(P, i, k0, end);
+            u32x4 o = {0, 0, 0, 0};
+            if (p) {
+                const int piece = piece_of(i) * CH;
+                int have;
+                if constexpr (ACROSS) {
+                    // the column clamp of init() does not hold pieces that end past the row
+                    const int w = width(P);
+                    p += first + piece - min(first + piece, max(w - CH, 0));
+                    have = w - (first + piece);
+                } else {
+                    have = end - (k0 + piece);
+                }
+                if (have >= CH) o = *reinterpret_cast<const u32x4_any*>(p);
+                else {
+                    VT t = {};
+#pragma unroll
+                    for (int j = 0; j < CH; ++j)
+                        if (j < have) t[j] = p[j];
+                    o = __builtin_bit_cast(u32x4, t);
+                }
+            }
+            v[i] = o;
+        }
+    }
+    __device__ __forceinline__ static void put(lds_char* tile, const u32x4* v) {
+#pragma unroll
+        for (int i = 0; i < COUNT; ++i) *(lds_u32x4*)(tile + (i * NT + (int)threadIdx.x) * 16) = v[i];
+    }
+};
+
+// Up to four values at p in the type that a run-time number names.
+__device__ __forceinline__ void store_as(int dtype, void* p, size_t at, f32x4 v, int have) {
+    if (dtype == DT_F32) store_part((float*)p + at, v, have);
+    else if (dtype == DT_BF16) store_part((bf16*)p + at, v, have);
+    else store_part((f16*)p + at, v, have);
+}
+
+// Four values from p on, those that exist.
+__device__ __forceinline__ f32x4 four_of(const float* p, int have) {
+    typedef f32x4 f32x4_any __attribute__((aligned(4)));
+    if (have >= 4) return *(const f32x4_any*)p;
+    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int q = 0; q < 3; ++q)
+        if (q < have) v[q] = p[q];
+    return v;
+}
+
+// The product's M in the rows of its output, and output row of tile row m, M or more if none:
+// dW_in's rows lie in [dg du] with a gap behind F.
+template <int MODE>
+__device__ __forceinline__ int out_row(const Product& P, int m) {
+    if constexpr (MODE == DWIN) return m < P.F ? m : m < P.Fp ? INT32_MAX : m + P.F - P.Fp;
+    return m;
+}
+
+// One tile of the product MODE: that of the block with number `block` of its grid
+// of mtiles x ntiles x splits.
+template <typename T, int MODE, typename TL, bool DMA>
+__device__ __forceinline__ void feed_tile(const Product& P, uint32_t block, int ntiles, int mtiles) {
+    using Block = typename Sums<T>::Block;
+    constexpr bool GATED = MODE == IN || MODE == IN8;
+    lds_char* const lds = (lds_char*)s_tiles;
+    const uint32_t lds_at = (uint32_t)(uintptr_t)lds;
+    const int wave = threadIdx.x / 64, lane = threadIdx.x & 63;
+    const int wm = wave / TL::WN, wn = wave % TL::WN;
+
+    // column tiles together with a group of row tiles, on one die
+    const int64_t per = (int64_t)mtiles * ntiles, id = die_order(block, per * P.splits);
+    if (id >= per * P.splits) return;
+    const int split = (int)(id / per);
+    const int64_t in = id - split * per, group = in / ((int64_t)TILE_GROUP * ntiles);
+    const int gin = (int)(in - group * TILE_GROUP * ntiles);
+    const int gm = (int)min((int64_t)TILE_GROUP, mtiles - group * TILE_GROUP);
+    const int mf = (int)(group * TILE_GROUP + gin % gm) * TL::BM;
+    const int nf = gin / gm * (GATED ? TL::BN / 2 : TL::BN);
+
+    constexpr int BK = TL::STEP / (int)sizeof(T), KS = TL::STEP / 32;
+    const int part = P.splits == 1 ? P.K : ((P.K + P.splits - 1) / P.splits + BK - 1) / BK * BK;
+    const int lo = (int)min((int64_t)P.K, (int64_t)split * part), end = (int)min((int64_t)P.K, (int64_t)lo + part);
+    const int steps = (int)(((int64_t)end - lo + BK - 1) / BK);
+
+    Loader<T, MODE, false, TL::BM, TL::NA, TL::NT, TL::STEP> la;
+    Loader<T, MODE, true, TL::BN, TL::NB, TL::NT, TL::STEP> lb;
+    using LA = decltype(la);
+    using LB = decltype(lb);
+    Block acc[TL::MI][TL::NI];
+#pragma unroll
+    for (int i = 0; i < TL::MI; ++i)
+#pragma unroll
+        for (int j = 0; j < TL::NI; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0;
+
+    if (steps > 0) {
+        la.init(P, mf);
+        lb.init(P, nf);
+        // Step t of the rows' operand lies at place t % AS, of the columns' at t % 2.
+        // The columns' step t + 2 is sent as soon as its place is free, at the end of
+        // step t; the rows' step t + 2 there too, or, with a third place, in two
+        // halves between the products of step t.  Steps past the last are sent too
+        // (zeros), so that every wait is the same.  Without DMA a step waits in
+        // registers for its place.
+        constexpr int AS = DMA ? TL::AS : 2;
+        constexpr bool HALVES = AS == 3;
+        static_assert(TL::BS == 2 && (AS == 2 || AS == 3), "places that the order of the steps is made for");
+        u32x4 ra[DMA ? 1 : TL::NA], rb[DMA ? 1 : TL::NB];
+        // where step t begins; past the end, from where nothing is read
+        auto from = [&](int t) { return (int)min((int64_t)end, lo + (int64_t)t * BK); };
+        auto send_a = [&](int t, int place) {
+            if constexpr (DMA) la.fill(P, from(t), end, lds_at + (uint32_t)place * TL::ABYTES);
+            else la.fetch(P, from(t), end, mf, ra);
+        };
+        auto send_b = [&](int t) {
+            if constexpr (DMA) lb.fill(P, from(t), end, lds_at + TL::AS * TL::ABYTES + (uint32_t)(t & 1) * TL::BBYTES);
+            else lb.fetch(P, from(t), end, nf, rb);
+        };
+        auto put = [&](int t) {
+            LA::put(lds + (t & 1) * TL::ABYTES, ra);
+            LB::put(lds + TL::AS * TL::ABYTES + (t & 1) * TL::BBYTES, rb);
+        };
+        // accesses of every wave after step 0's and, in the loop, after the next step's
+        constexpr int AFTER_0 = DMA ? TL::NA + TL::NB : 0, AFTER = HALVES ? TL::NA : 0;
+        if constexpr (DMA) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                send_a(t, t);
+                send_b(t);
+            }
+        } else {
+            send_a(0, 0);
+            send_b(0);
+            put(0);
+            send_a(1, 0);
+            send_b(1);
+        }
+        const Frag<T, LA::ACROSS, TL::BM, TL::STEP> fa(wm * TL::MI * 32);
+        const Frag<T, LB::ACROSS, TL::BN, TL::STEP> fb(wn * TL::NI * 32);
+        u32x4 a[2][TL::MI], b[2][TL::NI];
+        auto read = [&](int place, int t, int ks) {
+            lds_char* const ta = lds + place * TL::ABYTES;
+            lds_char* const tb = lds + TL::AS * TL::ABYTES + (t & 1) * TL::BBYTES;
+#pragma unroll
+            for (int i = 0; i < TL::MI; ++i) a[ks & 1][i] = fa.get(ta, i, ks);
+#pragma unroll
+            for (int j = 0; j < TL::NI; ++j) b[ks & 1][j] = fb.get(tb, j, ks);
+        };
+        constexpr int READS = TL::MI * decltype(fa)::READS + TL::NI * decltype(fb)::READS;
+        constexpr int PRODUCTS = TL::MI * TL::NI * (sizeof(T) == 4 ? 4 : 1);
+        stage_ready<AFTER_0>();
+        read(0, 0, 0);
+        // A k-step's operands are read while the one before is multiplied, the
+        // next step's first ones too: the wait for it stands before the last
+        // k-step's products, and what takes the freed places is sent there.
+        int place = 0;
+        for (int t = 0; t < steps; ++t) {
+            const int next = place + 1 == AS ? 0 : place + 1, free = next + 1 == AS ? 0 : next + 1;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                if (ks + 1 < KS) {
+                    if constexpr (HALVES) {
+                        const uint32_t to = lds_at + (uint32_t)free * TL::ABYTES;
+                        if (ks == 0) la.template fill<0, TL::NA / 2>(P, from(t + 2), end, to);
+                        else if (ks == 1) la.template fill<TL::NA / 2, TL::NA>(P, from(t + 2), end, to);
+                    }
+                    read(place, t, ks + 1);
+                } else {
+                    if constexpr (!DMA) put(t + 1);
+                    stage_ready<AFTER>();
+                    send_b(t + 2);
+                    if constexpr (!HALVES) send_a(t + 2, place);
+                    read(next, t + 1, 0);
+                }
+#pragma unroll
+                for (int i = 0; i < TL::MI; ++i)
+#pragma unroll
+                    for (int j = 0; j < TL::NI; ++j) {
+                        if constexpr (sizeof(T) == 1) acc[i][j] = mma8(a[ks & 1][i], b[ks & 1][j], acc[i][j]);
+                        else acc[i][j] = mma<T>(a[ks & 1][i], b[ks & 1][j], acc[i][j]);
+                    }
+                if constexpr (DMA) interleave<PRODUCTS, READS>();
+            }
+            place = next;
+        }
+        stage_ready<0>();                            // nothing may reach the LDS of a block that is gone
+    }
+
+    // The sums go through LDS, 32 rows of a wave at a time, from the matrix
+    // cores' layout (a lane has one column) to four neighbouring columns a lane,
+    // so that what is read and written beside them goes in whole lines.
+    constexpr int W = TL::NI * 32;
+    lds_float* const mine = (lds_float*)(lds + wave * 32 * W * 4);
+    constexpr int LANES = GATED ? W / 8 : W / 4, PASS = 64 / LANES;    // lanes a row, rows at once
+    const int c4 = lane % LANES * 4;
+#pragma unroll
+    for (int i = 0; i < TL::MI; ++i) {
+        wave_sync_lds();
+        // sum r of block (i, j): row 8 (r / 4) + 4 (lane / 32) + r % 4, column 32 j + lane % 32;
+        // the rows of the upper lanes are kept with their blocks in pairs swapped: other banks
+#pragma unroll
+        for (int j = 0; j < TL::NI; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const auto s = acc[i][j][r];
+                mine[(8 * (r / 4) + 4 * (lane >> 5) + r % 4) * W + ((j * 32) ^ (lane & 32)) + (lane & 31)] =
+                    __builtin_bit_cast(float, s);
+            }
+        wave_sync_lds();
+#pragma unroll 4
+        for (int p = 0; p < 32; p += PASS) {
+            const int at = p + lane / LANES, m = mf + (wm * TL::MI + i) * 32 + at;
+            auto bits = [&](int c) { return *(const lds_f32x4*)(mine + at * W + (c ^ ((at & 4) << 3))); };
+            auto whole = [&](int c) {
+                const i32x4 v = __builtin_bit_cast(i32x4, bits(c));
+                return f32x4{(float)v[0], (float)v[1], (float)v[2], (float)v[3]};
+            };
+            if constexpr (GATED) {
+                // columns 64 q + 0..31: gate of f 32 q + 0..31, the next 32: u
+                const int f = nf + wn * (W / 2) + c4, c = (c4 & ~31) * 2 + (c4 & 31);
+                if (m < P.M && f < P.Fp) {
+                    f32x4 g, u;
+                    if constexpr (MODE == IN8) {
+                        const float s = P.sa[m];
+                        g = whole(c) * four_of(P.sb + f, P.F - f) * s;
+                        u = whole(c + 32) * four_of(P.sb + P.F + f, P.F - f) * s;
+                    } else {
+                        g = bits(c);
+                        u = bits(c + 32);
+                    }
+                    float v[4], slope[4], h[4];
+                    activate<T>(P.act, g, v, slope);
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) h[q] = f + q < P.F ? v[q] * u[q] : 0.0f;
+                    if constexpr (MODE == IN8) {
+                        if (f < P.Fi) *(f32x4*)(P.h32 + (size_t)m * (size_t)P.Fi + f) = f32x4{h[0], h[1], h[2], h[3]};
+                    } else {
+                        store4((T*)P.h + (size_t)m * (size_t)P.Fp + f, h);
+                        if (P.pre && f < P.Fi) {
+                            float* pre = P.pre + (size_t)m * 2 * (size_t)P.Fi + f;
+                            *(f32x4*)pre = g;
+                            *(f32x4*)(pre + P.Fi) = u;
+                        }
+                    }
+                }
+            } else if constexpr (MODE == DH) {
+                const int f = nf + wn * W + c4;
+                if (m < P.M && f < P.Fp) {
+                    f32x4 g = {0.0f, 0.0f, 0.0f, 0.0f}, u = g;
+                    if (f < P.Fi) {
+                        const float* pre = P.pre + (size_t)m * 2 * (size_t)P.Fi + f;
+                        g = *(const f32x4*)pre;
+                        u = *(const f32x4*)(pre + P.Fi);
+                    }
+                    const f32x4 dh = bits(c4);
+                    float v[4], slope[4], dg[4], du[4];
+                    activate<T>(P.act, g, v, slope);
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const bool is = f + q < P.F;
+                        dg[q] = is ? dh[q] * u[q] * slope[q] : 0.0f;
+                        du[q] = is ? dh[q] * v[q] : 0.0f;
+                    }
+                    T* dpre = (T*)P.dpre + (size_t)m * 2 * (size_t)P.Fp + f;
+                    store4(dpre, dg);
+                    store4(dpre + P.Fp, du);
+                }
+            } else {
+                const int row = out_row<MODE>(P, m), c = nf + wn * W + c4;
+                const int M = MODE == DWIN ? 2 * P.F : P.M;
+                if (row < M && c < P.N) {
+                    if (P.splits > 1) {
+                        store_part(P.part + ((size_t)split * M + row) * (size_t)P.N + c, bits(c4), P.N - c);
+                    } else if constexpr (MODE == OUT8) {
+                        store_as(P.out_dtype, P.out, (size_t)row * (size_t)P.ldo + c,
+                                 whole(c4) * four_of(P.sb + c, P.N - c) * P.sa[row], P.N - c);
+                    } else {
+                        store_part((T*)P.out + (size_t)row * (size_t)P.ldo + c, bits(c4), P.N - c);
+                    }
+                }
+            }
+        }
+    }
+}
+
+template <typename T, int MODE, typename TL, bool DMA>
+__global__ void __launch_bounds__(TL::NT) k_feed(Product P, int ntiles, int mtiles) {
+    feed_tile<T, MODE, TL, DMA>(P, blockIdx.x, ntiles, mtiles);
+}
+
+// DX, DWIN and DWOUT need nothing of each other: one grid, so that one's last
+// tiles run beside the next one's first.
+struct GradProducts {
+    Product p[3];
+    int nt[3], mt[3];
+    uint32_t first[2];                // DWIN's and DWOUT's first blocks, multiples of XCDS
+};
+template <typename T, typename TL, bool DMA>
+__global__ void __launch_bounds__(TL::NT) k_feed_grads(GradProducts G) {
+    if (blockIdx.x < G.first[0]) feed_tile<T, DX, TL, DMA>(G.p[0], blockIdx.x, G.nt[0], G.mt[0]);
+    else if (blockIdx.x < G.first[1]) feed_tile<T, DWIN, TL, DMA>(G.p[1], blockIdx.x - G.first[0], G.nt[1], G.mt[1]);
+    else feed_tile<T, DWOUT, TL, DMA>(G.p[2], blockIdx.x - G.first[1], G.nt[2], G.mt[2]);
+}
+
+// The sums of up to three products that were made in part, added in order.
+struct Join {
+    const float* part;
+    void* out;
+    int64_t ldo;
+    int M, N, splits, dtype;
+    const float* sa;                  // whole numbers in part: their scales
+    const float* sb;
+};
+struct Joins {
+    Join j[3];
+    int count;
+};
+__global__ void __launch_bounds__(256) k_join(Joins A) {
+    for (int o = 0; o < A.count; ++o) {
+        const Join& J = A.j[o];
+        const int per = (J.N + 3) / 4;
+        const int64_t work = (int64_t)J.M * per;
+        const size_t each = (size_t)J.M * (size_t)J.N;
+        for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < work; i += (int64_t)gridDim.x * 256) {
+            const int row = (int)(i / per), c = (int)(i - (int64_t)row * per) * 4;
+            const float* p = J.part + (size_t)row * (size_t)J.N + c;
+            f32x4 s;
+            if (J.sa) {
+                i32x4 whole = {0, 0, 0, 0};
+                for (int k = 0; k < J.splits; ++k) whole += __builtin_bit_cast(i32x4, four_of(p + k * each, J.N - c));
+                s = f32x4{(float)whole[0], (float)whole[1], (float)whole[2], (float)whole[3]} *
+                    four_of(J.sb + c, J.N - c) * J.sa[row];
+            } else {
+                s = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+                for (int k = 0; k < J.splits; ++k) s += four_of(p + k * each, J.N - c);
+            }
+            store_as(J.dtype, J.out, (size_t)row * (size_t)J.ldo + c, s, J.N - c);
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Rows in 8 bits: codes of a 127th of the row's largest magnitude.
+// ---------------------------------------------------------------------------
+
+constexpr float ROW_LEAST = 0x1p-100f;           // a row whose largest magnitude is below counts as zeros
+
+__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
+
+// The scale of a row with this largest magnitude (as bits: infinities and NaN are
+// larger than numbers) and what its values are multiplied by; a row that is not
+// finite has zeros for codes and NaN for its scale.
+__device__ __forceinline__ float row_scale(uint32_t bits, float* unit) {
+    const float most = __uint_as_float(bits);
+    const bool finite = bits < 0x7F800000u, some = finite && most >= ROW_LEAST;
+    *unit = some ? 127.0f / most : 0.0f;
+    return !finite ? __uint_as_float(0x7FC00000u) : some ? most * (1.0f / 127.0f) : 0.0f;
+}
+__device__ __forceinline__ int row_code(float v, float unit) {
+    // unit 0: v may be infinite or NaN
+    return unit == 0.0f ? 0 : (int)fminf(fmaxf(rintf(v * unit), -127.0f), 127.0f);
+}
+template <typename T>
+__device__ __forceinline__ uint32_t chunk_most(const Chunk<T>& c) {
+    uint32_t most = 0;
+#pragma unroll
+    for (int i = 0; i < VEC<T>; ++i) {
+        const uint32_t b = magnitude(c.get(i));
+        most = most > b ? most : b;
+    }
+    return most;
+}
+// Codes of a chunk as bytes, to p (of any alignment when `have` of them exist only).
+template <typename T>
+__device__ __forceinline__ void chunk_codes(const Chunk<T>& c, float unit, int8_t* p, int have) {
+    if (have >= VEC<T>) {
+        uint32_t w[VEC<T> / 4];
+#pragma unroll
+        for (int i = 0; i < VEC<T> / 4; ++i) {
+            w[i] = 0;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) w[i] |= (uint32_t)(row_code(c.get(4 * i + q), unit) & 0xFF) << (8 * q);
+        }
+        typedef uint32_t WT __attribute__((ext_vector_type(VEC<T> / 4)));
+        typedef WT WTany __attribute__((aligned(1)));
+        WT o;
+#pragma unroll
+        for (int i = 0; i < VEC<T> / 4; ++i) o[i] = w[i];
+        *(WTany*)p = o;
+    } else {
+#pragma unroll
+        for (int q = 0; q < VEC<T>; ++q)
+            if (q < have) p[q] = (int8_t)row_code(c.get(q), unit);
+    }
+}
+
+// A row by LANES threads of a block (64: a wave, four rows a block; 256: the block), CHUNKS
+// pieces of 16 bytes a thread in registers; what does not fit there is read again.
+constexpr int QUANT_CHUNKS = 4;
+template <typename T, int LANES>
+__global__ void __launch_bounds__(256) k_quantize(const T* x, int64_t ldx, int64_t n, int D, int8_t* q, int64_t ldq, float* scale) {
+    __shared__ uint32_t s_most[4];
+    const int64_t row = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+    const int t = threadIdx.x % LANES;
+    if (LANES == 64 && row >= n) return;          // a wave by itself: no barrier below
+    const T* const r = x + (size_t)row * (size_t)ldx;
+    const int chunks = (D + VEC<T> - 1) / VEC<T>;
+    Chunk<T> c[QUANT_CHUNKS];
+    uint32_t most = 0;
+#pragma unroll
+    for (int i = 0; i < QUANT_CHUNKS; ++i) {
+        const int at = i * LANES + t;
+        c[i].raw = u32x4{0, 0, 0, 0};
+        if (at < chunks) c[i].raw = row_piece<T>(r, at * VEC<T>, D);
+    }
+#pragma unroll
+    for (int i = 0; i < QUANT_CHUNKS; ++i) most = max(most, chunk_most(c[i]));
+    for (int at = QUANT_CHUNKS * LANES + t; at < chunks; at += LANES) {
+        Chunk<T> d;
+        d.raw = row_piece<T>(r, at * VEC<T>, D);
+        most = max(most, chunk_most(d));
+    }
+    most = lanes_reduce<64>(most, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
+    if constexpr (LANES == 256) {
+        if ((threadIdx.x & 63) == 0) s_most[threadIdx.x / 64] = most;
+        __syncthreads();
+        most = max(max(s_most[0], s_most[1]), max(s_most[2], s_most[3]));
+    }
+    float unit;
+    const float s = row_scale(most, &unit);
+    int8_t* const o = q + (size_t)row * (size_t)ldq;
+#pragma unroll
+    for (int i = 0; i < QUANT_CHUNKS; ++i) {
+        const int at = i * LANES + t;
+        if (at < chunks) chunk_codes(c[i], unit, o + at * VEC<T>, D - at * VEC<T>);
+    }
+    for (int at = QUANT_CHUNKS * LANES + t; at < chunks; at += LANES) {
+        Chunk<T> d;
+        d.raw = row_piece<T>(r, at * VEC<T>, D);
+        chunk_codes(d, unit, o + at * VEC<T>, D - at * VEC<T>);
+    }
+    if (t == 0) scale[row] = s;
+}
+
+// ---------------------------------------------------------------------------
+// Few rows: the products are bound by the weights' bytes, each read once, and by
+// the launches.  Weights go straight from memory into the matrix instructions'
+// operands: a lane fetches 32 bytes in a row of one weight row, two instructions' worth, 16
+// weight rows and 16 rows of x a wave.  A block has 16 columns (IN: of h) and its
+// waves share the summed dimension, 128 bytes a row in turn; their sums meet in LDS.
+// ---------------------------------------------------------------------------
+
+constexpr int FEW_ROWS = 64;                     // rows of a call, up to four groups of 16
+constexpr int FEW_NT = 512;
+constexpr int FEW_VALUES = 16384;                // values of x that every block puts in 8 bits by itself
+
+// Where the rows of x come from: a lane's piece of 16 bytes' worth of T from value k on, fetched
+// as RAW pieces and taken apart into PARTS operands.
+template <typename T>
+struct FewRows {                                 // rows of T in memory
+    static constexpr int RAW = 1, PARTS = 1;
+    const T* base;
+    size_t ld;
+    int n;
+    __device__ __forceinline__ void load(int mb, int k, int K, u32x4 (&raw)[RAW]) const {
+        raw[0] = row_piece<T>(base + (size_t)min(mb * 16 + (int)(threadIdx.x & 15), n - 1) * ld, k, K);
+    }
+    __device__ __forceinline__ static void parts(const u32x4 (&raw)[RAW], u32x4 (&v)[PARTS]) { v[0] = raw[0]; }
+};
+template <typename T>
+struct FewHalves {                               // fp32 rows in two parts of T: 16 bits and more of each value
+    static constexpr int RAW = 2, PARTS = 2;
+    const float* base;
+    size_t ld;
+    int n;
+    __device__ __forceinline__ void load(int mb, int k, int K, u32x4 (&raw)[RAW]) const {
+        const float* row = base + (size_t)min(mb * 16 + (int)(threadIdx.x & 15), n - 1) * ld;
+        raw[0] = row_piece<float>(row, k, K);
+        raw[1] = row_piece<float>(row, k + 4, K);
+    }
+    __device__ __forceinline__ static void parts(const u32x4 (&raw)[RAW], u32x4 (&v)[PARTS]) {
+        typedef T VT __attribute__((ext_vector_type(8)));
+        VT hi, lo;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+            const float f = __builtin_bit_cast(f32x4, raw[q / 4])[q % 4];
+            hi[q] = (T)f;
+            lo[q] = (T)(f - (float)hi[q]);
+        }
+        v[0] = __builtin_bit_cast(u32x4, hi);
+        v[1] = __builtin_bit_cast(u32x4, lo);
+    }
+};
+struct FewCodes {                                // codes that the block put in LDS, `ld` bytes a row
+    static constexpr int RAW = 1, PARTS = 1;
+    const lds_char* base;
+    int ld, n;
+    __device__ __forceinline__ void load(int mb, int k, int K, u32x4 (&raw)[RAW]) const {
+        raw[0] = u32x4{0, 0, 0, 0};
+        if (k < K) raw[0] = *(const lds_u32x4*)(base + min(mb * 16 + (int)(threadIdx.x & 15), n - 1) * ld + k);
+    }
+    __device__ __forceinline__ static void parts(const u32x4 (&raw)[RAW], u32x4 (&v)[PARTS]) { v[0] = raw[0]; }
+};
+
+// acc[m][b] += M matrices' 16 rows w[m] times group b of 16 rows of x, from piece `from` of 128
+// bytes on, every `by`-th.
+template <typename T, int M, int MB, typename Src>
+__device__ __forceinline__ void few_sums(const T* const (&w)[M], const Src& x, int K, int from, int by,
+                                         typename Sums<T>::Four (&acc)[M][MB]) {
+    constexpr int CH = VEC<T>, STEP = 8 * CH;    // values in 128 bytes
+    constexpr int AHEAD = MB * Src::RAW >= 4 ? 2 : 4;    // pieces of a row under way
+    const int q = (threadIdx.x & 63) >> 4;
+    for (int k0 = from * STEP; k0 < K; k0 += by * AHEAD * STEP) {
+        u32x4 a[AHEAD][M][2], v[AHEAD][2][MB][Src::RAW];
+#pragma unroll
+        for (int s = 0; s < AHEAD; ++s)
+#pragma unroll
+            for (int o = 0; o < 2; ++o) {
+                const int k = k0 + s * by * STEP + (2 * q + o) * CH;
+#pragma unroll
+                for (int m = 0; m < M; ++m) a[s][m][o] = row_piece<T>(w[m], k, K);
+#pragma unroll
+                for (int b = 0; b < MB; ++b) x.load(b, k, K, v[s][o][b]);
+            }
+#pragma unroll
+        for (int s = 0; s < AHEAD; ++s)
+#pragma unroll
+            for (int o = 0; o < 2; ++o)
+#pragma unroll
+                for (int b = 0; b < MB; ++b) {
+                    u32x4 p[Src::PARTS];
+                    Src::parts(v[s][o][b], p);
+#pragma unroll
+                    for (int m = 0; m < M; ++m)
+#pragma unroll
+                        for (int i = 0; i < Src::PARTS; ++i) {
+                            if constexpr (sizeof(T) == 1) acc[m][b] = mma8(a[s][m][o], p[i], acc[m][b]);
+                            else acc[m][b] = mma16<T>(a[s][m][o], p[i], acc[m][b]);
+                        }
+                }
+    }
+}
+
+// The block's rows of x (type X) as codes in LDS, rows ld bytes apart, and their scales.
+template <typename X>
+__device__ __forceinline__ void few_codes(const Product& P, lds_char* codes, int ld, uint32_t* most, float* scale) {
+    constexpr int CH = VEC<X>, EACH = FEW_VALUES / CH / FEW_NT;
+    const int per = (P.K + 15) / 16 * (16 / CH), all = P.M * per;      // the last code piece is filled up with zeros
+    Chunk<X> c[EACH + 1];                         // rows of whole 16 codes may hold a little more than FEW_VALUES
+    if ((int)threadIdx.x < P.M) most[threadIdx.x] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i <= EACH; ++i) {
+        const int at = i * FEW_NT + (int)threadIdx.x;
+        c[i].raw = u32x4{0, 0, 0, 0};
+        if (at < all) c[i].raw = row_piece<X>((const X*)P.a + (size_t)(at / per) * (size_t)P.lda, at % per * CH, P.K);
+    }
+#pragma unroll
+    for (int i = 0; i <= EACH; ++i) {
+        const int at = i * FEW_NT + (int)threadIdx.x;
+        if (at < all) atomicMax(&most[at / per], chunk_most(c[i]));
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i <= EACH; ++i) {
+        const int at = i * FEW_NT + (int)threadIdx.x;
+        if (at < all) {
+            float unit;
+            row_scale(most[at / per], &unit);
+            chunk_codes(c[i], unit, (int8_t*)(codes + at / per * ld + at % per * CH), CH);
+        }
+    }
+    if ((int)threadIdx.x < P.M) {
+        float unit;
+        scale[threadIdx.x] = row_scale(most[threadIdx.x], &unit);
+    }
+    __syncthreads();
+}
+
+// MODE IN or OUT with T f32, bf16, f16; IN8 or OUT8 with int8_t, CODES: a's values become codes here.
+// OUT's rows are h in fp32.
+template <typename T, int MODE, int MB, bool CODES>
+__global__ void __launch_bounds__(FEW_NT) k_few(Product P) {
+    constexpr bool GATED = MODE == IN || MODE == IN8;
+    constexpr int M = GATED ? 2 : 1, WAVES = FEW_NT / 64;
+    using Four = typename Sums<T>::Four;
+    __shared__ Four s_sum[WAVES][M][64];
+    __shared__ float s_scale[FEW_ROWS];
+    __shared__ uint32_t s_most[FEW_ROWS];
+    const int wave = threadIdx.x / 64, lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+    const int first = blockIdx.x * 16;
+    const T* w[M];
+    w[0] = (const T*)P.b + (size_t)min(first + r, P.N - 1) * (size_t)P.ldb;
+    if constexpr (GATED) w[1] = w[0] + (size_t)P.F * (size_t)P.ldb;
+    Four acc[M][MB];
+#pragma unroll
+    for (int m = 0; m < M; ++m)
+#pragma unroll
+        for (int b = 0; b < MB; ++b) acc[m][b] = Four{0, 0, 0, 0};
+    if constexpr (CODES) {
+        lds_char* const codes = (lds_char*)s_tiles;
+        const int ld = (P.K + 15) / 16 * 16 + 16;        // rows begin at other banks
+        if (P.x_dtype == DT_F32) few_codes<float>(P, codes, ld, s_most, s_scale);
+        else if (P.x_dtype == DT_BF16) few_codes<bf16>(P, codes, ld, s_most, s_scale);
+        else few_codes<f16>(P, codes, ld, s_most, s_scale);
+        few_sums<T, M, MB>(w, FewCodes{codes, ld, P.M}, P.K, wave, WAVES, acc);
+    } else if constexpr (MODE == OUT && sizeof(T) == 2) {
+        few_sums<T, M, MB>(w, FewHalves<T>{(const float*)P.a, (size_t)P.lda, P.M}, P.K, wave, WAVES, acc);
+    } else {
+        few_sums<T, M, MB>(w, FewRows<T>{(const T*)P.a, (size_t)P.lda, P.M}, P.K, wave, WAVES, acc);
+    }
+#pragma unroll
+    for (int b = 0; b < MB; ++b) {
+        if (b) __syncthreads();                          // the sums of the rows before have been read
+#pragma unroll
+        for (int m = 0; m < M; ++m) s_sum[wave][m][lane] = acc[m][b];
+        __syncthreads();
+        // a lane has row r and columns first + 4 q .. + 3
+        const int row = b * 16 + r, c = first + 4 * q;
+        if (wave == 0 && row < P.M && c < P.N) {
+            Four t[M];
+#pragma unroll
+            for (int m = 0; m < M; ++m) {
+                t[m] = s_sum[0][m][lane];
+#pragma unroll
+                for (int o = 1; o < WAVES; ++o) t[m] += s_sum[o][m][lane];
+            }
+            f32x4 v[M];
+            if constexpr (sizeof(T) == 1) {
+                const float s = CODES ? s_scale[row] : P.sa[row];
+#pragma unroll
+                for (int m = 0; m < M; ++m)
+                    v[m] = f32x4{(float)t[m][0], (float)t[m][1], (float)t[m][2], (float)t[m][3]} *
+                           four_of(P.sb + m * P.F + c, P.N - c) * s;
+            } else {
+#pragma unroll
+                for (int m = 0; m < M; ++m) v[m] = t[m];
+            }
+            if constexpr (GATED) {
+                float a[4], slope[4], h[4];
+                activate<T>(P.act, v[0], a, slope);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) h[i] = c + i < P.F ? a[i] * v[M - 1][i] : 0.0f;
+                *(f32x4*)(P.h32 + (size_t)row * (size_t)P.Fi + c) = f32x4{h[0], h[1], h[2], h[3]};
+                if constexpr (sizeof(T) != 1) {
+                    if (P.h) store_part((T*)P.h + (size_t)row * (size_t)P.Fp + c, f32x4{h[0], h[1], h[2], h[3]}, P.Fp - c);
+                    if (P.pre) {
+                        float* pre = P.pre + (size_t)row * 2 * (size_t)P.Fi + c;
+                        *(f32x4*)pre = v[0];
+                        *(f32x4*)(pre + P.Fi) = v[M - 1];
+                    }
+                }
+            } else {
+                store_as(P.out_dtype, P.out, (size_t)row * (size_t)P.ldo + c, v[0], P.N - c);
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------
+
+using TileSmall = TileOf<64, 128, 2, 2, 128, 2, 2>;
+using TileLarge = TileOf<256, 256, 4, 2, 128, 3, 2>;
+
+constexpr int PART_BLOCKS = 512;      // blocks that keep the device busy
+constexpr int MOST_SPLITS = 64;
+constexpr int INT8_MOST = 131071;     // terms of 128 x 128 whose sum stays in 32 bits
+
+// Whether 256 x 256 tiles make a product of M x K by K x N (its sums' columns) faster than 64 x 128:
+// they fetch a third of the bytes, but there have to be enough of them, and a block of theirs has
+// its CU to itself, so that nothing covers its beginning and end unless K is long.  fp32 is bound by
+// its arithmetic, of which small tiles waste less at the edges.
+inline bool large_product(int bytes, int64_t M, int64_t N, int64_t K) {
+    return bytes <= 2 && K * bytes >= 768 && M >= 192 && N >= 192 && over(M, 256) * over(N, 256) >= 128;
+}
+
+// Parts of the summed dimension, so that few tiles fill the device: at least four steps each.
+inline int split_count(int64_t M, int64_t N, int64_t K, bool large, int bytes) {
+    const int64_t tiles = over(M, large ? 256 : 64) * over(N, large ? 256 : 128);
+    int64_t s = PART_BLOCKS / (tiles < 1 ? 1 : tiles);
+    const int64_t longest = K * bytes / (4 * 128);
+    if (s > longest) s = longest;
+    if (s > MOST_SPLITS) s = MOST_SPLITS;
+    return s < 1 ? 1 : (int)s;
+}
+
+template <typename TL>
+int64_t tile_grid(const Product& P, bool gated, int* nt, int* mt, int M) {
+    *nt = (int)over(P.N, gated ? TL::BN / 2 : TL::BN);
+    *mt = (int)over(M, TL::BM);
+    return over((int64_t)*nt * *mt * P.splits, XCDS) * XCDS;
+}
+inline bool grid_ok(int64_t blocks, int threads) { return blocks > 0 && blocks <= UINT32_MAX / threads; }
+
+// fp32 has no large tiles (large_product).
+template <typename T, typename F>
+auto by_tile(bool large, bool dma, const F& f) {
+    if constexpr (sizeof(T) <= 2) {
+        if (large) return dma ? f(TileLarge(), std::true_type()) : f(TileLarge(), std::false_type());
+    }
+    return dma ? f(TileSmall(), std::true_type()) : f(TileSmall(), std::false_type());
+}
+
+// Makes the tiles of one product; false: the grid would be too large.
+template <typename T, int MODE>
+bool run_tiles(const Product& P, bool large, bool dma, hipStream_t stream) {
+    return by_tile<T>(large, dma, [&](auto tl, auto d) {
+        using TL = decltype(tl);
+        int nt, mt;
+        const int64_t blocks = tile_grid<TL>(P, MODE == IN || MODE == IN8, &nt, &mt, P.M);
+        if (!grid_ok(blocks, TL::NT)) return false;
+        k_feed<T, MODE, TL, decltype(d)::value><<<(unsigned)blocks, TL::NT, TL::LDS, stream>>>(P, nt, mt);
+        return true;
+    });
+}
+
+inline void run_join(const Joins& J, hipStream_t stream) {
+    int64_t work = 0;
+    for (int i = 0; i < J.count; ++i) {
+        const int64_t w = (int64_t)J.j[i].M * over(J.j[i].N, 4);
+        work = w > work ? w : work;
+    }
+    if (J.count) k_join<<<launch_grid(work, 256, 8192), 256, 0, stream>>>(J);
+}
+
+template <typename T, int MODE, bool CODES>
+void run_few(const Product& P, hipStream_t stream) {
+    const unsigned blocks = (unsigned)over(P.N, 16);
+    const size_t lds = CODES ? (size_t)P.M * (size_t)((P.K + 15) / 16 * 16 + 16) : 0;
+    if (P.M <= 16) k_few<T, MODE, 1, CODES><<<blocks, FEW_NT, lds, stream>>>(P);
+    else if (P.M <= 32) k_few<T, MODE, 2, CODES><<<blocks, FEW_NT, lds, stream>>>(P);
+    else k_few<T, MODE, 4, CODES><<<blocks, FEW_NT, lds, stream>>>(P);
+}
+
+template <typename F>
+auto by_dtype(int dtype, const F& f) {
+    if (dtype == DT_F32) return f((float*)nullptr);
+    if (dtype == DT_BF16) return f((bf16*)nullptr);
+    return f((f16*)nullptr);
+}
+
+inline bool few_rows(int64_t n) { return n <= FEW_ROWS; }
+inline bool few_values(int64_t n, int64_t K) { return n * K <= FEW_VALUES; }
+
+inline bool feed_ranges_ok(int64_t n, int D, int F, int O) {
+    return n >= 0 && n < (1ll << 31) - 256 && D >= 1 && F >= 1 && O >= 1 && D <= (1 << 24) && F <= (1 << 24) && O <= (1 << 24);
+}
+
+struct FeedSizes {
+    int64_t n;
+    int D, F, O, bytes, Fp, Fi;
+    bool few, large_in, large_out, large_dh, large_grads;
+    int splits_out, splits[3];        // of y; of dx, dW_in, dW_out
+};
+inline FeedSizes feed_sizes(int dtype, int64_t n, int D, int F, int O) {
+    FeedSizes z;
+    const int b = dtype_bytes(dtype);
+    z.n = n, z.D = D, z.F = F, z.O = O, z.bytes = b;
+    z.Fp = up16(F, b);
+    z.Fi = up16(F, 4);
+    z.few = few_rows(n);
+    z.large_in = large_product(b, n, 2 * (int64_t)F, D);
+    z.large_out = large_product(b, n, O, F);
+    z.splits_out = split_count(n, O, F, z.large_out, b);
+    z.large_dh = large_product(b, n, F, O);
+    const int64_t K3 = (int64_t)z.Fp + F;
+    z.large_grads = large_product(b, n, D, K3) && large_product(b, 2 * (int64_t)F, D, n) && large_product(b, O, F, n);
+    z.splits[0] = split_count(n, D, K3, z.large_grads, b);
+    z.splits[1] = split_count(K3, D, n, z.large_grads, b);
+    z.splits[2] = split_count(O, F, n, z.large_grads, b);
+    return z;
+}
+
+struct FeedKept {                     // what the forward pass keeps
+    float* pre;
+    char* h;
+};
+inline size_t carve_kept(Carve& c, FeedKept* k, const FeedSizes& z) {
+    k->pre = c.take<float>((size_t)z.n * 2 * z.Fi);
+    k->h = c.take<char>((size_t)z.n * z.Fp * z.bytes);
+    return c.off;
+}
+struct FeedSpace {
+    char* h;
+    float* h32;
+    float* part;
+};
+inline size_t carve_forward(Carve& c, FeedSpace* s, const FeedSizes& z) {
+    s->h = c.take<char>((size_t)z.n * z.Fp * z.bytes);
+    s->h32 = z.few ? c.take<float>((size_t)z.n * z.Fi) : nullptr;
+    s->part = !z.few && z.splits_out > 1 ? c.take<float>((size_t)z.splits_out * z.n * z.O) : nullptr;
+    return c.off;
+}
+struct GradSpace {
+    char* dpre;
+    float* part[3];
+};
+inline size_t carve_backward(Carve& c, GradSpace* s, const FeedSizes& z) {
+    const int64_t M[3] = {z.n, 2 * (int64_t)z.F, z.O}, N[3] = {z.D, z.D, z.F};
+    s->dpre = c.take<char>((size_t)z.n * 2 * z.Fp * z.bytes);
+    for (int i = 0; i < 3; ++i) s->part[i] = z.splits[i] > 1 ? c.take<float>((size_t)z.splits[i] * M[i] * N[i]) : nullptr;
+    return c.off;
+}
+
+template <typename T>
+int run_feed(const FeedSizes& z, int act, int dtype, const void* x, int64_t ldx, const void* w_in, const void* w_out,
+             void* y, int64_t ldy, const FeedKept* kept, const FeedSpace& s, hipStream_t stream) {
+    Product P = {};
+    P.a = x, P.lda = ldx, P.b = w_in, P.ldb = z.D;
+    P.M = (int)z.n, P.N = z.F, P.K = z.D;
+    P.F = z.F, P.Fp = z.Fp, P.Fi = z.Fi, P.act = act, P.splits = 1;
+    P.pre = kept ? kept->pre : nullptr;
+    P.h = kept ? kept->h : z.few ? nullptr : s.h;
+    P.h32 = s.h32;
+    const int b = z.bytes;
+    if (z.few) run_few<T, IN, false>(P, stream);
+    else if (!run_tiles<T, IN>(P, z.large_in, pieces_ok(x, ldx, z.D, b) && pieces_ok(w_in, z.D, z.D, b), stream))
+        return fail(-1, "yabt_feed_forward: bad sizes");
+    Product Q = {};
+    Q.b = w_out, Q.ldb = z.F;
+    Q.M = (int)z.n, Q.N = z.O, Q.K = z.F;
+    Q.out = y, Q.ldo = ldy, Q.out_dtype = dtype, Q.splits = 1;
+    if (z.few) {
+        Q.a = s.h32, Q.lda = z.Fi;
+        run_few<T, OUT, false>(Q, stream);
+    } else {
+        Q.a = P.h, Q.lda = z.Fp, Q.splits = z.splits_out, Q.part = s.part;
+        if (!run_tiles<T, OUT>(Q, z.large_out, pieces_ok(w_out, z.F, z.F, b), stream))
+            return fail(-1, "yabt_feed_forward: bad sizes");
+        if (Q.splits > 1) run_join({{{s.part, y, ldy, Q.M, Q.N, Q.splits, dtype, nullptr, nullptr}}, 1}, stream);
+    }
+    return launch_status("yabt_feed_forward");
+}
+
+template <typename T>
+int run_feed_grad(const FeedSizes& z, int act, int dtype, const void* dy, int64_t lddy, const void* x, int64_t ldx,
+                  const void* w_in, const void* w_out, const FeedKept& kept, const GradSpace& s, void* dx, int64_t lddx,
+                  void* dw_in, void* dw_out, hipStream_t stream) {
+    const int b = z.bytes;
+    const bool dma = pieces_ok(x, ldx, z.D, b) && pieces_ok(dy, lddy, z.O, b) && pieces_ok(w_in, z.D, z.D, b) &&
+                     pieces_ok(w_out, z.F, z.F, b);
+    Product P = {};
+    P.a = dy, P.lda = lddy, P.b = w_out, P.ldb = z.F, P.bw = z.F;
+    P.M = (int)z.n, P.N = z.F, P.K = z.O;
+    P.F = z.F, P.Fp = z.Fp, P.Fi = z.Fi, P.act = act, P.splits = 1;
+    P.pre = kept.pre, P.dpre = s.dpre;
+    if (z.n > 0 && !run_tiles<T, DH>(P, z.large_dh, dma, stream)) return fail(-1, "yabt_feed_forward_grad: bad sizes");
+    GradProducts G = {};
+    for (auto& p : G.p) p.F = z.F, p.Fp = z.Fp, p.Fi = z.Fi, p.out_dtype = dtype;
+    Product &X = G.p[0], &I = G.p[1], &O = G.p[2];
+    X.a = s.dpre, X.lda = 2 * (int64_t)z.Fp, X.b = w_in, X.ldb = z.D, X.bw = z.D;
+    X.M = (int)z.n, X.N = z.D, X.K = z.Fp + z.F, X.out = dx, X.ldo = lddx;
+    I.a = s.dpre, I.lda = 2 * (int64_t)z.Fp, I.aw = 2 * z.Fp, I.b = x, I.ldb = ldx, I.bw = z.D;
+    I.M = z.Fp + z.F, I.N = z.D, I.K = (int)z.n, I.out = dw_in, I.ldo = z.D;
+    O.a = dy, O.lda = lddy, O.aw = z.O, O.b = kept.h, O.ldb = z.Fp, O.bw = z.Fp;
+    O.M = z.O, O.N = z.F, O.K = (int)z.n, O.out = dw_out, O.ldo = z.F;
+    for (int i = 0; i < 3; ++i) G.p[i].splits = z.splits[i], G.p[i].part = s.part[i];
+    const bool ok = by_tile<T>(z.large_grads, dma, [&](auto tl, auto d) {
+        using TL = decltype(tl);
+        const int64_t gx = tile_grid<TL>(X, false, &G.nt[0], &G.mt[0], X.M), gi = tile_grid<TL>(I, false, &G.nt[1], &G.mt[1], I.M),
+                      go = tile_grid<TL>(O, false, &G.nt[2], &G.mt[2], O.M);
+        if (!grid_ok(gx + gi + go, TL::NT)) return false;
+        G.first[0] = (uint32_t)gx;
+        G.first[1] = (uint32_t)(gx + gi);
+        k_feed_grads<T, TL, decltype(d)::value><<<(unsigned)(gx + gi + go), TL::NT, TL::LDS, stream>>>(G);
+        return true;
+    });
+    if (!ok) return fail(-1, "yabt_feed_forward_grad: bad sizes");
+    Joins J = {};
+    for (int i = 0; i < 3; ++i)
+        if (G.p[i].splits > 1)
+            J.j[J.count++] = {G.p[i].part, G.p[i].out, G.p[i].ldo, i == 1 ? 2 * z.F : G.p[i].M, G.p[i].N, G.p[i].splits,
+                              dtype, nullptr, nullptr};
+    run_join(J, stream);
+    return launch_status("yabt_feed_forward_grad");
+}
+
+int run_quantize(int dtype, const void* x, int64_t ldx, int64_t n, int D, int8_t* q, int64_t ldq, float* scale, hipStream_t stream) {
+    by_dtype(dtype, [&](auto* t) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        // rows that a wave holds in its registers, and longer ones by a block each
+        if (D <= 64 * QUANT_CHUNKS * VEC<T>) k_quantize<T, 64><<<(unsigned)over(n, 4), 256, 0, stream>>>((const T*)x, ldx, n, D, q, ldq, scale);
+        else k_quantize<T, 256><<<(unsigned)n, 256, 0, stream>>>((const T*)x, ldx, n, D, q, ldq, scale);
+        return 0;
+    });
+    return 0;
+}
+inline bool quantize_ok(int64_t n, int D) { return n >= 0 && n < (1 << 24) && D >= 1 && D <= (1 << 24); }
+
+// A product of codes: how it is made.
+struct Int8Sizes {
+    bool few, large;
+    int splits;
+};
+inline Int8Sizes int8_sizes(int64_t n, int64_t N, int64_t K) {
+    Int8Sizes z;
+    z.few = few_rows(n);
+    z.large = large_product(1, n, N, K);
+    z.splits = split_count(n, N, K, z.large, 1);
+    return z;
+}
+// y = (a b^T) scaled, a (n, K) codes; part: splits x n x N floats where it is made in parts.
+bool run_int8(const Int8Sizes& z, const int8_t* a, int64_t lda, const float* sa, int64_t n, int K, const int8_t* b, int64_t ldb,
+              const float* sb, int N, int out_dtype, void* y, int64_t ldy, float* part, hipStream_t stream) {
+    Product P = {};
+    P.a = a, P.lda = lda, P.b = b, P.ldb = ldb, P.M = (int)n, P.N = N, P.K = K, P.sa = sa, P.sb = sb;
+    P.out = y, P.ldo = ldy, P.out_dtype = out_dtype, P.splits = 1;
+    if (z.few) {
+        run_few<int8_t, OUT8, false>(P, stream);
+        return true;
+    }
+    P.splits = z.splits, P.part = part;
+    if (!run_tiles<int8_t, OUT8>(P, z.large, pieces_ok(a, lda, K, 1) && pieces_ok(b, ldb, K, 1), stream)) return false;
+    if (P.splits > 1) run_join({{{part, y, ldy, P.M, N, P.splits, out_dtype, sa, sb}}, 1}, stream);
+    return true;
+}
+
+struct Feed8Space {
+    int8_t* q;                        // codes of x, then of h
+    float* scale;
+    float* h32;
+    float* part;
+};
+inline size_t carve_feed8(Carve& c, Feed8Space* s, int64_t n, int D, int F, int O) {
+    const Int8Sizes z = int8_sizes(n, O, F);
+    const int64_t w = D > F ? D : F;
+    s->q = c.take<int8_t>((size_t)n * up16((int)w, 1));
+    s->scale = c.take<float>((size_t)n);
+    s->h32 = c.take<float>((size_t)n * up16(F, 4));
+    s->part = !z.few && z.splits > 1 ? c.take<float>((size_t)z.splits * n * O) : nullptr;
+    return c.off;
+}
+
+}  // namespace yabt
+
+using namespace yabt;
+
+extern "C" {
+
+size_t yabt_feed_forward_inner_bytes(int dtype, int64_t n, int D, int F, int O) {
+    if (!dtype_ok(dtype) || !feed_ranges_ok(n, D, F, O)) return 0;
+    Carve c{nullptr, 0};
+    FeedKept k;
+    return carve_kept(c, &k, feed_sizes(dtype, n, D, F, O)) + 256;
+}
+
+size_t yabt_feed_forward_workspace_bytes(int dtype, int64_t n, int D, int F, int O) {
+    if (!dtype_ok(dtype) || !feed_ranges_ok(n, D, F, O)) return 0;
+    Carve c{nullptr, 0};
+    FeedSpace s;
+    return carve_forward(c, &s, feed_sizes(dtype, n, D, F, O)) + 256;
+}
+
+int yabt_feed_forward(int dtype, int act, const void* x, int64_t ldx, int64_t n, int D, int F, int O, const void* w_in,
+                      const void* w_out, void* workspace, size_t workspace_bytes, void* out_inner, void* y, int64_t ldy,
+                      yabt_stream_t stream) {
+    if (!dtype_ok(dtype)) return fail(-1, "yabt_feed_forward: dtype is 0 (fp32), 1 (bf16) or 2 (fp16)");
+    if (act < SILU || act > RELU) return fail(-1, "yabt_feed_forward: the activation is 0 to 3");
+    if (!feed_ranges_ok(n, D, F, O) || ldx < D || ldy < O) return fail(-1, "yabt_feed_forward: bad sizes");
+    if (n == 0) return 0;
+    if (!x || !w_in || !w_out || !y) return fail(-1, "yabt_feed_forward: null pointer");
+    if (!workspace || workspace_bytes < yabt_feed_forward_workspace_bytes(dtype, n, D, F, O))
+        return fail(-2, "yabt_feed_forward: workspace too small");
+    const FeedSizes z = feed_sizes(dtype, n, D, F, O);
+    FeedKept kept;
+    if (out_inner) {
+        Carve c{(char*)align_up((size_t)out_inner, 256), 0};
+        carve_kept(c, &kept, z);
+    }
+    FeedSpace s;
+    Carve c{(char*)align_up((size_t)workspace, 256), 0};
+    carve_forward(c, &s, z);
+    return by_dtype(dtype, [&](auto* t) {
+        return run_feed<std::remove_pointer_t<decltype(t)>>(z, act, dtype, x, ldx, w_in, w_out, y, ldy,
+                                                            out_inner ? &kept : nullptr, s, (hipStream_t)stream);
+    });
+}
+
+size_t yabt_feed_forward_grad_workspace_bytes(int dtype, int64_t n, int D, int F, int O) {
+    if (!dtype_ok(dtype) || !feed_ranges_ok(n, D, F, O)) return 0;
+    Carve c{nullptr, 0};
+    GradSpace s;
+    return carve_backward(c, &s, feed_sizes(dtype, n, D, F, O)) + 256;
+}
+
+int yabt_feed_forward_grad(int dtype, int act, const void* dy, int64_t lddy, const void* x, int64_t ldx, int64_t n, int D,
+                           int F, int O, const void* w_in, const void* w_out, const void* inner, void* workspace,
+                           size_t workspace_bytes, void* dx, int64_t lddx, void* dw_in, void* dw_out, yabt_stream_t stream) {
+    if (!dtype_ok(dtype)) return fail(-1, "yabt_feed_forward_grad: dtype is 0 (fp32), 1 (bf16) or 2 (fp16)");
+    if (act < SILU || act > RELU) return fail(-1, "yabt_feed_forward_grad: the activation is 0 to 3");
+    if (!feed_ranges_ok(n, D, F, O) || ldx < D || lddy < O || lddx < D)
+        return fail(-1, "yabt_feed_forward_grad: bad sizes");
+    if (!w_in || !w_out || !dw_in || !dw_out || (n > 0 && (!x || !dy || !inner || !dx)))
+        return fail(-1, "yabt_feed_forward_grad: null pointer");
+    if (!workspace || workspace_bytes < yabt_feed_forward_grad_workspace_bytes(dtype, n, D, F, O))
+        return fail(-2, "yabt_feed_forward_grad: workspace too small");
+    const FeedSizes z = feed_sizes(dtype, n, D, F, O);
+    FeedKept kept;
+    Carve k{(char*)align_up((size_t)inner, 256), 0};
+    carve_kept(k, &kept, z);
+    GradSpace s;
+    Carve c{(char*)align_up((size_t)workspace, 256), 0};
+    carve_backward(c, &s, z);
+    return by_dtype(dtype, [&](auto* t) {
+        return run_feed_grad<std::remove_pointer_t<decltype(t)>>(z, act, dtype, dy, lddy, x, ldx, w_in, w_out, kept, s, dx,
+                                                                 lddx, dw_in, dw_out, (hipStream_t)stream);
+    });
+}
+
+int yabt_quantize_rows(int dtype, const void* x, int64_t ldx, int64_t n, int D, int8_t* out_codes, int64_t ldq,
+                       float* out_scale, yabt_stream_t stream) {
+    if (!dtype_ok(dtype)) return fail(-1, "yabt_quantize_rows: dtype is 0 (fp32), 1 (bf16) or 2 (fp16)");
+    if (!quantize_ok(n, D) || ldx < D || ldq < D) return fail(-1, "yabt_quantize_rows: bad sizes");
+    if (n == 0) return 0;
+    if (!x || !out_codes || !out_scale) return fail(-1, "yabt_quantize_rows: null pointer");
+    run_quantize(dtype, x, ldx, n, D, out_codes, ldq, out_scale, (hipStream_t)stream);
+    return launch_status("yabt_quantize_rows");
+}
+
+static bool int8_ranges_ok(int64_t n, int K, int N) {
+    return n >= 0 && n < (1 << 24) && K >= 1 && K <= INT8_MOST && N >= 1 && N <= (1 << 24);
+}
+
+size_t yabt_product_int8_workspace_bytes(int64_t n, int K, int N) {
+    if (!int8_ranges_ok(n, K, N)) return 0;
+    const Int8Sizes z = int8_sizes(n, N, K);
+    return (z.few || z.splits == 1 ? 0 : (size_t)z.splits * n * N * 4) + 256;
+}
+
+int yabt_product_int8(const int8_t* a, int64_t lda, const float* a_scale, int64_t n, int K, const int8_t* b, int64_t ldb,
+                      const float* b_scale, int N, int out_dtype, void* workspace, size_t workspace_bytes, void* y,
+                      int64_t ldy, yabt_stream_t stream) {
+    if (!dtype_ok(out_dtype)) return fail(-1, "yabt_product_int8: dtype is 0 (fp32), 1 (bf16) or 2 (fp16)");
+    if (!int8_ranges_ok(n, K, N) || lda < K || ldb < K || ldy < N) return fail(-1, "yabt_product_int8: bad sizes");
+    if (n == 0) return 0;
+    if (!a || !a_scale || !b || !b_scale || !y) return fail(-1, "yabt_product_int8: null pointer");
+    if (!workspace || workspace_bytes < yabt_product_int8_workspace_bytes(n, K, N))
+        return fail(-2, "yabt_product_int8: workspace too small");
+    if (!run_int8(int8_sizes(n, N, K), a, lda, a_scale, n, K, b, ldb, b_scale, N, out_dtype, y, ldy,
+                  (float*)align_up((size_t)workspace, 256), (hipStream_t)stream))
+        return fail(-1, "yabt_product_int8: bad sizes");
+    return launch_status("yabt_product_int8");
+}
+
+size_t yabt_feed_forward_int8_workspace_bytes(int64_t n, int D, int F, int O) {
+    if (!int8_ranges_ok(n, D, O) || !int8_ranges_ok(n, F, O)) return 0;
+    Carve c{nullptr, 0};
+    Feed8Space s;
+    return carve_feed8(c, &s, n, D, F, O) + 256;
+}
+
+int yabt_feed_forward_int8(int dtype, int act, const void* x, int64_t ldx, int64_t n, int D, int F, int O, const int8_t* w_in,
+                           const float* in_scale, const int8_t* w_out, const float* out_scale, void* workspace,
+                           size_t workspace_bytes, void* y, int64_t ldy, yabt_stream_t stream) {
+    if (!dtype_ok(dtype)) return fail(-1, "yabt_feed_forward_int8: dtype is 0 (fp32), 1 (bf16) or 2 (fp16)");
+    if (act < SILU || act > RELU) return fail(-1, "yabt_feed_forward_int8: the activation is 0 to 3");
+    if (!int8_ranges_ok(n, D, O) || !int8_ranges_ok(n, F, O) || ldx < D || ldy < O)
+        return fail(-1, "yabt_feed_forward_int8: bad sizes");
+    if (n == 0) return 0;
+    if (!x || !w_in || !in_scale || !w_out || !out_scale || !y) return fail(-1, "yabt_feed_forward_int8: null pointer");
+    if (!workspace || workspace_bytes < yabt_feed_forward_int8_workspace_bytes(n, D, F, O))
+        return fail(-2, "yabt_feed_forward_int8: workspace too small");
+    const hipStream_t on = (hipStream_t)stream;
+    Feed8Space s;
+    Carve c{(char*)align_up((size_t)workspace, 256), 0};
+    carve_feed8(c, &s, n, D, F, O);
+    const int Fi = up16(F, 4), dq = up16(D, 1), fq = up16(F, 1);
+    Product P = {};
+    P.b = w_in, P.ldb = D, P.M = (int)n, P.N = F, P.K = D, P.F = F, P.Fp = Fi, P.Fi = Fi, P.act = act, P.h32 = s.h32;
+    P.sb = in_scale, P.splits = 1;
+    if (few_rows(n) && few_values(n, D)) {
+        P.a = x, P.lda = ldx, P.x_dtype = dtype;
+        run_few<int8_t, IN8, true>(P, on);
+    } else {
+        run_quantize(dtype, x, ldx, n, D, s.q, dq, s.scale, on);
+        P.a = s.q, P.lda = dq, P.sa = s.scale;
+        if (few_rows(n)) run_few<int8_t, IN8, false>(P, on);
+        else if (!run_tiles<int8_t, IN8>(P, large_product(1, n, 2 * (int64_t)F, D), pieces_ok(s.q, dq, D, 1) && pieces_ok(w_in, D, D, 1), on))
+            return fail(-1, "yabt_feed_forward_int8: bad sizes");
+    }
+    if (few_rows(n) && few_values(n, F)) {
+        Product Q = {};
+        Q.a = s.h32, Q.lda = Fi, Q.x_dtype = DT_F32, Q.b = w_out, Q.ldb = F, Q.M = (int)n, Q.N = O, Q.K = F, Q.sb = out_scale;
+        Q.out = y, Q.ldo = ldy, Q.out_dtype = dtype, Q.splits = 1;
+        run_few<int8_t, OUT8, true>(Q, on);
+    } else {
+        run_quantize(DT_F32, s.h32, Fi, n, F, s.q, fq, s.scale, on);
+        if (!run_int8(int8_sizes(n, O, F), s.q, fq, s.scale, n, F, w_out, F, out_scale, O, dtype, y, ldy, s.part, on))
+            return fail(-1, "yabt_feed_forward_int8: bad sizes");
+    }
+    return launch_status("yabt_feed_forward_int8");
+}
+
+}  // extern "C"
