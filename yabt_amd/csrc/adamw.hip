@@ -328,7 +328,7 @@ int yabt_adamw_step(int count, const yabt_adamw_tensor* tensors, int bits, int64
     AdamwScalars S = {(float)(1.0 - beta1), (float)(1.0 - beta2), (float)(1.0 - lr * weight_decay), 0.0f, 0.0f, lr, beta1,
                       beta2, eps, step_device};
     if (!step_device) {
-        const double left = std::sqrt(1.0 - std::pow(beta2, (double)step));
+        const double left = std::pow(1.0 - std::pow(beta2, (double)step), 0.5);
         S.scale = (float)(lr * left / (1.0 - std::pow(beta1, (double)step)));
         S.eps = (float)(eps * left);
     }

@@ -15,11 +15,13 @@ Per row, with x the standardised inputs (missing ones, NaN or infinite, at their
 mean, 0, and columns that the fit saw no spread in always 0):
 
     r = x A;  a = layer_norm(r);  ids, weights = route(a G, k);
-    out = (r + sum_j weights_j expert_{ids_j}(a)) h
+    out = (r + sum_j weights_j expert_{ids_j}(a) + block(a)) h
 
-The passes are the operations of ``expert_ops`` and torch's plain matrix
-products; g comes from the booster's own losses (``boost_ops.grad_hess``);
-the parameters are fitted by Adam on mini-batches.  The gate's choice is
+where block, if there is one, is a gated feed-forward block that every row
+passes.  The passes are the operations of ``expert_ops`` and ``feed_ops`` and torch's
+plain matrix products; g comes from the booster's own losses (``boost_ops.grad_hess``);
+the parameters are fitted by AdamW (``optim.adamw_step``; without decay of the weights
+Adam) on mini-batches.  The gate's choice is
 balanced by a bias per expert that moves against its share of the rows, by a
 constant step, and takes no part in the weights.
 """
@@ -31,7 +33,7 @@ from dataclasses import dataclass
 import numpy as np
 import torch
 
-from . import boost_ops, expert_ops
+from . import boost_ops, expert_ops, feed_ops, optim
 
 
 @dataclass
@@ -49,6 +51,9 @@ class ExpertParams:
                                   # ("float16" ends at 65504: a fit or an answer that leaves it is an error)
     random_state: int = 0
     device: str = "cuda"
+    shared: int = 0               # inner width of the block that every row passes; 0: none
+    weight_decay: float = 0.0     # of the matrices, by step times learning rate
+    state_bits: int = 32          # of the fit's moments: 32, or 8 where memory is short
 
 
 _DTYPES = {"float32": torch.float32, "bfloat16": torch.bfloat16, "float16": torch.float16}
@@ -118,8 +123,11 @@ class ExpertStage:
             raise ValueError(f"scores must be one of {sorted(expert_ops.SCORES)}, got {p.scores!r}")
         if not 1 <= p.k <= min(p.experts, expert_ops.MAX_K) or p.experts > expert_ops.MAX_EXPERTS:
             raise ValueError(f"{p.k} of {p.experts} experts: at most {expert_ops.MAX_K} of {expert_ops.MAX_EXPERTS}")
-        if min(p.width, p.inner, p.batch_rows) < 1 or p.epochs < 0:
-            raise ValueError("width, inner and batch_rows must be positive, epochs not negative")
+        if min(p.width, p.inner, p.batch_rows) < 1 or p.epochs < 0 or p.shared < 0:
+            raise ValueError("width, inner and batch_rows must be positive, epochs and shared not negative")
+        if p.state_bits not in (32, 8) or not 0.0 <= p.weight_decay <= 1e30:
+            raise ValueError(f"state_bits must be 32 or 8 and weight_decay not negative, got {p.state_bits}, "
+                             f"{p.weight_decay}")
 
     def _inputs(self, X: np.ndarray) -> torch.Tensor:
         Xt = torch.as_tensor(np.asarray(X, dtype=np.float32), device=self.device_)
@@ -131,8 +139,13 @@ class ExpertStage:
     def _head(self) -> torch.Tensor:
         return self.weights_["head"] if self.unit_ is None else self.weights_["head"] * self.unit_
 
-    def _forward(self, x: torch.Tensor, keep: bool):
-        """(out (n,), what the backward pass needs)."""
+    def _shared_codes(self) -> tuple[torch.Tensor, ...]:
+        """The shared block's weights in 8 bits."""
+        w = self.weights_
+        return (*feed_ops.quantize_rows(w["shared_in"]), *feed_ops.quantize_rows(w["shared_out"]))
+
+    def _forward(self, x: torch.Tensor, keep: bool, codes: tuple[torch.Tensor, ...] | None = None):
+        """(out (n,), what the backward pass needs); codes: the shared block's weights in 8 bits."""
         w, p, dt = self.weights_, self.p, _DTYPES[self.p.dtype]
         r = x @ w["embed"]
         a, mean, rstd = expert_ops.layer_norm(r, w["norm"], w["shift"])
@@ -141,33 +154,55 @@ class ExpertStage:
         plan = expert_ops.expert_plan(ids, p.experts)
         ac, w_in, w_out = a.to(dt), w["w_in"].to(dt), w["w_out"].to(dt)
         if not keep:
-            y = expert_ops.expert_products(ac, plan, weights, w_in, w_out)
-            return (r + y) @ self._head(), None
+            s = r + expert_ops.expert_products(ac, plan, weights, w_in, w_out)
+            if codes is not None:
+                s = s + feed_ops.feed_forward_int8(ac, *codes)
+            elif p.shared:
+                s = s + feed_ops.feed_forward(ac, w["shared_in"].to(dt), w["shared_out"].to(dt))
+            return s @ self._head(), None
         y, inner = expert_ops.expert_products(ac, plan, weights, w_in, w_out, keep_inner=True)
-        s = r + y
-        return s @ self._head(), (x, r, mean, rstd, a, logits, ids, plan, weights, ac, w_in, w_out, inner, s)
+        s, block = r + y, None
+        if p.shared:
+            b_in, b_out = w["shared_in"].to(dt), w["shared_out"].to(dt)
+            z, b_inner = feed_ops.feed_forward(ac, b_in, b_out, keep_inner=True)
+            s, block = s + z, (b_in, b_out, b_inner)
+        return s @ self._head(), (x, r, mean, rstd, a, logits, ids, plan, weights, ac, w_in, w_out, inner, s, block)
 
     def _backward(self, g: torch.Tensor, kept) -> dict[str, torch.Tensor]:
         """Gradients of sum_t L_t / n, g = dL/dout, in every parameter."""
-        x, r, mean, rstd, a, logits, ids, plan, weights, ac, w_in, w_out, inner, s = kept
+        x, r, mean, rstd, a, logits, ids, plan, weights, ac, w_in, w_out, inner, s, block = kept
         w = self.weights_
         g = g / g.shape[0]
         if self.unit_ is not None:
             g = g * self.unit_
         ds = g[:, None] * w["head"]
-        if ac.dtype == torch.float16:
-            # float16 has too few powers of two for gradients as they come
-            unit = _half_unit(g, w["head"])
-            grads = expert_ops.expert_products_grad((ds * unit).half(), ac, plan, weights, w_in, w_out, inner)
-            dac, dweights, dw_in, dw_out = (t.float() / unit for t in grads)
-        else:
-            dac, dweights, dw_in, dw_out = expert_ops.expert_products_grad(ds.to(ac.dtype), ac, plan, weights, w_in,
-                                                                           w_out, inner)
+        # float16 has too few powers of two for gradients as they come
+        unit = _half_unit(g, w["head"]) if ac.dtype == torch.float16 else None
+        dy = (ds if unit is None else ds * unit).to(ac.dtype)
+        grads = expert_ops.expert_products_grad(dy, ac, plan, weights, w_in, w_out, inner)
+        if unit is not None:
+            grads = tuple(t.float() / unit for t in grads)
+        dac, dweights, dw_in, dw_out = grads
+        shared = {}
+        if block is not None:
+            b_in, b_out, b_inner = block
+            grads = tuple(t.float() for t in feed_ops.feed_forward_grad(dy, ac, b_in, b_out, b_inner))
+            if unit is not None:
+                grads = tuple(t / unit for t in grads)
+            dac = dac.float() + grads[0]
+            shared = dict(shared_in=grads[1], shared_out=grads[2])
         dlogits = expert_ops.route_grad(dweights, logits, ids, scores=self.p.scores)
         da = dac.float() + dlogits @ w["gate"]
         dr, dnorm, dshift = expert_ops.layer_norm_grad(da, r, mean, rstd, w["norm"])
         return dict(embed=x.t() @ (ds + dr), norm=dnorm, shift=dshift, gate=dlogits.t() @ a, w_in=dw_in.float(),
-                    w_out=dw_out.float(), head=s.t() @ g)
+                    w_out=dw_out.float(), head=s.t() @ g, **shared)
+
+    def _groups(self) -> list[tuple[list[str], float, optim.AdamWState]]:
+        """The parameters' names by what decays, with the moments before the first step."""
+        p, w = self.p, self.weights_
+        names = [list(w)] if p.weight_decay == 0.0 else [[m for m in w if w[m].dim() > 1], [m for m in w if w[m].dim() == 1]]
+        return [(part, decay, optim.adamw_state([w[m] for m in part], p.state_bits))
+                for part, decay in zip(names, (p.weight_decay, 0.0))]
 
     def fit(self, X: np.ndarray, y: np.ndarray, margin: np.ndarray | float = 0.0) -> "ExpertStage":
         """Fit to the loss at margin + out; margin (n,), the booster's on these rows, or one number."""
@@ -202,13 +237,15 @@ class ExpertStage:
                              w_in=normal(p.experts, 2 * p.inner, p.width, scale=p.width ** -0.5),
                              w_out=normal(p.experts, p.width, p.inner, scale=p.inner ** -0.5),
                              head=torch.zeros(p.width, device=dev))
+        if p.shared:
+            self.weights_.update(shared_in=normal(2 * p.shared, p.width, scale=p.width ** -0.5),
+                                 shared_out=normal(p.width, p.shared, scale=p.shared ** -0.5))
         self.bias_ = torch.zeros(p.experts, device=dev)
         self.unit_ = None
         if p.dtype == "float16" and n:
             g, _ = boost_ops.grad_hess(self.loss, base, yt)
             self.unit_ = _power_of_two((g.abs().median() / _HALF_ANSWER).clamp(1.0, 2.0 ** 100))
-        first = {m: torch.zeros_like(t) for m, t in self.weights_.items()}
-        second = {m: torch.zeros_like(t) for m, t in self.weights_.items()}
+        groups = self._groups()
         step = 0
         for _ in range(p.epochs):
             order = torch.randperm(n, generator=gen).to(dev)
@@ -217,11 +254,12 @@ class ExpertStage:
                 out, kept = self._forward(x[rows], keep=True)
                 g, _ = boost_ops.grad_hess(self.loss, base[rows] + out, yt[rows])
                 step += 1
-                scale = p.learning_rate * (1 - 0.999 ** step) ** 0.5 / (1 - 0.9 ** step)
-                for m, grad in self._backward(g, kept).items():
-                    first[m].lerp_(grad, 0.1)
-                    second[m].lerp_(grad.square(), 0.001)
-                    self.weights_[m].addcdiv_(first[m], second[m].sqrt() + 1e-8, value=-scale)
+                grads = self._backward(g, kept)
+                # 1e-8 beside the square root of the second moment as it is
+                eps = 1e-8 / (1 - 0.999 ** step) ** 0.5
+                for names, decay, state in groups:
+                    optim.adamw_step([self.weights_[m] for m in names], [grads[m] for m in names], state, step,
+                                     lr=p.learning_rate, eps=eps, weight_decay=decay)
                 # experts with more than their share become a little less likely
                 share = kept[7].offsets.diff().float()
                 self.bias_ -= p.balance_step * torch.sign(share - share.mean())
@@ -229,12 +267,16 @@ class ExpertStage:
             raise RuntimeError(f"the fit's parameters are not finite: y or margin are not, or passes in {p.dtype} "
                                "left the type's range")
 
-    def predict_margin(self, X: np.ndarray, margin: np.ndarray | float = 0.0) -> np.ndarray:
-        """margin + the stage's answer for each row; margin (n,) or one number."""
+    def predict_margin(self, X: np.ndarray, margin: np.ndarray | float = 0.0, int8: bool = False) -> np.ndarray:
+        """margin + the stage's answer for each row; margin (n,) or one number.  With
+        ``int8`` the shared block answers by 8-bit products."""
+        if int8 and not self.p.shared:
+            raise ValueError("int8 is of the shared block, and this stage has none (ExpertParams.shared)")
         with torch.cuda.device(self.device_):
             x = self._inputs(X)
             base = np.broadcast_to(np.asarray(margin, dtype=np.float32), (x.shape[0],))
-            parts = [self._forward(x[lo:lo + (1 << 18)], keep=False)[0] for lo in range(0, x.shape[0], 1 << 18)]
+            codes = self._shared_codes() if int8 else None
+            parts = [self._forward(x[lo:lo + (1 << 18)], False, codes)[0] for lo in range(0, x.shape[0], 1 << 18)]
             out = torch.cat(parts) if parts else x.new_zeros(0)
         if not bool(torch.isfinite(out).all()):
             raise RuntimeError(f"answers are not finite: passes in {self.p.dtype} left the type's range")
