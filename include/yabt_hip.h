@@ -636,8 +636,8 @@ int yabt_adamw_values(int count, const yabt_adamw_tensor *tensors, yabt_stream_t
  * all of `dtype`; act 0 silu (g / (1 + exp(-g))), 1 gelu (g times the normal
  * distribution function), 2 gelu_tanh (its usual form by tanh), 3 relu.
  * out_inner (yabt_feed_forward_inner_bytes, or NULL) keeps g and u in fp32 and h for
- * the backward pass.  h is rounded to `dtype` before the second product (16-bit
- * types, 64 rows or fewer: to two parts of it), so that in fp16 one beyond 65504
+ * the backward pass.  h is rounded to `dtype` before the second product (16 rows or
+ * fewer of narrow blocks: to two parts of it), so that in fp16 one beyond 65504
  * makes its row infinite or NaN; sums are fp32.  n below 2^31 - 256, D, F, O to 2^24.
  * Sums are added in an order that the sizes fix. */
 size_t yabt_feed_forward_inner_bytes(int dtype, int64_t n, int D, int F, int O);
@@ -664,7 +664,8 @@ int yabt_quantize_rows(int dtype, const void *x, int64_t ldx, int64_t n, int D, 
 
 /* y = a_scale[i] * (b_scale[o] * sum_k a[i, k] b[o, k]): codes a (n, K) with a scale for each
  * row, b (N, K) with one for each output column, to y (n, N) of out_dtype.  The sum
- * is exact (32 bits, K at most 131071) and rounded to fp32 once. */
+ * is exact (32 bits, K at most 131071) and rounded to fp32 once.  Where the size
+ * query answers 1, no workspace is needed. */
 size_t yabt_product_int8_workspace_bytes(int64_t n, int K, int N);
 int yabt_product_int8(const int8_t *a, int64_t lda, const float *a_scale, int64_t n, int K,
                       const int8_t *b, int64_t ldb, const float *b_scale, int N, int out_dtype,

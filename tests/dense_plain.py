@@ -101,7 +101,7 @@ def feed(x, w_in, w_out, act, dtype, dy=None):
     """{name: (value, bound)} of y and, with dy, dx, dw_in and dw_out: sums of K
     terms in float32 in any order (K + 8 units of the magnitudes' sum), slopes of at
     most 1.13 and curvatures of at most 1.2, h and the inner gradients rounded to the type
-    (h of 64 rows or fewer to two parts of it for y), one rounding of the result."""
+    (h of 16 rows or fewer to two parts of it for y), one rounding of the result."""
     n, F = x.shape[0], w_out.shape[1]
     u, tiny = UNIT[dtype], TINY[dtype]
     gam = lambda terms: (terms + 8) * U32  # noqa: E731
@@ -113,7 +113,7 @@ def feed(x, w_in, w_out, act, dtype, dy=None):
     h = a * v
     eh = 1.01 * (ea * np.abs(v) + np.abs(a) * ev + ea * ev) + 2 * U32 * np.abs(h)
     kept = eh + u * (np.abs(h) + eh) + tiny                       # h in the type
-    used = eh + (u * u * (np.abs(h) + eh) + 2 * tiny if n <= 64 else u * (np.abs(h) + eh) + tiny)
+    used = eh + (u * u * (np.abs(h) + eh) + 2 * tiny if n <= 16 else u * (np.abs(h) + eh) + tiny)
     y, ey = h @ w_out.T, (used + gam(2 * F) * (np.abs(h) + used)) @ np.abs(w_out).T
     out = {"y": (y, ey + u * (np.abs(y) + ey) + tiny)}
     if dy is None:

@@ -58,12 +58,12 @@ def test_python_entry():
         optim.adamw_step(p, g, optim.AdamWState(s.first, s.second, [torch.zeros(2)]), 1)
     with pytest.raises(ValueError, match="both scales"):
         optim.adamw_step(p, g, optim.AdamWState(s.first, []), 1)
-    with pytest.raises(ValueError, match="moments 0"):
+    with pytest.raises(ValueError, match="first moment 0"):
         optim.adamw_step(p, g, optim.AdamWState([torch.zeros(300, dtype=torch.float64)], s.second), 1)
     e = optim.adamw_state(p, bits=8)
     assert e.bits == 8 and e.first[0].dtype == torch.int8 and e.second[0].dtype == torch.uint8
     assert e.first_scale[0].shape == (2,)
-    with pytest.raises(ValueError, match="scales 0"):
+    with pytest.raises(ValueError, match="first scales 0"):
         optim.adamw_step(p, g, optim.AdamWState(e.first, e.second, [torch.zeros(1)], e.second_scale), 1)
     with pytest.raises(RuntimeError, match="autograd"):
         optim.adamw_step([torch.zeros(300, requires_grad=True)], g, s, 1)

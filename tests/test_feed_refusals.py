@@ -59,7 +59,8 @@ def test_8_bit_entries():
 
     for args, text in [(dict(dt=-1), "dtype"), (dict(lda=7), "bad sizes"), (dict(ldb=7), "bad sizes"), (dict(ldy=5), "bad sizes"),
                        (dict(K=0), "bad sizes"), (dict(N=0), "bad sizes"), (dict(K=131072, lda=131072, ldb=131072), "bad sizes"),
-                       (dict(n=1 << 24), "bad sizes"), (dict(p=0), "null pointer"), (dict(ws=16), "workspace")]:
+                       (dict(n=1 << 24), "bad sizes"), (dict(p=0), "null pointer"),
+                       (dict(n=100, K=2048, lda=2048, ldb=2048, ws=16), "workspace")]:
         refused(product(**args), text)
     assert product(n=0, p=0) == 0
     assert lib.yabt_product_int8_workspace_bytes(4, 0, 6) == 0

@@ -271,3 +271,29 @@ def test_on_another_stream_and_twice_the_same():
         torch.cuda.synchronize()
         out.append((d, s.first[0], s.second[0]))
     assert all(torch.equal(x, y) for x, y in zip(*out))
+
+
+def test_refused_on_the_device():
+    p, g = [torch.zeros(300, device="cuda") for _ in range(2)], [torch.zeros(300, device="cuda") for _ in range(2)]
+    s = optim.adamw_state(p)
+    for call, text in [(lambda: optim.adamw_step(p, g, s, 0), "counted"),
+                       (lambda: optim.adamw_step(p, g, s, torch.ones(1, device="cuda")), "int32"),
+                       (lambda: optim.adamw_step([p[0], p[0]], g, s, 1), "twice"),
+                       (lambda: optim.adamw_step(p, [g[0], g[1].view(30, 10)], s, 1), "shapes"),
+                       (lambda: optim.adamw_step(p, [g[0], g[1].double()], s, 1), "float32"),
+                       (lambda: optim.adamw_step(p, [g[0], g[1].cpu()], s, 1), "must be on"),
+                       (lambda: optim.adamw_step([p[0], torch.zeros(300, 2, device="cuda")[:, 0]], g, s, 1), "contiguous"),
+                       (lambda: optim.adamw_step([p[0][:299], p[1]], [g[0][:299], g[1]], s, 1), "first moment 0")]:
+        with pytest.raises(ValueError, match=text):
+            call()
+
+
+def test_a_parameter_that_requires_a_gradient():
+    p = torch.ones(10, device="cuda", requires_grad=True)
+    s = optim.adamw_state([p])
+    with pytest.raises(RuntimeError, match="autograd"):
+        optim.adamw_step([p], [torch.ones(10, device="cuda")], s, 1)
+    before = p._version
+    with torch.no_grad():
+        optim.adamw_step([p], [torch.ones(10, device="cuda")], s, 1)
+    assert p._version > before and bool((p < 1.0).all())

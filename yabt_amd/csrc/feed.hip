@@ -22,7 +22,7 @@
 // which are bound by the weights' bytes.
 //
 // 16-bit types: h, dg and du are rounded to the inputs' type, as the matrix cores
-// take them (for few rows, whose time is the weights', h is taken in two parts and
+// take them (for 16 rows or fewer, whose time is the weights', h is taken in two parts and
 // keeps 16 bits); g and u are kept in fp32 for the backward pass.  So an output has
 // two roundings behind it, its own and that of one factor.  8 bits: h is kept in fp32
 // until its row's largest magnitude is known, sums of codes are whole numbers.
@@ -49,7 +49,7 @@ struct Product {
     int act;
     float* pre;                       // (M, 2 Fi): g from 0, u from Fi, or NULL
     void* h;                          // (M, Fp), or NULL
-    float* h32;                       // (M, Fi): h of 8-bit products and of few rows
+    float* h32;                       // (M, Fi): h of 8-bit products and of 16 rows or fewer, or NULL
     void* dpre;                       // (M, 2 Fp): dg from 0, du from Fp
     void* out;
     int64_t ldo;
@@ -610,11 +610,13 @@ __global__ void __launch_bounds__(256) k_quantize(const T* x, int64_t ldx, int64
     const int chunks = (D + VEC<T> - 1) / VEC<T>;
     Chunk<T> c[QUANT_CHUNKS];
     uint32_t most = 0;
+    if (D % VEC<T> == 0) {
+        // past the end the last piece again, which leaves the largest as it is: loads without a branch between them
 #pragma unroll
-    for (int i = 0; i < QUANT_CHUNKS; ++i) {
-        const int at = i * LANES + t;
-        c[i].raw = u32x4{0, 0, 0, 0};
-        if (at < chunks) c[i].raw = row_piece<T>(r, at * VEC<T>, D);
+        for (int i = 0; i < QUANT_CHUNKS; ++i) c[i].load(r + min(i * LANES + t, chunks - 1) * VEC<T>);
+    } else {
+#pragma unroll
+        for (int i = 0; i < QUANT_CHUNKS; ++i) c[i].raw = row_piece<T>(r, min(i * LANES + t, chunks - 1) * VEC<T>, D);
     }
 #pragma unroll
     for (int i = 0; i < QUANT_CHUNKS; ++i) most = max(most, chunk_most(c[i]));
@@ -655,7 +657,17 @@ __global__ void __launch_bounds__(256) k_quantize(const T* x, int64_t ldx, int64
 
 constexpr int FEW_ROWS = 64;                     // rows of a call, up to four groups of 16
 constexpr int FEW_NT = 512;
+// pieces of 128 bytes a row that a wave holds, of weights and of x: with 32, the blocks of one group of rows
+// would be one a CU instead of two (1024 -> 4096 -> 1024, one row: 13.7 and 12.7 us)
+constexpr int few_held(int MB) { return MB > 1 ? 32 : 16; }
 constexpr int FEW_VALUES = 16384;                // values of x that every block puts in 8 bits by itself
+
+// 16 bytes of a row from value k on: all there (WHOLE), or its K values alone, zeros after them.
+template <typename T, bool WHOLE>
+__device__ __forceinline__ u32x4 few_piece(const T* row, int k, int K) {
+    if constexpr (WHOLE) return *reinterpret_cast<const u32x4_any*>(row + k);
+    else return row_piece<T>(row, k, K);
+}
 
 // Where the rows of x come from: a lane's piece of 16 bytes' worth of T from value k on, fetched
 // as RAW pieces and taken apart into PARTS operands.
@@ -665,8 +677,9 @@ struct FewRows {                                 // rows of T in memory
     const T* base;
     size_t ld;
     int n;
+    template <bool WHOLE>
     __device__ __forceinline__ void load(int mb, int k, int K, u32x4 (&raw)[RAW]) const {
-        raw[0] = row_piece<T>(base + (size_t)min(mb * 16 + (int)(threadIdx.x & 15), n - 1) * ld, k, K);
+        raw[0] = few_piece<T, WHOLE>(base + (size_t)min(mb * 16 + (int)(threadIdx.x & 15), n - 1) * ld, k, K);
     }
     __device__ __forceinline__ static void parts(const u32x4 (&raw)[RAW], u32x4 (&v)[PARTS]) { v[0] = raw[0]; }
 };
@@ -676,10 +689,11 @@ struct FewHalves {                               // fp32 rows in two parts of T:
     const float* base;
     size_t ld;
     int n;
+    template <bool WHOLE>
     __device__ __forceinline__ void load(int mb, int k, int K, u32x4 (&raw)[RAW]) const {
         const float* row = base + (size_t)min(mb * 16 + (int)(threadIdx.x & 15), n - 1) * ld;
-        raw[0] = row_piece<float>(row, k, K);
-        raw[1] = row_piece<float>(row, k + 4, K);
+        raw[0] = few_piece<float, WHOLE>(row, k, K);
+        raw[1] = few_piece<float, WHOLE>(row, k + 4, K);
     }
     __device__ __forceinline__ static void parts(const u32x4 (&raw)[RAW], u32x4 (&v)[PARTS]) {
         typedef T VT __attribute__((ext_vector_type(8)));
@@ -694,54 +708,72 @@ struct FewHalves {                               // fp32 rows in two parts of T:
         v[1] = __builtin_bit_cast(u32x4, lo);
     }
 };
-struct FewCodes {                                // codes that the block put in LDS, `ld` bytes a row
+struct FewCodes {                                // codes that the block put in LDS, `ld` bytes a row, zeros to whole pieces
     static constexpr int RAW = 1, PARTS = 1;
     const lds_char* base;
     int ld, n;
+    template <bool WHOLE>
     __device__ __forceinline__ void load(int mb, int k, int K, u32x4 (&raw)[RAW]) const {
         raw[0] = u32x4{0, 0, 0, 0};
-        if (k < K) raw[0] = *(const lds_u32x4*)(base + min(mb * 16 + (int)(threadIdx.x & 15), n - 1) * ld + k);
+        if (WHOLE || k < K) raw[0] = *(const lds_u32x4*)(base + min(mb * 16 + (int)(threadIdx.x & 15), n - 1) * ld + k);
     }
     __device__ __forceinline__ static void parts(const u32x4 (&raw)[RAW], u32x4 (&v)[PARTS]) { v[0] = raw[0]; }
 };
 
-// acc[m][b] += M matrices' 16 rows w[m] times group b of 16 rows of x, from piece `from` of 128
-// bytes on, every `by`-th.
+// acc[m][b] += M matrices' 16 rows w[m] times group b of 16 rows of x, over AHEAD pieces of 128
+// bytes, `by` pieces apart, the first from value k0 on.  WHOLE: they lie in the rows, and nothing
+// stands between their loads; else a branch for each, which costs more than the loads.
+template <typename T, int M, int MB, int AHEAD, bool WHOLE, typename Src>
+__device__ __forceinline__ void few_pieces(const T* const (&w)[M], const Src& x, int K, int k0, int by,
+                                           typename Sums<T>::Four (&acc)[M][MB]) {
+    constexpr int CH = VEC<T>, STEP = 8 * CH;    // values in 128 bytes
+    const int q = (threadIdx.x & 63) >> 4;
+    u32x4 a[AHEAD][M][2], v[AHEAD][2][MB][Src::RAW];
+#pragma unroll
+    for (int s = 0; s < AHEAD; ++s)
+#pragma unroll
+        for (int o = 0; o < 2; ++o) {
+            const int k = k0 + s * by * STEP + (2 * q + o) * CH;
+#pragma unroll
+            for (int m = 0; m < M; ++m) a[s][m][o] = few_piece<T, WHOLE>(w[m], k, K);
+#pragma unroll
+            for (int b = 0; b < MB; ++b) x.template load<WHOLE>(b, k, K, v[s][o][b]);
+        }
+#pragma unroll
+    for (int s = 0; s < AHEAD; ++s)
+#pragma unroll
+        for (int o = 0; o < 2; ++o)
+#pragma unroll
+            for (int b = 0; b < MB; ++b) {
+                u32x4 p[Src::PARTS];
+                Src::parts(v[s][o][b], p);
+#pragma unroll
+                for (int m = 0; m < M; ++m)
+#pragma unroll
+                    for (int i = 0; i < Src::PARTS; ++i) {
+                        if constexpr (sizeof(T) == 1) acc[m][b] = mma8(a[s][m][o], p[i], acc[m][b]);
+                        else acc[m][b] = mma16<T>(a[s][m][o], p[i], acc[m][b]);
+                    }
+            }
+}
+
+// The same over all of a row's pieces from number `from` on, every `by`-th: eight (or what registers
+// hold) under way at once, then four, two, one, and what is left of a piece.
 template <typename T, int M, int MB, typename Src>
 __device__ __forceinline__ void few_sums(const T* const (&w)[M], const Src& x, int K, int from, int by,
                                          typename Sums<T>::Four (&acc)[M][MB]) {
-    constexpr int CH = VEC<T>, STEP = 8 * CH;    // values in 128 bytes
-    constexpr int AHEAD = MB * Src::RAW >= 4 ? 2 : 4;    // pieces of a row under way
-    const int q = (threadIdx.x & 63) >> 4;
-    for (int k0 = from * STEP; k0 < K; k0 += by * AHEAD * STEP) {
-        u32x4 a[AHEAD][M][2], v[AHEAD][2][MB][Src::RAW];
-#pragma unroll
-        for (int s = 0; s < AHEAD; ++s)
-#pragma unroll
-            for (int o = 0; o < 2; ++o) {
-                const int k = k0 + s * by * STEP + (2 * q + o) * CH;
-#pragma unroll
-                for (int m = 0; m < M; ++m) a[s][m][o] = row_piece<T>(w[m], k, K);
-#pragma unroll
-                for (int b = 0; b < MB; ++b) x.load(b, k, K, v[s][o][b]);
-            }
-#pragma unroll
-        for (int s = 0; s < AHEAD; ++s)
-#pragma unroll
-            for (int o = 0; o < 2; ++o)
-#pragma unroll
-                for (int b = 0; b < MB; ++b) {
-                    u32x4 p[Src::PARTS];
-                    Src::parts(v[s][o][b], p);
-#pragma unroll
-                    for (int m = 0; m < M; ++m)
-#pragma unroll
-                        for (int i = 0; i < Src::PARTS; ++i) {
-                            if constexpr (sizeof(T) == 1) acc[m][b] = mma8(a[s][m][o], p[i], acc[m][b]);
-                            else acc[m][b] = mma16<T>(a[s][m][o], p[i], acc[m][b]);
-                        }
-                }
-    }
+    constexpr int STEP = 8 * VEC<T>;
+    int k0 = from * STEP;
+    const int each = by * STEP;
+    auto run = [&](auto ahead) {
+        constexpr int A = decltype(ahead)::value;
+        for (; k0 + (A - 1) * each + STEP <= K; k0 += A * each) few_pieces<T, M, MB, A, true>(w, x, K, k0, by, acc);
+    };
+    if constexpr (M + MB * Src::RAW <= few_held(MB) / 8) run(std::integral_constant<int, 8>());
+    if constexpr (M + MB * Src::RAW <= few_held(MB) / 4) run(std::integral_constant<int, 4>());
+    run(std::integral_constant<int, 2>());
+    run(std::integral_constant<int, 1>());
+    if (k0 < K) few_pieces<T, M, MB, 1, false>(w, x, K, k0, by, acc);
 }
 
 // The block's rows of x (type X) as codes in LDS, rows ld bytes apart, and their scales.
@@ -781,23 +813,28 @@ __device__ __forceinline__ void few_codes(const Product& P, lds_char* codes, int
 }
 
 // MODE IN or OUT with T f32, bf16, f16; IN8 or OUT8 with int8_t, CODES: a's values become codes here.
-// OUT's rows are h in fp32.
-template <typename T, int MODE, int MB, bool CODES>
+// OUT's rows are h, of up to 16 in fp32, of more in T.  A block makes R groups of 16 columns for MB
+// groups of 16 rows.
+template <typename T, int MODE, int MB, int R, bool CODES>
 __global__ void __launch_bounds__(FEW_NT) k_few(Product P) {
     constexpr bool GATED = MODE == IN || MODE == IN8;
-    constexpr int M = GATED ? 2 : 1, WAVES = FEW_NT / 64;
+    constexpr int G = GATED ? 2 : 1, WAVES = FEW_NT / 64;
     using Four = typename Sums<T>::Four;
-    __shared__ Four s_sum[WAVES][M][64];
+    constexpr int PAIRS = R * MB, AT_ONCE = PAIRS < 4 / G ? PAIRS : 4 / G;  // groups of columns and rows whose sums LDS holds: 32 KB
+    __shared__ Four s_sum[WAVES][AT_ONCE][G][64];
     __shared__ float s_scale[FEW_ROWS];
     __shared__ uint32_t s_most[FEW_ROWS];
     const int wave = threadIdx.x / 64, lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
-    const int first = blockIdx.x * 16;
-    const T* w[M];
-    w[0] = (const T*)P.b + (size_t)min(first + r, P.N - 1) * (size_t)P.ldb;
-    if constexpr (GATED) w[1] = w[0] + (size_t)P.F * (size_t)P.ldb;
-    Four acc[M][MB];
+    const int first = blockIdx.x * (16 * R);
+    const T* w[R * G];
 #pragma unroll
-    for (int m = 0; m < M; ++m)
+    for (int g = 0; g < R; ++g) {
+        w[g * G] = (const T*)P.b + (size_t)min(first + g * 16 + r, P.N - 1) * (size_t)P.ldb;
+        if constexpr (GATED) w[g * G + 1] = w[g * G] + (size_t)P.F * (size_t)P.ldb;
+    }
+    Four acc[R * G][MB];
+#pragma unroll
+    for (int m = 0; m < R * G; ++m)
 #pragma unroll
         for (int b = 0; b < MB; ++b) acc[m][b] = Four{0, 0, 0, 0};
     if constexpr (CODES) {
@@ -806,51 +843,54 @@ __global__ void __launch_bounds__(FEW_NT) k_few(Product P) {
         if (P.x_dtype == DT_F32) few_codes<float>(P, codes, ld, s_most, s_scale);
         else if (P.x_dtype == DT_BF16) few_codes<bf16>(P, codes, ld, s_most, s_scale);
         else few_codes<f16>(P, codes, ld, s_most, s_scale);
-        few_sums<T, M, MB>(w, FewCodes{codes, ld, P.M}, P.K, wave, WAVES, acc);
-    } else if constexpr (MODE == OUT && sizeof(T) == 2) {
-        few_sums<T, M, MB>(w, FewHalves<T>{(const float*)P.a, (size_t)P.lda, P.M}, P.K, wave, WAVES, acc);
+        few_sums<T, R * G, MB>(w, FewCodes{codes, ld, P.M}, P.K, wave, WAVES, acc);
+    } else if constexpr (MODE == OUT && sizeof(T) == 2 && MB == 1) {
+        few_sums<T, R * G, MB>(w, FewHalves<T>{(const float*)P.a, (size_t)P.lda, P.M}, P.K, wave, WAVES, acc);
     } else {
-        few_sums<T, M, MB>(w, FewRows<T>{(const T*)P.a, (size_t)P.lda, P.M}, P.K, wave, WAVES, acc);
+        few_sums<T, R * G, MB>(w, FewRows<T>{(const T*)P.a, (size_t)P.lda, P.M}, P.K, wave, WAVES, acc);
     }
 #pragma unroll
-    for (int b = 0; b < MB; ++b) {
-        if (b) __syncthreads();                          // the sums of the rows before have been read
+    for (int p0 = 0; p0 < PAIRS; p0 += AT_ONCE) {
+        if (p0) __syncthreads();                         // the sums before have been read
 #pragma unroll
-        for (int m = 0; m < M; ++m) s_sum[wave][m][lane] = acc[m][b];
+        for (int p = 0; p < AT_ONCE; ++p)
+#pragma unroll
+            for (int m = 0; m < G; ++m)
+                if (p0 + p < PAIRS) s_sum[wave][p][m][lane] = acc[(p0 + p) / MB * G + m][(p0 + p) % MB];
         __syncthreads();
-        // a lane has row r and columns first + 4 q .. + 3
-        const int row = b * 16 + r, c = first + 4 * q;
-        if (wave == 0 && row < P.M && c < P.N) {
-            Four t[M];
+        // a wave finishes a pair of groups: a lane has row r and columns c .. c + 3
+        const int pair = p0 + wave, row = pair % MB * 16 + r, c = first + pair / MB * 16 + 4 * q;
+        if (wave < AT_ONCE && pair < PAIRS && row < P.M && c < P.N) {
+            Four t[G];
 #pragma unroll
-            for (int m = 0; m < M; ++m) {
-                t[m] = s_sum[0][m][lane];
+            for (int m = 0; m < G; ++m) {
+                t[m] = s_sum[0][wave][m][lane];
 #pragma unroll
-                for (int o = 1; o < WAVES; ++o) t[m] += s_sum[o][m][lane];
+                for (int o = 1; o < WAVES; ++o) t[m] += s_sum[o][wave][m][lane];
             }
-            f32x4 v[M];
+            f32x4 v[G];
             if constexpr (sizeof(T) == 1) {
                 const float s = CODES ? s_scale[row] : P.sa[row];
 #pragma unroll
-                for (int m = 0; m < M; ++m)
+                for (int m = 0; m < G; ++m)
                     v[m] = f32x4{(float)t[m][0], (float)t[m][1], (float)t[m][2], (float)t[m][3]} *
                            four_of(P.sb + m * P.F + c, P.N - c) * s;
             } else {
 #pragma unroll
-                for (int m = 0; m < M; ++m) v[m] = t[m];
+                for (int m = 0; m < G; ++m) v[m] = t[m];
             }
             if constexpr (GATED) {
                 float a[4], slope[4], h[4];
                 activate<T>(P.act, v[0], a, slope);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) h[i] = c + i < P.F ? a[i] * v[M - 1][i] : 0.0f;
-                *(f32x4*)(P.h32 + (size_t)row * (size_t)P.Fi + c) = f32x4{h[0], h[1], h[2], h[3]};
+                for (int i = 0; i < 4; ++i) h[i] = c + i < P.F ? a[i] * v[G - 1][i] : 0.0f;
+                if (P.h32) *(f32x4*)(P.h32 + (size_t)row * (size_t)P.Fi + c) = f32x4{h[0], h[1], h[2], h[3]};
                 if constexpr (sizeof(T) != 1) {
                     if (P.h) store_part((T*)P.h + (size_t)row * (size_t)P.Fp + c, f32x4{h[0], h[1], h[2], h[3]}, P.Fp - c);
                     if (P.pre) {
                         float* pre = P.pre + (size_t)row * 2 * (size_t)P.Fi + c;
                         *(f32x4*)pre = v[0];
-                        *(f32x4*)(pre + P.Fi) = v[M - 1];
+                        *(f32x4*)(pre + P.Fi) = v[G - 1];
                     }
                 }
             } else {
@@ -881,7 +921,8 @@ inline bool large_product(int bytes, int64_t M, int64_t N, int64_t K) {
 
 // Parts of the summed dimension, so that few tiles fill the device: at least four steps each.
 inline int split_count(int64_t M, int64_t N, int64_t K, bool large, int bytes) {
-    const int64_t tiles = over(M, large ? 256 : 64) * over(N, large ? 256 : 128);
+    if (large) return 1;
+    const int64_t tiles = over(M, 64) * over(N, 128);
     int64_t s = PART_BLOCKS / (tiles < 1 ? 1 : tiles);
     const int64_t longest = K * bytes / (4 * 128);
     if (s > longest) s = longest;
@@ -928,13 +969,27 @@ inline void run_join(const Joins& J, hipStream_t stream) {
     if (J.count) k_join<<<launch_grid(work, 256, 8192), 256, 0, stream>>>(J);
 }
 
+template <typename T, int MODE, int MB, int R, bool CODES>
+void launch_few(const Product& P, hipStream_t stream) {
+    const size_t lds = CODES ? (size_t)P.M * (size_t)((P.K + 15) / 16 * 16 + 16) : 0;
+    k_few<T, MODE, MB, R, CODES><<<(unsigned)over(P.N, 16 * R), FEW_NT, lds, stream>>>(P);
+}
 template <typename T, int MODE, bool CODES>
 void run_few(const Product& P, hipStream_t stream) {
-    const unsigned blocks = (unsigned)over(P.N, 16);
-    const size_t lds = CODES ? (size_t)P.M * (size_t)((P.K + 15) / 16 * 16 + 16) : 0;
-    if (P.M <= 16) k_few<T, MODE, 1, CODES><<<blocks, FEW_NT, lds, stream>>>(P);
-    else if (P.M <= 32) k_few<T, MODE, 2, CODES><<<blocks, FEW_NT, lds, stream>>>(P);
-    else k_few<T, MODE, 4, CODES><<<blocks, FEW_NT, lds, stream>>>(P);
+    // more columns a block read x less often, but leave fewer blocks.  One group and two, us for the block: 2048 ->
+    // 5632 -> 2048, bf16, 24 rows 31.8 and 28.9, 64 rows 54.7 and 45.7; fp32 500 -> 700 -> 500, 20 rows 11.7 and
+    // 16.3; of y's 2048 columns 31.8 and 36.0 (24 rows)
+    auto by_rows = [&](auto r) {
+        constexpr int R = decltype(r)::value;
+        if (P.M <= 32) launch_few<T, MODE, 2, R, CODES>(P, stream);
+        else if (P.M <= 48) launch_few<T, MODE, 3, R, CODES>(P, stream);
+        else launch_few<T, MODE, 4, R, CODES>(P, stream);
+    };
+    if (P.M <= 16) return launch_few<T, MODE, 1, 1, CODES>(P, stream);
+    if constexpr (MODE == IN || MODE == IN8) {
+        if (over(P.N, 32) >= 128) return by_rows(std::integral_constant<int, 2>());
+    }
+    by_rows(std::integral_constant<int, 1>());
 }
 
 template <typename F>
@@ -951,10 +1006,19 @@ inline bool feed_ranges_ok(int64_t n, int D, int F, int O) {
     return n >= 0 && n < (1ll << 31) - 256 && D >= 1 && F >= 1 && O >= 1 && D <= (1 << 24) && F <= (1 << 24) && O <= (1 << 24);
 }
 
+// y: every block of its kernel for few rows reads all of h again, 16 columns a block (16 rows or
+// fewer: in fp32); tiles split over F read less but need a second launch to join them.  Few and tiles, us for
+// the block: 2048 -> 5632 -> 2048, bf16, 17 rows 26.9 and 26.3, 24 28.7 and 26.8, 48 38.6 and 31.3, 64 45.7 and
+// 35.4; 1024 -> 4096 -> 1024, 20 rows 19.9 and 19.0; fp32 500 -> 700 -> 500, 20 rows 16.4 and
+// 23.4, 48 20.9 and 26.2.  (8 bits: 5632 -> 2048, 24 rows 27.4 and 30.1, 64 37.9 and 37.2; 4096 -> 4096, 64
+// rows 15.4 and 18.2: few throughout.)
+inline bool few_answer(int64_t n, int64_t F, int64_t O, int bytes) { return over(O, 16) * n * F * bytes <= (8 << 20); }
+
 struct FeedSizes {
     int64_t n;
     int D, F, O, bytes, Fp, Fi;
-    bool few, large_in, large_out, large_dh, large_grads;
+    bool few, few_out, whole;         // few rows: h and y by their kernel; so few that h is kept in fp32 for y
+    bool large_in, large_out, large_dh, large_grads;
     int splits_out, splits[3];        // of y; of dx, dW_in, dW_out
 };
 inline FeedSizes feed_sizes(int dtype, int64_t n, int D, int F, int O) {
@@ -964,6 +1028,8 @@ inline FeedSizes feed_sizes(int dtype, int64_t n, int D, int F, int O) {
     z.Fp = up16(F, b);
     z.Fi = up16(F, 4);
     z.few = few_rows(n);
+    z.whole = n <= 16 && few_answer(n, F, O, 2);
+    z.few_out = z.whole || (n > 16 && z.few && few_answer(n, F, O, b));
     z.large_in = large_product(b, n, 2 * (int64_t)F, D);
     z.large_out = large_product(b, n, O, F);
     z.splits_out = split_count(n, O, F, z.large_out, b);
@@ -992,8 +1058,8 @@ struct FeedSpace {
 };
 inline size_t carve_forward(Carve& c, FeedSpace* s, const FeedSizes& z) {
     s->h = c.take<char>((size_t)z.n * z.Fp * z.bytes);
-    s->h32 = z.few ? c.take<float>((size_t)z.n * z.Fi) : nullptr;
-    s->part = !z.few && z.splits_out > 1 ? c.take<float>((size_t)z.splits_out * z.n * z.O) : nullptr;
+    s->h32 = z.whole ? c.take<float>((size_t)z.n * z.Fi) : nullptr;
+    s->part = !z.few_out && z.splits_out > 1 ? c.take<float>((size_t)z.splits_out * z.n * z.O) : nullptr;
     return c.off;
 }
 struct GradSpace {
@@ -1015,7 +1081,7 @@ int run_feed(const FeedSizes& z, int act, int dtype, const void* x, int64_t ldx,
     P.M = (int)z.n, P.N = z.F, P.K = z.D;
     P.F = z.F, P.Fp = z.Fp, P.Fi = z.Fi, P.act = act, P.splits = 1;
     P.pre = kept ? kept->pre : nullptr;
-    P.h = kept ? kept->h : z.few ? nullptr : s.h;
+    P.h = kept ? kept->h : z.whole ? nullptr : s.h;
     P.h32 = s.h32;
     const int b = z.bytes;
     if (z.few) run_few<T, IN, false>(P, stream);
@@ -1025,11 +1091,12 @@ int run_feed(const FeedSizes& z, int act, int dtype, const void* x, int64_t ldx,
     Q.b = w_out, Q.ldb = z.F;
     Q.M = (int)z.n, Q.N = z.O, Q.K = z.F;
     Q.out = y, Q.ldo = ldy, Q.out_dtype = dtype, Q.splits = 1;
-    if (z.few) {
-        Q.a = s.h32, Q.lda = z.Fi;
+    Q.a = P.h, Q.lda = z.Fp;
+    if (z.few_out) {
+        if (z.whole) Q.a = s.h32, Q.lda = z.Fi;
         run_few<T, OUT, false>(Q, stream);
     } else {
-        Q.a = P.h, Q.lda = z.Fp, Q.splits = z.splits_out, Q.part = s.part;
+        Q.splits = z.splits_out, Q.part = s.part;
         if (!run_tiles<T, OUT>(Q, z.large_out, pieces_ok(w_out, z.F, z.F, b), stream))
             return fail(-1, "yabt_feed_forward: bad sizes");
         if (Q.splits > 1) run_join({{{s.part, y, ldy, Q.M, Q.N, Q.splits, dtype, nullptr, nullptr}}, 1}, stream);
@@ -1229,7 +1296,7 @@ static bool int8_ranges_ok(int64_t n, int K, int N) {
 size_t yabt_product_int8_workspace_bytes(int64_t n, int K, int N) {
     if (!int8_ranges_ok(n, K, N)) return 0;
     const Int8Sizes z = int8_sizes(n, N, K);
-    return (z.few || z.splits == 1 ? 0 : (size_t)z.splits * n * N * 4) + 256;
+    return z.few || z.splits == 1 ? 1 : (size_t)z.splits * n * N * 4 + 256;
 }
 
 int yabt_product_int8(const int8_t* a, int64_t lda, const float* a_scale, int64_t n, int K, const int8_t* b, int64_t ldb,
@@ -1239,8 +1306,8 @@ int yabt_product_int8(const int8_t* a, int64_t lda, const float* a_scale, int64_
     if (!int8_ranges_ok(n, K, N) || lda < K || ldb < K || ldy < N) return fail(-1, "yabt_product_int8: bad sizes");
     if (n == 0) return 0;
     if (!a || !a_scale || !b || !b_scale || !y) return fail(-1, "yabt_product_int8: null pointer");
-    if (!workspace || workspace_bytes < yabt_product_int8_workspace_bytes(n, K, N))
-        return fail(-2, "yabt_product_int8: workspace too small");
+    const size_t need = yabt_product_int8_workspace_bytes(n, K, N);
+    if (need > 1 && (!workspace || workspace_bytes < need)) return fail(-2, "yabt_product_int8: workspace too small");
     if (!run_int8(int8_sizes(n, N, K), a, lda, a_scale, n, K, b, ldb, b_scale, N, out_dtype, y, ldy,
                   (float*)align_up((size_t)workspace, 256), (hipStream_t)stream))
         return fail(-1, "yabt_product_int8: bad sizes");

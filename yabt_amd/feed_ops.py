@@ -62,8 +62,8 @@ def feed_forward(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, *, ac
     "gelu_tanh" (its usual approximation) or "relu".  With ``keep_inner`` returns
     (y, inner), inner a buffer for the backward pass: g and u in float32 and act(g) * u.
 
-    16-bit types round act(g) * u to theirs before w_out (64 rows or fewer: keep 16
-    bits of it); in float16 one beyond 65504 makes its row infinite or NaN."""
+    16-bit types round act(g) * u to theirs before w_out (16 rows or fewer of narrow
+    blocks keep 16 bits of it); in float16 one beyond 65504 makes its row infinite or NaN."""
     if x.requires_grad or w_in.requires_grad or w_out.requires_grad:
         _unrecorded()
     act = _activation(activation)
@@ -159,10 +159,10 @@ def product_int8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scal
     if nbytes == 0:
         raise ValueError(f"product_int8: sizes out of range (K 1 to {MAX_INT8_TERMS}, N 1 to 2^24, n < 2^24), got "
                          f"{(n, K)} and {(N, K)}")
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes > 1 else None
     y = torch.empty((n, N), dtype=dtype, device=dev)
     _call("yabt_product_int8", dev, a.data_ptr(), _ld(a), sa.data_ptr(), n, K, b.data_ptr(), _ld(b), sb.data_ptr(), N,
-          DTYPES[dtype], ws.data_ptr(), nbytes, y.data_ptr(), N)
+          DTYPES[dtype], _at(ws), nbytes, y.data_ptr(), N)
     return y
 
 

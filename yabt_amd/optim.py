@@ -15,6 +15,8 @@ from __future__ import annotations
 
 import ctypes
 from dataclasses import dataclass
+from itertools import chain
+from operator import attrgetter
 
 import torch
 
@@ -45,53 +47,71 @@ class AdamWState:
         what they stand for now, in new ones."""
         if self.bits == 32:
             return self.first, self.second
-        dev = _state_device(self)
-        sizes = [t.numel() for t in self.first]
+        sizes = list(map(torch.Tensor.numel, self.first))
+        if not sizes:
+            return [], []
+        lists, dev = _checked(self, sizes)
         held = [(n + 63) // 64 * 64 for n in sizes]
-        both = [torch.empty(sum(held), dtype=torch.float32, device=dev).split(held) for _ in range(2)]
-        first, second = ([v[:n].view(t.shape) for v, n, t in zip(part, sizes, old)]
-                         for part, old in zip(both, (self.first, self.second)))
-        rows = [(a.data_ptr(), b.data_ptr(), c.data_ptr(), d.data_ptr(), e.data_ptr(), f.data_ptr(), n, 0)
-                for a, b, c, d, e, f, n in zip(first, second, self.first, self.second, self.first_scale,
-                                               self.second_scale, sizes)]
-        if rows:
-            expert_ops._call("yabt_adamw_values", dev, len(rows), _table(rows))
-        return first, second
+        # both moments' tensors in one buffer, each at a multiple of 256 bytes, all of a size next to its rest
+        parts = torch.empty(2 * sum(held), dtype=torch.float32, device=dev).split_with_sizes(
+            [m for n, h in zip(sizes, held) for m in (n, h - n)] * 2)[::2]
+        flat = parts[:len(sizes)], parts[len(sizes):]
+        rows = zip(*(map(torch.Tensor.data_ptr, part) for part in (*flat, *lists)), sizes, [0] * len(sizes))
+        expert_ops._call("yabt_adamw_values", dev, len(sizes), _table(rows))
+        return tuple([v if t.dim() == 1 else v.view(t.shape) for v, t in zip(part, self.first)] for part in flat)
 
 
-def _table(rows: list[tuple]) -> ctypes.Array:
+def _table(rows) -> ctypes.Array:
     """yabt_adamw_tensor's fields, eight 64-bit words a tensor."""
-    return (ctypes.c_int64 * (8 * len(rows)))(*[w for row in rows for w in row])
+    words = list(chain.from_iterable(rows))
+    return (ctypes.c_int64 * len(words))(*words)
 
 
-def _state_device(state: AdamWState) -> torch.device:
-    """The device of a state whose tensors fit each other."""
-    lists = (state.first, state.second, state.first_scale, state.second_scale)
-    if state.second_scale is None and state.first_scale is not None or state.first_scale is None and \
-            state.second_scale is not None or len({len(part) for part in lists if part is not None}) != 1:
+_TYPES = {32: (torch.float32, torch.float32), 8: (torch.int8, torch.uint8)}
+_DTYPE, _SHAPE, _NEEDS, _CUDA = (attrgetter(m) for m in ("dtype", "shape", "requires_grad", "is_cuda"))
+_numel, _contiguous, _device_number, _pointer = (getattr(torch.Tensor, m) for m in
+                                                 ("numel", "is_contiguous", "get_device", "data_ptr"))
+
+
+def _moments(state: AdamWState) -> list[list[torch.Tensor]]:
+    """The state's lists, if they fit each other."""
+    lists = [state.first, state.second]
+    if (state.first_scale is None) != (state.second_scale is None):
+        lists.append([])
+    elif state.first_scale is not None:
+        lists += [state.first_scale, state.second_scale]
+    if any(len(part) != len(state.first) for part in lists):
         raise ValueError("an AdamWState has a tensor of every moment (and of both scales, or of none) for each parameter")
-    dev = None
-    types = (torch.float32, torch.float32) if state.first_scale is None else (torch.int8, torch.uint8)
-    for i, m in enumerate(state.first):
-        v, n = state.second[i], m.numel()
-        if m.dtype != types[0] or v.dtype != types[1] or v.numel() != n:
-            raise ValueError(f"moments {i} must be {types[0]} and {types[1]} of one size, got {m.dtype} {tuple(m.shape)} "
-                             f"and {v.dtype} {tuple(v.shape)}")
-        parts = [m, v]
-        if state.first_scale is not None:
-            parts += [state.first_scale[i], state.second_scale[i]]
-            if any(t.dtype != torch.float32 or t.numel() != -(-n // BLOCK) for t in parts[2:]):
-                raise ValueError(f"scales {i} must be {-(-n // BLOCK)} float32 values, one for each {BLOCK}")
-        for t in parts:
-            if not t.is_cuda:
-                raise RuntimeError("moments must be on a HIP device: the step has no CPU form")
-            if not t.is_contiguous():
-                raise ValueError(f"moments {i} and their scales must be contiguous: they are written in place")
-            if dev is None:
-                dev = t.device
-            elif t.device != dev:
-                raise ValueError(f"all tensors must be on {dev}")
-    return dev
+    return lists
+
+
+def _checked(state: AdamWState, sizes: list[int]) -> tuple[list[list[torch.Tensor]], torch.device]:
+    """The moments' lists and their device: of these sizes, contiguous, on one device."""
+    lists = _moments(state)
+    types = _TYPES[state.bits] + (torch.float32, torch.float32)
+    blocks = [-(-n // BLOCK) for n in sizes]
+    # over whole lists, as a loop over the tensors takes as long as a step of small ones
+    every = list(chain.from_iterable(lists))
+    if any(set(map(_DTYPE, part)) != {dt} for part, dt in zip(lists, types)) or \
+            any(list(map(_numel, part)) != want for part, want in zip(lists, (sizes, sizes, blocks, blocks))) or \
+            not all(map(_contiguous, every)) or not all(map(_CUDA, every)) or len(set(map(_device_number, every))) != 1:
+        _refuse(lists, types, sizes, blocks)
+    return lists, every[0].device
+
+
+def _refuse(lists, types, sizes, blocks) -> None:
+    """What is wrong with the moments."""
+    for name, part, dt, want in zip(("first moment", "second moment", "first scales", "second scales"), lists, types,
+                                    (sizes, sizes, blocks, blocks)):
+        for i, (t, n) in enumerate(zip(part, want)):
+            if t.dtype != dt or t.numel() != n:
+                raise ValueError(f"{name} {i} must be {n} values of {dt}, got {t.numel()} of {t.dtype}")
+    for t in chain.from_iterable(lists):
+        if not t.is_cuda:
+            raise RuntimeError("moments must be on a HIP device: the step has no CPU form")
+        if not t.is_contiguous():
+            raise ValueError("moments and their scales must be contiguous: they are written in place")
+    raise ValueError("all tensors must be on one device")
 
 
 def adamw_state(params: list[torch.Tensor], bits: int = 32) -> AdamWState:
@@ -127,52 +147,57 @@ def adamw_step(params: list[torch.Tensor], grads: list[torch.Tensor | None], sta
     not finite makes the moments of its 256 values NaN."""
     if not len(params) == len(grads) == len(state.first):
         raise ValueError(f"{len(params)} parameters, {len(grads)} gradients and {len(state.first)} moments")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for part in (params, grads) for t in part):
-        expert_ops._unrecorded()
     b1, b2 = betas
     if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0 and 0.0 <= lr <= 1e30 and 0.0 <= eps <= 1e30
             and 0.0 <= weight_decay <= 1e30):
         raise ValueError(f"betas must be in [0, 1), lr, eps and weight_decay 0 to 1e30, got {betas}, {lr}, {eps}, "
                          f"{weight_decay}")
-    dev = _state_device(state)
+    if any(g is None for g in grads):
+        on = [i for i, g in enumerate(grads) if g is not None]
+        some = lambda part: None if part is None else [part[i] for i in on]  # noqa: E731
+        _moments(state)
+        state = AdamWState(*map(some, (state.first, state.second, state.first_scale, state.second_scale)))
+        params, grads = some(params), some(grads)
+    if not params:
+        _moments(state)
+        return
+    if torch.is_grad_enabled() and (any(map(_NEEDS, params)) or any(map(_NEEDS, grads))):
+        expert_ops._unrecorded()
+    sizes = list(map(_numel, params))
+    lists, dev = _checked(state, sizes)
     at, number = 0, 1
     if isinstance(step, torch.Tensor):
-        if step.dtype != torch.int32 or step.numel() != 1 or not step.is_cuda or dev is not None and step.device != dev:
+        if step.dtype != torch.int32 or step.numel() != 1 or step.device != dev:
             raise ValueError("step must be a number or one int32 on the parameters' device")
         at = step.data_ptr()
     else:
         number = int(step)
         if not 1 <= number < 2 ** 31:
             raise ValueError(f"steps are counted from 1 to 2^31 - 1, got {step}")
-        if dev is not None and torch.cuda.is_current_stream_capturing():
+        if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("a captured step would keep its number: pass step as an int32 device tensor")
-    rows, scales, seen, kept = [], state.bits == 8, set(), []
-    for i, (p, g) in enumerate(zip(params, grads)):
-        if g is None:
-            continue
-        n = p.numel()
-        m, v = state.first[i], state.second[i]
-        if p.dtype not in DTYPES or g.dtype not in DTYPES:
-            raise ValueError(f"parameter and gradient {i} must be float32, bfloat16 or float16, got {p.dtype}, {g.dtype}")
-        if g.shape != p.shape or m.numel() != n:
-            raise ValueError(f"parameter {i} has shape {tuple(p.shape)}, its gradient {tuple(g.shape)} and {m.numel()} "
-                             "moments")
-        if p.device != dev or g.device != dev:
-            raise ValueError(f"all tensors must be on {dev}")
-        if not p.is_contiguous():
-            raise ValueError(f"parameter {i} must be contiguous: it is written in place")
-        if not g.is_contiguous():
-            g = g.contiguous()
-            kept.append(g)                   # until the step is on its way
-        where = p.data_ptr()
-        if n and (where in seen or seen.add(where)):
-            raise ValueError(f"parameter {i} is in the list twice")
-        rows.append((where, g.data_ptr(), m.data_ptr(), v.data_ptr(),
-                     state.first_scale[i].data_ptr() if scales else 0,
-                     state.second_scale[i].data_ptr() if scales else 0, n, DTYPES[p.dtype] | DTYPES[g.dtype] << 32))
-    if rows:
-        expert_ops._call("yabt_adamw_step", dev, len(rows), _table(rows), state.bits, number, at, float(lr), float(b1),
-                         float(b2), float(eps), float(weight_decay))
+    if list(map(_SHAPE, params)) != list(map(_SHAPE, grads)):
+        raise ValueError(f"gradients must have their parameters' shapes, got {[tuple(g.shape) for g in grads]} for "
+                         f"{[tuple(p.shape) for p in params]}")
+    if any(n != dev.index for part in (params, grads) for n in map(_device_number, part)):
+        raise ValueError(f"all tensors must be on {dev}")
+    if not all(map(_contiguous, params)):
+        raise ValueError("parameters must be contiguous: they are written in place")
+    if not all(map(_contiguous, grads)):
+        grads = [g.contiguous() for g in grads]          # held until the step is on its way
+    try:
+        types = [DTYPES[p] | DTYPES[g] << 32 for p, g in zip(map(_DTYPE, params), map(_DTYPE, grads))]
+    except KeyError as e:
+        raise ValueError(f"parameters and gradients must be float32, bfloat16 or float16, got {e.args[0]}") from None
+    where = list(map(_pointer, params))
+    filled = [p for p, n in zip(where, sizes) if n]
+    if len(set(filled)) < len(filled):
+        raise ValueError("a parameter is in the list twice")
+    none = [0] * len(params)
+    first, second, *scales = (list(map(_pointer, part)) for part in lists)
+    rows = zip(where, map(_pointer, grads), first, second, *(scales or (none, none)), sizes, types)
+    expert_ops._call("yabt_adamw_step", dev, len(params), _table(rows), state.bits, number, at, float(lr), float(b1),
+                     float(b2), float(eps), float(weight_decay))
     for p in params:
         if p.requires_grad:
             torch.autograd.graph.increment_version(p)
