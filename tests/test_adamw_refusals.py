@@ -1,6 +1,8 @@
 """What an AdamW step refuses, without a device; and its plain form against
 differences of the quantity that it minimises in one step."""
 
+import ctypes
+
 import numpy as np
 import pytest
 import torch
@@ -15,7 +17,7 @@ def refused(rc, text):
 
 
 def words(n=4, p=16, g=16, m=16, v=16, sm=16, sv=16, pt=0, gt=0):
-    return optim._table([(p, g, m, v, sm, sv, n, pt | gt << 32)])
+    return (ctypes.c_int64 * 8)(p, g, m, v, sm, sv, n, pt | gt << 32)
 
 
 def test_c_entry():

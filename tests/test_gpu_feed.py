@@ -107,7 +107,8 @@ def large(n, D, F, O, dt, act):
     return got
 
 
-@pytest.mark.parametrize("n,D,F,O", [(2048, 384, 2048, 4096), (2050, 392, 2056, 4104), (4100, 2048, 1025, 2049)])
+@pytest.mark.parametrize("n,D,F,O", [(2048, 384, 2048, 4096), (2050, 392, 2056, 4104), (4100, 2048, 1025, 2049),
+                                     (4096, 2048, 2048, 4096), (4120, 2056, 2064, 4104), (4097, 2049, 2050, 4099), (16_390, 520, 600, 512)])
 @pytest.mark.parametrize("dt", TYPES[1:], ids=name)
 def test_large_tiles(n, D, F, O, dt):
     print(f"feed large n={n} D={D} F={F} O={O} {name(dt)}", flush=True)

@@ -73,13 +73,14 @@ __device__ __forceinline__ i32x4 mma8(u32x4 a, u32x4 b, i32x4 c) {
 
 // The activation of four gates and its derivative.  16 bits: the hardware's exp2 and
 // reciprocal (gate_sigmoid), and for the normal distribution function the approximation
-// 7.1.26 of Abramowitz and Stegun's handbook, off by 7.5e-8 at most; fp32 and 8 bits, whose
-// codes a small error would move: the accurate functions.
+// 7.1.26 of Abramowitz and Stegun's handbook, off by 7.5e-8 at most.  8 bits too: an h that is
+// off by 2^-20 of itself has another code once in 10^4 times or less; the accurate ones take
+// 12 of 466 us of 16 384 x 2048 -> 5632.  fp32: the accurate functions.
 template <typename T>
 __device__ __forceinline__ float gate_normal(float g) {
     const float x = fabsf(g) * 0.70710678f;
     float tail;                        // of the distribution, beyond |g|
-    if constexpr (sizeof(T) == 2) {
+    if constexpr (sizeof(T) != 4) {
         const float t = __builtin_amdgcn_rcpf(1.0f + 0.3275911f * x);
         const float p = t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
         tail = 0.5f * p * __expf(-x * x);
@@ -90,12 +91,11 @@ __device__ __forceinline__ float gate_normal(float g) {
 }
 template <typename T>
 __device__ __forceinline__ void activate(int act, f32x4 g, float (&v)[4], float (&slope)[4]) {
-    using S = std::conditional_t<sizeof(T) == 2, T, float>;
     switch (act) {
         case SILU:
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                const float s = gate_sigmoid<S>(g[q]);
+                const float s = gate_sigmoid<T>(g[q]);
                 v[q] = g[q] * s;
                 slope[q] = s * (1.0f + g[q] * (1.0f - s));
             }
@@ -103,10 +103,10 @@ __device__ __forceinline__ void activate(int act, f32x4 g, float (&v)[4], float 
         case GELU:
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                const float p = gate_normal<S>(g[q]), e = -0.5f * g[q] * g[q];
+                const float p = gate_normal<T>(g[q]), e = -0.5f * g[q] * g[q];
                 v[q] = g[q] * p;
                 // far out the density is 0, and g times it too
-                slope[q] = p + (e > -87.0f ? g[q] * 0.39894228f * (sizeof(T) == 2 ? __expf(e) : expf(e)) : 0.0f);
+                slope[q] = p + (e > -87.0f ? g[q] * 0.39894228f * (sizeof(T) != 4 ? __expf(e) : expf(e)) : 0.0f);
             }
             break;
         case GELU_TANH:
@@ -114,7 +114,7 @@ __device__ __forceinline__ void activate(int act, f32x4 g, float (&v)[4], float 
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 const float g2 = fminf(g[q] * g[q], 1e8f);
-                const float s = gate_sigmoid<S>(1.5957691216f * g[q] * (1.0f + 0.044715f * g2));
+                const float s = gate_sigmoid<T>(1.5957691216f * g[q] * (1.0f + 0.044715f * g2));
                 v[q] = g[q] * s;
                 slope[q] = s + g[q] * s * (1.0f - s) * 1.5957691216f * (1.0f + 0.134145f * g2);
             }
@@ -257,10 +257,16 @@ __device__ __forceinline__ int out_row(const Product& P, int m) {
     return m;
 }
 
-// One tile of the product MODE: that of the block with number `block` of its grid
-// of mtiles x ntiles x splits.
+// The tiles of a product that a grid makes: mt x nt x splits, or `count` of them from `first` on,
+// by `blocks` thread blocks (a multiple of XCDS, so that a block's number tells its die).
+struct Tiles {
+    int nt, mt;
+    uint32_t first, count, blocks;
+};
+
+// One tile of the product MODE: that of the block with number `block` of the product's.
 template <typename T, int MODE, typename TL, bool DMA>
-__device__ __forceinline__ void feed_tile(const Product& P, uint32_t block, int ntiles, int mtiles) {
+__device__ __forceinline__ void feed_tile(const Product& P, uint32_t block, const Tiles& G) {
     using Block = typename Sums<T>::Block;
     constexpr bool GATED = MODE == IN || MODE == IN8;
     lds_char* const lds = (lds_char*)s_tiles;
@@ -269,13 +275,14 @@ __device__ __forceinline__ void feed_tile(const Product& P, uint32_t block, int 
     const int wm = wave / TL::WN, wn = wave % TL::WN;
 
     // column tiles together with a group of row tiles, on one die
-    const int64_t per = (int64_t)mtiles * ntiles, id = die_order(block, per * P.splits);
-    if (id >= per * P.splits) return;
+    const int64_t place = die_order(block, G.count);
+    if (place >= G.count) return;
+    const uint32_t id = G.first + (uint32_t)place, per = (uint32_t)G.mt * (uint32_t)G.nt;
     const int split = (int)(id / per);
-    const int64_t in = id - split * per, group = in / ((int64_t)TILE_GROUP * ntiles);
-    const int gin = (int)(in - group * TILE_GROUP * ntiles);
-    const int gm = (int)min((int64_t)TILE_GROUP, mtiles - group * TILE_GROUP);
-    const int mf = (int)(group * TILE_GROUP + gin % gm) * TL::BM;
+    const uint32_t in = id - split * per, whole_group = TILE_GROUP * (uint32_t)G.nt, group = in / whole_group;
+    const int gin = (int)(in - group * whole_group);
+    const int gm = min(TILE_GROUP, G.mt - (int)group * TILE_GROUP);
+    const int mf = ((int)group * TILE_GROUP + gin % gm) * TL::BM;
     const int nf = gin / gm * (GATED ? TL::BN / 2 : TL::BN);
 
     constexpr int BK = TL::STEP / (int)sizeof(T), KS = TL::STEP / 32;
@@ -486,22 +493,27 @@ __device__ __forceinline__ void feed_tile(const Product& P, uint32_t block, int 
 }
 
 template <typename T, int MODE, typename TL, bool DMA>
-__global__ void __launch_bounds__(TL::NT) k_feed(Product P, int ntiles, int mtiles) {
-    feed_tile<T, MODE, TL, DMA>(P, blockIdx.x, ntiles, mtiles);
+__global__ void __launch_bounds__(TL::NT) k_feed(Product P, Tiles G) {
+    feed_tile<T, MODE, TL, DMA>(P, blockIdx.x, G);
 }
 
-// DX, DWIN and DWOUT need nothing of each other: one grid, so that one's last
-// tiles run beside the next one's first.
+// Products that need nothing of each other share a grid, so that one's last tiles run beside the
+// next one's first: DW_OUT, which needs h and dy alone, with DH, and DX, DW_IN and the rest of DW_OUT.
 struct GradProducts {
     Product p[3];
-    int nt[3], mt[3];
-    uint32_t first[2];                // DWIN's and DWOUT's first blocks, multiples of XCDS
+    Tiles g[3];
 };
 template <typename T, typename TL, bool DMA>
+__global__ void __launch_bounds__(TL::NT) k_feed_inner_grad(Product out, Tiles go, Product dh, Tiles gh) {
+    if (blockIdx.x < go.blocks) feed_tile<T, DWOUT, TL, DMA>(out, blockIdx.x, go);
+    else feed_tile<T, DH, TL, DMA>(dh, blockIdx.x - go.blocks, gh);
+}
+template <typename T, typename TL, bool DMA>
 __global__ void __launch_bounds__(TL::NT) k_feed_grads(GradProducts G) {
-    if (blockIdx.x < G.first[0]) feed_tile<T, DX, TL, DMA>(G.p[0], blockIdx.x, G.nt[0], G.mt[0]);
-    else if (blockIdx.x < G.first[1]) feed_tile<T, DWIN, TL, DMA>(G.p[1], blockIdx.x - G.first[0], G.nt[1], G.mt[1]);
-    else feed_tile<T, DWOUT, TL, DMA>(G.p[2], blockIdx.x - G.first[1], G.nt[2], G.mt[2]);
+    const uint32_t first = G.g[0].blocks, second = first + G.g[1].blocks;
+    if (blockIdx.x < first) feed_tile<T, DX, TL, DMA>(G.p[0], blockIdx.x, G.g[0]);
+    else if (blockIdx.x < second) feed_tile<T, DWIN, TL, DMA>(G.p[1], blockIdx.x - first, G.g[1]);
+    else feed_tile<T, DWOUT, TL, DMA>(G.p[2], blockIdx.x - second, G.g[2]);
 }
 
 // The sums of up to three products that were made in part, added in order.
@@ -907,6 +919,7 @@ __global__ void __launch_bounds__(FEW_NT) k_few(Product P) {
 using TileSmall = TileOf<64, 128, 2, 2, 128, 2, 2>;
 using TileLarge = TileOf<256, 256, 4, 2, 128, 3, 2>;
 
+constexpr int CUS = 256;
 constexpr int PART_BLOCKS = 512;      // blocks that keep the device busy
 constexpr int MOST_SPLITS = 64;
 constexpr int INT8_MOST = 131071;     // terms of 128 x 128 whose sum stays in 32 bits
@@ -930,13 +943,29 @@ inline int split_count(int64_t M, int64_t N, int64_t K, bool large, int bytes) {
     return s < 1 ? 1 : (int)s;
 }
 
+// All tiles of a product; false: more than a grid can have.
 template <typename TL>
-int64_t tile_grid(const Product& P, bool gated, int* nt, int* mt, int M) {
-    *nt = (int)over(P.N, gated ? TL::BN / 2 : TL::BN);
-    *mt = (int)over(M, TL::BM);
-    return over((int64_t)*nt * *mt * P.splits, XCDS) * XCDS;
+bool all_tiles(const Product& P, bool gated, Tiles* g) {
+    g->nt = (int)over(P.N, gated ? TL::BN / 2 : TL::BN);
+    g->mt = (int)over(P.M, TL::BM);
+    const double count = (double)g->nt * g->mt * P.splits;
+    if (count * TL::NT > 4e9) return false;      // with the other products of a grid below 2^32 threads, checked there
+    g->first = 0;
+    g->count = (uint32_t)g->nt * (uint32_t)g->mt * (uint32_t)P.splits;
+    g->blocks = (uint32_t)(over(g->count, XCDS) * XCDS);
+    return true;
 }
-inline bool grid_ok(int64_t blocks, int threads) { return blocks > 0 && blocks <= UINT32_MAX / threads; }
+// The last `count` tiles in a grid of their own.
+inline Tiles take_last(Tiles* g, uint32_t count) {
+    Tiles last = *g;
+    g->count -= count;
+    g->blocks = (uint32_t)(over(g->count, XCDS) * XCDS);
+    last.first += g->count;
+    last.count = count;
+    last.blocks = (uint32_t)(over(count, XCDS) * XCDS);
+    return last;
+}
+inline bool grid_ok(int64_t blocks, int threads) { return blocks <= UINT32_MAX / threads; }
 
 // fp32 has no large tiles (large_product).
 template <typename T, typename F>
@@ -952,10 +981,9 @@ template <typename T, int MODE>
 bool run_tiles(const Product& P, bool large, bool dma, hipStream_t stream) {
     return by_tile<T>(large, dma, [&](auto tl, auto d) {
         using TL = decltype(tl);
-        int nt, mt;
-        const int64_t blocks = tile_grid<TL>(P, MODE == IN || MODE == IN8, &nt, &mt, P.M);
-        if (!grid_ok(blocks, TL::NT)) return false;
-        k_feed<T, MODE, TL, decltype(d)::value><<<(unsigned)blocks, TL::NT, TL::LDS, stream>>>(P, nt, mt);
+        Tiles g;
+        if (!all_tiles<TL>(P, MODE == IN || MODE == IN8, &g) || !grid_ok(g.blocks, TL::NT)) return false;
+        k_feed<T, MODE, TL, decltype(d)::value><<<g.blocks, TL::NT, TL::LDS, stream>>>(P, g);
         return true;
     });
 }
@@ -1006,6 +1034,25 @@ inline bool feed_ranges_ok(int64_t n, int D, int F, int O) {
     return n >= 0 && n < (1ll << 31) - 256 && D >= 1 && F >= 1 && O >= 1 && D <= (1 << 24) && F <= (1 << 24) && O <= (1 << 24);
 }
 
+// The three gradients by 256 x 256 tiles, side by side, those of more steps than a CU's share of
+// all in parts (of 16 steps at least).  Large and small, us for forward and backward, bf16: 8192 x 1024, 2816: 620 and
+// 703; 4096 x 2048, 2048: 360 and 446; 2048 x 2048, 5632: 590 and 624.
+inline bool large_gradients(int bytes, const int64_t (&M)[3], const int64_t (&N)[3], const int64_t (&K)[3], int (&splits)[3]) {
+    int64_t tiles[3], steps[3], all = 0, count = 0;
+    for (int i = 0; i < 3; ++i) {
+        if (bytes > 2 || K[i] * bytes < 768 || M[i] < 192 || N[i] < 192) return false;
+        tiles[i] = over(M[i], 256) * over(N[i], 256), steps[i] = over(K[i] * bytes, 128);
+        all += tiles[i] * steps[i];
+    }
+    const int64_t share = all / CUS < 16 ? 16 : all / CUS;
+    for (int i = 0; i < 3; ++i) {
+        const int64_t s = over(steps[i], share);
+        splits[i] = (int)(s < MOST_SPLITS ? s : MOST_SPLITS);
+        count += tiles[i] * splits[i];
+    }
+    return count >= 200;
+}
+
 // y: every block of its kernel for few rows reads all of h again, 16 columns a block (16 rows or
 // fewer: in fp32); tiles split over F read less but need a second launch to join them.  Few and tiles, us for
 // the block: 2048 -> 5632 -> 2048, bf16, 17 rows 26.9 and 26.3, 24 28.7 and 26.8, 48 38.6 and 31.3, 64 45.7 and
@@ -1034,12 +1081,23 @@ inline FeedSizes feed_sizes(int dtype, int64_t n, int D, int F, int O) {
     z.large_out = large_product(b, n, O, F);
     z.splits_out = split_count(n, O, F, z.large_out, b);
     z.large_dh = large_product(b, n, F, O);
-    const int64_t K3 = (int64_t)z.Fp + F;
-    z.large_grads = large_product(b, n, D, K3) && large_product(b, 2 * (int64_t)F, D, n) && large_product(b, O, F, n);
-    z.splits[0] = split_count(n, D, K3, z.large_grads, b);
-    z.splits[1] = split_count(K3, D, n, z.large_grads, b);
-    z.splits[2] = split_count(O, F, n, z.large_grads, b);
+    const int64_t M[3] = {n, (int64_t)z.Fp + F, O}, N[3] = {D, D, F}, K[3] = {(int64_t)z.Fp + F, n, n};
+    z.large_grads = large_gradients(b, M, N, K, z.splits);
+    if (!z.large_grads)
+        for (int i = 0; i < 3; ++i) z.splits[i] = split_count(M[i], N[i], K[i], false, b);
     return z;
+}
+
+// How many tiles of dW_out are made beside dh: with large tiles, of which a CU takes one at a time, so many that
+// the others' grid is whole rounds of tiles, where that round costs more than what it adds to dh's.
+// 8192 x 2048, 5632 (784 tiles, dh's 704): 16 of them.
+inline uint32_t beside_inner_grad(const FeedSizes& z, uint32_t dh, const Tiles (&g)[3]) {
+    const uint32_t rest = (g[0].count + g[1].count + g[2].count) % CUS;
+    if (!z.large_grads || rest == 0 || rest > g[2].count) return 0;
+    const double each = (double)z.n / 64 / z.splits[2], each_dh = (double)z.O / 64 + 22;   // steps; dh's end takes as long as 22
+    const double rounds = (double)over(dh, CUS), idle = rounds * CUS - dh;
+    const double more = (rest * each - idle * each_dh) / CUS, longer = each - rounds * each_dh;
+    return (more > 0 ? more : 0) + (longer > 0 ? longer : 0) < 0.9 * each ? rest : 0;
 }
 
 struct FeedKept {                     // what the forward pass keeps
@@ -1116,7 +1174,6 @@ int run_feed_grad(const FeedSizes& z, int act, int dtype, const void* dy, int64_
     P.M = (int)z.n, P.N = z.F, P.K = z.O;
     P.F = z.F, P.Fp = z.Fp, P.Fi = z.Fi, P.act = act, P.splits = 1;
     P.pre = kept.pre, P.dpre = s.dpre;
-    if (z.n > 0 && !run_tiles<T, DH>(P, z.large_dh, dma, stream)) return fail(-1, "yabt_feed_forward_grad: bad sizes");
     GradProducts G = {};
     for (auto& p : G.p) p.F = z.F, p.Fp = z.Fp, p.Fi = z.Fi, p.out_dtype = dtype;
     Product &X = G.p[0], &I = G.p[1], &O = G.p[2];
@@ -1129,12 +1186,21 @@ int run_feed_grad(const FeedSizes& z, int act, int dtype, const void* dy, int64_
     for (int i = 0; i < 3; ++i) G.p[i].splits = z.splits[i], G.p[i].part = s.part[i];
     const bool ok = by_tile<T>(z.large_grads, dma, [&](auto tl, auto d) {
         using TL = decltype(tl);
-        const int64_t gx = tile_grid<TL>(X, false, &G.nt[0], &G.mt[0], X.M), gi = tile_grid<TL>(I, false, &G.nt[1], &G.mt[1], I.M),
-                      go = tile_grid<TL>(O, false, &G.nt[2], &G.mt[2], O.M);
-        if (!grid_ok(gx + gi + go, TL::NT)) return false;
-        G.first[0] = (uint32_t)gx;
-        G.first[1] = (uint32_t)(gx + gi);
-        k_feed_grads<T, TL, decltype(d)::value><<<(unsigned)(gx + gi + go), TL::NT, TL::LDS, stream>>>(G);
+        for (int i = 0; i < 3; ++i)
+            if (!all_tiles<TL>(G.p[i], false, &G.g[i])) return false;
+        if (!grid_ok((int64_t)G.g[0].blocks + G.g[1].blocks + G.g[2].blocks, TL::NT)) return false;
+        Tiles gh;
+        if (z.large_dh == z.large_grads) {
+            if (!all_tiles<TL>(P, false, &gh)) return false;
+            Tiles go = take_last(&G.g[2], beside_inner_grad(z, gh.count, G.g));
+            if (!grid_ok((int64_t)go.blocks + gh.blocks, TL::NT)) return false;
+            if (go.blocks + gh.blocks)
+                k_feed_inner_grad<T, TL, decltype(d)::value><<<go.blocks + gh.blocks, TL::NT, TL::LDS, stream>>>(O, go, P, gh);
+        } else if (z.n > 0 && !run_tiles<T, DH>(P, z.large_dh, dma, stream)) {
+            return false;
+        }
+        k_feed_grads<T, TL, decltype(d)::value>
+            <<<G.g[0].blocks + G.g[1].blocks + G.g[2].blocks, TL::NT, TL::LDS, stream>>>(G);
         return true;
     });
     if (!ok) return fail(-1, "yabt_feed_forward_grad: bad sizes");

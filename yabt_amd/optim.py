@@ -13,7 +13,7 @@ graph.
 
 from __future__ import annotations
 
-import ctypes
+from array import array
 from dataclasses import dataclass
 from itertools import chain
 from operator import attrgetter
@@ -47,7 +47,7 @@ class AdamWState:
         what they stand for now, in new ones."""
         if self.bits == 32:
             return self.first, self.second
-        sizes = list(map(torch.Tensor.numel, self.first))
+        sizes = list(map(_numel, self.first))
         if not sizes:
             return [], []
         lists, dev = _checked(self, sizes)
@@ -56,19 +56,18 @@ class AdamWState:
         parts = torch.empty(2 * sum(held), dtype=torch.float32, device=dev).split_with_sizes(
             [m for n, h in zip(sizes, held) for m in (n, h - n)] * 2)[::2]
         flat = parts[:len(sizes)], parts[len(sizes):]
-        rows = zip(*(map(torch.Tensor.data_ptr, part) for part in (*flat, *lists)), sizes, [0] * len(sizes))
-        expert_ops._call("yabt_adamw_values", dev, len(sizes), _table(rows))
+        table = _table(zip(*(map(_pointer, part) for part in (*flat, *lists)), sizes, [0] * len(sizes)))
+        expert_ops._call("yabt_adamw_values", dev, len(sizes), table.buffer_info()[0])
         return tuple([v if t.dim() == 1 else v.view(t.shape) for v, t in zip(part, self.first)] for part in flat)
 
 
-def _table(rows) -> ctypes.Array:
-    """yabt_adamw_tensor's fields, eight 64-bit words a tensor."""
-    words = list(chain.from_iterable(rows))
-    return (ctypes.c_int64 * len(words))(*words)
+def _table(rows) -> array:
+    """yabt_adamw_tensor's fields, eight 64-bit words a tensor, to be held while their address is in use."""
+    return array("q", chain.from_iterable(rows))
 
 
 _TYPES = {32: (torch.float32, torch.float32), 8: (torch.int8, torch.uint8)}
-_DTYPE, _SHAPE, _NEEDS, _CUDA = (attrgetter(m) for m in ("dtype", "shape", "requires_grad", "is_cuda"))
+_DTYPE, _SHAPE, _NEEDS = (attrgetter(m) for m in ("dtype", "shape", "requires_grad"))
 _numel, _contiguous, _device_number, _pointer = (getattr(torch.Tensor, m) for m in
                                                  ("numel", "is_contiguous", "get_device", "data_ptr"))
 
@@ -94,7 +93,7 @@ def _checked(state: AdamWState, sizes: list[int]) -> tuple[list[list[torch.Tenso
     every = list(chain.from_iterable(lists))
     if any(set(map(_DTYPE, part)) != {dt} for part, dt in zip(lists, types)) or \
             any(list(map(_numel, part)) != want for part, want in zip(lists, (sizes, sizes, blocks, blocks))) or \
-            not all(map(_contiguous, every)) or not all(map(_CUDA, every)) or len(set(map(_device_number, every))) != 1:
+            not all(map(_contiguous, every)) or len(numbers := set(map(_device_number, every))) != 1 or -1 in numbers:
         _refuse(lists, types, sizes, blocks)
     return lists, every[0].device
 
@@ -179,7 +178,7 @@ def adamw_step(params: list[torch.Tensor], grads: list[torch.Tensor | None], sta
     if list(map(_SHAPE, params)) != list(map(_SHAPE, grads)):
         raise ValueError(f"gradients must have their parameters' shapes, got {[tuple(g.shape) for g in grads]} for "
                          f"{[tuple(p.shape) for p in params]}")
-    if any(n != dev.index for part in (params, grads) for n in map(_device_number, part)):
+    if set(map(_device_number, chain(params, grads))) != {dev.index}:
         raise ValueError(f"all tensors must be on {dev}")
     if not all(map(_contiguous, params)):
         raise ValueError("parameters must be contiguous: they are written in place")
@@ -195,8 +194,8 @@ def adamw_step(params: list[torch.Tensor], grads: list[torch.Tensor | None], sta
         raise ValueError("a parameter is in the list twice")
     none = [0] * len(params)
     first, second, *scales = (list(map(_pointer, part)) for part in lists)
-    rows = zip(where, map(_pointer, grads), first, second, *(scales or (none, none)), sizes, types)
-    expert_ops._call("yabt_adamw_step", dev, len(params), _table(rows), state.bits, number, at, float(lr), float(b1),
+    table = _table(zip(where, map(_pointer, grads), first, second, *(scales or (none, none)), sizes, types))
+    expert_ops._call("yabt_adamw_step", dev, len(params), table.buffer_info()[0], state.bits, number, at, float(lr), float(b1),
                      float(b2), float(eps), float(weight_decay))
     for p in params:
         if p.requires_grad:
