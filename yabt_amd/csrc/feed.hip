@@ -231,6 +231,182 @@ struct Loader {
     }
 };
 
+// fp32 values in three parts of bf16, 8 bits of the significand each: x = hi + mid + lo exactly, each
+// part cut off, so that none is larger than x.  A product of two has nine products of parts; the
+// three smallest, at most 2^-23 of it together, are left out.
+__device__ __forceinline__ void in_parts(u32x4 a, u32x4 b, u32x4 (&part)[3]) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        uint32_t x[2], r[2], l[2];
+#pragma unroll
+        for (int o = 0; o < 2; ++o) {
+            const int at = 2 * q + o;
+            x[o] = at < 4 ? a[at] : b[at - 4];
+            r[o] = __float_as_uint(__uint_as_float(x[o]) - __uint_as_float(x[o] & 0xFFFF0000u));
+            l[o] = __float_as_uint(__uint_as_float(r[o]) - __uint_as_float(r[o] & 0xFFFF0000u));
+        }
+        part[0][q] = __builtin_amdgcn_perm(x[1], x[0], 0x07060302u);     // the upper halves of both
+        part[1][q] = __builtin_amdgcn_perm(r[1], r[0], 0x07060302u);
+        part[2][q] = __builtin_amdgcn_perm(l[1], l[0], 0x07060302u);
+    }
+}
+
+// BM x BN sums of fp32 by WM x WN waves, in steps of 32 places of the summed dimension; LDS
+// holds two steps of both operands, in three parts of bf16.
+template <int BM_, int BN_, int WM_, int WN_>
+struct TileParts {
+    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, STEP = 128;
+    static constexpr int NT = 64 * WM * WN;
+    static constexpr int MI = BM / WM / 32, NI = BN / WN / 32;
+    static constexpr int APART = BM * 64, BPART = BN * 64, PLACE = 3 * (APART + BPART);   // a part's bytes, a step's
+    static constexpr int LDS = 2 * PLACE;
+    static constexpr int NA = APART / 16 / NT, NB = BPART / 16 / NT;                      // pieces of 8 values a thread
+    static_assert(NA >= 1 && NB >= 1 && NI % 2 == 0, "whole pieces a thread, gate and up in one wave");
+    static_assert(LDS <= 160 * 1024 && BM / MI * BN * 4 <= LDS, "a block's LDS");
+};
+
+// The pieces (8 values) of an fp32 operand that a thread brings to LDS in parts: laid out as bf16 in
+// steps of 64 bytes.
+template <int MODE, bool SIDE_B, int W, int COUNT, int NT>
+struct PartsLoader {
+    using Layout = Loader<bf16, MODE, SIDE_B, W, COUNT, NT, 64>;
+    static constexpr bool ACROSS = Layout::ACROSS;
+    const float* ptr[COUNT];
+    u32x4 v[2][COUNT][2];      // two steps' pieces on their way
+
+    __device__ __forceinline__ void init(const Product& P, int first) {
+        const float* const base = (const float*)(SIDE_B ? P.b : P.a);
+        const size_t ld = (size_t)(SIDE_B ? P.ldb : P.lda);
+#pragma unroll
+        for (int i = 0; i < COUNT; ++i) {
+            const int r = Layout::row_of(i);
+            if constexpr (Layout::GATED) {
+                const int f = min(first + (r >> 6) * 32 + (r & 31), P.F - 1);
+                ptr[i] = base + (size_t)((r >> 5 & 1 ? P.F : 0) + f) * ld;
+            } else if constexpr (!ACROSS) {
+                ptr[i] = base + (size_t)min(first + r, (SIDE_B ? P.N : P.M) - 1) * ld;
+            } else {
+                ptr[i] = base + min(first + Layout::piece_of(i) * 8, Layout::width(P) - 1);
+            }
+        }
+    }
+    // the step from k0 on; what does not exist is zero
+    template <int SET>
+    __device__ __forceinline__ void fetch(const Product& P, int k0, int end, int first) {
+#pragma unroll
+        for (int i = 0; i < COUNT; ++i) {
+            const float* p = ptr[i];
+            int have;
+            if constexpr (!ACROSS) {
+                const int k = k0 + Layout::piece_of(i) * 8;
+                have = end - k;
+                p += k;
+            } else {
+                int kk = k0 + Layout::row_of(i);
+                have = kk < end ? Layout::width(P) - (first + Layout::piece_of(i) * 8) : 0;
+                if constexpr (MODE == DX) {
+                    // [dg du] has du from Fp on, W_in its rows from F on
+                    if (kk >= P.F) {
+                        if (kk < P.Fp) have = 0;
+                        kk += P.F - P.Fp;
+                    }
+                }
+                p += (size_t)kk * (size_t)(SIDE_B ? P.ldb : P.lda);
+            }
+            u32x4 a = {0, 0, 0, 0}, b = a;
+            if (have >= 8) {
+                a = *reinterpret_cast<const u32x4_any*>(p);
+                b = *reinterpret_cast<const u32x4_any*>(p + 4);
+            } else {
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    if (q < have) a[q] = __float_as_uint(p[q]);
+#pragma unroll
+                for (int q = 0; q < 3; ++q)
+                    if (q + 4 < have) b[q] = __float_as_uint(p[q + 4]);
+            }
+            v[SET][i][0] = a;
+            v[SET][i][1] = b;
+        }
+    }
+    template <int SET>
+    __device__ __forceinline__ void put(lds_char* tile) const {
+#pragma unroll
+        for (int i = 0; i < COUNT; ++i) {
+            u32x4 part[3];
+            in_parts(v[SET][i][0], v[SET][i][1], part);
+#pragma unroll
+            for (int o = 0; o < 3; ++o) *(lds_u32x4*)(tile + o * (W * 64) + (i * NT + (int)threadIdx.x) * 16) = part[o];
+        }
+    }
+};
+
+// acc += the tile's products over [lo, end) in parts.
+template <int MODE, typename TL>
+__device__ __forceinline__ void parts_sums(const Product& P, int mf, int nf, int lo, int end, int steps,
+                                           f32x16 (&acc)[TL::MI][TL::NI]) {
+    lds_char* const lds = (lds_char*)s_tiles;
+    const int wave = threadIdx.x / 64, wm = wave / TL::WN, wn = wave % TL::WN;
+    PartsLoader<MODE, false, TL::BM, TL::NA, TL::NT> la;
+    PartsLoader<MODE, true, TL::BN, TL::NB, TL::NT> lb;
+    la.init(P, mf);
+    lb.init(P, nf);
+    const Frag<bf16, decltype(la)::ACROSS, TL::BM, 64> fa(wm * TL::MI * 32);
+    const Frag<bf16, decltype(lb)::ACROSS, TL::BN, 64> fb(wn * TL::NI * 32);
+    auto fetch = [&](auto set, int t) {
+        if (t >= steps) return;
+        la.template fetch<decltype(set)::value>(P, lo + t * 32, end, mf);
+        lb.template fetch<decltype(set)::value>(P, lo + t * 32, end, nf);
+    };
+    auto put = [&](auto set) {
+        lds_char* const place = lds + decltype(set)::value * TL::PLACE;
+        la.template put<decltype(set)::value>(place);
+        lb.template put<decltype(set)::value>(place + 3 * TL::APART);
+    };
+    auto products = [&](auto set) {
+        lds_char* const ta = lds + decltype(set)::value * TL::PLACE;
+        lds_char* const tb = ta + 3 * TL::APART;
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+            u32x4 a[3][TL::MI], b[3][TL::NI];
+#pragma unroll
+            for (int o = 0; o < 3; ++o) {
+#pragma unroll
+                for (int i = 0; i < TL::MI; ++i) a[o][i] = fa.get(ta + o * TL::APART, i, ks);
+#pragma unroll
+                for (int j = 0; j < TL::NI; ++j) b[o][j] = fb.get(tb + o * TL::BPART, j, ks);
+            }
+            // the small products first
+#pragma unroll
+            for (int sum = 2; sum >= 0; --sum)
+#pragma unroll
+                for (int o = 0; o <= sum; ++o)
+#pragma unroll
+                    for (int i = 0; i < TL::MI; ++i)
+#pragma unroll
+                        for (int j = 0; j < TL::NI; ++j) acc[i][j] = mma<bf16>(a[o][i], b[sum - o][j], acc[i][j]);
+        }
+    };
+    constexpr std::integral_constant<int, 0> even;
+    constexpr std::integral_constant<int, 1> odd;
+    fetch(even, 0);
+    fetch(odd, 1);
+    put(even);
+    fetch(even, 2);
+    for (int t = 0; t < steps; t += 2) {
+        __syncthreads();                         // step t is there, and what was read of the other place is read
+        if (t + 1 < steps) put(odd);
+        fetch(odd, t + 3);
+        products(even);
+        if (t + 1 >= steps) break;
+        __syncthreads();
+        if (t + 2 < steps) put(even);
+        fetch(even, t + 4);
+        products(odd);
+    }
+    __syncthreads();                             // the sums leave through the same LDS
+}
+
 // Up to four values at p in the type that a run-time number names.
 __device__ __forceinline__ void store_as(int dtype, void* p, size_t at, f32x4 v, int have) {
     if (dtype == DT_F32) store_part((float*)p + at, v, have);
@@ -290,10 +466,6 @@ __device__ __forceinline__ void feed_tile(const Product& P, uint32_t block, cons
     const int lo = (int)min((int64_t)P.K, (int64_t)split * part), end = (int)min((int64_t)P.K, (int64_t)lo + part);
     const int steps = (int)(((int64_t)end - lo + BK - 1) / BK);
 
-    Loader<T, MODE, false, TL::BM, TL::NA, TL::NT, TL::STEP> la;
-    Loader<T, MODE, true, TL::BN, TL::NB, TL::NT, TL::STEP> lb;
-    using LA = decltype(la);
-    using LB = decltype(lb);
     Block acc[TL::MI][TL::NI];
 #pragma unroll
     for (int i = 0; i < TL::MI; ++i)
@@ -302,7 +474,13 @@ __device__ __forceinline__ void feed_tile(const Product& P, uint32_t block, cons
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0;
 
-    if (steps > 0) {
+    if constexpr (sizeof(T) == 4) {
+        if (steps > 0) parts_sums<MODE, TL>(P, mf, nf, lo, end, steps, acc);
+    } else if (steps > 0) {
+        Loader<T, MODE, false, TL::BM, TL::NA, TL::NT, TL::STEP> la;
+        Loader<T, MODE, true, TL::BN, TL::NB, TL::NT, TL::STEP> lb;
+        using LA = decltype(la);
+        using LB = decltype(lb);
         la.init(P, mf);
         lb.init(P, nf);
         // Step t of the rows' operand lies at place t % AS, of the columns' at t % 2.
@@ -356,7 +534,7 @@ __device__ __forceinline__ void feed_tile(const Product& P, uint32_t block, cons
             for (int j = 0; j < TL::NI; ++j) b[ks & 1][j] = fb.get(tb, j, ks);
         };
         constexpr int READS = TL::MI * decltype(fa)::READS + TL::NI * decltype(fb)::READS;
-        constexpr int PRODUCTS = TL::MI * TL::NI * (sizeof(T) == 4 ? 4 : 1);
+        constexpr int PRODUCTS = TL::MI * TL::NI;
         stage_ready<AFTER_0>();
         read(0, 0, 0);
         // A k-step's operands are read while the one before is multiplied, the
@@ -918,6 +1096,7 @@ __global__ void __launch_bounds__(FEW_NT) k_few(Product P) {
 
 using TileSmall = TileOf<64, 128, 2, 2, 128, 2, 2>;
 using TileLarge = TileOf<256, 256, 4, 2, 128, 3, 2>;
+using TileWhole = TileParts<64, 128, 2, 2>;       // fp32
 
 constexpr int CUS = 256;
 constexpr int PART_BLOCKS = 512;      // blocks that keep the device busy
@@ -967,13 +1146,15 @@ inline Tiles take_last(Tiles* g, uint32_t count) {
 }
 inline bool grid_ok(int64_t blocks, int threads) { return blocks <= UINT32_MAX / threads; }
 
-// fp32 has no large tiles (large_product).
+// fp32: in parts, whatever its rows' alignment.
 template <typename T, typename F>
 auto by_tile(bool large, bool dma, const F& f) {
-    if constexpr (sizeof(T) <= 2) {
+    if constexpr (sizeof(T) == 4) {
+        return f(TileWhole(), std::false_type());
+    } else {
         if (large) return dma ? f(TileLarge(), std::true_type()) : f(TileLarge(), std::false_type());
+        return dma ? f(TileSmall(), std::true_type()) : f(TileSmall(), std::false_type());
     }
-    return dma ? f(TileSmall(), std::true_type()) : f(TileSmall(), std::false_type());
 }
 
 // Makes the tiles of one product; false: the grid would be too large.
