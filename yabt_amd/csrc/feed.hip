@@ -1096,25 +1096,31 @@ __global__ void __launch_bounds__(FEW_NT) k_few(Product P) {
 
 using TileSmall = TileOf<64, 128, 2, 2, 128, 2, 2>;
 using TileLarge = TileOf<256, 256, 4, 2, 128, 3, 2>;
-using TileWhole = TileParts<64, 128, 2, 2>;       // fp32
+using PartsSmall = TileParts<64, 128, 2, 2>;     // fp32
+using PartsLarge = TileParts<128, 256, 2, 4>;
+// Tiles of a product of M x N sums.
+inline int64_t tile_count(int bytes, bool large, int64_t M, int64_t N) {
+    return over(M, large ? (bytes == 4 ? 128 : 256) : 64) * over(N, large ? 256 : 128);
+}
 
 constexpr int CUS = 256;
 constexpr int PART_BLOCKS = 512;      // blocks that keep the device busy
 constexpr int MOST_SPLITS = 64;
 constexpr int INT8_MOST = 131071;     // terms of 128 x 128 whose sum stays in 32 bits
 
-// Whether 256 x 256 tiles make a product of M x K by K x N (its sums' columns) faster than 64 x 128:
-// they fetch a third of the bytes, but there have to be enough of them, and a block of theirs has
-// its CU to itself, so that nothing covers its beginning and end unless K is long.  fp32 is bound by
-// its arithmetic, of which small tiles waste less at the edges.
+// Whether large tiles make a product of M x K by K x N (its sums' columns) faster than small ones: they
+// fetch less, or take less apart (fp32), but there have to be enough of them, and a block of theirs has
+// its CU to itself, so that nothing covers its beginning and end unless K is long.  fp32, small and
+// large, us: 4096 x 2048 -> 4096 -> 2048 1240 and 1020, 3000 x 700, 2000, forward and backward 634 and 590; 128 x
+// 128 tiles lie between them where products are large and behind both where they are small.
 inline bool large_product(int bytes, int64_t M, int64_t N, int64_t K) {
-    return bytes <= 2 && K * bytes >= 768 && M >= 192 && N >= 192 && over(M, 256) * over(N, 256) >= 128;
+    return K * bytes >= 768 && M >= 192 && N >= 192 && tile_count(bytes, true, M, N) >= (bytes == 4 ? 200 : 128);
 }
 
 // Parts of the summed dimension, so that few tiles fill the device: at least four steps each.
 inline int split_count(int64_t M, int64_t N, int64_t K, bool large, int bytes) {
     if (large) return 1;
-    const int64_t tiles = over(M, 64) * over(N, 128);
+    const int64_t tiles = tile_count(bytes, false, M, N);
     int64_t s = PART_BLOCKS / (tiles < 1 ? 1 : tiles);
     const int64_t longest = K * bytes / (4 * 128);
     if (s > longest) s = longest;
@@ -1150,7 +1156,7 @@ inline bool grid_ok(int64_t blocks, int threads) { return blocks <= UINT32_MAX /
 template <typename T, typename F>
 auto by_tile(bool large, bool dma, const F& f) {
     if constexpr (sizeof(T) == 4) {
-        return f(TileWhole(), std::false_type());
+        return large ? f(PartsLarge(), std::false_type()) : f(PartsSmall(), std::false_type());
     } else {
         if (large) return dma ? f(TileLarge(), std::true_type()) : f(TileLarge(), std::false_type());
         return dma ? f(TileSmall(), std::true_type()) : f(TileSmall(), std::false_type());
@@ -1215,14 +1221,14 @@ inline bool feed_ranges_ok(int64_t n, int D, int F, int O) {
     return n >= 0 && n < (1ll << 31) - 256 && D >= 1 && F >= 1 && O >= 1 && D <= (1 << 24) && F <= (1 << 24) && O <= (1 << 24);
 }
 
-// The three gradients by 256 x 256 tiles, side by side, those of more steps than a CU's share of
+// The three gradients by large tiles, side by side, those of more steps than a CU's share of
 // all in parts (of 16 steps at least).  Large and small, us for forward and backward, bf16: 8192 x 1024, 2816: 620 and
 // 703; 4096 x 2048, 2048: 360 and 446; 2048 x 2048, 5632: 590 and 624.
 inline bool large_gradients(int bytes, const int64_t (&M)[3], const int64_t (&N)[3], const int64_t (&K)[3], int (&splits)[3]) {
     int64_t tiles[3], steps[3], all = 0, count = 0;
     for (int i = 0; i < 3; ++i) {
-        if (bytes > 2 || K[i] * bytes < 768 || M[i] < 192 || N[i] < 192) return false;
-        tiles[i] = over(M[i], 256) * over(N[i], 256), steps[i] = over(K[i] * bytes, 128);
+        if (K[i] * bytes < 768 || M[i] < 192 || N[i] < 192) return false;
+        tiles[i] = tile_count(bytes, true, M[i], N[i]), steps[i] = over(K[i] * bytes, 128);
         all += tiles[i] * steps[i];
     }
     const int64_t share = all / CUS < 16 ? 16 : all / CUS;
@@ -1275,7 +1281,7 @@ inline FeedSizes feed_sizes(int dtype, int64_t n, int D, int F, int O) {
 inline uint32_t beside_inner_grad(const FeedSizes& z, uint32_t dh, const Tiles (&g)[3]) {
     const uint32_t rest = (g[0].count + g[1].count + g[2].count) % CUS;
     if (!z.large_grads || rest == 0 || rest > g[2].count) return 0;
-    const double each = (double)z.n / 64 / z.splits[2], each_dh = (double)z.O / 64 + 22;   // steps; dh's end takes as long as 22
+    const double each = (double)z.n * z.bytes / 128 / z.splits[2], each_dh = (double)z.O * z.bytes / 128 + 22;   // steps; dh's end takes as long as 22
     const double rounds = (double)over(dh, CUS), idle = rounds * CUS - dh;
     const double more = (rest * each - idle * each_dh) / CUS, longer = each - rounds * each_dh;
     return (more > 0 ? more : 0) + (longer > 0 ? longer : 0) < 0.9 * each ? rest : 0;
