@@ -128,6 +128,11 @@ __device__ __forceinline__ void activate(int act, f32x4 g, float (&v)[4], float 
     }
 }
 
+// As lds_fill, from an address that is the same for the wave and 32 bits of its lanes' own.
+__device__ __forceinline__ void lds_fill_from(const char* from, uint32_t off, uint32_t base) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(from), "s"(base));
+}
+
 // The pieces of an operand that a thread brings to LDS.  Pieces past the end of the
 // summed dimension are zero, rows and columns past the product's end repeat the last
 // (their sums are not stored).
@@ -138,6 +143,11 @@ struct Loader {
     static constexpr int CH = VEC<T>;
     static constexpr int PER_ROW = ACROSS ? W * (int)sizeof(T) / 16 : STEP / 16;
     const T* ptr[COUNT];       // along: the row, at this piece; across: column of the piece, from row 0
+    // straight to LDS: bytes from where the tile begins, which is the same for the block and moves with the step, so
+    // that a step's addresses cost no vector instruction (they took a tenth of the issue slots otherwise)
+    uint32_t off[COUNT];
+    const char* begin;
+    size_t step;               // bytes from one step to the next
 
     __device__ __forceinline__ static int row_of(int i) { return (i * NT + (int)threadIdx.x) / PER_ROW; }
     __device__ __forceinline__ static int piece_of(int i) {
@@ -146,10 +156,12 @@ struct Loader {
     }
     __device__ __forceinline__ static int width(const Product& P) { return SIDE_B ? P.bw : P.aw; }
 
-    // first: the tile's first row or column of the operand
-    __device__ __forceinline__ void init(const Product& P, int first) {
+    // first: the tile's first row or column of the operand; lo: where its steps begin
+    __device__ __forceinline__ void init(const Product& P, int first, int lo) {
         const T* const base = (const T*)(SIDE_B ? P.b : P.a);
         const size_t ld = (size_t)(SIDE_B ? P.ldb : P.lda);
+        begin = (const char*)(ACROSS ? base + (size_t)lo * ld + first : base + (size_t)first * ld + lo);
+        step = ACROSS ? STEP / sizeof(T) * ld * sizeof(T) : STEP;
 #pragma unroll
         for (int i = 0; i < COUNT; ++i) {
             const int r = row_of(i), piece = piece_of(i) * CH;
@@ -157,10 +169,15 @@ struct Loader {
                 // gate and up rows alternately by 32
                 const int f = min(first + (r >> 6) * 32 + (r & 31), P.F - 1);
                 ptr[i] = base + (size_t)((r >> 5 & 1 ? P.F : 0) + f) * ld + piece;
+                off[i] = (uint32_t)((r >> 5 & 1 ? P.F : 0) + f - first) * (uint32_t)(ld * sizeof(T)) + piece * sizeof(T);
             } else if constexpr (!ACROSS) {
-                ptr[i] = base + (size_t)min(first + r, (SIDE_B ? P.N : P.M) - 1) * ld + piece;
+                const int row = min(first + r, (SIDE_B ? P.N : P.M) - 1);
+                ptr[i] = base + (size_t)row * ld + piece;
+                off[i] = (uint32_t)(row - first) * (uint32_t)(ld * sizeof(T)) + piece * sizeof(T);
             } else {
-                ptr[i] = base + min(first + piece, max(width(P) - CH, 0));
+                const int column = min(first + piece, max(width(P) - CH, 0));
+                ptr[i] = base + column;
+                off[i] = (uint32_t)r * (uint32_t)(ld * sizeof(T)) + (uint32_t)(column - first) * sizeof(T);
             }
         }
     }
@@ -183,14 +200,22 @@ struct Loader {
         }
     }
 
-    // pieces LO .. HI - 1 of the step from k0 on
+    // pieces LO .. HI - 1 of step t, which begins at k0 (at the end or before it)
     template <int LO = 0, int HI = COUNT>
-    __device__ __forceinline__ void fill(const Product& P, int k0, int end, uint32_t lds) const {
+    __device__ __forceinline__ void fill(const Product& P, int t, int k0, int end, uint32_t lds) const {
+        auto place = [&](int i) {
+            return __builtin_amdgcn_readfirstlane(lds + (uint32_t)(i * NT * 16) + ((threadIdx.x & ~63u) << 4));
+        };
+        if (k0 + STEP / (int)sizeof(T) <= end) {
+            const char* const from = begin + (size_t)t * step;
 #pragma unroll
-        for (int i = LO; i < HI; ++i) {
-            const T* p = at(P, i, k0, end);
-            const uint32_t base = lds + (uint32_t)(i * NT * 16) + ((threadIdx.x & ~63u) << 4);
-            lds_fill(p ? (const void*)p : (const void*)&g_zeros, __builtin_amdgcn_readfirstlane(base));
+            for (int i = LO; i < HI; ++i) lds_fill_from(from, off[i], place(i));
+        } else {
+#pragma unroll
+            for (int i = LO; i < HI; ++i) {
+                const T* p = at(P, i, k0, end);
+                lds_fill(p ? (const void*)p : (const void*)&g_zeros, place(i));
+            }
         }
     }
 
@@ -481,8 +506,8 @@ __device__ __forceinline__ void feed_tile(const Product& P, uint32_t block, cons
         Loader<T, MODE, true, TL::BN, TL::NB, TL::NT, TL::STEP> lb;
         using LA = decltype(la);
         using LB = decltype(lb);
-        la.init(P, mf);
-        lb.init(P, nf);
+        la.init(P, mf, lo);
+        lb.init(P, nf, lo);
         // Step t of the rows' operand lies at place t % AS, of the columns' at t % 2.
         // The columns' step t + 2 is sent as soon as its place is free, at the end of
         // step t; the rows' step t + 2 there too, or, with a third place, in two
@@ -496,11 +521,11 @@ __device__ __forceinline__ void feed_tile(const Product& P, uint32_t block, cons
         // where step t begins; past the end, from where nothing is read
         auto from = [&](int t) { return (int)min((int64_t)end, lo + (int64_t)t * BK); };
         auto send_a = [&](int t, int place) {
-            if constexpr (DMA) la.fill(P, from(t), end, lds_at + (uint32_t)place * TL::ABYTES);
+            if constexpr (DMA) la.fill(P, t, from(t), end, lds_at + (uint32_t)place * TL::ABYTES);
             else la.fetch(P, from(t), end, mf, ra);
         };
         auto send_b = [&](int t) {
-            if constexpr (DMA) lb.fill(P, from(t), end, lds_at + TL::AS * TL::ABYTES + (uint32_t)(t & 1) * TL::BBYTES);
+            if constexpr (DMA) lb.fill(P, t, from(t), end, lds_at + TL::AS * TL::ABYTES + (uint32_t)(t & 1) * TL::BBYTES);
             else lb.fetch(P, from(t), end, nf, rb);
         };
         auto put = [&](int t) {
@@ -548,8 +573,8 @@ __device__ __forceinline__ void feed_tile(const Product& P, uint32_t block, cons
                 if (ks + 1 < KS) {
                     if constexpr (HALVES) {
                         const uint32_t to = lds_at + (uint32_t)free * TL::ABYTES;
-                        if (ks == 0) la.template fill<0, TL::NA / 2>(P, from(t + 2), end, to);
-                        else if (ks == 1) la.template fill<TL::NA / 2, TL::NA>(P, from(t + 2), end, to);
+                        if (ks == 0) la.template fill<0, TL::NA / 2>(P, t + 2, from(t + 2), end, to);
+                        else if (ks == 1) la.template fill<TL::NA / 2, TL::NA>(P, t + 2, from(t + 2), end, to);
                     }
                     read(place, t, ks + 1);
                 } else {
@@ -1108,6 +1133,13 @@ constexpr int PART_BLOCKS = 512;      // blocks that keep the device busy
 constexpr int MOST_SPLITS = 64;
 constexpr int INT8_MOST = 131071;     // terms of 128 x 128 whose sum stays in 32 bits
 
+// Whether a tile's rows of an operand, `rows` of them ld apart, lie within 32 bits of where it begins.
+inline bool near_ok(int64_t rows, int64_t ld, int bytes) { return rows <= (1ll << 31) / (ld * bytes); }
+// Whether an operand's rows, of `width` values and ld apart, may go straight to LDS.
+inline bool straight_ok(const void* p, int64_t ld, int width, int bytes, int64_t rows = 256) {
+    return pieces_ok(p, ld, width, bytes) && near_ok(rows, ld, bytes);
+}
+
 // Whether large tiles make a product of M x K by K x N (its sums' columns) faster than small ones: they
 // fetch less, or take less apart (fp32), but there have to be enough of them, and a block of theirs has
 // its CU to itself, so that nothing covers its beginning and end unless K is long.  fp32, small and
@@ -1330,7 +1362,7 @@ int run_feed(const FeedSizes& z, int act, int dtype, const void* x, int64_t ldx,
     P.h32 = s.h32;
     const int b = z.bytes;
     if (z.few) run_few<T, IN, false>(P, stream);
-    else if (!run_tiles<T, IN>(P, z.large_in, pieces_ok(x, ldx, z.D, b) && pieces_ok(w_in, z.D, z.D, b), stream))
+    else if (!run_tiles<T, IN>(P, z.large_in, straight_ok(x, ldx, z.D, b) && straight_ok(w_in, z.D, z.D, b, (int64_t)z.F + 256), stream))
         return fail(-1, "yabt_feed_forward: bad sizes");
     Product Q = {};
     Q.b = w_out, Q.ldb = z.F;
@@ -1342,7 +1374,7 @@ int run_feed(const FeedSizes& z, int act, int dtype, const void* x, int64_t ldx,
         run_few<T, OUT, false>(Q, stream);
     } else {
         Q.splits = z.splits_out, Q.part = s.part;
-        if (!run_tiles<T, OUT>(Q, z.large_out, pieces_ok(w_out, z.F, z.F, b), stream))
+        if (!run_tiles<T, OUT>(Q, z.large_out, straight_ok(w_out, z.F, z.F, b) && near_ok(256, z.Fp, b), stream))
             return fail(-1, "yabt_feed_forward: bad sizes");
         if (Q.splits > 1) run_join({{{s.part, y, ldy, Q.M, Q.N, Q.splits, dtype, nullptr, nullptr}}, 1}, stream);
     }
@@ -1354,8 +1386,8 @@ int run_feed_grad(const FeedSizes& z, int act, int dtype, const void* dy, int64_
                   const void* w_in, const void* w_out, const FeedKept& kept, const GradSpace& s, void* dx, int64_t lddx,
                   void* dw_in, void* dw_out, hipStream_t stream) {
     const int b = z.bytes;
-    const bool dma = pieces_ok(x, ldx, z.D, b) && pieces_ok(dy, lddy, z.O, b) && pieces_ok(w_in, z.D, z.D, b) &&
-                     pieces_ok(w_out, z.F, z.F, b);
+    const bool dma = straight_ok(x, ldx, z.D, b) && straight_ok(dy, lddy, z.O, b) && straight_ok(w_in, z.D, z.D, b) &&
+                     straight_ok(w_out, z.F, z.F, b) && near_ok(256, 2 * (int64_t)z.Fp, b);
     Product P = {};
     P.a = dy, P.lda = lddy, P.b = w_out, P.ldb = z.F, P.bw = z.F;
     P.M = (int)z.n, P.N = z.F, P.K = z.O;
@@ -1435,7 +1467,7 @@ bool run_int8(const Int8Sizes& z, const int8_t* a, int64_t lda, const float* sa,
         return true;
     }
     P.splits = z.splits, P.part = part;
-    if (!run_tiles<int8_t, OUT8>(P, z.large, pieces_ok(a, lda, K, 1) && pieces_ok(b, ldb, K, 1), stream)) return false;
+    if (!run_tiles<int8_t, OUT8>(P, z.large, straight_ok(a, lda, K, 1) && straight_ok(b, ldb, K, 1), stream)) return false;
     if (P.splits > 1) run_join({{{part, y, ldy, P.M, N, P.splits, out_dtype, sa, sb}}, 1}, stream);
     return true;
 }
@@ -1600,7 +1632,7 @@ int yabt_feed_forward_int8(int dtype, int act, const void* x, int64_t ldx, int64
         run_quantize(dtype, x, ldx, n, D, s.q, dq, s.scale, on);
         P.a = s.q, P.lda = dq, P.sa = s.scale;
         if (few_rows(n)) run_few<int8_t, IN8, false>(P, on);
-        else if (!run_tiles<int8_t, IN8>(P, large_product(1, n, 2 * (int64_t)F, D), pieces_ok(s.q, dq, D, 1) && pieces_ok(w_in, D, D, 1), on))
+        else if (!run_tiles<int8_t, IN8>(P, large_product(1, n, 2 * (int64_t)F, D), straight_ok(s.q, dq, D, 1) && straight_ok(w_in, D, D, 1, (int64_t)F + 256), on))
             return fail(-1, "yabt_feed_forward_int8: bad sizes");
     }
     if (few_rows(n) && few_values(n, F)) {
