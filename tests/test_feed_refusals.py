@@ -44,6 +44,11 @@ def test_block_entries():
         assert sizes(1, 1000, 64, 32, 64) >= 1000 * 32 * 2
     assert lib.yabt_feed_forward_inner_bytes(0, 1000, 64, 33, 64) >= 1000 * 4 * (2 * 36 + 36)
     assert lib.yabt_feed_forward_int8_workspace_bytes(10, 0, 4, 4) == 0
+    # 2^31 rows' tiles of 64 x 128 have 2^33 threads
+    assert lib.yabt_feed_forward_workspace_bytes(0, (1 << 31) - 1000, 1, 1, 1) == 0
+    refused(call(n=(1 << 31) - 1000), "bad sizes")
+    refused(grad(F=1 << 24, D=1 << 24, ldx=1 << 24), "bad sizes")
+    refused(codes(n=(1 << 24) - 1, O=1 << 24, ldy=1 << 24), "bad sizes")
 
 
 def test_8_bit_entries():

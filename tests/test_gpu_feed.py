@@ -50,7 +50,8 @@ def check(args, act, got=None):
 # tiles; O other than D; a long sum with few tiles
 SIZES = [(1, 1, 1, 1), (2, 3, 1, 5), (16, 64, 32, 64), (17, 20, 7, 33), (33, 136, 72, 16), (64, 100, 61, 100),
          (65, 64, 64, 64), (66, 28, 65, 30), (130, 129, 130, 128), (257, 100, 60, 100), (129, 128, 256, 1),
-         (700, 50, 33, 40), (100, 40, 3000, 24), (1500, 16, 24, 8), (48, 200, 2050, 700), (20, 520, 2048, 1100)]
+         (700, 50, 33, 40), (100, 40, 3000, 24), (1500, 16, 24, 8), (48, 200, 2050, 700), (20, 520, 2048, 1100),
+         (200, 1024, 640, 520), (90, 520, 1040, 72)]
 
 
 @pytest.mark.parametrize("dt", TYPES, ids=name)

@@ -73,7 +73,7 @@ def want(a, sa, b, sb, dt):
 
 @pytest.mark.parametrize("dt", TYPES, ids=name)
 @pytest.mark.parametrize("n,K,N", [(1, 1, 1), (1, 300, 17), (15, 16, 33), (16, 128, 16), (17, 127, 40), (40, 500, 21), (64, 1000, 100),
-                                   (65, 64, 64), (100, 100, 130), (300, 257, 129), (129, 2048, 64), (70, 9000, 30)])
+                                   (65, 64, 64), (100, 100, 130), (300, 257, 129), (129, 2048, 64), (70, 9000, 30), (400, 1104, 8000)])
 def test_products(n, K, N, dt):
     gen = torch.Generator().manual_seed(K)
     a = torch.randint(-128, 128, (n, K), generator=gen, dtype=torch.int8)
@@ -138,7 +138,7 @@ def block(n, D, F, O, dt, seed):
 @pytest.mark.parametrize("dt", TYPES, ids=name)
 @pytest.mark.parametrize("n,D,F,O", [(1, 1, 1, 1), (1, 1000, 300, 40), (5, 33, 17, 20), (16, 1024, 64, 32), (17, 1025, 50, 64),
                                      (64, 256, 257, 30), (64, 250, 255, 30), (33, 100, 700, 100), (65, 64, 64, 64),
-                                     (130, 100, 61, 100), (300, 72, 400, 33), (70, 40, 5000, 16)])
+                                     (130, 100, 61, 100), (300, 72, 400, 33), (70, 40, 5000, 16), (100, 1040, 130, 50)])
 def test_block_in_8_bits(n, D, F, O, dt):
     act = ACTS[(n + D) % 4]
     print(f"feed8 n={n} D={D} F={F} O={O} {act} {name(dt)}", flush=True)

@@ -508,15 +508,15 @@ __device__ __forceinline__ void feed_tile(const Product& P, uint32_t block, cons
         using LB = decltype(lb);
         la.init(P, mf, lo);
         lb.init(P, nf, lo);
-        // Step t of the rows' operand lies at place t % AS, of the columns' at t % 2.
-        // The columns' step t + 2 is sent as soon as its place is free, at the end of
-        // step t; the rows' step t + 2 there too, or, with a third place, in two
-        // halves between the products of step t.  Steps past the last are sent too
-        // (zeros), so that every wait is the same.  Without DMA a step waits in
-        // registers for its place.
-        constexpr int AS = DMA ? TL::AS : 2;
-        constexpr bool HALVES = AS == 3;
-        static_assert(TL::BS == 2 && (AS == 2 || AS == 3), "places that the order of the steps is made for");
+        // Step t of the rows' operand lies at place t % AS, of the columns' at t % BS.  As
+        // many steps as there are places are under way; a place is sent its next step as
+        // soon as it is free, at the end of the step it held.  With one place more for the rows
+        // than for the columns (HALVES), theirs is sent in two halves between the products of
+        // step t.  Steps past the last are sent too (zeros), so that every wait is the same.
+        // Without DMA there are two places, and a step waits in registers for its own.
+        constexpr int AS = DMA ? TL::AS : 2, BS = DMA ? TL::BS : 2;
+        constexpr bool HALVES = AS == BS + 1;
+        static_assert(AS == BS || (AS == 3 && BS == 2), "places that the order of the steps is made for");
         u32x4 ra[DMA ? 1 : TL::NA], rb[DMA ? 1 : TL::NB];
         // where step t begins; past the end, from where nothing is read
         auto from = [&](int t) { return (int)min((int64_t)end, lo + (int64_t)t * BK); };
@@ -524,8 +524,8 @@ __device__ __forceinline__ void feed_tile(const Product& P, uint32_t block, cons
             if constexpr (DMA) la.fill(P, t, from(t), end, lds_at + (uint32_t)place * TL::ABYTES);
             else la.fetch(P, from(t), end, mf, ra);
         };
-        auto send_b = [&](int t) {
-            if constexpr (DMA) lb.fill(P, t, from(t), end, lds_at + TL::AS * TL::ABYTES + (uint32_t)(t & 1) * TL::BBYTES);
+        auto send_b = [&](int t, int place) {
+            if constexpr (DMA) lb.fill(P, t, from(t), end, lds_at + TL::AS * TL::ABYTES + (uint32_t)place * TL::BBYTES);
             else lb.fetch(P, from(t), end, nf, rb);
         };
         auto put = [&](int t) {
@@ -533,56 +533,56 @@ __device__ __forceinline__ void feed_tile(const Product& P, uint32_t block, cons
             LB::put(lds + TL::AS * TL::ABYTES + (t & 1) * TL::BBYTES, rb);
         };
         // accesses of every wave after step 0's and, in the loop, after the next step's
-        constexpr int AFTER_0 = DMA ? TL::NA + TL::NB : 0, AFTER = HALVES ? TL::NA : 0;
+        constexpr int AFTER_0 = DMA ? (BS - 1) * (TL::NA + TL::NB) : 0;
+        constexpr int AFTER = HALVES ? TL::NA : DMA ? (BS - 2) * (TL::NA + TL::NB) : 0;
+        static_assert(AFTER_0 < 63, "what a wait can count");
         if constexpr (DMA) {
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
+            for (int t = 0; t < BS; ++t) {
                 send_a(t, t);
-                send_b(t);
+                send_b(t, t);
             }
         } else {
             send_a(0, 0);
-            send_b(0);
+            send_b(0, 0);
             put(0);
             send_a(1, 0);
-            send_b(1);
+            send_b(1, 0);
         }
         const Frag<T, LA::ACROSS, TL::BM, TL::STEP> fa(wm * TL::MI * 32);
         const Frag<T, LB::ACROSS, TL::BN, TL::STEP> fb(wn * TL::NI * 32);
         u32x4 a[2][TL::MI], b[2][TL::NI];
-        auto read = [&](int place, int t, int ks) {
-            lds_char* const ta = lds + place * TL::ABYTES;
-            lds_char* const tb = lds + TL::AS * TL::ABYTES + (t & 1) * TL::BBYTES;
+        auto read = [&](int pa, int pb, int ks) {
+            lds_char* const ta = lds + pa * TL::ABYTES;
+            lds_char* const tb = lds + TL::AS * TL::ABYTES + pb * TL::BBYTES;
 #pragma unroll
             for (int i = 0; i < TL::MI; ++i) a[ks & 1][i] = fa.get(ta, i, ks);
 #pragma unroll
             for (int j = 0; j < TL::NI; ++j) b[ks & 1][j] = fb.get(tb, j, ks);
         };
-        constexpr int READS = TL::MI * decltype(fa)::READS + TL::NI * decltype(fb)::READS;
-        constexpr int PRODUCTS = TL::MI * TL::NI;
         stage_ready<AFTER_0>();
         read(0, 0, 0);
         // A k-step's operands are read while the one before is multiplied, the
         // next step's first ones too: the wait for it stands before the last
         // k-step's products, and what takes the freed places is sent there.
-        int place = 0;
+        int pa = 0, pb = 0;
         for (int t = 0; t < steps; ++t) {
-            const int next = place + 1 == AS ? 0 : place + 1, free = next + 1 == AS ? 0 : next + 1;
+            const int na = pa + 1 == AS ? 0 : pa + 1, nb = pb + 1 == BS ? 0 : pb + 1;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 if (ks + 1 < KS) {
                     if constexpr (HALVES) {
-                        const uint32_t to = lds_at + (uint32_t)free * TL::ABYTES;
+                        const uint32_t to = lds_at + (uint32_t)(na + 1 == AS ? 0 : na + 1) * TL::ABYTES;
                         if (ks == 0) la.template fill<0, TL::NA / 2>(P, t + 2, from(t + 2), end, to);
                         else if (ks == 1) la.template fill<TL::NA / 2, TL::NA>(P, t + 2, from(t + 2), end, to);
                     }
-                    read(place, t, ks + 1);
+                    read(pa, pb, ks + 1);
                 } else {
                     if constexpr (!DMA) put(t + 1);
                     stage_ready<AFTER>();
-                    send_b(t + 2);
-                    if constexpr (!HALVES) send_a(t + 2, place);
-                    read(next, t + 1, 0);
+                    send_b(t + BS, pb);
+                    if constexpr (!HALVES) send_a(t + AS, pa);
+                    read(na, nb, 0);
                 }
 #pragma unroll
                 for (int i = 0; i < TL::MI; ++i)
@@ -591,9 +591,9 @@ __device__ __forceinline__ void feed_tile(const Product& P, uint32_t block, cons
                         if constexpr (sizeof(T) == 1) acc[i][j] = mma8(a[ks & 1][i], b[ks & 1][j], acc[i][j]);
                         else acc[i][j] = mma<T>(a[ks & 1][i], b[ks & 1][j], acc[i][j]);
                     }
-                if constexpr (DMA) interleave<PRODUCTS, READS>();
             }
-            place = next;
+            pa = na;
+            pb = nb;
         }
         stage_ready<0>();                            // nothing may reach the LDS of a block that is gone
     }
@@ -1120,6 +1120,7 @@ __global__ void __launch_bounds__(FEW_NT) k_few(Product P) {
 // ---------------------------------------------------------------------------
 
 using TileSmall = TileOf<64, 128, 2, 2, 128, 2, 2>;
+using TileDeep = TileOf<64, 128, 2, 2, 128, 3, 3>;
 using TileLarge = TileOf<256, 256, 4, 2, 128, 3, 2>;
 using PartsSmall = TileParts<64, 128, 2, 2>;     // fp32
 using PartsLarge = TileParts<128, 256, 2, 4>;
@@ -1202,6 +1203,15 @@ bool run_tiles(const Product& P, bool large, bool dma, hipStream_t stream) {
         using TL = decltype(tl);
         Tiles g;
         if (!all_tiles<TL>(P, MODE == IN || MODE == IN8, &g) || !grid_ok(g.blocks, TL::NT)) return false;
+        // no more blocks than two a CU: three steps under way in each instead of two, which leaves room for
+        // two.  Two and three, us: 128 x 2048 -> 5632 -> 2048, bf16, 37.2 and 32.4; 534 x 1000 -> 760 26.9 and
+        // 23.5; steps too few to fill the places, 48 rows' y, 31.3 and 32.3.
+        if constexpr (std::is_same_v<TL, TileSmall> && decltype(d)::value) {
+            if (g.blocks <= 2 * CUS && (int64_t)P.K * (int)sizeof(T) / P.splits >= 8 * 128) {
+                k_feed<T, MODE, TileDeep, true><<<g.blocks, TileDeep::NT, TileDeep::LDS, stream>>>(P, g);
+                return true;
+            }
+        }
         k_feed<T, MODE, TL, decltype(d)::value><<<g.blocks, TL::NT, TL::LDS, stream>>>(P, g);
         return true;
     });
@@ -1317,6 +1327,26 @@ inline uint32_t beside_inner_grad(const FeedSizes& z, uint32_t dh, const Tiles (
     const double rounds = (double)over(dh, CUS), idle = rounds * CUS - dh;
     const double more = (rest * each - idle * each_dh) / CUS, longer = each - rounds * each_dh;
     return (more > 0 ? more : 0) + (longer > 0 ? longer : 0) < 0.9 * each ? rest : 0;
+}
+
+// A launch has fewer than 2^32 threads: whether those of the block's products have.
+inline bool tiles_fit(bool large, double tiles) { return tiles * (large ? 512 : 256) < 4e9; }
+inline double tiles_of(int bytes, bool large, double M, double N) {
+    return (double)tile_count(bytes, large, (int64_t)M, (int64_t)N);
+}
+inline bool feed_grids_ok(const FeedSizes& z) {
+    const int b = z.bytes;
+    const double dh = tiles_of(b, z.large_dh, z.n, z.F), x = tiles_of(b, z.large_grads, z.n, z.D) * z.splits[0],
+                 i = tiles_of(b, z.large_grads, (double)z.Fp + z.F, z.D) * z.splits[1],
+                 o = tiles_of(b, z.large_grads, z.O, z.F) * z.splits[2];
+    return tiles_fit(z.large_in, tiles_of(b, z.large_in, z.n, 2.0 * z.F)) &&
+           tiles_fit(z.large_out, tiles_of(b, z.large_out, z.n, z.O) * z.splits_out) && tiles_fit(z.large_dh, dh + o) &&
+           tiles_fit(z.large_grads, x + i + o);
+}
+inline bool feed_sizes_ok(int dtype, int64_t n, int D, int F, int O, FeedSizes* z) {
+    if (!dtype_ok(dtype) || !feed_ranges_ok(n, D, F, O)) return false;
+    *z = feed_sizes(dtype, n, D, F, O);
+    return feed_grids_ok(*z);
 }
 
 struct FeedKept {                     // what the forward pass keeps
@@ -1495,17 +1525,19 @@ using namespace yabt;
 extern "C" {
 
 size_t yabt_feed_forward_inner_bytes(int dtype, int64_t n, int D, int F, int O) {
-    if (!dtype_ok(dtype) || !feed_ranges_ok(n, D, F, O)) return 0;
+    FeedSizes z;
+    if (!feed_sizes_ok(dtype, n, D, F, O, &z)) return 0;
     Carve c{nullptr, 0};
     FeedKept k;
-    return carve_kept(c, &k, feed_sizes(dtype, n, D, F, O)) + 256;
+    return carve_kept(c, &k, z) + 256;
 }
 
 size_t yabt_feed_forward_workspace_bytes(int dtype, int64_t n, int D, int F, int O) {
-    if (!dtype_ok(dtype) || !feed_ranges_ok(n, D, F, O)) return 0;
+    FeedSizes z;
+    if (!feed_sizes_ok(dtype, n, D, F, O, &z)) return 0;
     Carve c{nullptr, 0};
     FeedSpace s;
-    return carve_forward(c, &s, feed_sizes(dtype, n, D, F, O)) + 256;
+    return carve_forward(c, &s, z) + 256;
 }
 
 int yabt_feed_forward(int dtype, int act, const void* x, int64_t ldx, int64_t n, int D, int F, int O, const void* w_in,
@@ -1513,12 +1545,12 @@ int yabt_feed_forward(int dtype, int act, const void* x, int64_t ldx, int64_t n,
                       yabt_stream_t stream) {
     if (!dtype_ok(dtype)) return fail(-1, "yabt_feed_forward: dtype is 0 (fp32), 1 (bf16) or 2 (fp16)");
     if (act < SILU || act > RELU) return fail(-1, "yabt_feed_forward: the activation is 0 to 3");
-    if (!feed_ranges_ok(n, D, F, O) || ldx < D || ldy < O) return fail(-1, "yabt_feed_forward: bad sizes");
+    FeedSizes z;
+    if (!feed_sizes_ok(dtype, n, D, F, O, &z) || ldx < D || ldy < O) return fail(-1, "yabt_feed_forward: bad sizes");
     if (n == 0) return 0;
     if (!x || !w_in || !w_out || !y) return fail(-1, "yabt_feed_forward: null pointer");
     if (!workspace || workspace_bytes < yabt_feed_forward_workspace_bytes(dtype, n, D, F, O))
         return fail(-2, "yabt_feed_forward: workspace too small");
-    const FeedSizes z = feed_sizes(dtype, n, D, F, O);
     FeedKept kept;
     if (out_inner) {
         Carve c{(char*)align_up((size_t)out_inner, 256), 0};
@@ -1534,10 +1566,11 @@ int yabt_feed_forward(int dtype, int act, const void* x, int64_t ldx, int64_t n,
 }
 
 size_t yabt_feed_forward_grad_workspace_bytes(int dtype, int64_t n, int D, int F, int O) {
-    if (!dtype_ok(dtype) || !feed_ranges_ok(n, D, F, O)) return 0;
+    FeedSizes z;
+    if (!feed_sizes_ok(dtype, n, D, F, O, &z)) return 0;
     Carve c{nullptr, 0};
     GradSpace s;
-    return carve_backward(c, &s, feed_sizes(dtype, n, D, F, O)) + 256;
+    return carve_backward(c, &s, z) + 256;
 }
 
 int yabt_feed_forward_grad(int dtype, int act, const void* dy, int64_t lddy, const void* x, int64_t ldx, int64_t n, int D,
@@ -1545,13 +1578,13 @@ int yabt_feed_forward_grad(int dtype, int act, const void* dy, int64_t lddy, con
                            size_t workspace_bytes, void* dx, int64_t lddx, void* dw_in, void* dw_out, yabt_stream_t stream) {
     if (!dtype_ok(dtype)) return fail(-1, "yabt_feed_forward_grad: dtype is 0 (fp32), 1 (bf16) or 2 (fp16)");
     if (act < SILU || act > RELU) return fail(-1, "yabt_feed_forward_grad: the activation is 0 to 3");
-    if (!feed_ranges_ok(n, D, F, O) || ldx < D || lddy < O || lddx < D)
+    FeedSizes z;
+    if (!feed_sizes_ok(dtype, n, D, F, O, &z) || ldx < D || lddy < O || lddx < D)
         return fail(-1, "yabt_feed_forward_grad: bad sizes");
     if (!w_in || !w_out || !dw_in || !dw_out || (n > 0 && (!x || !dy || !inner || !dx)))
         return fail(-1, "yabt_feed_forward_grad: null pointer");
     if (!workspace || workspace_bytes < yabt_feed_forward_grad_workspace_bytes(dtype, n, D, F, O))
         return fail(-2, "yabt_feed_forward_grad: workspace too small");
-    const FeedSizes z = feed_sizes(dtype, n, D, F, O);
     FeedKept kept;
     Carve k{(char*)align_up((size_t)inner, 256), 0};
     carve_kept(k, &kept, z);
@@ -1575,7 +1608,14 @@ int yabt_quantize_rows(int dtype, const void* x, int64_t ldx, int64_t n, int D, 
 }
 
 static bool int8_ranges_ok(int64_t n, int K, int N) {
-    return n >= 0 && n < (1 << 24) && K >= 1 && K <= INT8_MOST && N >= 1 && N <= (1 << 24);
+    if (!(n >= 0 && n < (1 << 24) && K >= 1 && K <= INT8_MOST && N >= 1 && N <= (1 << 24))) return false;
+    const Int8Sizes z = int8_sizes(n, N, K);
+    return tiles_fit(z.large, tiles_of(1, z.large, n, N) * z.splits);
+}
+static bool feed8_ranges_ok(int64_t n, int D, int F, int O) {
+    if (!int8_ranges_ok(n, F, O) || D < 1 || D > INT8_MOST || F < 1 || F > INT8_MOST) return false;
+    const bool large = large_product(1, n, 2 * (int64_t)F, D);
+    return tiles_fit(large, tiles_of(1, large, n, 2.0 * F));
 }
 
 size_t yabt_product_int8_workspace_bytes(int64_t n, int K, int N) {
@@ -1600,7 +1640,7 @@ int yabt_product_int8(const int8_t* a, int64_t lda, const float* a_scale, int64_
 }
 
 size_t yabt_feed_forward_int8_workspace_bytes(int64_t n, int D, int F, int O) {
-    if (!int8_ranges_ok(n, D, O) || !int8_ranges_ok(n, F, O)) return 0;
+    if (!feed8_ranges_ok(n, D, F, O)) return 0;
     Carve c{nullptr, 0};
     Feed8Space s;
     return carve_feed8(c, &s, n, D, F, O) + 256;
@@ -1611,7 +1651,7 @@ int yabt_feed_forward_int8(int dtype, int act, const void* x, int64_t ldx, int64
                            size_t workspace_bytes, void* y, int64_t ldy, yabt_stream_t stream) {
     if (!dtype_ok(dtype)) return fail(-1, "yabt_feed_forward_int8: dtype is 0 (fp32), 1 (bf16) or 2 (fp16)");
     if (act < SILU || act > RELU) return fail(-1, "yabt_feed_forward_int8: the activation is 0 to 3");
-    if (!int8_ranges_ok(n, D, O) || !int8_ranges_ok(n, F, O) || ldx < D || ldy < O)
+    if (!feed8_ranges_ok(n, D, F, O) || ldx < D || ldy < O)
         return fail(-1, "yabt_feed_forward_int8: bad sizes");
     if (n == 0) return 0;
     if (!x || !w_in || !in_scale || !w_out || !out_scale || !y) return fail(-1, "yabt_feed_forward_int8: null pointer");

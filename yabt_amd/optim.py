@@ -14,6 +14,7 @@ graph.
 from __future__ import annotations
 
 from array import array
+from contextlib import nullcontext
 from dataclasses import dataclass
 from itertools import chain
 from operator import attrgetter
@@ -173,7 +174,9 @@ def adamw_step(params: list[torch.Tensor], grads: list[torch.Tensor | None], sta
         number = int(step)
         if not 1 <= number < 2 ** 31:
             raise ValueError(f"steps are counted from 1 to 2^31 - 1, got {step}")
-        if torch.cuda.is_current_stream_capturing():
+        with torch.cuda.device(dev) if torch._C._cuda_getDevice() != dev.index else nullcontext():
+            capturing = torch.cuda.is_current_stream_capturing()
+        if capturing:
             raise RuntimeError("a captured step would keep its number: pass step as an int32 device tensor")
     if list(map(_SHAPE, params)) != list(map(_SHAPE, grads)):
         raise ValueError(f"gradients must have their parameters' shapes, got {[tuple(g.shape) for g in grads]} for "
