@@ -472,7 +472,7 @@ __device__ __forceinline__ void feed_tile(const Product& P, uint32_t block, cons
     constexpr bool GATED = MODE == IN || MODE == IN8;
     lds_char* const lds = (lds_char*)s_tiles;
     const uint32_t lds_at = (uint32_t)(uintptr_t)lds;
-    const int wave = threadIdx.x / 64, lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x & 63;
     const int wm = wave / TL::WN, wn = wave % TL::WN;
 
     // column tiles together with a group of row tiles, on one die
@@ -600,11 +600,103 @@ __device__ __forceinline__ void feed_tile(const Product& P, uint32_t block, cons
 
     // The sums go through LDS, 32 rows of a wave at a time, from the matrix
     // cores' layout (a lane has one column) to four neighbouring columns a lane,
-    // so that what is read and written beside them goes in whole lines.
+    // so that what is read and written beside them goes in whole lines.  Of a tile that
+    // lies inside the product nothing is checked.
     constexpr int W = TL::NI * 32;
     lds_float* const mine = (lds_float*)(lds + wave * 32 * W * 4);
     constexpr int LANES = GATED ? W / 8 : W / 4, PASS = 64 / LANES;    // lanes a row, rows at once
-    const int c4 = lane % LANES * 4;
+    const int c4 = lane % LANES * 4, first = nf + wn * (GATED ? W / 2 : W);   // this lane's columns: first + c4 .. + 3
+    const int width = GATED || MODE == DH ? P.Fp : P.N;
+    const bool inside = mf + TL::BM <= P.M && nf + (GATED ? TL::BN / 2 : TL::BN) <= P.N && (P.F == P.Fp || !(GATED || MODE == DH || MODE == DWIN));
+    f32x4 scale[2];                   // of 8-bit products: the columns'
+    if constexpr (MODE == IN8 || MODE == OUT8) {
+        if (first + c4 < P.N) {
+            scale[0] = four_of(P.sb + first + c4, P.N - (first + c4));
+            if constexpr (MODE == IN8) scale[1] = four_of(P.sb + P.F + first + c4, P.F - (first + c4));
+        }
+    }
+    // where the rows of block i begin in an array of this pitch, and this lane's bytes from there
+    auto row0 = [&](auto* base, int i, int p, int64_t pitch) {
+        return base + (size_t)(mf + (wm * TL::MI + i) * 32 + p) * (size_t)pitch + first;
+    };
+    auto lane_at = [&](int64_t pitch) { return (uint32_t)(lane / LANES) * (uint32_t)pitch + (uint32_t)c4; };
+    const uint32_t at_h = lane_at(P.Fp), at_pre = lane_at(2 * (int64_t)P.Fi), at_dpre = lane_at(2 * (int64_t)P.Fp),
+                   at_h32 = lane_at(P.Fi), at_out = lane_at(P.splits > 1 ? P.N : 0);
+    auto rows = [&](auto whole_tile, int i) {
+        constexpr bool WHOLE = decltype(whole_tile)::value;
+        const int f = first + c4;
+#pragma unroll 4
+        for (int p = 0; p < 32; p += PASS) {
+            const int at = p + lane / LANES, m = mf + (wm * TL::MI + i) * 32 + at;
+            if (!WHOLE && !(m < P.M && f < width)) continue;
+            auto bits = [&](int c) { return *(const lds_f32x4*)(mine + at * W + (c ^ ((at & 4) << 3))); };
+            auto whole = [&](int c) {
+                const i32x4 v = __builtin_bit_cast(i32x4, bits(c));
+                return f32x4{(float)v[0], (float)v[1], (float)v[2], (float)v[3]};
+            };
+            auto is = [&](int q) { return WHOLE || f + q < P.F; };
+            if constexpr (GATED) {
+                // columns 64 q + 0..31: gate of f 32 q + 0..31, the next 32: u
+                const int c = (c4 & ~31) * 2 + (c4 & 31);
+                f32x4 g, u;
+                if constexpr (MODE == IN8) {
+                    const float s = P.sa[m];
+                    g = whole(c) * scale[0] * s;
+                    u = whole(c + 32) * scale[1] * s;
+                } else {
+                    g = bits(c);
+                    u = bits(c + 32);
+                }
+                float v[4], slope[4], h[4];
+                activate<T>(P.act, g, v, slope);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) h[q] = is(q) ? v[q] * u[q] : 0.0f;
+                if constexpr (MODE == IN8) {
+                    if (WHOLE || f < P.Fi) *(f32x4*)(row0(P.h32, i, p, P.Fi) + at_h32) = f32x4{h[0], h[1], h[2], h[3]};
+                } else {
+                    store4(row0((T*)P.h, i, p, P.Fp) + at_h, h);
+                    if (P.pre && (WHOLE || f < P.Fi)) {
+                        float* const pre = row0(P.pre, i, p, 2 * (int64_t)P.Fi);
+                        *(f32x4*)(pre + at_pre) = g;
+                        *(f32x4*)(pre + P.Fi + at_pre) = u;
+                    }
+                }
+            } else if constexpr (MODE == DH) {
+                f32x4 g = {0.0f, 0.0f, 0.0f, 0.0f}, u = g;
+                if (WHOLE || f < P.Fi) {
+                    const float* const pre = row0(P.pre, i, p, 2 * (int64_t)P.Fi);
+                    g = *(const f32x4*)(pre + at_pre);
+                    u = *(const f32x4*)(pre + P.Fi + at_pre);
+                }
+                const f32x4 dh = bits(c4);
+                float v[4], slope[4], dg[4], du[4];
+                activate<T>(P.act, g, v, slope);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    dg[q] = is(q) ? dh[q] * u[q] * slope[q] : 0.0f;
+                    du[q] = is(q) ? dh[q] * v[q] : 0.0f;
+                }
+                T* const dpre = row0((T*)P.dpre, i, p, 2 * (int64_t)P.Fp);
+                store4(dpre + at_dpre, dg);
+                store4(dpre + P.Fp + at_dpre, du);
+            } else {
+                const int M = MODE == DWIN ? 2 * P.F : P.M;
+                if (WHOLE && P.splits > 1) {
+                    store_part(row0(P.part + (size_t)split * M * (size_t)P.N, i, p, P.N) + at_out, bits(c4), 4);
+                    continue;
+                }
+                const int row = out_row<MODE>(P, m), have = WHOLE ? 4 : P.N - f;
+                if (!WHOLE && row >= M) continue;
+                if (P.splits > 1) {
+                    store_part(P.part + ((size_t)split * M + row) * (size_t)P.N + f, bits(c4), have);
+                } else if constexpr (MODE == OUT8) {
+                    store_as(P.out_dtype, P.out, (size_t)row * (size_t)P.ldo + f, whole(c4) * scale[0] * P.sa[row], have);
+                } else {
+                    store_part((T*)P.out + (size_t)row * (size_t)P.ldo + f, bits(c4), have);
+                }
+            }
+        }
+    };
 #pragma unroll
     for (int i = 0; i < TL::MI; ++i) {
         wave_sync_lds();
@@ -619,79 +711,8 @@ __device__ __forceinline__ void feed_tile(const Product& P, uint32_t block, cons
                     __builtin_bit_cast(float, s);
             }
         wave_sync_lds();
-#pragma unroll 4
-        for (int p = 0; p < 32; p += PASS) {
-            const int at = p + lane / LANES, m = mf + (wm * TL::MI + i) * 32 + at;
-            auto bits = [&](int c) { return *(const lds_f32x4*)(mine + at * W + (c ^ ((at & 4) << 3))); };
-            auto whole = [&](int c) {
-                const i32x4 v = __builtin_bit_cast(i32x4, bits(c));
-                return f32x4{(float)v[0], (float)v[1], (float)v[2], (float)v[3]};
-            };
-            if constexpr (GATED) {
-                // columns 64 q + 0..31: gate of f 32 q + 0..31, the next 32: u
-                const int f = nf + wn * (W / 2) + c4, c = (c4 & ~31) * 2 + (c4 & 31);
-                if (m < P.M && f < P.Fp) {
-                    f32x4 g, u;
-                    if constexpr (MODE == IN8) {
-                        const float s = P.sa[m];
-                        g = whole(c) * four_of(P.sb + f, P.F - f) * s;
-                        u = whole(c + 32) * four_of(P.sb + P.F + f, P.F - f) * s;
-                    } else {
-                        g = bits(c);
-                        u = bits(c + 32);
-                    }
-                    float v[4], slope[4], h[4];
-                    activate<T>(P.act, g, v, slope);
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) h[q] = f + q < P.F ? v[q] * u[q] : 0.0f;
-                    if constexpr (MODE == IN8) {
-                        if (f < P.Fi) *(f32x4*)(P.h32 + (size_t)m * (size_t)P.Fi + f) = f32x4{h[0], h[1], h[2], h[3]};
-                    } else {
-                        store4((T*)P.h + (size_t)m * (size_t)P.Fp + f, h);
-                        if (P.pre && f < P.Fi) {
-                            float* pre = P.pre + (size_t)m * 2 * (size_t)P.Fi + f;
-                            *(f32x4*)pre = g;
-                            *(f32x4*)(pre + P.Fi) = u;
-                        }
-                    }
-                }
-            } else if constexpr (MODE == DH) {
-                const int f = nf + wn * W + c4;
-                if (m < P.M && f < P.Fp) {
-                    f32x4 g = {0.0f, 0.0f, 0.0f, 0.0f}, u = g;
-                    if (f < P.Fi) {
-                        const float* pre = P.pre + (size_t)m * 2 * (size_t)P.Fi + f;
-                        g = *(const f32x4*)pre;
-                        u = *(const f32x4*)(pre + P.Fi);
-                    }
-                    const f32x4 dh = bits(c4);
-                    float v[4], slope[4], dg[4], du[4];
-                    activate<T>(P.act, g, v, slope);
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const bool is = f + q < P.F;
-                        dg[q] = is ? dh[q] * u[q] * slope[q] : 0.0f;
-                        du[q] = is ? dh[q] * v[q] : 0.0f;
-                    }
-                    T* dpre = (T*)P.dpre + (size_t)m * 2 * (size_t)P.Fp + f;
-                    store4(dpre, dg);
-                    store4(dpre + P.Fp, du);
-                }
-            } else {
-                const int row = out_row<MODE>(P, m), c = nf + wn * W + c4;
-                const int M = MODE == DWIN ? 2 * P.F : P.M;
-                if (row < M && c < P.N) {
-                    if (P.splits > 1) {
-                        store_part(P.part + ((size_t)split * M + row) * (size_t)P.N + c, bits(c4), P.N - c);
-                    } else if constexpr (MODE == OUT8) {
-                        store_as(P.out_dtype, P.out, (size_t)row * (size_t)P.ldo + c,
-                                 whole(c4) * four_of(P.sb + c, P.N - c) * P.sa[row], P.N - c);
-                    } else {
-                        store_part((T*)P.out + (size_t)row * (size_t)P.ldo + c, bits(c4), P.N - c);
-                    }
-                }
-            }
-        }
+        if (inside) rows(std::true_type(), i);
+        else rows(std::false_type(), i);
     }
 }
 
