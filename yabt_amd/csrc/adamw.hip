@@ -15,7 +15,9 @@
 // The update is made with the new moments before they are rounded.
 //
 // Bound by its bytes: 28 a value (26 with 16-bit gradients), 16 (14) with 8-bit
-// moments.  A wave takes blocks of 256 values, four a lane, so that a block's largest
+// moments: 40M fp32 values with bf16 gradients 196 us, 5.3 TB/s, a copy's rate; 120M with
+// 8-bit moments 356 us, 4.7 TB/s (three square roots and a quotient a value beside the bytes),
+// the values they stand for 215 us, 5.6 TB/s.  A wave takes blocks of 256 values, four a lane, so that a block's largest
 // needs no LDS; a thread block takes 4096 of one tensor, which it finds by one ballot
 // over the tensors' first blocks, passed by value: one launch for up to 48 tensors, and
 // nothing to copy to the device first.

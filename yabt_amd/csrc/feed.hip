@@ -21,6 +21,15 @@
 // are read with the transposing LDS loads.  Few rows have kernels of their own,
 // which are bound by the weights' bytes.
 //
+// 8192 x 2048 -> 5632 -> 2048, bf16, forward and backward: h with g and u kept 366 us (378 GFLOP), y
+// 150 (189), the inner gradient 284 (189), the three others 722 (945): 1030, 1260, 670 and 1310
+// TFLOP/s, the matrix cores at work 54, 74, 37 and 74% of the time; the library's plain products of
+// these sizes reach 980 to 1510.  What is between them: a block has its CU to itself, so that the end of
+// a tile, where all CUs read and write at once (h with g and u 0.46 GB, the inner gradient 0.55 GB), is
+// not covered, and neither is its first step; and h has 5.5 rounds of 256 tiles.
+// 8192 x 4096 x 4096 in 8 bits: 133 us, 2070 TOP/s (the library's reaches 2110 at 8192 x 8192 x 8192).
+// 4096 x 2048 -> 4096 -> 2048, fp32: 1020 us, 202 TFLOP/s (the library's fp32 product: 153).
+//
 // 16-bit types: h, dg and du are rounded to the inputs' type, as the matrix cores
 // take them (for 16 rows or fewer, whose time is the weights', h is taken in two parts and
 // keeps 16 bits); g and u are kept in fp32 for the backward pass.  So an output has
@@ -74,8 +83,8 @@ __device__ __forceinline__ i32x4 mma8(u32x4 a, u32x4 b, i32x4 c) {
 // The activation of four gates and its derivative.  16 bits: the hardware's exp2 and
 // reciprocal (gate_sigmoid), and for the normal distribution function the approximation
 // 7.1.26 of Abramowitz and Stegun's handbook, off by 7.5e-8 at most.  8 bits too: an h that is
-// off by 2^-20 of itself has another code once in 10^4 times or less; the accurate ones take
-// 12 of 466 us of 16 384 x 2048 -> 5632.  fp32: the accurate functions.
+// off by 2^-20 of itself has another code once in 4000 times at most, and the accurate ones made
+// h of 16 384 x 2048 -> 5632 take 466 us instead of 415.  fp32: the accurate functions.
 template <typename T>
 __device__ __forceinline__ float gate_normal(float g) {
     const float x = fabsf(g) * 0.70710678f;
@@ -144,7 +153,8 @@ struct Loader {
     static constexpr int PER_ROW = ACROSS ? W * (int)sizeof(T) / 16 : STEP / 16;
     const T* ptr[COUNT];       // along: the row, at this piece; across: column of the piece, from row 0
     // straight to LDS: bytes from where the tile begins, which is the same for the block and moves with the step, so
-    // that a step's addresses cost no vector instruction (they took a tenth of the issue slots otherwise)
+    // that a step's addresses cost no vector instruction (8192 x 2048, 5632, forward and backward: 1493 us, and
+    // 1609 with 64-bit addresses a lane)
     uint32_t off[COUNT];
     const char* begin;
     size_t step;               // bytes from one step to the next
@@ -833,8 +843,9 @@ __device__ __forceinline__ void chunk_codes(const Chunk<T>& c, float unit, int8_
     }
 }
 
-// A row by LANES threads of a block (64: a wave, four rows a block; 256: the block), CHUNKS
-// pieces of 16 bytes a thread in registers; what does not fit there is read again.
+// A row by LANES threads of a block (64: a wave, four rows a block; 256: the block), QUANT_CHUNKS
+// pieces of 16 bytes a thread in registers; what does not fit there is read again.  Bound by its
+// bytes: 16 384 x 5632 of fp32 86 us, 5.4 TB/s; 8192 x 4096 of bf16 19.3 us, 5.2 TB/s.
 constexpr int QUANT_CHUNKS = 4;
 template <typename T, int LANES>
 __global__ void __launch_bounds__(256) k_quantize(const T* x, int64_t ldx, int64_t n, int D, int8_t* q, int64_t ldq, float* scale) {
@@ -889,6 +900,9 @@ __global__ void __launch_bounds__(256) k_quantize(const T* x, int64_t ldx, int64
 // operands: a lane fetches 32 bytes in a row of one weight row, two instructions' worth, 16
 // weight rows and 16 rows of x a wave.  A block has 16 columns (IN: of h) and its
 // waves share the summed dimension, 128 bytes a row in turn; their sums meet in LDS.
+// One row, bf16, 1024 -> 4096 -> 1024: 5.7 and 6.9 us for 17 and 8 MB, mostly launch and one round
+// trip of loads; 2048 -> 5632 -> 2048: 22 us together for 69 MB.  From 16 rows on x, which every
+// block reads again, costs as much as the weights.
 // ---------------------------------------------------------------------------
 
 constexpr int FEW_ROWS = 64;                     // rows of a call, up to four groups of 16
@@ -1140,6 +1154,8 @@ __global__ void __launch_bounds__(FEW_NT) k_few(Product P) {
 // host
 // ---------------------------------------------------------------------------
 
+// 16384 x 2048 -> 5632 -> 2048 in 8 bits, us: 256 x 256 700, 128 x 256 (one block a CU, eight waves) 852, 128 x 128 (two
+// blocks) 826; 8192 x 4096 x 4096 158, 197 and 191.
 using TileSmall = TileOf<64, 128, 2, 2, 128, 2, 2>;
 using TileDeep = TileOf<64, 128, 2, 2, 128, 3, 3>;
 using TileLarge = TileOf<256, 256, 4, 2, 128, 3, 2>;
@@ -1344,7 +1360,8 @@ inline FeedSizes feed_sizes(int dtype, int64_t n, int D, int F, int O) {
 inline uint32_t beside_inner_grad(const FeedSizes& z, uint32_t dh, const Tiles (&g)[3]) {
     const uint32_t rest = (g[0].count + g[1].count + g[2].count) % CUS;
     if (!z.large_grads || rest == 0 || rest > g[2].count) return 0;
-    const double each = (double)z.n * z.bytes / 128 / z.splits[2], each_dh = (double)z.O * z.bytes / 128 + 22;   // steps; dh's end takes as long as 22
+    // in steps; the end of dh's tiles, which read g and u and write dg and du, takes as long as 22
+    const double each = (double)z.n * z.bytes / 128 / z.splits[2], each_dh = (double)z.O * z.bytes / 128 + 22;
     const double rounds = (double)over(dh, CUS), idle = rounds * CUS - dh;
     const double more = (rest * each - idle * each_dh) / CUS, longer = each - rounds * each_dh;
     return (more > 0 ? more : 0) + (longer > 0 ? longer : 0) < 0.9 * each ? rest : 0;
