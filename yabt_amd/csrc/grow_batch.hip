@@ -106,7 +106,7 @@ struct State {
     int32_t n_pend;                      // Pend entries used
     int32_t round;                       // controllers run
     uint32_t scan_ticket;                // splits whose scan blocks have all finished
-    int32_t pad;
+    int32_t scan_word;                   // (round << 8) | n_round, the scan launch's exit test (k_scan)
     int32_t root_pend;                   // the root's computed split, -1: none
     float root_gain;                     // the root's table gain
     int32_t round_pend[KMAX];            // this round's Pend entries
@@ -211,6 +211,7 @@ __global__ void k_setup_finish(Args A) {
     st->n_round = 0;
     st->n_pend = 0;
     st->round = 0;
+    st->scan_word = 0;
     st->scan_ticket = 0;
     for (int i = 0; i < KMAX; ++i) st->split_ticket[i] = 0;
     st->root_pend = -1;
@@ -1035,6 +1036,7 @@ __device__ __forceinline__ void control(const Args& A, Table& T, int nn, int na,
         st->n_round = done ? 0 : j;
         const int r = st->round + 1;
         st->round = r;
+        st->scan_word = (r << 8) | (done ? 0 : j);
         // the host's view: round and done in one store
         volatile Flags* fl = A.flags;
         fl->word = ((r + 1) << 1) | done;
@@ -1078,8 +1080,14 @@ constexpr size_t SCAN_XCHG_BYTES = (size_t)(CT / WAVE) * 12 * WAVE * sizeof(int6
 // scans both children of the round's split y (wave w: feature w % SCAN_FEATS,
 // child w / SCAN_FEATS).  Each block publishes its best record per child;
 // the last block to take a ticket is the controller.
+// The blocks of y at or past the round's count take no ticket, so the
+// controller does not wait for them: on a device busy with other streams one
+// may start after the controller has planned the next, larger round.  The
+// launch is therefore told its round (`round`), and the round and its count
+// are read as one word: a late block finds either this round's word, whose
+// count it is past, or the next round's, which is not its own.
 template <bool ROOT>
-__global__ void __launch_bounds__(ROOT ? SCAN_FEATS * WAVE : CT) k_scan(Args A) {
+__global__ void __launch_bounds__(ROOT ? SCAN_FEATS * WAVE : CT) k_scan(Args A, int round) {
     constexpr int NT = ROOT ? SCAN_FEATS * WAVE : CT;
     constexpr int NC = ROOT ? 1 : 2;
     State* st = A.st;
@@ -1088,12 +1096,14 @@ __global__ void __launch_bounds__(ROOT ? SCAN_FEATS * WAVE : CT) k_scan(Args A) 
     // the words of State this block needs, loaded before the exit test (y <
     // KMAX indexes them all): the split's Pend index and its gather pieces'
     // range do not wait for the test
-    const int32_t done = st->done, nr = ROOT ? 1 : st->n_round;
+    const int32_t done = st->done, word = ROOT ? 0 : st->scan_word;
+    const int nr = ROOT ? 1 : word & 255;
+    const bool idle = !ROOT && ((word >> 8) != round || y >= nr);
     const int pidx = ROOT ? 0 : st->round_pend[y];
     const int u0 = ROOT ? 0 : st->unit_off[y], u1 = ROOT ? 0 : st->unit_off[y + 1];
     // one test over all of them (none is negative in a live round), so that
     // they are loaded together rather than after the branch
-    if ((done != 0) | (y >= nr) | ((pidx | u0 | u1) < 0)) return;
+    if ((done != 0) | idle | ((pidx | u0 | u1) < 0)) return;
     // the start of the controller's table, loaded by every block together
     // with its bins (whichever block finishes last is the controller and
     // holds it in registers by then): leaf t and computed split t (a
@@ -1576,7 +1586,7 @@ int yabt_grow_batched(const uint8_t* bins_fm, int64_t ld_fm, const uint8_t* bins
                      &A.st->done);
     const int scan_grid = (F + SCAN_FEATS - 1) / SCAN_FEATS;
     const size_t table_lds = table_carve(nullptr, max_leaves, A.pend_cap, nullptr);
-    k_scan<true><<<scan_grid, SCAN_FEATS * WAVE, table_lds, stream>>>(A);
+    k_scan<true><<<scan_grid, SCAN_FEATS * WAVE, table_lds, stream>>>(A, 0);
     const size_t scan_lds = table_lds > SCAN_XCHG_BYTES ? table_lds : SCAN_XCHG_BYTES;
     int lrc = launch_status("yabt_grow_batched launch");
     if (lrc) return lrc;
@@ -1604,7 +1614,7 @@ int yabt_grow_batched(const uint8_t* bins_fm, int64_t ld_fm, const uint8_t* bins
         k_part<<<PART_BLOCKS, SB, 0, stream>>>(bins_fm, ld_fm, n, A.st, A.pend);
         k_gather<<<tiles * gather_units(tiles), HBLOCK, 0, stream>>>(bins_rm, ld_rm, grad, hess, A.gh, F, A.q, A.dflt,
                                                                          A.st, A.pend, A.pieces);
-        k_scan<false><<<dim3(scan_grid, KMAX), CT, scan_lds, stream>>>(A);
+        k_scan<false><<<dim3(scan_grid, KMAX), CT, scan_lds, stream>>>(A, r);
         if ((lrc = launch_status("yabt_grow_batched launch"))) return lrc;
     }
     if (out_leaf_of_row && n > 0) {
