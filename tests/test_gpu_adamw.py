@@ -297,3 +297,21 @@ def test_a_parameter_that_requires_a_gradient():
     with torch.no_grad():
         optim.adamw_step([p], [torch.ones(10, device="cuda")], s, 1)
     assert p._version > before and bool((p < 1.0).all())
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_moment_twice_is_refused(bits):
+    p = [torch.ones(300, device="cuda"), torch.ones(300, device="cuda"), torch.ones(0, device="cuda"),
+         torch.ones(0, device="cuda")]
+    g = [torch.ones_like(t) for t in p]
+    s = optim.adamw_state(p, bits)
+    optim.adamw_step(p, g, s, 1)                      # two empty tensors are not one twice
+    moved = [t.clone() for t in p]
+    names = ["first", "second"] + ["first_scale", "second_scale"] * (bits == 8)
+    for name in names:
+        part = getattr(s, name)
+        kept, part[1] = part[1], part[0]
+        with pytest.raises(ValueError, match="twice"):
+            optim.adamw_step(p, g, s, 2)
+        part[1] = kept
+    assert all(torch.equal(a, b) for a, b in zip(p, moved))

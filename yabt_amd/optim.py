@@ -192,11 +192,14 @@ def adamw_step(params: list[torch.Tensor], grads: list[torch.Tensor | None], sta
     except KeyError as e:
         raise ValueError(f"parameters and gradients must be float32, bfloat16 or float16, got {e.args[0]}") from None
     where = list(map(_pointer, params))
-    filled = [p for p, n in zip(where, sizes) if n]
-    if len(set(filled)) < len(filled):
-        raise ValueError("a parameter is in the list twice")
     none = [0] * len(params)
     first, second, *scales = (list(map(_pointer, part)) for part in lists)
+    written = [where, first, second, *scales]
+    if len(set(chain.from_iterable(written))) < len(written) * len(sizes):
+        # empty tensors have one address, null
+        written = [at for part in written for at, n in zip(part, sizes) if n]
+        if len(set(written)) < len(written):
+            raise ValueError("a parameter or a moment is in the lists twice")
     table = _table(zip(where, map(_pointer, grads), first, second, *(scales or (none, none)), sizes, types))
     expert_ops._call("yabt_adamw_step", dev, len(params), table.buffer_info()[0], state.bits, number, at, float(lr), float(b1),
                      float(b2), float(eps), float(weight_decay))
