@@ -649,7 +649,8 @@ int yabt_feed_forward(int dtype, int act, const void *x, int64_t ldx, int64_t n,
 
 /* Its gradients from dy (n, O) and the forward pass's inner: dx (n, D), dw_in
  * (2 F, D), dw_out (O, F), all of `dtype`.  The inner gradients are rounded to
- * `dtype`, in fp16 with its range.  n = 0 gives zeros for the weights. */
+ * `dtype`, in fp16 with its range.  inner, if it was moved, begins as far from a multiple
+ * of 256 bytes as it did.  n = 0 gives zeros for the weights. */
 size_t yabt_feed_forward_grad_workspace_bytes(int dtype, int64_t n, int D, int F, int O);
 int yabt_feed_forward_grad(int dtype, int act, const void *dy, int64_t lddy, const void *x, int64_t ldx,
                            int64_t n, int D, int F, int O, const void *w_in, const void *w_out,

@@ -193,3 +193,33 @@ def test_half_beyond_its_range():
         y = X.feed_forward(x, w_in, w_out, activation="relu")
         keep = torch.arange(n, device="cuda") != 2
         assert bool(torch.isfinite(y[keep]).all()) and not bool(torch.isfinite(y[2]).all())
+
+
+def test_an_inner_that_was_moved():
+    """From a multiple of 256 bytes on it serves as it did; elsewhere its parts would be
+    looked for beside where they are, and it is refused."""
+    x, w_in, w_out, dy = (t.cuda() for t in inputs(70, 40, 24, 30, torch.bfloat16, 6))
+    y, inner = X.feed_forward(x, w_in, w_out, keep_inner=True)
+    want = X.feed_forward_grad(dy, x, w_in, w_out, inner)
+    packed = torch.zeros(inner.numel() + 1024, dtype=torch.uint8, device="cuda")
+    for at in (0, 512, 768):
+        packed[at:at + inner.numel()] = inner
+        got = X.feed_forward_grad(dy, x, w_in, w_out, packed[at:at + inner.numel()])
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), at
+    for at in (16, 128, 300):
+        with pytest.raises(ValueError, match="multiple of 256"):
+            X.feed_forward_grad(dy, x, w_in, w_out, packed[at:at + inner.numel()])
+
+
+@pytest.mark.parametrize("n", [5, 40, 90, 700])
+def test_a_float32_row_that_is_not_finite_stays_alone(n):
+    x, w_in, w_out, dy = (t.cuda() for t in inputs(n, 64, 40, 32, torch.float32, 4))
+    want, inner = X.feed_forward(x, w_in, w_out, keep_inner=True)
+    dx = X.feed_forward_grad(dy, x, w_in, w_out, inner)[0]
+    bad = x.clone()
+    bad[n - 2, 7], bad[1, 0] = float("nan"), float("inf")
+    got, inner = X.feed_forward(bad, w_in, w_out, keep_inner=True)
+    keep = torch.ones(n, dtype=torch.bool, device="cuda")
+    keep[n - 2] = keep[1] = False
+    assert torch.equal(got[keep], want[keep]) and not bool(torch.isfinite(got[~keep]).any())
+    assert torch.equal(X.feed_forward_grad(dy, bad, w_in, w_out, inner)[0][keep], dx[keep])

@@ -63,7 +63,8 @@ def feed_forward(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, *, ac
     (y, inner), inner a buffer for the backward pass: g and u in float32 and act(g) * u.
 
     16-bit types round act(g) * u to theirs before w_out (16 rows or fewer of narrow
-    blocks keep 16 bits of it); in float16 one beyond 65504 makes its row infinite or NaN."""
+    blocks keep 16 bits of it); in float16 one beyond 65504 makes its row infinite or NaN.
+    In float32 an infinite x or weight may count as NaN."""
     if x.requires_grad or w_in.requires_grad or w_out.requires_grad:
         _unrecorded()
     act = _activation(activation)
@@ -99,8 +100,9 @@ def feed_forward_grad(dy: torch.Tensor, x: torch.Tensor, w_in: torch.Tensor, w_o
     if nbytes == 0:
         raise ValueError("feed_forward_grad: sizes out of range (D, F, O <= 2^24, n < 2^31 - 256, tiles of fewer than 2^32 threads)")
     size = int(lib.yabt_feed_forward_inner_bytes(dt, n, D, F, O))
-    if inner.dtype != torch.uint8 or tuple(inner.shape) != (size,) or inner.device != dev or not inner.is_contiguous():
-        raise ValueError(f"inner must be what feed_forward kept, {size} bytes on {dev}")
+    if inner.dtype != torch.uint8 or tuple(inner.shape) != (size,) or inner.device != dev or \
+            not inner.is_contiguous() or inner.data_ptr() % 256:
+        raise ValueError(f"inner must be what feed_forward kept, {size} bytes on {dev} from a multiple of 256 on")
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     dx = torch.empty((n, D), dtype=x.dtype, device=dev)
     dw_in, dw_out = torch.empty_like(w_in), torch.empty_like(w_out)
