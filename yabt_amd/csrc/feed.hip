@@ -54,7 +54,8 @@ struct Product {
     int64_t lda, ldb;
     int M, N, K;
     int aw, bw;                       // an operand across K: its width in memory
-    int F, Fp, Fi;                    // inner width; up to whole 16 bytes: the pitch of h, half of [dg du]'s; up to a multiple of 4
+    int F, Fp, Fi;                    // inner width; up to whole 16 bytes: the pitch of h, half of [dg du]'s; up to a
+                                      // multiple of 4
     int act;
     float* pre;                       // (M, 2 Fi): g from 0, u from Fi, or NULL
     void* h;                          // (M, Fp), or NULL
@@ -91,7 +92,8 @@ __device__ __forceinline__ float gate_normal(float g) {
     float tail;                        // of the distribution, beyond |g|
     if constexpr (sizeof(T) != 4) {
         const float t = __builtin_amdgcn_rcpf(1.0f + 0.3275911f * x);
-        const float p = t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+        const float p =
+            t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
         tail = 0.5f * p * __expf(-x * x);
     } else {
         tail = 0.5f * erfcf(x);
@@ -617,7 +619,8 @@ __device__ __forceinline__ void feed_tile(const Product& P, uint32_t block, cons
     constexpr int LANES = GATED ? W / 8 : W / 4, PASS = 64 / LANES;    // lanes a row, rows at once
     const int c4 = lane % LANES * 4, first = nf + wn * (GATED ? W / 2 : W);   // this lane's columns: first + c4 .. + 3
     const int width = GATED || MODE == DH ? P.Fp : P.N;
-    const bool inside = mf + TL::BM <= P.M && nf + (GATED ? TL::BN / 2 : TL::BN) <= P.N && (P.F == P.Fp || !(GATED || MODE == DH || MODE == DWIN));
+    const bool inside = mf + TL::BM <= P.M && nf + (GATED ? TL::BN / 2 : TL::BN) <= P.N &&
+                        (P.F == P.Fp || !(GATED || MODE == DH || MODE == DWIN));
     f32x4 scale[2];                   // of 8-bit products: the columns'
     if constexpr (MODE == IN8 || MODE == OUT8) {
         if (first + c4 < P.N) {
@@ -848,7 +851,8 @@ __device__ __forceinline__ void chunk_codes(const Chunk<T>& c, float unit, int8_
 // bytes: 16 384 x 5632 of fp32 86 us, 5.4 TB/s; 8192 x 4096 of bf16 19.3 us, 5.2 TB/s.
 constexpr int QUANT_CHUNKS = 4;
 template <typename T, int LANES>
-__global__ void __launch_bounds__(256) k_quantize(const T* x, int64_t ldx, int64_t n, int D, int8_t* q, int64_t ldq, float* scale) {
+__global__ void __launch_bounds__(256) k_quantize(const T* x, int64_t ldx, int64_t n, int D, int8_t* q, int64_t ldq,
+                                                  float* scale) {
     __shared__ uint32_t s_most[4];
     const int64_t row = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
     const int t = threadIdx.x % LANES;
@@ -1070,7 +1074,8 @@ __global__ void __launch_bounds__(FEW_NT) k_few(Product P) {
     constexpr bool GATED = MODE == IN || MODE == IN8;
     constexpr int G = GATED ? 2 : 1, WAVES = FEW_NT / 64;
     using Four = typename Sums<T>::Four;
-    constexpr int PAIRS = R * MB, AT_ONCE = PAIRS < 4 / G ? PAIRS : 4 / G;  // groups of columns and rows whose sums LDS holds: 32 KB
+    // groups of columns and rows, and how many of their sums LDS holds: 32 KB
+    constexpr int PAIRS = R * MB, AT_ONCE = PAIRS < 4 / G ? PAIRS : 4 / G;
     __shared__ Four s_sum[WAVES][AT_ONCE][G][64];
     __shared__ float s_scale[FEW_ROWS];
     __shared__ uint32_t s_most[FEW_ROWS];
@@ -1297,13 +1302,15 @@ inline bool few_rows(int64_t n) { return n <= FEW_ROWS; }
 inline bool few_values(int64_t n, int64_t K) { return n * K <= FEW_VALUES; }
 
 inline bool feed_ranges_ok(int64_t n, int D, int F, int O) {
-    return n >= 0 && n < (1ll << 31) - 256 && D >= 1 && F >= 1 && O >= 1 && D <= (1 << 24) && F <= (1 << 24) && O <= (1 << 24);
+    return n >= 0 && n < (1ll << 31) - 256 && D >= 1 && F >= 1 && O >= 1 && D <= (1 << 24) && F <= (1 << 24) &&
+           O <= (1 << 24);
 }
 
 // The three gradients by large tiles, side by side, those of more steps than a CU's share of
 // all in parts (of 16 steps at least).  Large and small, us for forward and backward, bf16: 8192 x 1024, 2816: 620 and
 // 703; 4096 x 2048, 2048: 360 and 446; 2048 x 2048, 5632: 590 and 624.
-inline bool large_gradients(int bytes, const int64_t (&M)[3], const int64_t (&N)[3], const int64_t (&K)[3], int (&splits)[3]) {
+inline bool large_gradients(int bytes, const int64_t (&M)[3], const int64_t (&N)[3], const int64_t (&K)[3],
+                            int (&splits)[3]) {
     int64_t tiles[3], steps[3], all = 0, count = 0;
     for (int i = 0; i < 3; ++i) {
         if (K[i] * bytes < 768 || M[i] < 192 || N[i] < 192) return false;
@@ -1430,7 +1437,8 @@ int run_feed(const FeedSizes& z, int act, int dtype, const void* x, int64_t ldx,
     P.h32 = s.h32;
     const int b = z.bytes;
     if (z.few) run_few<T, IN, false>(P, stream);
-    else if (!run_tiles<T, IN>(P, z.large_in, straight_ok(x, ldx, z.D, b) && straight_ok(w_in, z.D, z.D, b, (int64_t)z.F + 256), stream))
+    else if (!run_tiles<T, IN>(P, z.large_in,
+                               straight_ok(x, ldx, z.D, b) && straight_ok(w_in, z.D, z.D, b, (int64_t)z.F + 256), stream))
         return fail(-1, "yabt_feed_forward: bad sizes");
     Product Q = {};
     Q.b = w_out, Q.ldb = z.F;
@@ -1482,7 +1490,8 @@ int run_feed_grad(const FeedSizes& z, int act, int dtype, const void* dy, int64_
             Tiles go = take_last(&G.g[2], beside_inner_grad(z, gh.count, G.g));
             if (!grid_ok((int64_t)go.blocks + gh.blocks, TL::NT)) return false;
             if (go.blocks + gh.blocks)
-                k_feed_inner_grad<T, TL, decltype(d)::value><<<go.blocks + gh.blocks, TL::NT, TL::LDS, stream>>>(O, go, P, gh);
+                k_feed_inner_grad<T, TL, decltype(d)::value>
+                    <<<go.blocks + gh.blocks, TL::NT, TL::LDS, stream>>>(O, go, P, gh);
         } else if (z.n > 0 && !run_tiles<T, DH>(P, z.large_dh, dma, stream)) {
             return false;
         }
@@ -1500,11 +1509,13 @@ int run_feed_grad(const FeedSizes& z, int act, int dtype, const void* dy, int64_
     return launch_status("yabt_feed_forward_grad");
 }
 
-int run_quantize(int dtype, const void* x, int64_t ldx, int64_t n, int D, int8_t* q, int64_t ldq, float* scale, hipStream_t stream) {
+int run_quantize(int dtype, const void* x, int64_t ldx, int64_t n, int D, int8_t* q, int64_t ldq, float* scale,
+                 hipStream_t stream) {
     by_dtype(dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
         // rows that a wave holds in its registers, and longer ones by a block each
-        if (D <= 64 * QUANT_CHUNKS * VEC<T>) k_quantize<T, 64><<<(unsigned)over(n, 4), 256, 0, stream>>>((const T*)x, ldx, n, D, q, ldq, scale);
+        if (D <= 64 * QUANT_CHUNKS * VEC<T>)
+            k_quantize<T, 64><<<(unsigned)over(n, 4), 256, 0, stream>>>((const T*)x, ldx, n, D, q, ldq, scale);
         else k_quantize<T, 256><<<(unsigned)n, 256, 0, stream>>>((const T*)x, ldx, n, D, q, ldq, scale);
         return 0;
     });
@@ -1525,8 +1536,8 @@ inline Int8Sizes int8_sizes(int64_t n, int64_t N, int64_t K) {
     return z;
 }
 // y = (a b^T) scaled, a (n, K) codes; part: splits x n x N floats where it is made in parts.
-bool run_int8(const Int8Sizes& z, const int8_t* a, int64_t lda, const float* sa, int64_t n, int K, const int8_t* b, int64_t ldb,
-              const float* sb, int N, int out_dtype, void* y, int64_t ldy, float* part, hipStream_t stream) {
+bool run_int8(const Int8Sizes& z, const int8_t* a, int64_t lda, const float* sa, int64_t n, int K, const int8_t* b,
+              int64_t ldb, const float* sb, int N, int out_dtype, void* y, int64_t ldy, float* part, hipStream_t stream) {
     Product P = {};
     P.a = a, P.lda = lda, P.b = b, P.ldb = ldb, P.M = (int)n, P.N = N, P.K = K, P.sa = sa, P.sb = sb;
     P.out = y, P.ldo = ldy, P.out_dtype = out_dtype, P.splits = 1;
@@ -1684,8 +1695,8 @@ size_t yabt_feed_forward_int8_workspace_bytes(int64_t n, int D, int F, int O) {
     return carve_feed8(c, &s, n, D, F, O) + 256;
 }
 
-int yabt_feed_forward_int8(int dtype, int act, const void* x, int64_t ldx, int64_t n, int D, int F, int O, const int8_t* w_in,
-                           const float* in_scale, const int8_t* w_out, const float* out_scale, void* workspace,
+int yabt_feed_forward_int8(int dtype, int act, const void* x, int64_t ldx, int64_t n, int D, int F, int O,
+                           const int8_t* w_in, const float* in_scale, const int8_t* w_out, const float* out_scale, void* workspace,
                            size_t workspace_bytes, void* y, int64_t ldy, yabt_stream_t stream) {
     if (!dtype_ok(dtype)) return fail(-1, "yabt_feed_forward_int8: dtype is 0 (fp32), 1 (bf16) or 2 (fp16)");
     if (act < SILU || act > RELU) return fail(-1, "yabt_feed_forward_int8: the activation is 0 to 3");
@@ -1710,13 +1721,14 @@ int yabt_feed_forward_int8(int dtype, int act, const void* x, int64_t ldx, int64
         run_quantize(dtype, x, ldx, n, D, s.q, dq, s.scale, on);
         P.a = s.q, P.lda = dq, P.sa = s.scale;
         if (few_rows(n)) run_few<int8_t, IN8, false>(P, on);
-        else if (!run_tiles<int8_t, IN8>(P, large_product(1, n, 2 * (int64_t)F, D), straight_ok(s.q, dq, D, 1) && straight_ok(w_in, D, D, 1, (int64_t)F + 256), on))
+        else if (!run_tiles<int8_t, IN8>(P, large_product(1, n, 2 * (int64_t)F, D),
+                                         straight_ok(s.q, dq, D, 1) && straight_ok(w_in, D, D, 1, (int64_t)F + 256), on))
             return fail(-1, "yabt_feed_forward_int8: bad sizes");
     }
     if (few_rows(n) && few_values(n, F)) {
         Product Q = {};
-        Q.a = s.h32, Q.lda = Fi, Q.x_dtype = DT_F32, Q.b = w_out, Q.ldb = F, Q.M = (int)n, Q.N = O, Q.K = F, Q.sb = out_scale;
-        Q.out = y, Q.ldo = ldy, Q.out_dtype = dtype, Q.splits = 1;
+        Q.a = s.h32, Q.lda = Fi, Q.x_dtype = DT_F32, Q.b = w_out, Q.ldb = F, Q.M = (int)n, Q.N = O, Q.K = F;
+        Q.sb = out_scale, Q.out = y, Q.ldo = ldy, Q.out_dtype = dtype, Q.splits = 1;
         run_few<int8_t, OUT8, true>(Q, on);
     } else {
         run_quantize(DT_F32, s.h32, Fi, n, F, s.q, fq, s.scale, on);
