@@ -28,7 +28,7 @@
 // a tile, where all CUs read and write at once (h with g and u 0.46 GB, the inner gradient 0.55 GB), is
 // not covered, and neither is its first step; and h has 5.5 rounds of 256 tiles.
 // 8192 x 4096 x 4096 in 8 bits: 133 us, 2070 TOP/s (the library's reaches 2110 at 8192 x 8192 x 8192).
-// 4096 x 2048 -> 4096 -> 2048, fp32: 1020 us, 202 TFLOP/s (the library's fp32 product: 153).
+// 4096 x 2048 -> 4096 -> 2048, fp32: 1030 us, 200 TFLOP/s (the library's fp32 product: 153).
 //
 // 16-bit types: h, dg and du are rounded to the inputs' type, as the matrix cores
 // take them (for 16 rows or fewer, whose time is the weights', h is taken in two parts and
@@ -378,7 +378,8 @@ struct PartsLoader {
     }
 };
 
-// acc += the tile's products over [lo, end) in parts.
+// acc += the tile's products over [lo, end) in parts.  The upper parts' products have sums of their
+// own, which are rounded once a product; those of the small ones join them at the end.
 template <int MODE, typename TL>
 __device__ __forceinline__ void parts_sums(const Product& P, int mf, int nf, int lo, int end, int steps,
                                            f32x16 (&acc)[TL::MI][TL::NI]) {
@@ -400,6 +401,13 @@ __device__ __forceinline__ void parts_sums(const Product& P, int mf, int nf, int
         la.template put<decltype(set)::value>(place);
         lb.template put<decltype(set)::value>(place + 3 * TL::APART);
     };
+    f32x16 small[TL::MI][TL::NI];
+#pragma unroll
+    for (int i = 0; i < TL::MI; ++i)
+#pragma unroll
+        for (int j = 0; j < TL::NI; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) small[i][j][r] = 0.0f;
     auto products = [&](auto set) {
         lds_char* const ta = lds + decltype(set)::value * TL::PLACE;
         lds_char* const tb = ta + 3 * TL::APART;
@@ -413,7 +421,6 @@ __device__ __forceinline__ void parts_sums(const Product& P, int mf, int nf, int
 #pragma unroll
                 for (int j = 0; j < TL::NI; ++j) b[o][j] = fb.get(tb + o * TL::BPART, j, ks);
             }
-            // the small products first
 #pragma unroll
             for (int sum = 2; sum >= 0; --sum)
 #pragma unroll
@@ -421,7 +428,10 @@ __device__ __forceinline__ void parts_sums(const Product& P, int mf, int nf, int
 #pragma unroll
                     for (int i = 0; i < TL::MI; ++i)
 #pragma unroll
-                        for (int j = 0; j < TL::NI; ++j) acc[i][j] = mma<bf16>(a[o][i], b[sum - o][j], acc[i][j]);
+                        for (int j = 0; j < TL::NI; ++j) {
+                            f32x16& to = sum ? small[i][j] : acc[i][j];
+                            to = mma<bf16>(a[o][i], b[sum - o][j], to);
+                        }
         }
     };
     constexpr std::integral_constant<int, 0> even;
@@ -441,6 +451,10 @@ __device__ __forceinline__ void parts_sums(const Product& P, int mf, int nf, int
         fetch(even, t + 4);
         products(odd);
     }
+#pragma unroll
+    for (int i = 0; i < TL::MI; ++i)
+#pragma unroll
+        for (int j = 0; j < TL::NI; ++j) acc[i][j] += small[i][j];
     __syncthreads();                             // the sums leave through the same LDS
 }
 
