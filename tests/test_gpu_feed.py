@@ -223,3 +223,33 @@ def test_a_float32_row_that_is_not_finite_stays_alone(n):
     keep[n - 2] = keep[1] = False
     assert torch.equal(got[keep], want[keep]) and not bool(torch.isfinite(got[~keep]).any())
     assert torch.equal(X.feed_forward_grad(dy, bad, w_in, w_out, inner)[0][keep], dx[keep])
+
+
+# few tiles over a long sum, which is made in parts: of [g u] over D, of dh over O; inner widths that are
+# and are not whole pieces, one tile and many
+@pytest.mark.parametrize("dt", TYPES, ids=name)
+@pytest.mark.parametrize("n,D,F,O", [(65, 2600, 17, 2000), (83, 2520, 256, 2520), (130, 4001, 33, 1500),
+                                     (300, 3000, 64, 40), (300, 40, 64, 3100), (777, 500, 1333, 500)])
+def test_few_tiles_over_long_sums(n, D, F, O, dt):
+    check(inputs(n, D, F, O, dt, n + F), "gelu")
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=name)
+def test_few_tiles_over_long_sums_without_a_kept_inner(dt):
+    x, w_in, w_out, _ = (t.cuda() for t in inputs(83, 2520, 250, 60, dt, 8))
+    assert torch.equal(X.feed_forward(x, w_in, w_out), X.feed_forward(x, w_in, w_out, keep_inner=True)[0])
+
+
+def test_sums_in_parts_captured_and_replayed():
+    x, w_in, w_out, dy = (t.cuda() for t in inputs(83, 2520, 250, 2000, torch.float32, 9))
+    run(x, w_in, w_out, dy, "silu")
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run(x, w_in, w_out, dy, "silu")
+    for k in range(4):
+        x.mul_(-0.75), dy.add_(0.25)
+        graph.replay()
+        want = run(x, w_in, w_out, dy, "silu")
+        torch.cuda.synchronize()
+        assert all(torch.equal(got[m], want[m]) for m in want), k

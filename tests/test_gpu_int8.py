@@ -202,3 +202,19 @@ def test_no_rows():
     assert q.shape == (0, 24) and s.shape == (0,)
     assert X.product_int8(q, s, w[0], w[1]).shape == (0, 20)
     assert X.feed_forward_int8(x.cuda(), *w).shape == (0, 12)
+
+
+# few tiles over a long sum: [g u] is made in parts
+@pytest.mark.parametrize("dt", TYPES, ids=name)
+@pytest.mark.parametrize("n,D,F,O", [(65, 9000, 17, 30), (83, 2520, 256, 40), (300, 8192, 130, 33), (100, 4096, 1021, 16)])
+def test_block_of_few_tiles_over_long_sums(n, D, F, O, dt):
+    x, *w = block(n, D, F, O, dt, n + D)
+    y = X.feed_forward_int8(x.cuda(), *w, activation="gelu_tanh")
+    value, bound = feed8(x.float().numpy(), *(t.cpu().numpy() for t in w), "gelu_tanh")
+    # feed8 bounds the value before it is rounded to the type: half a step of it, or of the type's least values
+    bound = bound + UNIT[name(dt)] * (np.abs(value) + bound) + (2.0 ** -25 if dt == torch.float16 else 2.0 ** -133)
+    got, most = y.double().cpu().numpy(), torch.finfo(dt).max
+    # rounding to the type makes what is half a step past its largest value infinite
+    past = np.isinf(got) & (np.sign(got) * value + bound > most)
+    off = np.where(past, 0.0, np.abs(got - value))
+    assert np.all(off <= bound), f"{np.max(off / bound):.3g} of the bound"

@@ -66,7 +66,8 @@ struct Product {
     int out_dtype;
     const float* sa;                  // scales of rows and columns (IN8: of gates, then of u)
     const float* sb;
-    float* part;                      // (splits, M, N) where splits > 1: the sums in part (OUT8: as int32)
+    float* part;                      // (splits, M, N) where splits > 1: the sums in part (8 bits: as int32); IN
+                                      // (splits, M, 2 Fi): of g from 0, of u from Fi; DH (splits, M, Fi)
     int splits;
     int x_dtype;                      // few rows of 8 bits: the type of a's values
 };
@@ -665,6 +666,14 @@ __device__ __forceinline__ void feed_tile(const Product& P, uint32_t block, cons
             if constexpr (GATED) {
                 // columns 64 q + 0..31: gate of f 32 q + 0..31, the next 32: u
                 const int c = (c4 & ~31) * 2 + (c4 & 31);
+                if (P.splits > 1) {
+                    if (WHOLE || f < P.Fi) {
+                        float* const to = row0(P.part + (size_t)split * P.M * 2 * (size_t)P.Fi, i, p, 2 * (int64_t)P.Fi);
+                        *(f32x4*)(to + at_pre) = bits(c);
+                        *(f32x4*)(to + P.Fi + at_pre) = bits(c + 32);
+                    }
+                    continue;
+                }
                 f32x4 g, u;
                 if constexpr (MODE == IN8) {
                     const float s = P.sa[m];
@@ -689,6 +698,11 @@ __device__ __forceinline__ void feed_tile(const Product& P, uint32_t block, cons
                     }
                 }
             } else if constexpr (MODE == DH) {
+                if (P.splits > 1) {
+                    if (WHOLE || f < P.Fi)
+                        *(f32x4*)(row0(P.part + (size_t)split * P.M * (size_t)P.Fi, i, p, P.Fi) + at_h32) = bits(c4);
+                    continue;
+                }
                 f32x4 g = {0.0f, 0.0f, 0.0f, 0.0f}, u = g;
                 if (WHOLE || f < P.Fi) {
                     const float* const pre = row0(P.pre, i, p, 2 * (int64_t)P.Fi);
@@ -801,6 +815,66 @@ __global__ void __launch_bounds__(256) k_join(Joins A) {
                 for (int k = 0; k < J.splits; ++k) s += four_of(p + k * each, J.N - c);
             }
             store_as(J.dtype, J.out, (size_t)row * (size_t)J.ldo + c, s, J.N - c);
+        }
+    }
+}
+
+// The same for IN, IN8 and DH, whose sums become h, or dg and du, here.
+template <typename T, int MODE>
+__global__ void __launch_bounds__(256) k_join_inner(Product P) {
+    const int per = P.Fp / 4;
+    const int64_t work = (int64_t)P.M * per;
+    const size_t pitch = (MODE == DH ? 1 : 2) * (size_t)P.Fi, each = (size_t)P.M * pitch;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < work; i += (int64_t)gridDim.x * 256) {
+        const size_t m = (size_t)(i / per);
+        const int f = (int)(i - (int64_t)m * per) * 4;
+        const bool there = f < P.Fi;
+        f32x4 g = {0.0f, 0.0f, 0.0f, 0.0f}, u = g, dh = g;
+        if (there) {
+            const float* p = P.part + m * pitch + f;
+            if constexpr (MODE == IN8) {
+                i32x4 sg = {0, 0, 0, 0}, su = sg;
+#pragma unroll 4
+                for (int k = 0; k < P.splits; ++k, p += each) {
+                    sg += *(const i32x4*)p;
+                    su += *(const i32x4*)(p + P.Fi);
+                }
+                const float s = P.sa[m];
+                g = f32x4{(float)sg[0], (float)sg[1], (float)sg[2], (float)sg[3]} * four_of(P.sb + f, P.F - f) * s;
+                u = f32x4{(float)su[0], (float)su[1], (float)su[2], (float)su[3]} * four_of(P.sb + P.F + f, P.F - f) * s;
+            } else if constexpr (MODE == IN) {
+#pragma unroll 4
+                for (int k = 0; k < P.splits; ++k, p += each) {
+                    g += *(const f32x4*)p;
+                    u += *(const f32x4*)(p + P.Fi);
+                }
+            } else {
+#pragma unroll 4
+                for (int k = 0; k < P.splits; ++k, p += each) dh += *(const f32x4*)p;
+                g = *(const f32x4*)(P.pre + m * 2 * P.Fi + f);
+                u = *(const f32x4*)(P.pre + m * 2 * P.Fi + P.Fi + f);
+            }
+        }
+        float v[4], slope[4], a[4], b[4];
+        activate<T>(P.act, g, v, slope);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const bool is = f + q < P.F;
+            a[q] = !is ? 0.0f : MODE == DH ? dh[q] * u[q] * slope[q] : v[q] * u[q];
+            b[q] = is && MODE == DH ? dh[q] * v[q] : 0.0f;
+        }
+        if constexpr (MODE == DH) {
+            T* const to = (T*)P.dpre + m * 2 * P.Fp + f;
+            store4(to, a);
+            store4(to + P.Fp, b);
+        } else if constexpr (MODE == IN8) {
+            *(f32x4*)(P.h32 + m * P.Fi + f) = f32x4{a[0], a[1], a[2], a[3]};
+        } else {
+            store4((T*)P.h + m * P.Fp + f, a);
+            if (P.pre && there) {
+                *(f32x4*)(P.pre + m * 2 * P.Fi + f) = g;
+                *(f32x4*)(P.pre + m * 2 * P.Fi + P.Fi + f) = u;
+            }
         }
     }
 }
@@ -1217,6 +1291,18 @@ inline int split_count(int64_t M, int64_t N, int64_t K, bool large, int bytes) {
     return s < 1 ? 1 : (int)s;
 }
 
+// The same of the products that become h (IN), or dg and du (DH), whose join is a launch more that reads the
+// parts: where the steps that a block is spared take longer.  A step takes about 0.38 us, DH's 0.6 (0.9 where
+// W_out's rows are not whole pieces), fp32's 1.1, the launch 5 and 100 parts of tiles 1.2.  Whole and in parts, us for the block: fp32 83 x 2520 -> 256
+// -> 2520 106 and 28, 1000 x 2048 -> 512 100 and 61; bf16 83 x 2520 24.5 and 15.5, but 534 x 1000 -> 760 23.5
+// and 27.2 (it stays whole); 8 bits 100 x 4096 -> 1024 33.1 and 28.9, but 1000 x 2048 -> 512 27.0 and 32.9.
+inline int inner_split_count(int mode, int64_t M, int64_t N, int64_t K, bool large, int bytes) {
+    const int s = split_count(M, N, K, large, bytes);
+    const double each = bytes == 4 ? 1.1 : mode != DH ? 0.38 : N * bytes % 16 ? 0.9 : 0.6, steps = (double)over(K * bytes, 128);
+    const double spared = steps * (1.0 - 1.0 / s) * each, more = 5.0 + 0.012 * s * (double)tile_count(bytes, false, M, N);
+    return spared > more ? s : 1;
+}
+
 // All tiles of a product; false: more than a grid can have.
 template <typename TL>
 bool all_tiles(const Product& P, bool gated, Tiles* g) {
@@ -1280,6 +1366,12 @@ inline void run_join(const Joins& J, hipStream_t stream) {
         work = w > work ? w : work;
     }
     if (J.count) k_join<<<launch_grid(work, 256, 8192), 256, 0, stream>>>(J);
+}
+
+template <typename T, int MODE>
+void run_join_inner(const Product& P, hipStream_t stream) {
+    const int64_t work = (int64_t)P.M * (P.Fp / 4);
+    if (P.splits > 1 && work > 0) k_join_inner<T, MODE><<<launch_grid(work, 256, 8192), 256, 0, stream>>>(P);
 }
 
 template <typename T, int MODE, int MB, int R, bool CODES>
@@ -1353,7 +1445,8 @@ struct FeedSizes {
     int D, F, O, bytes, Fp, Fi;
     bool few, few_out, whole;         // few rows: h and y by their kernel; so few that h is kept in fp32 for y
     bool large_in, large_out, large_dh, large_grads;
-    int splits_out, splits[3];        // of y; of dx, dW_in, dW_out
+    int splits_in, splits_out;        // of [g u], of y
+    int splits_dh, splits[3];         // of dh; of dx, dW_in, dW_out
 };
 inline FeedSizes feed_sizes(int dtype, int64_t n, int D, int F, int O) {
     FeedSizes z;
@@ -1367,7 +1460,9 @@ inline FeedSizes feed_sizes(int dtype, int64_t n, int D, int F, int O) {
     z.large_in = large_product(b, n, 2 * (int64_t)F, D);
     z.large_out = large_product(b, n, O, F);
     z.splits_out = split_count(n, O, F, z.large_out, b);
+    z.splits_in = z.few ? 1 : inner_split_count(IN, n, 2 * (int64_t)F, D, z.large_in, b);
     z.large_dh = large_product(b, n, F, O);
+    z.splits_dh = inner_split_count(DH, n, F, O, z.large_dh, b);
     const int64_t M[3] = {n, (int64_t)z.Fp + F, O}, N[3] = {D, D, F}, K[3] = {(int64_t)z.Fp + F, n, n};
     z.large_grads = large_gradients(b, M, N, K, z.splits);
     if (!z.large_grads)
@@ -1420,21 +1515,25 @@ inline size_t carve_kept(Carve& c, FeedKept* k, const FeedSizes& z) {
 struct FeedSpace {
     char* h;
     float* h32;
+    float* part_in;
     float* part;
 };
 inline size_t carve_forward(Carve& c, FeedSpace* s, const FeedSizes& z) {
     s->h = c.take<char>((size_t)z.n * z.Fp * z.bytes);
     s->h32 = z.whole ? c.take<float>((size_t)z.n * z.Fi) : nullptr;
+    s->part_in = z.splits_in > 1 ? c.take<float>((size_t)z.splits_in * z.n * 2 * z.Fi) : nullptr;
     s->part = !z.few_out && z.splits_out > 1 ? c.take<float>((size_t)z.splits_out * z.n * z.O) : nullptr;
     return c.off;
 }
 struct GradSpace {
     char* dpre;
+    float* part_dh;
     float* part[3];
 };
 inline size_t carve_backward(Carve& c, GradSpace* s, const FeedSizes& z) {
     const int64_t M[3] = {z.n, 2 * (int64_t)z.F, z.O}, N[3] = {z.D, z.D, z.F};
     s->dpre = c.take<char>((size_t)z.n * 2 * z.Fp * z.bytes);
+    s->part_dh = z.splits_dh > 1 ? c.take<float>((size_t)z.splits_dh * z.n * z.Fi) : nullptr;
     for (int i = 0; i < 3; ++i) s->part[i] = z.splits[i] > 1 ? c.take<float>((size_t)z.splits[i] * M[i] * N[i]) : nullptr;
     return c.off;
 }
@@ -1445,7 +1544,7 @@ int run_feed(const FeedSizes& z, int act, int dtype, const void* x, int64_t ldx,
     Product P = {};
     P.a = x, P.lda = ldx, P.b = w_in, P.ldb = z.D;
     P.M = (int)z.n, P.N = z.F, P.K = z.D;
-    P.F = z.F, P.Fp = z.Fp, P.Fi = z.Fi, P.act = act, P.splits = 1;
+    P.F = z.F, P.Fp = z.Fp, P.Fi = z.Fi, P.act = act, P.splits = z.splits_in, P.part = s.part_in;
     P.pre = kept ? kept->pre : nullptr;
     P.h = kept ? kept->h : z.whole ? nullptr : s.h;
     P.h32 = s.h32;
@@ -1454,6 +1553,7 @@ int run_feed(const FeedSizes& z, int act, int dtype, const void* x, int64_t ldx,
     else if (!run_tiles<T, IN>(P, z.large_in,
                                straight_ok(x, ldx, z.D, b) && straight_ok(w_in, z.D, z.D, b, (int64_t)z.F + 256), stream))
         return fail(-1, "yabt_feed_forward: bad sizes");
+    run_join_inner<T, IN>(P, stream);
     Product Q = {};
     Q.b = w_out, Q.ldb = z.F;
     Q.M = (int)z.n, Q.N = z.O, Q.K = z.F;
@@ -1481,7 +1581,7 @@ int run_feed_grad(const FeedSizes& z, int act, int dtype, const void* dy, int64_
     Product P = {};
     P.a = dy, P.lda = lddy, P.b = w_out, P.ldb = z.F, P.bw = z.F;
     P.M = (int)z.n, P.N = z.F, P.K = z.O;
-    P.F = z.F, P.Fp = z.Fp, P.Fi = z.Fi, P.act = act, P.splits = 1;
+    P.F = z.F, P.Fp = z.Fp, P.Fi = z.Fi, P.act = act, P.splits = z.splits_dh, P.part = s.part_dh;
     P.pre = kept.pre, P.dpre = s.dpre;
     GradProducts G = {};
     for (auto& p : G.p) p.F = z.F, p.Fp = z.Fp, p.Fi = z.Fi, p.out_dtype = dtype;
@@ -1509,6 +1609,7 @@ int run_feed_grad(const FeedSizes& z, int act, int dtype, const void* dy, int64_
         } else if (z.n > 0 && !run_tiles<T, DH>(P, z.large_dh, dma, stream)) {
             return false;
         }
+        run_join_inner<T, DH>(P, stream);
         k_feed_grads<T, TL, decltype(d)::value>
             <<<G.g[0].blocks + G.g[1].blocks + G.g[2].blocks, TL::NT, TL::LDS, stream>>>(G);
         return true;
@@ -1569,14 +1670,21 @@ struct Feed8Space {
     int8_t* q;                        // codes of x, then of h
     float* scale;
     float* h32;
+    float* part_in;
     float* part;
 };
+inline int splits_in8(int64_t n, int D, int F) {
+    const int64_t N = 2 * (int64_t)F;
+    return few_rows(n) ? 1 : inner_split_count(IN, n, N, D, large_product(1, n, N, D), 1);
+}
 inline size_t carve_feed8(Carve& c, Feed8Space* s, int64_t n, int D, int F, int O) {
     const Int8Sizes z = int8_sizes(n, O, F);
     const int64_t w = D > F ? D : F;
     s->q = c.take<int8_t>((size_t)n * up16((int)w, 1));
     s->scale = c.take<float>((size_t)n);
+    const int in = splits_in8(n, D, F);
     s->h32 = c.take<float>((size_t)n * up16(F, 4));
+    s->part_in = in > 1 ? c.take<float>((size_t)in * n * 2 * up16(F, 4)) : nullptr;
     s->part = !z.few && z.splits > 1 ? c.take<float>((size_t)z.splits * n * O) : nullptr;
     return c.off;
 }
@@ -1727,7 +1835,7 @@ int yabt_feed_forward_int8(int dtype, int act, const void* x, int64_t ldx, int64
     const int Fi = up16(F, 4), dq = up16(D, 1), fq = up16(F, 1);
     Product P = {};
     P.b = w_in, P.ldb = D, P.M = (int)n, P.N = F, P.K = D, P.F = F, P.Fp = Fi, P.Fi = Fi, P.act = act, P.h32 = s.h32;
-    P.sb = in_scale, P.splits = 1;
+    P.sb = in_scale, P.splits = splits_in8(n, D, F), P.part = s.part_in;
     if (few_rows(n) && few_values(n, D)) {
         P.a = x, P.lda = ldx, P.x_dtype = dtype;
         run_few<int8_t, IN8, true>(P, on);
@@ -1738,6 +1846,7 @@ int yabt_feed_forward_int8(int dtype, int act, const void* x, int64_t ldx, int64
         else if (!run_tiles<int8_t, IN8>(P, large_product(1, n, 2 * (int64_t)F, D),
                                          straight_ok(s.q, dq, D, 1) && straight_ok(w_in, D, D, 1, (int64_t)F + 256), on))
             return fail(-1, "yabt_feed_forward_int8: bad sizes");
+        run_join_inner<int8_t, IN8>(P, on);
     }
     if (few_rows(n) && few_values(n, F)) {
         Product Q = {};
