@@ -676,7 +676,8 @@ int yabt_product_int8(const int8_t *a, int64_t lda, const float *a_scale, int64_
 
 /* yabt_feed_forward with both weights in 8 bits (w_in (2 F, D) and w_out (O, F), a
  * scale for each row): x's rows are put in 8 bits as yabt_quantize_rows does, g, u
- * and h are fp32, and h's rows are put in 8 bits in the same way.  D and F to 131071. */
+ * and h are fp32 (act(g) within (20 + 2 g^2) 2^-24 of itself for gelu, else (8 + 10 |z|) 2^-24, z the
+ * sigmoid's argument), and h's rows are put in 8 bits in the same way.  D and F to 131071. */
 size_t yabt_feed_forward_int8_workspace_bytes(int64_t n, int D, int F, int O);
 int yabt_feed_forward_int8(int dtype, int act, const void *x, int64_t ldx, int64_t n, int D, int F, int O,
                            const int8_t *w_in, const float *in_scale, const int8_t *w_out,

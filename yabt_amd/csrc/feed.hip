@@ -83,21 +83,37 @@ __device__ __forceinline__ i32x4 mma8(u32x4 a, u32x4 b, i32x4 c) {
 }
 
 // The activation of four gates and its derivative.  16 bits: the hardware's exp2 and
-// reciprocal (gate_sigmoid), and for the normal distribution function the approximation
-// 7.1.26 of Abramowitz and Stegun's handbook, off by 7.5e-8 at most.  8 bits too: an h that is
-// off by 2^-20 of itself has another code once in 4000 times at most, and the accurate ones made
-// h of 16 384 x 2048 -> 5632 take 466 us instead of 415.  fp32: the accurate functions.
+// reciprocal (gate_sigmoid), and for the normal distribution function normal_tail.  8 bits too: with
+// U = 2^-24, silu's and gelu_tanh's factor is off by (8 + 10 |z|) U of itself at most (z the sigmoid's argument), gelu's
+// by (20 + 2 g^2) U, so that h of gates to -8 (silu: to -20) is within 2^-16 and has another code once in
+// some 250 times at worst, near 0 once in thousands; the accurate functions
+// made h of 16 384 x 2048 -> 5632 take 466 us instead of 415.  fp32: the accurate functions.
+//
+// Phi(-a) / exp(-a^2 / 2), a >= 0, is half the scaled complementary error function of x = a / sqrt(2).
+// In t = 1 / (1 + 0.33 x) it is t times a polynomial, fitted here to the least largest relative error, 2^-23.5 for x to
+// 9.5 (beyond, the exponential is 0): relative, because a negative gate's whole factor is this tail.
+__device__ __forceinline__ float normal_tail(float a) {
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.23334524f, a, 1.0f));
+    float p = fmaf(-0.0679644f, t, 0.23134412f);
+    p = fmaf(p, t, -0.17771947f);
+    p = fmaf(p, t, 0.2062708f);
+    p = fmaf(p, t, 0.022505322f);
+    p = fmaf(p, t, 0.100961916f);
+    p = fmaf(p, t, 0.091418624f);
+    p = fmaf(p, t, 0.093183056f);
+    return p * t;
+}
+// The normal distribution function at g and exp(-g^2 / 2).
 template <typename T>
-__device__ __forceinline__ float gate_normal(float g) {
-    const float x = fabsf(g) * 0.70710678f;
+__device__ __forceinline__ float gate_normal(float g, float* density) {
+    const float e = -0.5f * g * g;
     float tail;                        // of the distribution, beyond |g|
     if constexpr (sizeof(T) != 4) {
-        const float t = __builtin_amdgcn_rcpf(1.0f + 0.3275911f * x);
-        const float p =
-            t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
-        tail = 0.5f * p * __expf(-x * x);
+        *density = __expf(e);
+        tail = normal_tail(fabsf(g)) * *density;
     } else {
-        tail = 0.5f * erfcf(x);
+        *density = expf(e);
+        tail = 0.5f * erfcf(fabsf(g) * 0.70710678f);
     }
     return g > 0.0f ? 1.0f - tail : tail;
 }
@@ -115,10 +131,11 @@ __device__ __forceinline__ void activate(int act, f32x4 g, float (&v)[4], float 
         case GELU:
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                const float p = gate_normal<T>(g[q]), e = -0.5f * g[q] * g[q];
+                float d;
+                const float p = gate_normal<T>(g[q], &d);
                 v[q] = g[q] * p;
-                // far out the density is 0, and g times it too
-                slope[q] = p + (e > -87.0f ? g[q] * 0.39894228f * (sizeof(T) != 4 ? __expf(e) : expf(e)) : 0.0f);
+                // far out the density is 0, and an infinite g times it too
+                slope[q] = p + (d > 0.0f ? g[q] * 0.39894228f * d : 0.0f);
             }
             break;
         case GELU_TANH:

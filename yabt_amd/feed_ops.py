@@ -171,8 +171,9 @@ def product_int8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scal
 def feed_forward_int8(x: torch.Tensor, w_in: torch.Tensor, in_scale: torch.Tensor, w_out: torch.Tensor,
                       out_scale: torch.Tensor, *, activation: str = "silu") -> torch.Tensor:
     """``feed_forward`` with its weights in 8 bits, each ``quantize_rows`` of the
-    weight: x's rows are put in 8 bits, g, u and h = act(g) * u are float32, and h's
-    rows are put in 8 bits before w_out.  y (n, O) in x's type."""
+    weight: x's rows are put in 8 bits, g, u and h = act(g) * u are float32, act(g) off
+    by up to (20 + 2 g^2) 2^-24 of itself (gelu) or (8 + 10 |z|) 2^-24, z the sigmoid's
+    argument, and h's rows are put in 8 bits before w_out.  y (n, O) in x's type."""
     if x.requires_grad or in_scale.requires_grad or out_scale.requires_grad:
         _unrecorded()
     act = _activation(activation)
