@@ -621,13 +621,16 @@ typedef struct {
  * bits p moves by the moments before they are rounded; a v above 0 keeps a code above
  * 0; a block whose largest magnitude is below 2^-100 is held as zeros, one that is not
  * finite as NaN.  step_device, if not NULL, is read on the device in place of `step`, so
- * that a captured call counts on; numbers below 1 count as 1. */
+ * that a captured call counts on; numbers below 1 count as 1.  Status -3: tensors that are
+ * written overlap, or a gradient overlaps one (its own param or moment may lie on it, from
+ * the same address on with values of as many bytes). */
 int yabt_adamw_step(int count, const yabt_adamw_tensor *tensors, int bits, int64_t step,
                     const int32_t *step_device, double lr, double beta1, double beta2, double eps,
                     double weight_decay, yabt_stream_t stream);
 
 /* The values that 8-bit moments stand for: those of `first` as n floats to
- * `param`, those of `second` to `grad`, which is written here; the types are not read. */
+ * `param`, those of `second` to `grad`, which is written here; the types are not read.
+ * Status -3: what is written overlaps, or overlaps what is read. */
 int yabt_adamw_values(int count, const yabt_adamw_tensor *tensors, yabt_stream_t stream);
 
 /* A gated feed-forward block over n rows:

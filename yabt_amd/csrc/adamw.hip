@@ -25,7 +25,10 @@
 #include "expert.h"
 #include "yabt_hip.h"
 
+#include <algorithm>
 #include <cmath>
+#include <memory>
+#include <new>
 
 namespace yabt {
 
@@ -304,6 +307,39 @@ int adamw_launches(const char* what, int count, const Entry& entry, const Launch
 
 constexpr int64_t ADAMW_MOST = (int64_t)((1 << 24) - 1) * ADAMW_CHUNK;
 
+// Bytes [lo, hi) of tensor `of`, whose values have `each` bytes.
+struct Span {
+    uintptr_t lo, hi;
+    int of, each;
+};
+
+// Whether what a call writes overlaps, or is overlapped by what it reads: thread blocks would meet there in no
+// order.  spans(i, write, read) names tensor i's, up to WRITES and READS of them.  `own_read`: a tensor's own values may be
+// read where they are written, from the same place on in the same width (a thread reads what it alone writes, before).
+// 0, or fails.
+template <int WRITES, int READS, typename Spans>
+int adamw_apart(const char* message, int count, bool own_read, const Spans& spans) {
+    std::unique_ptr<Span[]> written(new (std::nothrow) Span[(size_t)count * WRITES]),
+        read(new (std::nothrow) Span[(size_t)count * READS]);
+    if (!written || !read) return fail(-2, "yabt_adamw: no host memory");
+    Span *w = written.get(), *r = read.get();
+    for (int i = 0; i < count; ++i)
+        spans(i, [&](const void* p, int64_t n, int each) { *w++ = {(uintptr_t)p, (uintptr_t)p + (size_t)n * each, i, each}; },
+              [&](const void* p, int64_t n, int each) { *r++ = {(uintptr_t)p, (uintptr_t)p + (size_t)n * each, i, each}; });
+    const Span* const first = written.get();
+    std::sort(written.get(), w, [](const Span& a, const Span& b) { return a.lo < b.lo; });
+    for (const Span* s = first; s + 1 < w; ++s)
+        if (s->hi > s[1].lo) return fail(-3, message);
+    for (const Span* s = read.get(); s < r; ++s) {
+        // the written spans lie apart: those that begin below s's end, from the last one backwards
+        const Span* t = std::lower_bound(first, (const Span*)w, s->hi, [](const Span& a, uintptr_t at) { return a.lo < at; });
+        while (t > first && (--t)->hi > s->lo)
+            if (!(own_read && t->of == s->of && t->lo == s->lo && t->each == s->each)) return fail(-3, message);
+    }
+    return 0;
+}
+inline int64_t adamw_scales(int64_t n) { return (n + ADAMW_BLOCK - 1) / ADAMW_BLOCK; }
+
 }  // namespace yabt
 
 using namespace yabt;
@@ -327,6 +363,20 @@ int yabt_adamw_step(int count, const yabt_adamw_tensor* tensors, int bits, int64
         if (t.n > 0 && (!t.param || !t.grad || !t.first || !t.second || (bits == 8 && (!t.first_scale || !t.second_scale))))
             return fail(-1, "yabt_adamw_step: null pointer");
     }
+    const int apart = adamw_apart<5, 1>(
+        "yabt_adamw_step: tensors overlap", count, true, [&](int i, const auto& write, const auto& read) {
+            const yabt_adamw_tensor& t = tensors[i];
+            if (t.n == 0) return;
+            write(t.param, t.n, dtype_bytes(t.param_dtype));
+            write(t.first, t.n, bits / 8);
+            write(t.second, t.n, bits / 8);
+            if (bits == 8) {
+                write(t.first_scale, adamw_scales(t.n), 4);
+                write(t.second_scale, adamw_scales(t.n), 4);
+            }
+            read(t.grad, t.n, dtype_bytes(t.grad_dtype));
+        });
+    if (apart) return apart;
     AdamwScalars S = {(float)(1.0 - beta1), (float)(1.0 - beta2), (float)(1.0 - lr * weight_decay), 0.0f, 0.0f, lr, beta1,
                       beta2, eps, step_device};
     if (!step_device) {
@@ -356,6 +406,18 @@ int yabt_adamw_values(int count, const yabt_adamw_tensor* tensors, yabt_stream_t
         if (t.n > 0 && (!t.param || !t.grad || !t.first || !t.second || !t.first_scale || !t.second_scale))
             return fail(-1, "yabt_adamw_values: null pointer");
     }
+    const int apart = adamw_apart<2, 4>(
+        "yabt_adamw_values: tensors overlap", count, false, [&](int i, const auto& write, const auto& read) {
+            const yabt_adamw_tensor& t = tensors[i];
+            if (t.n == 0) return;
+            write(t.param, t.n, 4);
+            write(t.grad, t.n, 4);
+            read(t.first, t.n, 1);
+            read(t.second, t.n, 1);
+            read(t.first_scale, adamw_scales(t.n), 4);
+            read(t.second_scale, adamw_scales(t.n), 4);
+        });
+    if (apart) return apart;
     return adamw_launches(
         "yabt_adamw_values", count,
         [&](int i) {

@@ -144,7 +144,10 @@ def adamw_step(params: list[torch.Tensor], grads: list[torch.Tensor | None], sta
     so that a captured graph that adds one to it counts on (a plain number would
     stay what it was, and is refused while a graph is captured).  With 8-bit
     moments p moves by the moments before they are rounded; a gradient that is
-    not finite makes the moments of its 256 values NaN."""
+    not finite makes the moments of its 256 values NaN.
+
+    Parameters, moments and scales may not overlap, nor a gradient any of them but its
+    own parameter or moment, from the same place on in values of the same width."""
     if not len(params) == len(grads) == len(state.first):
         raise ValueError(f"{len(params)} parameters, {len(grads)} gradients and {len(state.first)} moments")
     b1, b2 = betas
@@ -194,15 +197,15 @@ def adamw_step(params: list[torch.Tensor], grads: list[torch.Tensor | None], sta
     where = list(map(_pointer, params))
     none = [0] * len(params)
     first, second, *scales = (list(map(_pointer, part)) for part in lists)
-    written = [where, first, second, *scales]
-    if len(set(chain.from_iterable(written))) < len(written) * len(sizes):
-        # empty tensors have one address, null
-        written = [at for part in written for at, n in zip(part, sizes) if n]
-        if len(set(written)) < len(written):
-            raise ValueError("a parameter or a moment is in the lists twice")
     table = _table(zip(where, map(_pointer, grads), first, second, *(scales or (none, none)), sizes, types))
-    expert_ops._call("yabt_adamw_step", dev, len(params), table.buffer_info()[0], state.bits, number, at, float(lr), float(b1),
-                     float(b2), float(eps), float(weight_decay))
+    try:
+        expert_ops._call("yabt_adamw_step", dev, len(params), table.buffer_info()[0], state.bits, number, at, float(lr),
+                         float(b1), float(b2), float(eps), float(weight_decay))
+    except RuntimeError as e:
+        if "tensors overlap" in str(e):
+            raise ValueError("a parameter or a moment is in the lists twice, overlaps another, or is overlapped by a "
+                             "gradient that is not all its own") from None
+        raise
     for p in params:
         if p.requires_grad:
             torch.autograd.graph.increment_version(p)
