@@ -206,6 +206,5 @@ def adamw_step(params: list[torch.Tensor], grads: list[torch.Tensor | None], sta
             raise ValueError("a parameter or a moment is in the lists twice, overlaps another, or is overlapped by a "
                              "gradient that is not all its own") from None
         raise
-    for p in params:
-        if p.requires_grad:
-            torch.autograd.graph.increment_version(p)
+    # also of tensors without a gradient of their own: a backward pass may have kept them
+    torch.autograd.graph.increment_version(list(chain(params, *lists)))
