@@ -19,7 +19,7 @@ neither waits nor reads anything back, so it can be captured into a HIP graph.
 Autograd does not see these calls: a program takes the gradients from the
 ``_grad`` functions itself.  A tensor that requires a gradient is therefore
 refused while autograd records; under ``torch.no_grad()``, as in a backward pass
-of one's own, it is taken as it is.
+of one's own, it is taken as it is.  A dual tensor with a tangent (forward mode) is refused too.
 """
 
 from __future__ import annotations
@@ -27,6 +27,7 @@ from __future__ import annotations
 from dataclasses import dataclass
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -57,6 +58,14 @@ def _unrecorded() -> None:
         raise RuntimeError("the expert layer's calls are not recorded by autograd, and a tensor requires a gradient: "
                            "call them under torch.no_grad() and take the gradients from the _grad functions, or "
                            "detach it")
+
+
+def _no_tangents(*tensors: torch.Tensor | None) -> None:
+    """The same for forward mode, whose dual tensors require no gradient: called while a level of it is open."""
+    if torch._C._is_fwd_grad_enabled() and any(t is not None and forward_ad.unpack_dual(t).tangent is not None
+                                               for t in tensors):
+        raise RuntimeError("these calls are not seen by autograd's forward mode, and a tensor has a tangent: pass the "
+                           "primal (torch.autograd.forward_ad.unpack_dual), and make the tangent from the formulas")
 
 
 def _matrix(t: torch.Tensor, what: str, dtype: torch.dtype | None = None) -> torch.Tensor:
@@ -98,6 +107,8 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     + bias in x's type, mean and rstd (n,) float32 for the backward pass."""
     if x.requires_grad or weight is not None and weight.requires_grad or bias is not None and bias.requires_grad:
         _unrecorded()
+    if forward_ad._current_level >= 0:
+        _no_tangents(x, weight, bias)
     x = _matrix(x, "x")
     (n, D), dev = x.shape, x.device
     if D == 0:
@@ -116,6 +127,8 @@ def layer_norm_grad(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd:
     rstd it returned: dx in x's type, dweight and dbias (D,) float32."""
     if any(t is not None and t.requires_grad for t in (dy, x, mean, rstd, weight)):
         _unrecorded()
+    if forward_ad._current_level >= 0:
+        _no_tangents(dy, x, mean, rstd, weight)
     x = _matrix(x, "x")
     dy = _matrix(dy, "dy", x.dtype)
     (n, D), dev = x.shape, x.device
@@ -156,6 +169,8 @@ def route(logits: torch.Tensor, k: int, *, scores: str = "softmax", bias: torch.
     row's chosen scores."""
     if logits.requires_grad or bias is not None and bias.requires_grad:
         _unrecorded()
+    if forward_ad._current_level >= 0:
+        _no_tangents(logits, bias)
     logits = _matrix(logits, "logits")
     (n, E), dev = logits.shape, logits.device
     how = _scores(scores)
@@ -180,6 +195,8 @@ def route_grad(dweights: torch.Tensor, logits: torch.Tensor, ids: torch.Tensor, 
     choice (ids) held fixed; a balancing bias has none."""
     if dweights.requires_grad or logits.requires_grad:
         _unrecorded()
+    if forward_ad._current_level >= 0:
+        _no_tangents(dweights, logits)
     logits = _matrix(logits, "logits")
     (n, E), dev = logits.shape, logits.device
     how = _scores(scores)
@@ -281,6 +298,8 @@ def expert_products(x: torch.Tensor, plan: ExpertPlan, weights: torch.Tensor, w_
     not; in float16 one beyond 65504 makes its row infinite or NaN."""
     if x.requires_grad or weights.requires_grad or w_in.requires_grad or w_out.requires_grad:
         _unrecorded()
+    if forward_ad._current_level >= 0:
+        _no_tangents(x, weights, w_in, w_out)
     x, weights, w_in, w_out, n, k, D, F, E = _expert_args(x, plan, weights, w_in, w_out)
     dev, dt, lib = x.device, DTYPES[x.dtype], _lib.load()
     nbytes = lib.yabt_experts_workspace_bytes(dt, n, k, D, F, E)
@@ -304,6 +323,8 @@ def expert_products_grad(dy: torch.Tensor, x: torch.Tensor, plan: ExpertPlan, we
     if dy.requires_grad or x.requires_grad or weights.requires_grad or w_in.requires_grad or w_out.requires_grad or \
             inner.requires_grad:
         _unrecorded()
+    if forward_ad._current_level >= 0:
+        _no_tangents(dy, x, weights, w_in, w_out, inner)
     x, weights, w_in, w_out, n, k, D, F, E = _expert_args(x, plan, weights, w_in, w_out)
     dy = _matrix(dy, "dy", x.dtype)
     dev, dt, lib = x.device, DTYPES[x.dtype], _lib.load()

@@ -10,15 +10,16 @@ Beside its routed experts a layer may have a block that every row passes.
 Values are float32, bfloat16 or float16, sums float32, those of 8-bit codes exact.
 Every call runs on the current stream and neither waits nor reads anything back, so
 it can be captured into a HIP graph.  Autograd does not see these calls: a tensor
-that requires a gradient is refused while it records, as in ``expert_ops``.
+that requires a gradient is refused while it records, and one with a tangent, as in ``expert_ops``.
 """
 
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
-from .expert_ops import DTYPES, _at, _call, _ld, _matrix, _unrecorded, _vector
+from .expert_ops import DTYPES, _at, _call, _ld, _matrix, _no_tangents, _unrecorded, _vector
 
 ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2, "relu": 3}
 MAX_INT8_TERMS = 131071        # of a sum of 8-bit products that stays in 32 bits
@@ -67,6 +68,8 @@ def feed_forward(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, *, ac
     In float32 an infinite x or weight may count as NaN."""
     if x.requires_grad or w_in.requires_grad or w_out.requires_grad:
         _unrecorded()
+    if forward_ad._current_level >= 0:
+        _no_tangents(x, w_in, w_out)
     act = _activation(activation)
     x, w_in, w_out, n, D, F, O = _block(x, w_in, w_out, None)
     dev, dt, lib = x.device, DTYPES[x.dtype], _lib.load()
@@ -90,6 +93,8 @@ def feed_forward_grad(dy: torch.Tensor, x: torch.Tensor, w_in: torch.Tensor, w_o
     scale dy for them and the results back."""
     if dy.requires_grad or x.requires_grad or w_in.requires_grad or w_out.requires_grad:
         _unrecorded()
+    if forward_ad._current_level >= 0:
+        _no_tangents(dy, x, w_in, w_out)
     act = _activation(activation)
     x, w_in, w_out, n, D, F, O = _block(x, w_in, w_out, None)
     dy = _matrix(dy, "dy", x.dtype)
@@ -119,6 +124,8 @@ def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     scale NaN.  Of a weight (O, D), its rows are the output's channels."""
     if x.requires_grad:
         _unrecorded()
+    if forward_ad._current_level >= 0:
+        _no_tangents(x)
     x = _matrix(x, "x")
     (n, D), dev = x.shape, x.device
     if D < 1 or n >= 1 << 24 or D > 1 << 24:
@@ -149,6 +156,8 @@ def product_int8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scal
     131071) and rounded to float32 once."""
     if a_scale.requires_grad or b_scale.requires_grad:
         _unrecorded()
+    if forward_ad._current_level >= 0:
+        _no_tangents(a_scale, b_scale)
     if dtype not in DTYPES:
         raise ValueError(f"dtype must be float32, bfloat16 or float16, got {dtype}")
     a, b = _codes(a, "a"), _codes(b, "b")
@@ -176,6 +185,8 @@ def feed_forward_int8(x: torch.Tensor, w_in: torch.Tensor, in_scale: torch.Tenso
     argument, and h's rows are put in 8 bits before w_out.  y (n, O) in x's type."""
     if x.requires_grad or in_scale.requires_grad or out_scale.requires_grad:
         _unrecorded()
+    if forward_ad._current_level >= 0:
+        _no_tangents(x, in_scale, out_scale)
     act = _activation(activation)
     x, w_in, w_out, n, D, F, O = _block(x, w_in, w_out, torch.int8)
     dev, lib = x.device, _lib.load()

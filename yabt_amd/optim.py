@@ -20,6 +20,7 @@ from itertools import chain
 from operator import attrgetter
 
 import torch
+from torch.autograd import forward_ad
 
 from . import expert_ops
 from .expert_ops import DTYPES
@@ -166,6 +167,8 @@ def adamw_step(params: list[torch.Tensor], grads: list[torch.Tensor | None], sta
         return
     if torch.is_grad_enabled() and (any(map(_NEEDS, params)) or any(map(_NEEDS, grads))):
         expert_ops._unrecorded()
+    if forward_ad._current_level >= 0:
+        expert_ops._no_tangents(*params, *grads, *chain.from_iterable(_moments(state)))
     sizes = list(map(_numel, params))
     lists, dev = _checked(state, sizes)
     at, number = 0, 1
