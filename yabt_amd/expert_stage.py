@@ -128,6 +128,8 @@ class ExpertStage:
         if p.state_bits not in (32, 8) or not 0.0 <= p.weight_decay <= 1e30:
             raise ValueError(f"state_bits must be 32 or 8 and weight_decay not negative, got {p.state_bits}, "
                              f"{p.weight_decay}")
+        if p.weight_decay > 0.0 and p.learning_rate < 0.0:
+            raise ValueError(f"a learning_rate below 0 has no weight_decay, got {p.learning_rate}, {p.weight_decay}")
 
     def _inputs(self, X: np.ndarray) -> torch.Tensor:
         Xt = torch.as_tensor(np.asarray(X, dtype=np.float32), device=self.device_)
@@ -257,9 +259,12 @@ class ExpertStage:
                 grads = self._backward(g, kept)
                 # 1e-8 beside the square root of the second moment as it is
                 eps = 1e-8 / (1 - 0.999 ** step) ** 0.5
+                if p.learning_rate < 0.0:
+                    # up the gradient, which a step of the opposite one does with the same bits
+                    grads = {m: -t for m, t in grads.items()}
                 for names, decay, state in groups:
                     optim.adamw_step([self.weights_[m] for m in names], [grads[m] for m in names], state, step,
-                                     lr=p.learning_rate, eps=eps, weight_decay=decay)
+                                     lr=abs(p.learning_rate), eps=eps, weight_decay=decay)
                 # experts with more than their share become a little less likely
                 share = kept[7].offsets.diff().float()
                 self.bias_ -= p.balance_step * torch.sign(share - share.mean())
