@@ -650,6 +650,13 @@ int yabt_feed_forward(int dtype, int act, const void *x, int64_t ldx, int64_t n,
                       const void *w_in, const void *w_out, void *workspace, size_t workspace_bytes,
                       void *out_inner, void *y, int64_t ldy, yabt_stream_t stream);
 
+/* Which kernels make the block's products of these sizes, for tests and profiles; -1
+ * where they are out of range.  Bits 0 and 1: h and y by the kernel for few rows; bits 2 to
+ * 5: large tiles (256 x 256, fp32 128 x 256; else 64 x 128) for h, y, the inner gradient, and the
+ * three other gradients; bits 6 to 9: these in parts over the summed dimension (the last: any of
+ * the three); bit 10: y of h in fp32 (fp32) or in two parts of the type. */
+int yabt_feed_forward_forms(int dtype, int64_t n, int D, int F, int O);
+
 /* Its gradients from dy (n, O) and the forward pass's inner: dx (n, D), dw_in
  * (2 F, D), dw_out (O, F), all of `dtype`.  The inner gradients are rounded to
  * `dtype`, in fp16 with its range.  inner, if it was moved, begins as far from a multiple
@@ -686,6 +693,9 @@ int yabt_feed_forward_int8(int dtype, int act, const void *x, int64_t ldx, int64
                            const int8_t *w_in, const float *in_scale, const int8_t *w_out,
                            const float *out_scale, void *workspace, size_t workspace_bytes, void *y,
                            int64_t ldy, yabt_stream_t stream);
+/* As yabt_feed_forward_forms, bits 0 to 3, 6 and 7 (256 x 256 tiles); bits 10 and 11: x and h are put
+ * in 8 bits by the products' blocks. */
+int yabt_feed_forward_int8_forms(int64_t n, int D, int F, int O);
 
 #ifdef __cplusplus
 }

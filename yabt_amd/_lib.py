@@ -121,6 +121,8 @@ SIGNATURES = {
     "yabt_feed_forward_grad_workspace_bytes": (_sz, [_int, _i64, _int, _int, _int]),
     "yabt_feed_forward_grad": (_int, [_int, _int, _vp, _i64, _vp, _i64, _i64, _int, _int, _int, _vp, _vp, _vp, _vp,
                                       _sz, _vp, _i64, _vp, _vp, _vp]),
+    "yabt_feed_forward_forms": (_int, [_int, _i64, _int, _int, _int]),
+    "yabt_feed_forward_int8_forms": (_int, [_i64, _int, _int, _int]),
     "yabt_quantize_rows": (_int, [_int, _vp, _i64, _i64, _int, _vp, _i64, _vp, _vp]),
     "yabt_product_int8_workspace_bytes": (_sz, [_i64, _int, _int]),
     "yabt_product_int8": (_int, [_vp, _i64, _vp, _i64, _int, _vp, _i64, _vp, _int, _int, _vp, _sz, _vp, _i64, _vp]),

@@ -1753,6 +1753,15 @@ int yabt_feed_forward(int dtype, int act, const void* x, int64_t ldx, int64_t n,
     });
 }
 
+int yabt_feed_forward_forms(int dtype, int64_t n, int D, int F, int O) {
+    FeedSizes z;
+    if (!feed_sizes_ok(dtype, n, D, F, O, &z)) return -1;
+    return (int)z.few | (int)z.few_out << 1 | (int)(z.large_in && !z.few) << 2 | (int)(z.large_out && !z.few_out) << 3 |
+           (int)z.large_dh << 4 | (int)z.large_grads << 5 | (int)(z.splits_in > 1) << 6 |
+           (int)(!z.few_out && z.splits_out > 1) << 7 | (int)(z.splits_dh > 1) << 8 |
+           (int)(z.splits[0] > 1 || z.splits[1] > 1 || z.splits[2] > 1) << 9 | (int)z.whole << 10;
+}
+
 size_t yabt_feed_forward_grad_workspace_bytes(int dtype, int64_t n, int D, int F, int O) {
     FeedSizes z;
     if (!feed_sizes_ok(dtype, n, D, F, O, &z)) return 0;
@@ -1832,6 +1841,15 @@ size_t yabt_feed_forward_int8_workspace_bytes(int64_t n, int D, int F, int O) {
     Carve c{nullptr, 0};
     Feed8Space s;
     return carve_feed8(c, &s, n, D, F, O) + 256;
+}
+
+int yabt_feed_forward_int8_forms(int64_t n, int D, int F, int O) {
+    if (!feed8_ranges_ok(n, D, F, O)) return -1;
+    const Int8Sizes z = int8_sizes(n, O, F);
+    const bool few = few_rows(n), large = large_product(1, n, 2 * (int64_t)F, D);
+    return (int)few | (int)few << 1 | (int)(large && !few) << 2 | (int)(z.large && !few) << 3 |
+           (int)(splits_in8(n, D, F) > 1) << 6 | (int)(z.splits > 1 && !few) << 7 | (int)(few && few_values(n, D)) << 10 |
+           (int)(few && few_values(n, F)) << 11;
 }
 
 int yabt_feed_forward_int8(int dtype, int act, const void* x, int64_t ldx, int64_t n, int D, int F, int O,
