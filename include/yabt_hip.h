@@ -642,6 +642,8 @@ int yabt_adamw_values(int count, const yabt_adamw_tensor *tensors, yabt_stream_t
  * the backward pass.  h is rounded to `dtype` before the second product (16 rows or
  * fewer of narrow blocks: to two parts of it), so that in fp16 one beyond 65504
  * makes its row infinite or NaN; sums are fp32.  n below 2^31 - 256, D, F, O to 2^24.
+ * In fp32 an infinite x or weight may count as NaN, and values below 2^-110 are taken to 2^-133 (the
+ * forward pass of 64 rows or fewer in full).
  * Sums are added in an order that the sizes fix.  Sizes whose launches would have 2^32
  * threads are refused; the size queries then answer 0 (8-bit products too). */
 size_t yabt_feed_forward_inner_bytes(int dtype, int64_t n, int D, int F, int O);

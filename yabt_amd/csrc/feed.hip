@@ -288,7 +288,10 @@ struct Loader {
 
 // fp32 values in three parts of bf16, 8 bits of the significand each: x = hi + mid + lo exactly, each
 // part cut off, so that none is larger than x.  A product of two has nine products of parts; the
-// three smallest, at most 2^-23 of it together, are left out.
+// three smallest are left out.  mid ends at 2^-7 of x and lo at 2^-15, so they are up to 2^-21 of the product
+// together, 2^-24.5 on average, and have its sign: sums of terms of one sign come out low by as much (with nearest parts
+// they would not, but values next to the largest would become infinite).  A part ends at bf16's least step, 2^-133:
+// values below 2^-110 are taken to that.
 __device__ __forceinline__ void in_parts(u32x4 a, u32x4 b, u32x4 (&part)[3]) {
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
