@@ -639,9 +639,9 @@ int yabt_adamw_values(int count, const yabt_adamw_tensor *tensors, yabt_stream_t
  * all of `dtype`; act 0 silu (g / (1 + exp(-g))), 1 gelu (g times the normal
  * distribution function), 2 gelu_tanh (its usual form by tanh), 3 relu.
  * out_inner (yabt_feed_forward_inner_bytes, or NULL) keeps g and u in fp32 and h for
- * the backward pass.  h is rounded to `dtype` before the second product (16 rows or
- * fewer of narrow blocks: to two parts of it), so that in fp16 one beyond 65504
- * makes its row infinite or NaN; sums are fp32.  n below 2^31 - 256, D, F, O to 2^24.
+ * the backward pass.  h is rounded to `dtype` before the second product (in small blocks,
+ * 24 / F + 6 / min(D, O) > n / 128, and for y of 16 rows or fewer with n F O <= 2^26 to two parts of it), so that in fp16 one
+ * beyond 65504 makes its row infinite or NaN; sums are fp32.  n below 2^31 - 256, D, F, O to 2^24.
  * In fp32 an infinite x or weight may count as NaN, and values below 2^-110 are taken to 2^-133 (the
  * forward pass of 64 rows or fewer in full).
  * Sums are added in an order that the sizes fix.  Sizes whose launches would have 2^32
@@ -656,12 +656,13 @@ int yabt_feed_forward(int dtype, int act, const void *x, int64_t ldx, int64_t n,
  * where they are out of range.  Bits 0 and 1: h and y by the kernel for few rows; bits 2 to
  * 5: large tiles (256 x 256, fp32 128 x 256; else 64 x 128) for h, y, the inner gradient, and the
  * three other gradients; bits 6 to 9: these in parts over the summed dimension (the last: any of
- * the three); bit 10: y of h in fp32 (fp32) or in two parts of the type. */
+ * the three); bit 10: y by the kernel for few rows of h in fp32; bit 11: h and the inner gradients
+ * in two parts of the type. */
 int yabt_feed_forward_forms(int dtype, int64_t n, int D, int F, int O);
 
 /* Its gradients from dy (n, O) and the forward pass's inner: dx (n, D), dw_in
  * (2 F, D), dw_out (O, F), all of `dtype`.  The inner gradients are rounded to
- * `dtype`, in fp16 with its range.  inner, if it was moved, begins as far from a multiple
+ * `dtype` (in small blocks to two parts of it), in fp16 with its range.  inner, if it was moved, begins as far from a multiple
  * of 256 bytes as it did.  n = 0 gives zeros for the weights. */
 size_t yabt_feed_forward_grad_workspace_bytes(int dtype, int64_t n, int D, int F, int O);
 int yabt_feed_forward_grad(int dtype, int act, const void *dy, int64_t lddy, const void *x, int64_t ldx,

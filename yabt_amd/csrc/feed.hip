@@ -31,9 +31,11 @@
 // 4096 x 2048 -> 4096 -> 2048, fp32: 1030 us, 200 TFLOP/s (the library's fp32 product: 153).
 //
 // 16-bit types: h, dg and du are rounded to the inputs' type, as the matrix cores
-// take them (for 16 rows or fewer, whose time is the weights', h is taken in two parts and
-// keeps 16 bits); g and u are kept in fp32 for the backward pass.  So an output has
-// two roundings behind it, its own and that of one factor.  8 bits: h is kept in fp32
+// take them; g and u are kept in fp32 for the backward pass.  So an output has
+// two roundings behind it, its own and that of one factor, and 1.41 times the error of its own, where
+// many values average.  In a small block (twice_ok) one large value may decide, and the error was up to 2.2 times; there
+// h, dg and du are kept in two parts of the type, 16 bits or more, and their products made of both.  y of 16 rows or
+// fewer, whose time is the weights', takes h in two parts too, unless the block is so wide that y goes by tiles.  8 bits: h is kept in fp32
 // until its row's largest magnitude is known, sums of codes are whole numbers.
 
 #include "tiles.h"
@@ -70,6 +72,8 @@ struct Product {
                                       // (splits, M, 2 Fi): of g from 0, of u from Fi; DH (splits, M, Fi)
     int splits;
     int x_dtype;                      // few rows of 8 bits: the type of a's values
+    int64_t again;                    // values from h's, or dpre's, first part to its second, 0: it has one
+    int64_t again_a, again_b;         // the same of an operand in two parts (TWICE); of the other 0
 };
 
 template <typename T> struct Sums { using Four = f32x4; using Block = f32x16; };
@@ -165,7 +169,8 @@ __device__ __forceinline__ void lds_fill_from(const char* from, uint32_t off, ui
 // The pieces of an operand that a thread brings to LDS.  Pieces past the end of the
 // summed dimension are zero, rows and columns past the product's end repeat the last
 // (their sums are not stored).
-template <typename T, int MODE, bool SIDE_B, int W, int COUNT, int NT, int STEP>
+// PAIR: the rows' operand in two parts of the type, their rows alternately by 32.
+template <typename T, int MODE, bool SIDE_B, int W, int COUNT, int NT, int STEP, bool PAIR = false>
 struct Loader {
     static constexpr bool ACROSS = SIDE_B ? MODE >= DH : MODE >= DWIN;
     static constexpr bool GATED = SIDE_B && (MODE == IN || MODE == IN8);
@@ -200,6 +205,12 @@ struct Loader {
                 const int f = min(first + (r >> 6) * 32 + (r & 31), P.F - 1);
                 ptr[i] = base + (size_t)((r >> 5 & 1 ? P.F : 0) + f) * ld + piece;
                 off[i] = (uint32_t)((r >> 5 & 1 ? P.F : 0) + f - first) * (uint32_t)(ld * sizeof(T)) + piece * sizeof(T);
+            } else if constexpr (PAIR) {
+                static_assert(!SIDE_B && !ACROSS, "of the rows' operand along the summed dimension");
+                const int row = min(first + (r >> 6) * 32 + (r & 31), P.M - 1);
+                const size_t part = r >> 5 & 1 ? (size_t)P.again_a : 0;
+                ptr[i] = base + (size_t)row * ld + piece + part;
+                off[i] = (uint32_t)(row - first) * (uint32_t)(ld * sizeof(T)) + (piece + (uint32_t)part) * sizeof(T);
             } else if constexpr (!ACROSS) {
                 const int row = min(first + r, (SIDE_B ? P.N : P.M) - 1);
                 ptr[i] = base + (size_t)row * ld + piece;
@@ -230,28 +241,28 @@ struct Loader {
         }
     }
 
-    // pieces LO .. HI - 1 of step t, which begins at k0 (at the end or before it)
+    // pieces LO .. HI - 1 of step t, which begins at k0 (at the end or before it), `again` values further on
     template <int LO = 0, int HI = COUNT>
-    __device__ __forceinline__ void fill(const Product& P, int t, int k0, int end, uint32_t lds) const {
+    __device__ __forceinline__ void fill(const Product& P, int t, int k0, int end, uint32_t lds, int64_t again = 0) const {
         auto place = [&](int i) {
             return __builtin_amdgcn_readfirstlane(lds + (uint32_t)(i * NT * 16) + ((threadIdx.x & ~63u) << 4));
         };
         if (k0 + STEP / (int)sizeof(T) <= end) {
-            const char* const from = begin + (size_t)t * step;
+            const char* const from = begin + (size_t)t * step + (size_t)again * sizeof(T);
 #pragma unroll
             for (int i = LO; i < HI; ++i) lds_fill_from(from, off[i], place(i));
         } else {
 #pragma unroll
             for (int i = LO; i < HI; ++i) {
                 const T* p = at(P, i, k0, end);
-                lds_fill(p ? (const void*)p : (const void*)&g_zeros, place(i));
+                lds_fill(p ? (const void*)(p + again) : (const void*)&g_zeros, place(i));
             }
         }
     }
 
     // the same through registers, for rows at any address: the values that
     // exist, zeros for the others
-    __device__ __forceinline__ void fetch(const Product& P, int k0, int end, int first, u32x4* v) const {
+    __device__ __forceinline__ void fetch(const Product& P, int k0, int end, int first, u32x4* v, int64_t again = 0) const {
         typedef T VT __attribute__((ext_vector_type(CH)));
 #pragma unroll
         for (int i = 0; i < COUNT; ++i) {
@@ -260,6 +271,7 @@ struct Loader {
             if (p) {
                 const int piece = piece_of(i) * CH;
                 int have;
+                p += again;
                 if constexpr (ACROSS) {
                     // the column clamp of init() does not hold pieces that end past the row
                     const int w = width(P);
@@ -315,7 +327,7 @@ template <int BM_, int BN_, int WM_, int WN_>
 struct TileParts {
     static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, STEP = 128;
     static constexpr int NT = 64 * WM * WN;
-    static constexpr int MI = BM / WM / 32, NI = BN / WN / 32;
+    static constexpr int MI = BM / WM / 32, NI = BN / WN / 32, ROWS = BM;
     static constexpr int APART = BM * 64, BPART = BN * 64, PLACE = 3 * (APART + BPART);   // a part's bytes, a step's
     static constexpr int LDS = 2 * PLACE;
     static constexpr int NA = APART / 16 / NT, NB = BPART / 16 / NT;                      // pieces of 8 values a thread
@@ -512,6 +524,21 @@ struct Tiles {
     uint32_t first, count, blocks;
 };
 
+// Small tiles of a product with an operand in two parts of the type.  Of the rows' operand along the summed dimension
+// both parts are rows of one tile, so that the columns' is read once (PAIR); else every step is made twice, of the first part and
+// of the second, the other operand the same (TWICE: dW_in and dW_out, whose sums over a small block's rows have few steps).
+struct TilePair : TileOf<128, 128, 2, 2, 128, 2, 2> { static constexpr int ROWS = 64; };
+struct TileTwice : TileOf<64, 128, 2, 2, 128, 2, 2> {};
+template <typename TL> constexpr bool PAIR = std::is_same_v<TL, TilePair>;
+template <typename TL> constexpr bool TWICE = std::is_same_v<TL, TileTwice>;
+
+// What a value's rounding to T leaves of it, the second part.
+template <typename T>
+__device__ __forceinline__ void rest_of(const float* v, float (&rest)[4]) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) rest[q] = v[q] - (float)(T)v[q];
+}
+
 // One tile of the product MODE: that of the block with number `block` of the product's.
 template <typename T, int MODE, typename TL, bool DMA>
 __device__ __forceinline__ void feed_tile(const Product& P, uint32_t block, const Tiles& G) {
@@ -530,13 +557,13 @@ __device__ __forceinline__ void feed_tile(const Product& P, uint32_t block, cons
     const uint32_t in = id - split * per, whole_group = TILE_GROUP * (uint32_t)G.nt, group = in / whole_group;
     const int gin = (int)(in - group * whole_group);
     const int gm = min(TILE_GROUP, G.mt - (int)group * TILE_GROUP);
-    const int mf = ((int)group * TILE_GROUP + gin % gm) * TL::BM;
+    const int mf = ((int)group * TILE_GROUP + gin % gm) * TL::ROWS;
     const int nf = gin / gm * (GATED ? TL::BN / 2 : TL::BN);
 
     constexpr int BK = TL::STEP / (int)sizeof(T), KS = TL::STEP / 32;
     const int part = P.splits == 1 ? P.K : ((P.K + P.splits - 1) / P.splits + BK - 1) / BK * BK;
     const int lo = (int)min((int64_t)P.K, (int64_t)split * part), end = (int)min((int64_t)P.K, (int64_t)lo + part);
-    const int steps = (int)(((int64_t)end - lo + BK - 1) / BK);
+    const int steps = (int)(((int64_t)end - lo + BK - 1) / BK) * (TWICE<TL> ? 2 : 1);
 
     Block acc[TL::MI][TL::NI];
 #pragma unroll
@@ -549,7 +576,7 @@ __device__ __forceinline__ void feed_tile(const Product& P, uint32_t block, cons
     if constexpr (sizeof(T) == 4) {
         if (steps > 0) parts_sums<MODE, TL>(P, mf, nf, lo, end, steps, acc);
     } else if (steps > 0) {
-        Loader<T, MODE, false, TL::BM, TL::NA, TL::NT, TL::STEP> la;
+        Loader<T, MODE, false, TL::BM, TL::NA, TL::NT, TL::STEP, PAIR<TL>> la;
         Loader<T, MODE, true, TL::BN, TL::NB, TL::NT, TL::STEP> lb;
         using LA = decltype(la);
         using LB = decltype(lb);
@@ -566,14 +593,18 @@ __device__ __forceinline__ void feed_tile(const Product& P, uint32_t block, cons
         static_assert(AS == BS || (AS == 3 && BS == 2), "places that the order of the steps is made for");
         u32x4 ra[DMA ? 1 : TL::NA], rb[DMA ? 1 : TL::NB];
         // where step t begins; past the end, from where nothing is read
-        auto from = [&](int t) { return (int)min((int64_t)end, lo + (int64_t)t * BK); };
+        auto of = [&](int t) { return TWICE<TL> ? t >> 1 : t; };
+        auto from = [&](int t) { return (int)min((int64_t)end, lo + (int64_t)of(t) * BK); };
         auto send_a = [&](int t, int place) {
-            if constexpr (DMA) la.fill(P, t, from(t), end, lds_at + (uint32_t)place * TL::ABYTES);
-            else la.fetch(P, from(t), end, mf, ra);
+            const int64_t again = TWICE<TL> && (t & 1) ? P.again_a : 0;
+            if constexpr (DMA) la.fill(P, of(t), from(t), end, lds_at + (uint32_t)place * TL::ABYTES, again);
+            else la.fetch(P, from(t), end, mf, ra, again);
         };
         auto send_b = [&](int t, int place) {
-            if constexpr (DMA) lb.fill(P, t, from(t), end, lds_at + TL::AS * TL::ABYTES + (uint32_t)place * TL::BBYTES);
-            else lb.fetch(P, from(t), end, nf, rb);
+            const int64_t again = TWICE<TL> && (t & 1) ? P.again_b : 0;
+            if constexpr (DMA)
+                lb.fill(P, of(t), from(t), end, lds_at + TL::AS * TL::ABYTES + (uint32_t)place * TL::BBYTES, again);
+            else lb.fetch(P, from(t), end, nf, rb, again);
         };
         auto put = [&](int t) {
             LA::put(lds + (t & 1) * TL::ABYTES, ra);
@@ -644,6 +675,11 @@ __device__ __forceinline__ void feed_tile(const Product& P, uint32_t block, cons
         }
         stage_ready<0>();                            // nothing may reach the LDS of a block that is gone
     }
+    constexpr int MI = PAIR<TL> ? 1 : TL::MI;        // blocks of rows of the product
+    if constexpr (PAIR<TL>) {
+#pragma unroll
+        for (int j = 0; j < TL::NI; ++j) acc[0][j] += acc[1][j];
+    }
 
     // The sums go through LDS, 32 rows of a wave at a time, from the matrix
     // cores' layout (a lane has one column) to four neighbouring columns a lane,
@@ -654,7 +690,7 @@ __device__ __forceinline__ void feed_tile(const Product& P, uint32_t block, cons
     constexpr int LANES = GATED ? W / 8 : W / 4, PASS = 64 / LANES;    // lanes a row, rows at once
     const int c4 = lane % LANES * 4, first = nf + wn * (GATED ? W / 2 : W);   // this lane's columns: first + c4 .. + 3
     const int width = GATED || MODE == DH ? P.Fp : P.N;
-    const bool inside = mf + TL::BM <= P.M && nf + (GATED ? TL::BN / 2 : TL::BN) <= P.N &&
+    const bool inside = mf + TL::ROWS <= P.M && nf + (GATED ? TL::BN / 2 : TL::BN) <= P.N &&
                         (P.F == P.Fp || !(GATED || MODE == DH || MODE == DWIN));
     f32x4 scale[2];                   // of 8-bit products: the columns'
     if constexpr (MODE == IN8 || MODE == OUT8) {
@@ -665,7 +701,7 @@ __device__ __forceinline__ void feed_tile(const Product& P, uint32_t block, cons
     }
     // where the rows of block i begin in an array of this pitch, and this lane's bytes from there
     auto row0 = [&](auto* base, int i, int p, int64_t pitch) {
-        return base + (size_t)(mf + (wm * TL::MI + i) * 32 + p) * (size_t)pitch + first;
+        return base + (size_t)(mf + (wm * MI + i) * 32 + p) * (size_t)pitch + first;
     };
     auto lane_at = [&](int64_t pitch) { return (uint32_t)(lane / LANES) * (uint32_t)pitch + (uint32_t)c4; };
     const uint32_t at_h = lane_at(P.Fp), at_pre = lane_at(2 * (int64_t)P.Fi), at_dpre = lane_at(2 * (int64_t)P.Fp),
@@ -675,7 +711,7 @@ __device__ __forceinline__ void feed_tile(const Product& P, uint32_t block, cons
         const int f = first + c4;
 #pragma unroll 4
         for (int p = 0; p < 32; p += PASS) {
-            const int at = p + lane / LANES, m = mf + (wm * TL::MI + i) * 32 + at;
+            const int at = p + lane / LANES, m = mf + (wm * MI + i) * 32 + at;
             if (!WHOLE && !(m < P.M && f < width)) continue;
             auto bits = [&](int c) { return *(const lds_f32x4*)(mine + at * W + (c ^ ((at & 4) << 3))); };
             auto whole = [&](int c) {
@@ -710,7 +746,15 @@ __device__ __forceinline__ void feed_tile(const Product& P, uint32_t block, cons
                 if constexpr (MODE == IN8) {
                     if (WHOLE || f < P.Fi) *(f32x4*)(row0(P.h32, i, p, P.Fi) + at_h32) = f32x4{h[0], h[1], h[2], h[3]};
                 } else {
-                    store4(row0((T*)P.h, i, p, P.Fp) + at_h, h);
+                    T* const to = row0((T*)P.h, i, p, P.Fp) + at_h;
+                    store4(to, h);
+                    if constexpr (sizeof(T) == 2 && TL::ROWS <= 64) {
+                        if (P.again) {
+                            float rest[4];
+                            rest_of<T>(h, rest);
+                            store4(to + P.again, rest);
+                        }
+                    }
                     if (P.pre && (WHOLE || f < P.Fi)) {
                         float* const pre = row0(P.pre, i, p, 2 * (int64_t)P.Fi);
                         *(f32x4*)(pre + at_pre) = g;
@@ -740,6 +784,15 @@ __device__ __forceinline__ void feed_tile(const Product& P, uint32_t block, cons
                 T* const dpre = row0((T*)P.dpre, i, p, 2 * (int64_t)P.Fp);
                 store4(dpre + at_dpre, dg);
                 store4(dpre + P.Fp + at_dpre, du);
+                if constexpr (sizeof(T) == 2 && TL::ROWS <= 64) {
+                    if (P.again) {
+                        float rest[4];
+                        rest_of<T>(dg, rest);
+                        store4(dpre + P.again + at_dpre, rest);
+                        rest_of<T>(du, rest);
+                        store4(dpre + P.again + P.Fp + at_dpre, rest);
+                    }
+                }
             } else {
                 const int M = MODE == DWIN ? 2 * P.F : P.M;
                 if (WHOLE && P.splits > 1) {
@@ -759,7 +812,7 @@ __device__ __forceinline__ void feed_tile(const Product& P, uint32_t block, cons
         }
     };
 #pragma unroll
-    for (int i = 0; i < TL::MI; ++i) {
+    for (int i = 0; i < MI; ++i) {
         wave_sync_lds();
         // sum r of block (i, j): row 8 (r / 4) + 4 (lane / 32) + r % 4, column 32 j + lane % 32;
         // the rows of the upper lanes are kept with their blocks in pairs swapped: other banks
@@ -793,10 +846,11 @@ __global__ void __launch_bounds__(TL::NT) k_feed_inner_grad(Product out, Tiles g
     if (blockIdx.x < go.blocks) feed_tile<T, DWOUT, TL, DMA>(out, blockIdx.x, go);
     else feed_tile<T, DH, TL, DMA>(dh, blockIdx.x - go.blocks, gh);
 }
-template <typename T, typename TL, bool DMA>
+template <typename T, typename TL, bool DMA, typename TLX = TL>
 __global__ void __launch_bounds__(TL::NT) k_feed_grads(GradProducts G) {
+    static_assert(TLX::NT == TL::NT, "threads of a block");
     const uint32_t first = G.g[0].blocks, second = first + G.g[1].blocks;
-    if (blockIdx.x < first) feed_tile<T, DX, TL, DMA>(G.p[0], blockIdx.x, G.g[0]);
+    if (blockIdx.x < first) feed_tile<T, DX, TLX, DMA>(G.p[0], blockIdx.x, G.g[0]);
     else if (blockIdx.x < second) feed_tile<T, DWIN, TL, DMA>(G.p[1], blockIdx.x - first, G.g[1]);
     else feed_tile<T, DWOUT, TL, DMA>(G.p[2], blockIdx.x - second, G.g[2]);
 }
@@ -887,10 +941,23 @@ __global__ void __launch_bounds__(256) k_join_inner(Product P) {
             T* const to = (T*)P.dpre + m * 2 * P.Fp + f;
             store4(to, a);
             store4(to + P.Fp, b);
+            if (sizeof(T) == 2 && P.again) {
+                float rest[4];
+                rest_of<T>(a, rest);
+                store4(to + P.again, rest);
+                rest_of<T>(b, rest);
+                store4(to + P.again + P.Fp, rest);
+            }
         } else if constexpr (MODE == IN8) {
             *(f32x4*)(P.h32 + m * P.Fi + f) = f32x4{a[0], a[1], a[2], a[3]};
         } else {
-            store4((T*)P.h + m * P.Fp + f, a);
+            T* const to = (T*)P.h + m * P.Fp + f;
+            store4(to, a);
+            if (sizeof(T) == 2 && P.again) {
+                float rest[4];
+                rest_of<T>(a, rest);
+                store4(to + P.again, rest);
+            }
             if (P.pre && there) {
                 *(f32x4*)(P.pre + m * 2 * P.Fi + f) = g;
                 *(f32x4*)(P.pre + m * 2 * P.Fi + P.Fi + f) = u;
@@ -1174,10 +1241,10 @@ __device__ __forceinline__ void few_codes(const Product& P, lds_char* codes, int
     __syncthreads();
 }
 
-// MODE IN or OUT with T f32, bf16, f16; IN8 or OUT8 with int8_t, CODES: a's values become codes here.
-// OUT's rows are h, of up to 16 in fp32, of more in T.  A block makes R groups of 16 columns for MB
-// groups of 16 rows.
-template <typename T, int MODE, int MB, int R, bool CODES>
+// MODE IN or OUT with T f32, bf16, f16; IN8 or OUT8 with int8_t, FLOATS: a's values become codes here.
+// OUT's rows are h, in fp32 for up to 16 of them and with FLOATS, taken in two parts of a 16-bit T, else in T.  A block
+// makes R groups of 16 columns for MB groups of 16 rows.
+template <typename T, int MODE, int MB, int R, bool FLOATS>
 __global__ void __launch_bounds__(FEW_NT) k_few(Product P) {
     constexpr bool GATED = MODE == IN || MODE == IN8;
     constexpr int G = GATED ? 2 : 1, WAVES = FEW_NT / 64;
@@ -1200,14 +1267,14 @@ __global__ void __launch_bounds__(FEW_NT) k_few(Product P) {
     for (int m = 0; m < R * G; ++m)
 #pragma unroll
         for (int b = 0; b < MB; ++b) acc[m][b] = Four{0, 0, 0, 0};
-    if constexpr (CODES) {
+    if constexpr (FLOATS && sizeof(T) == 1) {
         lds_char* const codes = (lds_char*)s_tiles;
         const int ld = (P.K + 15) / 16 * 16 + 16;        // rows begin at other banks
         if (P.x_dtype == DT_F32) few_codes<float>(P, codes, ld, s_most, s_scale);
         else if (P.x_dtype == DT_BF16) few_codes<bf16>(P, codes, ld, s_most, s_scale);
         else few_codes<f16>(P, codes, ld, s_most, s_scale);
         few_sums<T, R * G, MB>(w, FewCodes{codes, ld, P.M}, P.K, wave, WAVES, acc);
-    } else if constexpr (MODE == OUT && sizeof(T) == 2 && MB == 1) {
+    } else if constexpr (MODE == OUT && sizeof(T) == 2 && (MB == 1 || FLOATS)) {
         few_sums<T, R * G, MB>(w, FewHalves<T>{(const float*)P.a, (size_t)P.lda, P.M}, P.K, wave, WAVES, acc);
     } else {
         few_sums<T, R * G, MB>(w, FewRows<T>{(const T*)P.a, (size_t)P.lda, P.M}, P.K, wave, WAVES, acc);
@@ -1233,7 +1300,7 @@ __global__ void __launch_bounds__(FEW_NT) k_few(Product P) {
             }
             f32x4 v[G];
             if constexpr (sizeof(T) == 1) {
-                const float s = CODES ? s_scale[row] : P.sa[row];
+                const float s = FLOATS ? s_scale[row] : P.sa[row];
 #pragma unroll
                 for (int m = 0; m < G; ++m)
                     v[m] = f32x4{(float)t[m][0], (float)t[m][1], (float)t[m][2], (float)t[m][3]} *
@@ -1249,7 +1316,15 @@ __global__ void __launch_bounds__(FEW_NT) k_few(Product P) {
                 for (int i = 0; i < 4; ++i) h[i] = c + i < P.F ? a[i] * v[G - 1][i] : 0.0f;
                 if (P.h32) *(f32x4*)(P.h32 + (size_t)row * (size_t)P.Fi + c) = f32x4{h[0], h[1], h[2], h[3]};
                 if constexpr (sizeof(T) != 1) {
-                    if (P.h) store_part((T*)P.h + (size_t)row * (size_t)P.Fp + c, f32x4{h[0], h[1], h[2], h[3]}, P.Fp - c);
+                    if (P.h) {
+                        T* const to = (T*)P.h + (size_t)row * (size_t)P.Fp + c;
+                        store_part(to, f32x4{h[0], h[1], h[2], h[3]}, P.Fp - c);
+                        if (sizeof(T) == 2 && P.again) {
+                            float rest[4];
+                            rest_of<T>(h, rest);
+                            store_part(to + P.again, f32x4{rest[0], rest[1], rest[2], rest[3]}, P.Fp - c);
+                        }
+                    }
                     if (P.pre) {
                         float* pre = P.pre + (size_t)row * 2 * (size_t)P.Fi + c;
                         *(f32x4*)pre = v[0];
@@ -1327,7 +1402,7 @@ inline int inner_split_count(int mode, int64_t M, int64_t N, int64_t K, bool lar
 template <typename TL>
 bool all_tiles(const Product& P, bool gated, Tiles* g) {
     g->nt = (int)over(P.N, gated ? TL::BN / 2 : TL::BN);
-    g->mt = (int)over(P.M, TL::BM);
+    g->mt = (int)over(P.M, TL::ROWS);
     const double count = (double)g->nt * g->mt * P.splits;
     if (count * TL::NT > 4e9) return false;      // with the other products of a grid below 2^32 threads, checked there
     g->first = 0;
@@ -1361,7 +1436,7 @@ auto by_tile(bool large, bool dma, const F& f) {
 // Makes the tiles of one product; false: the grid would be too large.
 template <typename T, int MODE>
 bool run_tiles(const Product& P, bool large, bool dma, hipStream_t stream) {
-    return by_tile<T>(large, dma, [&](auto tl, auto d) {
+    auto launch = [&](auto tl, auto d) {
         using TL = decltype(tl);
         Tiles g;
         if (!all_tiles<TL>(P, MODE == IN || MODE == IN8, &g) || !grid_ok(g.blocks, TL::NT)) return false;
@@ -1376,7 +1451,11 @@ bool run_tiles(const Product& P, bool large, bool dma, hipStream_t stream) {
         }
         k_feed<T, MODE, TL, decltype(d)::value><<<g.blocks, TL::NT, TL::LDS, stream>>>(P, g);
         return true;
-    });
+    };
+    if constexpr (MODE == OUT && sizeof(T) == 2) {
+        if (P.again_a) return dma ? launch(TilePair(), std::true_type()) : launch(TilePair(), std::false_type());
+    }
+    return by_tile<T>(large, dma, launch);
 }
 
 inline void run_join(const Joins& J, hipStream_t stream) {
@@ -1394,23 +1473,23 @@ void run_join_inner(const Product& P, hipStream_t stream) {
     if (P.splits > 1 && work > 0) k_join_inner<T, MODE><<<launch_grid(work, 256, 8192), 256, 0, stream>>>(P);
 }
 
-template <typename T, int MODE, int MB, int R, bool CODES>
+template <typename T, int MODE, int MB, int R, bool FLOATS>
 void launch_few(const Product& P, hipStream_t stream) {
-    const size_t lds = CODES ? (size_t)P.M * (size_t)((P.K + 15) / 16 * 16 + 16) : 0;
-    k_few<T, MODE, MB, R, CODES><<<(unsigned)over(P.N, 16 * R), FEW_NT, lds, stream>>>(P);
+    const size_t lds = FLOATS && sizeof(T) == 1 ? (size_t)P.M * (size_t)((P.K + 15) / 16 * 16 + 16) : 0;
+    k_few<T, MODE, MB, R, FLOATS><<<(unsigned)over(P.N, 16 * R), FEW_NT, lds, stream>>>(P);
 }
-template <typename T, int MODE, bool CODES>
+template <typename T, int MODE, bool FLOATS>
 void run_few(const Product& P, hipStream_t stream) {
     // more columns a block read x less often, but leave fewer blocks.  One group and two, us for the block: 2048 ->
     // 5632 -> 2048, bf16, 24 rows 31.8 and 28.9, 64 rows 54.7 and 45.7; fp32 500 -> 700 -> 500, 20 rows 11.7 and
     // 16.3; of y's 2048 columns 31.8 and 36.0 (24 rows)
     auto by_rows = [&](auto r) {
         constexpr int R = decltype(r)::value;
-        if (P.M <= 32) launch_few<T, MODE, 2, R, CODES>(P, stream);
-        else if (P.M <= 48) launch_few<T, MODE, 3, R, CODES>(P, stream);
-        else launch_few<T, MODE, 4, R, CODES>(P, stream);
+        if (P.M <= 32) launch_few<T, MODE, 2, R, FLOATS>(P, stream);
+        else if (P.M <= 48) launch_few<T, MODE, 3, R, FLOATS>(P, stream);
+        else launch_few<T, MODE, 4, R, FLOATS>(P, stream);
     };
-    if (P.M <= 16) return launch_few<T, MODE, 1, 1, CODES>(P, stream);
+    if (P.M <= 16) return launch_few<T, MODE, 1, 1, FLOATS && sizeof(T) == 1>(P, stream);
     if constexpr (MODE == IN || MODE == IN8) {
         if (over(P.N, 32) >= 128) return by_rows(std::integral_constant<int, 2>());
     }
@@ -1460,10 +1539,21 @@ inline bool large_gradients(int bytes, const int64_t (&M)[3], const int64_t (&N)
 // rows 15.4 and 18.2: few throughout.)
 inline bool few_answer(int64_t n, int64_t F, int64_t O, int bytes) { return over(O, 16) * n * F * bytes <= (8 << 20); }
 
+// A small block: one large value of h, or of an output, may decide the error of all, and h, dg and du are taken in two parts
+// of a 16-bit type.  The error's square is that of one rounding times 1 + a weighted mean over h's values (their fourth
+// moment is some 24 squares of the second) over one over the outputs' (6): a variance of 24 / (n F) + 6 / (n min(D, O)), up
+// to 1 / 128 left as it is.  Of 44 500 random blocks more than 1.5 times one rounding's error had 19% of those
+// below (up to 2.2 times) and 0.5% of the others.
+inline bool twice_ok(int64_t n, int D, int F, int O, int bytes) {
+    const double w = D < O ? D : O;
+    return bytes == 2 && 128.0 * (24.0 / F + 6.0 / w) > (double)n && n * F < (1 << 28);      // parts: 32 bits apart
+}
+
 struct FeedSizes {
     int64_t n;
     int D, F, O, bytes, Fp, Fi;
-    bool few, few_out, whole;         // few rows: h and y by their kernel; so few that h is kept in fp32 for y
+    bool few, few_out, whole;         // few rows: h and y by their kernel; h is kept in fp32 for y
+    bool twice;                       // h, dg and du in two parts
     bool large_in, large_out, large_dh, large_grads;
     int splits_in, splits_out;        // of [g u], of y
     int splits_dh, splits[3];         // of dh; of dx, dW_in, dW_out
@@ -1475,8 +1565,6 @@ inline FeedSizes feed_sizes(int dtype, int64_t n, int D, int F, int O) {
     z.Fp = up16(F, b);
     z.Fi = up16(F, 4);
     z.few = few_rows(n);
-    z.whole = n <= 16 && few_answer(n, F, O, 2);
-    z.few_out = z.whole || (n > 16 && z.few && few_answer(n, F, O, b));
     z.large_in = large_product(b, n, 2 * (int64_t)F, D);
     z.large_out = large_product(b, n, O, F);
     z.splits_out = split_count(n, O, F, z.large_out, b);
@@ -1485,8 +1573,11 @@ inline FeedSizes feed_sizes(int dtype, int64_t n, int D, int F, int O) {
     z.splits_dh = inner_split_count(DH, n, F, O, z.large_dh, b);
     const int64_t M[3] = {n, (int64_t)z.Fp + F, O}, N[3] = {D, D, F}, K[3] = {(int64_t)z.Fp + F, n, n};
     z.large_grads = large_gradients(b, M, N, K, z.splits);
-    if (!z.large_grads)
-        for (int i = 0; i < 3; ++i) z.splits[i] = split_count(M[i], N[i], K[i], false, b);
+    z.twice = twice_ok(n, D, F, O, b) && !(z.large_in || z.large_out || z.large_dh || z.large_grads);
+    z.whole = (n <= 16 || (z.few && z.twice && n * F < 16384)) && few_answer(n, F, O, 2);
+    z.few_out = z.whole || (n > 16 && z.few && !z.twice && few_answer(n, F, O, b));
+    if (!z.large_grads)                   // of the products whose steps are made twice, as many as of twice the length
+        for (int i = 0; i < 3; ++i) z.splits[i] = split_count(M[i], N[i], K[i] * (z.twice && i ? 2 : 1), false, b);
     return z;
 }
 
@@ -1529,7 +1620,7 @@ struct FeedKept {                     // what the forward pass keeps
 };
 inline size_t carve_kept(Carve& c, FeedKept* k, const FeedSizes& z) {
     k->pre = c.take<float>((size_t)z.n * 2 * z.Fi);
-    k->h = c.take<char>((size_t)z.n * z.Fp * z.bytes);
+    k->h = c.take<char>((size_t)z.n * z.Fp * z.bytes * (z.twice ? 2 : 1));
     return c.off;
 }
 struct FeedSpace {
@@ -1539,7 +1630,7 @@ struct FeedSpace {
     float* part;
 };
 inline size_t carve_forward(Carve& c, FeedSpace* s, const FeedSizes& z) {
-    s->h = c.take<char>((size_t)z.n * z.Fp * z.bytes);
+    s->h = c.take<char>((size_t)z.n * z.Fp * z.bytes * (z.twice ? 2 : 1));
     s->h32 = z.whole ? c.take<float>((size_t)z.n * z.Fi) : nullptr;
     s->part_in = z.splits_in > 1 ? c.take<float>((size_t)z.splits_in * z.n * 2 * z.Fi) : nullptr;
     s->part = !z.few_out && z.splits_out > 1 ? c.take<float>((size_t)z.splits_out * z.n * z.O) : nullptr;
@@ -1552,7 +1643,7 @@ struct GradSpace {
 };
 inline size_t carve_backward(Carve& c, GradSpace* s, const FeedSizes& z) {
     const int64_t M[3] = {z.n, 2 * (int64_t)z.F, z.O}, N[3] = {z.D, z.D, z.F};
-    s->dpre = c.take<char>((size_t)z.n * 2 * z.Fp * z.bytes);
+    s->dpre = c.take<char>((size_t)z.n * 2 * z.Fp * z.bytes * (z.twice ? 2 : 1));
     s->part_dh = z.splits_dh > 1 ? c.take<float>((size_t)z.splits_dh * z.n * z.Fi) : nullptr;
     for (int i = 0; i < 3; ++i) s->part[i] = z.splits[i] > 1 ? c.take<float>((size_t)z.splits[i] * M[i] * N[i]) : nullptr;
     return c.off;
@@ -1568,6 +1659,7 @@ int run_feed(const FeedSizes& z, int act, int dtype, const void* x, int64_t ldx,
     P.pre = kept ? kept->pre : nullptr;
     P.h = kept ? kept->h : z.whole ? nullptr : s.h;
     P.h32 = s.h32;
+    P.again = z.twice ? z.n * z.Fp : 0;
     const int b = z.bytes;
     if (z.few) run_few<T, IN, false>(P, stream);
     else if (!run_tiles<T, IN>(P, z.large_in,
@@ -1581,9 +1673,14 @@ int run_feed(const FeedSizes& z, int act, int dtype, const void* x, int64_t ldx,
     Q.a = P.h, Q.lda = z.Fp;
     if (z.few_out) {
         if (z.whole) Q.a = s.h32, Q.lda = z.Fi;
-        run_few<T, OUT, false>(Q, stream);
+        if constexpr (sizeof(T) == 2) {
+            if (z.whole) run_few<T, OUT, true>(Q, stream);
+            else run_few<T, OUT, false>(Q, stream);
+        } else {
+            run_few<T, OUT, false>(Q, stream);
+        }
     } else {
-        Q.splits = z.splits_out, Q.part = s.part;
+        Q.splits = z.splits_out, Q.part = s.part, Q.again_a = P.again;
         if (!run_tiles<T, OUT>(Q, z.large_out, straight_ok(w_out, z.F, z.F, b) && near_ok(256, z.Fp, b), stream))
             return fail(-1, "yabt_feed_forward: bad sizes");
         if (Q.splits > 1) run_join({{{s.part, y, ldy, Q.M, Q.N, Q.splits, dtype, nullptr, nullptr}}, 1}, stream);
@@ -1602,7 +1699,7 @@ int run_feed_grad(const FeedSizes& z, int act, int dtype, const void* dy, int64_
     P.a = dy, P.lda = lddy, P.b = w_out, P.ldb = z.F, P.bw = z.F;
     P.M = (int)z.n, P.N = z.F, P.K = z.O;
     P.F = z.F, P.Fp = z.Fp, P.Fi = z.Fi, P.act = act, P.splits = z.splits_dh, P.part = s.part_dh;
-    P.pre = kept.pre, P.dpre = s.dpre;
+    P.pre = kept.pre, P.dpre = s.dpre, P.again = z.twice ? z.n * 2 * z.Fp : 0;
     GradProducts G = {};
     for (auto& p : G.p) p.F = z.F, p.Fp = z.Fp, p.Fi = z.Fi, p.out_dtype = dtype;
     Product &X = G.p[0], &I = G.p[1], &O = G.p[2];
@@ -1613,27 +1710,47 @@ int run_feed_grad(const FeedSizes& z, int act, int dtype, const void* dy, int64_
     O.a = dy, O.lda = lddy, O.aw = z.O, O.b = kept.h, O.ldb = z.Fp, O.bw = z.Fp;
     O.M = z.O, O.N = z.F, O.K = (int)z.n, O.out = dw_out, O.ldo = z.F;
     for (int i = 0; i < 3; ++i) G.p[i].splits = z.splits[i], G.p[i].part = s.part[i];
-    const bool ok = by_tile<T>(z.large_grads, dma, [&](auto tl, auto d) {
+    X.again_a = I.again_a = P.again, O.again_b = z.twice ? z.n * z.Fp : 0;
+    auto launch_with = [&](auto tl, auto d, auto tlx) {
         using TL = decltype(tl);
-        for (int i = 0; i < 3; ++i)
-            if (!all_tiles<TL>(G.p[i], false, &G.g[i])) return false;
-        if (!grid_ok((int64_t)G.g[0].blocks + G.g[1].blocks + G.g[2].blocks, TL::NT)) return false;
-        Tiles gh;
-        if (z.large_dh == z.large_grads) {
-            if (!all_tiles<TL>(P, false, &gh)) return false;
-            Tiles go = take_last(&G.g[2], beside_inner_grad(z, gh.count, G.g));
-            if (!grid_ok((int64_t)go.blocks + gh.blocks, TL::NT)) return false;
-            if (go.blocks + gh.blocks)
-                k_feed_inner_grad<T, TL, decltype(d)::value>
-                    <<<go.blocks + gh.blocks, TL::NT, TL::LDS, stream>>>(O, go, P, gh);
-        } else if (z.n > 0 && !run_tiles<T, DH>(P, z.large_dh, dma, stream)) {
+        using TLX = decltype(tlx);
+        if (!all_tiles<TLX>(X, false, &G.g[0]) || !all_tiles<TL>(I, false, &G.g[1]) || !all_tiles<TL>(O, false, &G.g[2]))
             return false;
+        if (!grid_ok((int64_t)G.g[0].blocks + G.g[1].blocks + G.g[2].blocks, TL::NT)) return false;
+        bool shared = false;
+        if constexpr (!TWICE<TL>) {                  // the inner gradient's own operands have one part
+            if (z.large_dh == z.large_grads) {
+                Tiles gh;
+                if (!all_tiles<TL>(P, false, &gh)) return false;
+                Tiles go = take_last(&G.g[2], beside_inner_grad(z, gh.count, G.g));
+                if (!grid_ok((int64_t)go.blocks + gh.blocks, TL::NT)) return false;
+                if (go.blocks + gh.blocks)
+                    k_feed_inner_grad<T, TL, decltype(d)::value>
+                        <<<go.blocks + gh.blocks, TL::NT, TL::LDS, stream>>>(O, go, P, gh);
+                shared = true;
+            }
         }
+        if (!shared && z.n > 0 && !run_tiles<T, DH>(P, z.large_dh, dma, stream)) return false;
         run_join_inner<T, DH>(P, stream);
-        k_feed_grads<T, TL, decltype(d)::value>
-            <<<G.g[0].blocks + G.g[1].blocks + G.g[2].blocks, TL::NT, TL::LDS, stream>>>(G);
+        constexpr int lds = TLX::LDS > TL::LDS ? TLX::LDS : TL::LDS;
+        k_feed_grads<T, TL, decltype(d)::value, TLX>
+            <<<G.g[0].blocks + G.g[1].blocks + G.g[2].blocks, TL::NT, lds, stream>>>(G);
         return true;
-    });
+    };
+    auto launch = [&](auto tl, auto d) { return launch_with(tl, d, tl); };
+    bool ok;
+    if (sizeof(T) == 4 || !z.twice) {
+        ok = by_tile<T>(z.large_grads, dma, launch);
+    } else if constexpr (sizeof(T) == 2) {
+        // dx by pairs, whose 64 KB of LDS leave two blocks a CU, unless the grid has more of them.  In one part, by pairs
+        // and with every step twice, us for forward and backward, bf16: 4 x 512 -> 2000 -> 512 27.4, 28.8 and 30.4; one row of
+        // 2048 -> 2048 -> 2048 43.2, 48.5 and 45.6
+        int64_t blocks = 0;
+        for (int i = 0; i < 3; ++i) blocks += tile_count(b, false, G.p[i].M, G.p[i].N) * z.splits[i];
+        ok = !dma                ? launch_with(TileTwice(), std::false_type(), TilePair())
+             : blocks <= 2 * CUS ? launch_with(TileTwice(), std::true_type(), TilePair())
+                                 : launch(TileTwice(), std::true_type());
+    }
     if (!ok) return fail(-1, "yabt_feed_forward_grad: bad sizes");
     Joins J = {};
     for (int i = 0; i < 3; ++i)
@@ -1762,7 +1879,7 @@ int yabt_feed_forward_forms(int dtype, int64_t n, int D, int F, int O) {
     return (int)z.few | (int)z.few_out << 1 | (int)(z.large_in && !z.few) << 2 | (int)(z.large_out && !z.few_out) << 3 |
            (int)z.large_dh << 4 | (int)z.large_grads << 5 | (int)(z.splits_in > 1) << 6 |
            (int)(!z.few_out && z.splits_out > 1) << 7 | (int)(z.splits_dh > 1) << 8 |
-           (int)(z.splits[0] > 1 || z.splits[1] > 1 || z.splits[2] > 1) << 9 | (int)z.whole << 10;
+           (int)(z.splits[0] > 1 || z.splits[1] > 1 || z.splits[2] > 1) << 9 | (int)z.whole << 10 | (int)z.twice << 11;
 }
 
 size_t yabt_feed_forward_grad_workspace_bytes(int dtype, int64_t n, int D, int F, int O) {

@@ -33,6 +33,7 @@ struct TileOf {
     static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, STEP = STEP_, AS = AS_, BS = BS_;
     static constexpr int NT = 64 * WM * WN;
     static constexpr int MI = BM / WM / 32, NI = BN / WN / 32;    // 32 x 32 blocks a wave makes
+    static constexpr int ROWS = BM;                               // of the product
     static constexpr int ABYTES = BM * STEP, BBYTES = BN * STEP;
     static constexpr int LDS = AS * ABYTES + BS * BBYTES;
     static constexpr int NA = ABYTES / 16 / NT, NB = BBYTES / 16 / NT;

@@ -63,8 +63,9 @@ def feed_forward(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, *, ac
     "gelu_tanh" (its usual approximation) or "relu".  With ``keep_inner`` returns
     (y, inner), inner a buffer for the backward pass: g and u in float32 and act(g) * u.
 
-    16-bit types round act(g) * u to theirs before w_out (16 rows or fewer of narrow
-    blocks keep 16 bits of it); in float16 one beyond 65504 makes its row infinite or NaN.
+    16-bit types round act(g) * u to theirs before w_out, and the inner gradients; small
+    blocks (24 / F + 6 / min(D, O) > n / 128) keep 16 bits of them, and y of 16 rows or fewer
+    (n F O <= 2^26) of act(g) * u; in float16 one beyond 65504 makes its row infinite or NaN.
     In float32 an infinite x or weight may count as NaN, and of more than 64 rows x, weights
     and act(g) * u below 2^-110 are taken to 2^-133 (their gradients' factors too)."""
     if x.requires_grad or w_in.requires_grad or w_out.requires_grad:
