@@ -314,25 +314,29 @@ struct Span {
 };
 
 // Whether what a call writes overlaps, or is overlapped by what it reads: thread blocks would meet there in no
-// order.  spans(i, write, read) names tensor i's, up to WRITES and READS of them.  `own_read`: a tensor's own values may be
-// read where they are written, from the same place on in the same width (a thread reads what it alone writes, before).
-// 0, or fails.
+// order.  spans(i, write, read) names tensor i's, up to WRITES and READS of them.  `own_read`: a tensor's own values
+// may be read where they are written, from the same place on in the same width (a thread reads what it alone
+// writes, before).  0, or fails.
 template <int WRITES, int READS, typename Spans>
 int adamw_apart(const char* message, int count, bool own_read, const Spans& spans) {
     std::unique_ptr<Span[]> written(new (std::nothrow) Span[(size_t)count * WRITES]),
         read(new (std::nothrow) Span[(size_t)count * READS]);
     if (!written || !read) return fail(-2, "yabt_adamw: no host memory");
     Span *w = written.get(), *r = read.get();
-    for (int i = 0; i < count; ++i)
-        spans(i, [&](const void* p, int64_t n, int each) { *w++ = {(uintptr_t)p, (uintptr_t)p + (size_t)n * each, i, each}; },
-              [&](const void* p, int64_t n, int each) { *r++ = {(uintptr_t)p, (uintptr_t)p + (size_t)n * each, i, each}; });
+    auto into = [](Span*& to, int i) {
+        return [&to, i](const void* p, int64_t n, int each) {
+            *to++ = {(uintptr_t)p, (uintptr_t)p + (size_t)n * each, i, each};
+        };
+    };
+    for (int i = 0; i < count; ++i) spans(i, into(w, i), into(r, i));
     const Span* const first = written.get();
     std::sort(written.get(), w, [](const Span& a, const Span& b) { return a.lo < b.lo; });
     for (const Span* s = first; s + 1 < w; ++s)
         if (s->hi > s[1].lo) return fail(-3, message);
     for (const Span* s = read.get(); s < r; ++s) {
         // the written spans lie apart: those that begin below s's end, from the last one backwards
-        const Span* t = std::lower_bound(first, (const Span*)w, s->hi, [](const Span& a, uintptr_t at) { return a.lo < at; });
+        const Span* t =
+            std::lower_bound(first, (const Span*)w, s->hi, [](const Span& a, uintptr_t at) { return a.lo < at; });
         while (t > first && (--t)->hi > s->lo)
             if (!(own_read && t->of == s->of && t->lo == s->lo && t->each == s->each)) return fail(-3, message);
     }

@@ -32,11 +32,13 @@
 //
 // 16-bit types: h, dg and du are rounded to the inputs' type, as the matrix cores
 // take them; g and u are kept in fp32 for the backward pass.  So an output has
-// two roundings behind it, its own and that of one factor, and 1.41 times the error of its own, where
-// many values average.  In a small block (twice_ok) one large value may decide, and the error was up to 2.2 times; there
-// h, dg and du are kept in two parts of the type, 16 bits or more, and their products made of both.  y of 16 rows or
-// fewer, whose time is the weights', takes h in two parts too, unless the block is so wide that y goes by tiles.  8 bits: h is kept in fp32
-// until its row's largest magnitude is known, sums of codes are whole numbers.
+// two roundings behind it, its own and that of one factor, and 1.41 times the error
+// of its own, where many values average.  In a small block (twice_ok) one large
+// value may decide, and the error was up to 2.2 times; there h, dg and du are kept in
+// two parts of the type, 16 bits or more, and their products made of both.  y of
+// 16 rows or fewer, whose time is the weights', takes h in two parts too, unless the
+// block is so wide that y goes by tiles.  8 bits: h is kept in fp32 until its row's
+// largest magnitude is known, sums of codes are whole numbers.
 
 #include "tiles.h"
 #include "yabt_hip.h"
@@ -524,9 +526,10 @@ struct Tiles {
     uint32_t first, count, blocks;
 };
 
-// Small tiles of a product with an operand in two parts of the type.  Of the rows' operand along the summed dimension
-// both parts are rows of one tile, so that the columns' is read once (PAIR); else every step is made twice, of the first part and
-// of the second, the other operand the same (TWICE: dW_in and dW_out, whose sums over a small block's rows have few steps).
+// Small tiles of a product with an operand in two parts of the type.  Of the rows' operand along the summed
+// dimension both parts are rows of one tile, so that the columns' is read once (PAIR); else every step is made twice,
+// of the first part and of the second, the other operand the same (TWICE: dW_in and dW_out, whose sums over a small
+// block's rows have few steps).
 struct TilePair : TileOf<128, 128, 2, 2, 128, 2, 2> { static constexpr int ROWS = 64; };
 struct TileTwice : TileOf<64, 128, 2, 2, 128, 2, 2> {};
 template <typename TL> constexpr bool PAIR = std::is_same_v<TL, TilePair>;
@@ -1370,7 +1373,9 @@ inline bool straight_ok(const void* p, int64_t ld, int width, int bytes, int64_t
 // fetch less, or take less apart (fp32), but there have to be enough of them, and a block of theirs has
 // its CU to itself, so that nothing covers its beginning and end unless K is long.  fp32, small and
 // large, us: 4096 x 2048 -> 4096 -> 2048 1240 and 1020, 3000 x 700, 2000, forward and backward 634 and 590; 128 x
-// 128 tiles lie between them where products are large and behind both where they are small.
+// 128 tiles lie between them where products are large and behind both where they are small.  16 and 8 bits, small and
+// large by the number of large ones, us: bf16 n x 2048 -> 2048 -> 4096 64 tiles 55 and 87, 96 77 and 88, 128 105 and 89,
+// 256 180 and 123; 8-bit products n x 2048 x 4096 96 tiles 23.8 and 31.6, 128 33.5 and 32.0, 256 55 and 41.
 inline bool large_product(int bytes, int64_t M, int64_t N, int64_t K) {
     return K * bytes >= 768 && M >= 192 && N >= 192 && tile_count(bytes, true, M, N) >= (bytes == 4 ? 200 : 128);
 }
@@ -1388,12 +1393,13 @@ inline int split_count(int64_t M, int64_t N, int64_t K, bool large, int bytes) {
 
 // The same of the products that become h (IN), or dg and du (DH), whose join is a launch more that reads the
 // parts: where the steps that a block is spared take longer.  A step takes about 0.38 us, DH's 0.6 (0.9 where
-// W_out's rows are not whole pieces), fp32's 1.1, the launch 5 and 100 parts of tiles 1.2.  Whole and in parts, us for the block: fp32 83 x 2520 -> 256
-// -> 2520 106 and 28, 1000 x 2048 -> 512 100 and 61; bf16 83 x 2520 24.5 and 15.5, but 534 x 1000 -> 760 23.5
+// W_out's rows are not whole pieces), fp32's 1.1, the launch 5 and 100 parts of tiles 1.2.  Whole and in
+// parts, us for the block: fp32 83 x 2520 -> 256 -> 2520 106 and 28, 1000 x 2048 -> 512 100 and 61; bf16 83 x 2520 24.5 and 15.5, but 534 x 1000 -> 760 23.5
 // and 27.2 (it stays whole); 8 bits 100 x 4096 -> 1024 33.1 and 28.9, but 1000 x 2048 -> 512 27.0 and 32.9.
 inline int inner_split_count(int mode, int64_t M, int64_t N, int64_t K, bool large, int bytes) {
     const int s = split_count(M, N, K, large, bytes);
-    const double each = bytes == 4 ? 1.1 : mode != DH ? 0.38 : N * bytes % 16 ? 0.9 : 0.6, steps = (double)over(K * bytes, 128);
+    const double each = bytes == 4 ? 1.1 : mode != DH ? 0.38 : N * bytes % 16 ? 0.9 : 0.6;
+    const double steps = (double)over(K * bytes, 128);
     const double spared = steps * (1.0 - 1.0 / s) * each, more = 5.0 + 0.012 * s * (double)tile_count(bytes, false, M, N);
     return spared > more ? s : 1;
 }
@@ -1539,11 +1545,11 @@ inline bool large_gradients(int bytes, const int64_t (&M)[3], const int64_t (&N)
 // rows 15.4 and 18.2: few throughout.)
 inline bool few_answer(int64_t n, int64_t F, int64_t O, int bytes) { return over(O, 16) * n * F * bytes <= (8 << 20); }
 
-// A small block: one large value of h, or of an output, may decide the error of all, and h, dg and du are taken in two parts
-// of a 16-bit type.  The error's square is that of one rounding times 1 + a weighted mean over h's values (their fourth
-// moment is some 24 squares of the second) over one over the outputs' (6): a variance of 24 / (n F) + 6 / (n min(D, O)), up
-// to 1 / 128 left as it is.  Of 44 500 random blocks more than 1.5 times one rounding's error had 19% of those
-// below (up to 2.2 times) and 0.5% of the others.
+// A small block: one large value of h, or of an output, may decide the error of all, and h, dg and du are taken in
+// two parts of a 16-bit type.  The error's square is that of one rounding times 1 + a weighted mean over h's values
+// (their fourth moment is some 24 squares of the second) over one over the outputs' (6): a variance of 24 / (n F) +
+// 6 / (n min(D, O)), up to 1 / 128 left as it is.  Of 44 500 random blocks more than 1.5 times one rounding's error
+// had 19% of those below (up to 2.2 times) and 0.5% of the others.
 inline bool twice_ok(int64_t n, int D, int F, int O, int bytes) {
     const double w = D < O ? D : O;
     return bytes == 2 && 128.0 * (24.0 / F + 6.0 / w) > (double)n && n * F < (1 << 28);      // parts: 32 bits apart
@@ -1742,9 +1748,9 @@ int run_feed_grad(const FeedSizes& z, int act, int dtype, const void* dy, int64_
     if (sizeof(T) == 4 || !z.twice) {
         ok = by_tile<T>(z.large_grads, dma, launch);
     } else if constexpr (sizeof(T) == 2) {
-        // dx by pairs, whose 64 KB of LDS leave two blocks a CU, unless the grid has more of them.  In one part, by pairs
-        // and with every step twice, us for forward and backward, bf16: 4 x 512 -> 2000 -> 512 27.4, 28.8 and 30.4; one row of
-        // 2048 -> 2048 -> 2048 43.2, 48.5 and 45.6
+        // dx by pairs, whose 64 KB of LDS leave two blocks a CU, unless the grid has more of them.  In one part, by
+        // pairs and with every step twice, us for forward and backward, bf16: 4 x 512 -> 2000 -> 512 27.4, 28.8 and
+        // 30.4; one row of 2048 -> 2048 -> 2048 43.2, 48.5 and 45.6
         int64_t blocks = 0;
         for (int i = 0; i < 3; ++i) blocks += tile_count(b, false, G.p[i].M, G.p[i].N) * z.splits[i];
         ok = !dma                ? launch_with(TileTwice(), std::false_type(), TilePair())

@@ -55,7 +55,7 @@ def _call(name: str, dev: torch.device, *args) -> None:
 def _unrecorded() -> None:
     """A call's tensor requires a gradient, which autograd would silently not get."""
     if torch.is_grad_enabled():
-        raise RuntimeError("the expert layer's calls are not recorded by autograd, and a tensor requires a gradient: "
+        raise RuntimeError("these calls are not recorded by autograd, and a tensor requires a gradient: "
                            "call them under torch.no_grad() and take the gradients from the _grad functions, or "
                            "detach it")
 
@@ -73,7 +73,7 @@ def _matrix(t: torch.Tensor, what: str, dtype: torch.dtype | None = None) -> tor
     if t.dim() != 2:
         raise ValueError(f"{what} must be a matrix, got shape {tuple(t.shape)}")
     if not t.is_cuda:
-        raise RuntimeError(f"{what} must be on a HIP device: the expert layer has no CPU form")
+        raise RuntimeError(f"{what} must be on a HIP device: this call has no CPU form")
     if t.dtype not in DTYPES or (dtype is not None and t.dtype != dtype):
         raise ValueError(f"{what} must be {dtype or 'float32, bfloat16 or float16'}, got {t.dtype}")
     rows, cols = t.shape

@@ -77,7 +77,8 @@ def feed_forward(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, *, ac
     dev, dt, lib = x.device, DTYPES[x.dtype], _lib.load()
     nbytes = lib.yabt_feed_forward_workspace_bytes(dt, n, D, F, O)
     if nbytes == 0:
-        raise ValueError("feed_forward: sizes out of range (D, F, O <= 2^24, n < 2^31 - 256, tiles of fewer than 2^32 threads)")
+        raise ValueError("feed_forward: sizes out of range (D, F, O <= 2^24, n < 2^31 - 256, tiles of fewer than 2^32 "
+                         "threads)")
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     y = torch.empty((n, O), dtype=x.dtype, device=dev)
     inner = None
@@ -105,7 +106,8 @@ def feed_forward_grad(dy: torch.Tensor, x: torch.Tensor, w_in: torch.Tensor, w_o
         raise ValueError(f"dy must have shape {(n, O)} on {dev}, got {tuple(dy.shape)}")
     nbytes = int(lib.yabt_feed_forward_grad_workspace_bytes(dt, n, D, F, O))
     if nbytes == 0:
-        raise ValueError("feed_forward_grad: sizes out of range (D, F, O <= 2^24, n < 2^31 - 256, tiles of fewer than 2^32 threads)")
+        raise ValueError("feed_forward_grad: sizes out of range (D, F, O <= 2^24, n < 2^31 - 256, tiles of fewer than 2^32 "
+                         "threads)")
     size = int(lib.yabt_feed_forward_inner_bytes(dt, n, D, F, O))
     if inner.dtype != torch.uint8 or tuple(inner.shape) != (size,) or inner.device != dev or \
             not inner.is_contiguous() or inner.data_ptr() % 256:
