@@ -642,6 +642,7 @@ int yabt_adamw_values(int count, const yabt_adamw_tensor *tensors, yabt_stream_t
  * the backward pass.  h is rounded to `dtype` before the second product (in small blocks,
  * 24 / F + 6 / min(D, O) > n / 128, and for y of 16 rows or fewer with n F O <= 2^26 to two parts of it), so that in fp16 one
  * beyond 65504 makes its row infinite or NaN; sums are fp32.  n below 2^31 - 256, D, F, O to 2^24.
+ * Where h, or an inner gradient, has two parts, an infinite weight, x or dy that it is multiplied by counts as NaN.
  * In fp32 an infinite x or weight may count as NaN, and values below 2^-110 are taken to 2^-133 (the
  * forward pass of 64 rows or fewer in full).
  * Sums are added in an order that the sizes fix.  Sizes whose launches would have 2^32

@@ -493,6 +493,13 @@ __device__ __forceinline__ void parts_sums(const Product& P, int mf, int nf, int
     __syncthreads();                             // the sums leave through the same LDS
 }
 
+// What is left of v beside its first part; 0 where that is infinite, whose sum with it would be NaN.
+template <typename T>
+__device__ __forceinline__ float second_part(float v, T first) {
+    const float rest = v - (float)first;
+    return fabsf(rest) <= 3.402823466e38f ? rest : 0.0f;
+}
+
 // Up to four values at p in the type that a run-time number names.
 __device__ __forceinline__ void store_as(int dtype, void* p, size_t at, f32x4 v, int have) {
     if (dtype == DT_F32) store_part((float*)p + at, v, have);
@@ -535,11 +542,11 @@ struct TileTwice : TileOf<64, 128, 2, 2, 128, 2, 2> {};
 template <typename TL> constexpr bool PAIR = std::is_same_v<TL, TilePair>;
 template <typename TL> constexpr bool TWICE = std::is_same_v<TL, TileTwice>;
 
-// What a value's rounding to T leaves of it, the second part.
+// What values' roundings to T leave of them, the second parts.
 template <typename T>
 __device__ __forceinline__ void rest_of(const float* v, float (&rest)[4]) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) rest[q] = v[q] - (float)(T)v[q];
+    for (int q = 0; q < 4; ++q) rest[q] = second_part(v[q], (T)v[q]);
 }
 
 // One tile of the product MODE: that of the block with number `block` of the product's.
@@ -1134,7 +1141,7 @@ struct FewHalves {                               // fp32 rows in two parts of T:
         for (int q = 0; q < 8; ++q) {
             const float f = __builtin_bit_cast(f32x4, raw[q / 4])[q % 4];
             hi[q] = (T)f;
-            lo[q] = (T)(f - (float)hi[q]);
+            lo[q] = (T)second_part(f, hi[q]);
         }
         v[0] = __builtin_bit_cast(u32x4, hi);
         v[1] = __builtin_bit_cast(u32x4, lo);

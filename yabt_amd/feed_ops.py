@@ -65,7 +65,8 @@ def feed_forward(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, *, ac
 
     16-bit types round act(g) * u to theirs before w_out, and the inner gradients; small
     blocks (24 / F + 6 / min(D, O) > n / 128) keep 16 bits of them, and y of 16 rows or fewer
-    (n F O <= 2^26) of act(g) * u; in float16 one beyond 65504 makes its row infinite or NaN.
+    (n F O <= 2^26) of act(g) * u; what they are multiplied by there, a weight, x or dy, counts
+    as NaN where it is infinite.  In float16 an act(g) * u beyond 65504 makes its row infinite or NaN.
     In float32 an infinite x or weight may count as NaN, and of more than 64 rows x, weights
     and act(g) * u below 2^-110 are taken to 2^-133 (their gradients' factors too)."""
     if x.requires_grad or w_in.requires_grad or w_out.requires_grad:
