@@ -493,11 +493,12 @@ __device__ __forceinline__ void parts_sums(const Product& P, int mf, int nf, int
     __syncthreads();                             // the sums leave through the same LDS
 }
 
-// What is left of v beside its first part; 0 where that is infinite, whose sum with it would be NaN.
+// What is left of v beside its first part, or beside the type's largest value where that is infinite: infinity less
+// infinity would be NaN, which the product's sum then is.
 template <typename T>
 __device__ __forceinline__ float second_part(float v, T first) {
-    const float rest = v - (float)first;
-    return fabsf(rest) <= 3.402823466e38f ? rest : 0.0f;
+    constexpr float most = std::is_same_v<T, f16> ? 65504.0f : std::is_same_v<T, bf16> ? 0x1.FEp127f : 0x1.FFFFFEp127f;
+    return v - __builtin_amdgcn_fmed3f((float)first, -most, most);
 }
 
 // Up to four values at p in the type that a run-time number names.
